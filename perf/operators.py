@@ -167,7 +167,7 @@ def prepare(case, seed):
         s["bias"] = (0.1 if c["score"] == "sigmoid" else 0.5 / E) * _randn(g, (E,)) if c["bias"] else None
         s["ids"], s["w"] = torch.empty((T, k), dtype=torch.int32, device="cuda"), torch.empty((T, k), device="cuda")
         s["offsets"], s["inv"] = torch.empty(E + 1, dtype=torch.int32, device="cuda"), torch.empty((T, k), dtype=torch.int32, device="cuda")
-        s["work"] = torch.empty(4 * (E + 1) * (T * k // 256 + 3), dtype=torch.uint8, device="cuda")
+        s["work"] = torch.empty(4 * E * (-(-T // 32) + 1), dtype=torch.uint8, device="cuda")
         return s
     if c["op"] == "quant":
         T, K, k = c["T"], c["K"], c["k"]
