@@ -19,7 +19,9 @@ SYMBOLS = ("moe_layer_create", "moe_layer_destroy", "moe_layer_forward", "moe_la
            "moe_layer_wire_row_bytes", "moe_layer_received_ids_device", "moe_layer_gather_rows_device", "moe_layer_experts_device", "moe_layer_shared_device",
            "moe_layer_combine_device", "moe_layer_read_groups", "moe_layer_read_quantized", "moe_layer_read_logits",
            "moe_layer_read_config", "moe_layer_forward_residual_device", "moe_rmsnorm_rows_device", "moe_layer_dispatch_row_bytes", "moe_layer_dispatch_plan_device", "moe_layer_dispatch_rows_device",
-           "moe_layer_experts_partial_device", "moe_layer_combine_partials_device", "moe_gguf_open", "moe_gguf_close", "moe_gguf_layers", "moe_gguf_tensors", "moe_layer_create_from_gguf")
+           "moe_layer_experts_partial_device", "moe_layer_combine_partials_device", "moe_gguf_open", "moe_gguf_close", "moe_gguf_layers", "moe_gguf_tensors", "moe_layer_create_from_gguf",
+           "moe_route_work_bytes", "moe_route_logits_device", "moe_mx4_scale_row_bytes", "moe_mx4_quantize_rows_device", "moe_mx4_dequantize_rows_device",
+           "moe_mx4_from_blocks_device", "moe_mx4_product_device", "moe_mx4_gate_up_device", "moe_combine_rows_device", "moe_ops_error")
 
 
 class Config(C.Structure):
@@ -54,12 +56,22 @@ class Stats(C.Structure):
                                           "last_tiles", "last_experts_hit", "last_tensor_rows")]
 
 
+class RouteConfig(C.Structure):
+    _fields_ = [("n_experts", C.c_uint32), ("n_used", C.c_uint32), ("score", C.c_uint32), ("n_groups", C.c_uint32),
+                ("n_groups_used", C.c_uint32), ("no_renorm", C.c_uint32), ("scale", C.c_float), ("logits_type", C.c_uint32)]
+
+
+class Mx4Weights(C.Structure):
+    _fields_ = [("n_experts", C.c_uint32), ("n_out", C.c_uint32), ("n_in", C.c_uint32), ("reserved", C.c_uint32),
+                ("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p)]
+
+
 class AbiRow(C.Structure):
     _fields_ = [("name", C.c_char_p), ("offset", C.c_uint32), ("size", C.c_uint32)]
 
 
 STRUCTS = {"moe_gguf_tensor": GgufTensor, "moe_layer_config": Config, "moe_layer_weights": Weights, "moe_tile": Tile, "moe_group": Group, "moe_layer_stats": Stats,
-           "moe_abi_row": AbiRow}
+           "moe_route_config": RouteConfig, "moe_mx4_weights": Mx4Weights, "moe_abi_row": AbiRow}
 
 _lib = None
 
@@ -124,6 +136,19 @@ def lib():
         L.moe_layer_combine_device.argtypes = [vp, vp, u32, vp, vp]
         L.moe_route_rows_static.argtypes = [vp, u32, u32, vp, vp, u32, u32, vp, vp, vp, vp]
         L.moe_route_rows_static_error.restype = C.c_char_p
+        u64 = C.c_uint64
+        L.moe_route_work_bytes.argtypes = [u32, u32]
+        L.moe_route_work_bytes.restype = u64
+        L.moe_route_logits_device.argtypes = [C.POINTER(RouteConfig), vp, u64, vp, u32, vp, vp, vp, vp, vp, u64, vp]
+        L.moe_mx4_scale_row_bytes.argtypes = [u32]
+        L.moe_mx4_scale_row_bytes.restype = u32
+        L.moe_mx4_quantize_rows_device.argtypes = [vp, u32, u64, u32, u32, vp, u32, u32, vp, vp, vp]
+        L.moe_mx4_dequantize_rows_device.argtypes = [vp, vp, u32, u32, vp, u32, vp]
+        L.moe_mx4_from_blocks_device.argtypes = [vp, u32, u32, vp, vp, vp]
+        L.moe_mx4_product_device.argtypes = [C.POINTER(Mx4Weights), vp, vp, u32, vp, vp, u32, vp]
+        L.moe_mx4_gate_up_device.argtypes = [C.POINTER(Mx4Weights), vp, vp, u32, vp, C.c_float, vp, vp, vp]
+        L.moe_combine_rows_device.argtypes = [vp, u32, u32, vp, vp, u32, u32, u32, vp, vp, vp]
+        L.moe_ops_error.restype = C.c_char_p
         L.moe_abi_layout.argtypes = [C.POINTER(AbiRow), u32]
         L.moe_abi_layout.restype = u32
         _lib = L

@@ -1564,6 +1564,10 @@ MOE_API uint32_t moe_abi_layout(moe_abi_row *table, uint32_t cap) {
       ROW(moe_group, slot), ROW(moe_group, start), ROW(moe_group, n),
       ROW(moe_gguf_tensor, name), ROW(moe_gguf_tensor, type), ROW(moe_gguf_tensor, n_dims), ROW(moe_gguf_tensor, shape),
       ROW(moe_gguf_tensor, offset), ROW(moe_gguf_tensor, bytes),
+      ROW(moe_route_config, n_experts), ROW(moe_route_config, n_used), ROW(moe_route_config, score), ROW(moe_route_config, n_groups),
+      ROW(moe_route_config, n_groups_used), ROW(moe_route_config, no_renorm), ROW(moe_route_config, scale), ROW(moe_route_config, logits_type),
+      ROW(moe_mx4_weights, n_experts), ROW(moe_mx4_weights, n_out), ROW(moe_mx4_weights, n_in), ROW(moe_mx4_weights, reserved),
+      ROW(moe_mx4_weights, codes_dev), ROW(moe_mx4_weights, scales_dev),
       ROW(moe_abi_row, name), ROW(moe_abi_row, offset), ROW(moe_abi_row, size),
 #undef ROW
       {"moe_layer_config", 0, (uint32_t)sizeof(moe_layer_config)},
@@ -1572,6 +1576,8 @@ MOE_API uint32_t moe_abi_layout(moe_abi_row *table, uint32_t cap) {
       {"moe_group", 0, (uint32_t)sizeof(moe_group)},
       {"moe_gguf_tensor", 0, (uint32_t)sizeof(moe_gguf_tensor)},
       {"moe_layer_stats", 0, (uint32_t)sizeof(moe_layer_stats)},
+      {"moe_route_config", 0, (uint32_t)sizeof(moe_route_config)},
+      {"moe_mx4_weights", 0, (uint32_t)sizeof(moe_mx4_weights)},
       {"moe_abi_row", 0, (uint32_t)sizeof(moe_abi_row)},
   };
   const uint32_t n = (uint32_t)(sizeof(rows) / sizeof(rows[0]));

@@ -1,0 +1,202 @@
+// Rows to and from microscaled 4-bit floating point, and the combine without a layer. All are single passes over their data: what
+// bounds them is HBM.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "mx4.cuh"
+#include "ops_common.h"
+
+namespace moe {
+namespace {
+
+constexpr uint32_t kRowsMaxUsed = 16;
+
+// A thread takes 8 values, four threads a block of 32, a CTA 2,048 values of one row (grid.x the row, grid.y the piece). The block's
+// largest magnitude is an integer maximum over the four threads: magnitudes order as their bits do.
+template <class X>
+__global__ void __launch_bounds__(256) k_mx4_quantize(const X *x, uint64_t stride, uint32_t K, const int32_t *inv, uint32_t n_used, uint32_t R,
+                                                      uint8_t *codes, uint8_t *scales) {
+  dependents_may_launch(), wait_for_predecessors();
+  const uint64_t t = blockIdx.x;
+  const uint32_t k = (blockIdx.y * 256 + threadIdx.x) * 8;
+  const bool in = k < K;  // K is a multiple of 32: a block's four threads alike
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (in) load8(x + t * stride + k, v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const uint32_t scale = mx_scale_of(m);
+  const float f = mx_inverse(scale);
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] *= f;
+  const uint32_t c = scale == 255 ? 0u : mx_codes8(v);
+  const uint32_t srow = mx_scale_row_bytes(K), b = k / kMxBlock;
+  const uint32_t n = inv ? n_used : 1;
+  for (uint32_t j = 0; j < n; j++) {
+    const uint64_t r = inv ? (uint64_t)(uint32_t)inv[t * n_used + j] : t;
+    if (r >= R) continue;
+    if (in) *(uint32_t *)(codes + r * (K / 2) + k / 2) = c;
+    if (threadIdx.x % 4 == 0 && b < srow) scales[r * srow + b] = in ? (uint8_t)scale : 0;
+  }
+}
+
+template <class Y>
+__global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, uint32_t K, Y *out) {
+  dependents_may_launch(), wait_for_predecessors();
+  const uint64_t r = blockIdx.x;
+  const uint32_t k = (blockIdx.y * 256 + threadIdx.x) * 8;
+  if (k >= K) return;
+  float v[8];
+  mx_values8(*(const uint32_t *)(codes + r * (K / 2) + k / 2), v);
+  const float f = mx_scale(scales[r * mx_scale_row_bytes(K) + k / kMxBlock]);
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] *= f;
+  store8(out + r * K + k, v);
+}
+
+// A thread a block of the file: its bytes hold value j and value j + 16, the rows' hold neighbours.
+__global__ void __launch_bounds__(256) k_mx4_from_blocks(const uint8_t *blocks, uint32_t K, uint8_t *codes, uint8_t *scales) {
+  dependents_may_launch(), wait_for_predecessors();
+  const uint64_t r = blockIdx.x;
+  const uint32_t b = blockIdx.y * 256 + threadIdx.x, srow = mx_scale_row_bytes(K);
+  if (b >= srow) return;
+  if (b >= K / kMxBlock) {
+    scales[r * srow + b] = 0;
+    return;
+  }
+  const uint8_t *p = blocks + (r * (K / kMxBlock) + b) * 17;
+  scales[r * srow + b] = p[0];
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const uint32_t lo = p[1 + i], hi = p[2 + i];
+    w[i / 8] |= ((lo & 15u) | (hi & 15u) << 4) << (i / 2 % 4 * 8);
+    w[2 + i / 8] |= (lo >> 4 | (hi >> 4) << 4) << (i / 2 % 4 * 8);
+  }
+  *(uint4 *)(codes + r * (K / 2) + b * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A thread takes 8 columns of a row and loads its n_used results before it adds the first.
+template <class Y>
+__global__ void __launch_bounds__(256) k_combine_rows(const Y *y, uint32_t R, const int32_t *inv, const float *w, uint32_t n_used, uint32_t E,
+                                                      const float *res, float *out) {
+  dependents_may_launch(), wait_for_predecessors();
+  const uint64_t t = blockIdx.x;
+  const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 8;
+  if (c >= E) return;
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+  for (uint32_t j = 0; j < n_used; j++) {
+    const uint32_t r = (uint32_t)inv[t * n_used + j];
+    if (r >= R) continue;
+    const float wj = w[t * n_used + j];
+    float v[8];
+    load8(y + (uint64_t)r * E + c, v);
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc[i] = fmaf(wj, v[i], acc[i]);
+  }
+  if (res) {
+    float v[8];
+    load8(res + t * E + c, v);
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc[i] += v[i];
+  }
+  store8(out + t * E + c, acc);
+}
+
+// Grids of (rows, pieces of a row): rows up to 2^31 - 1.
+dim3 rows_grid(uint32_t rows, uint32_t per_row) { return dim3(rows, (per_row + 255) / 256); }
+
+void need_mx_row(uint32_t K) { need(K >= kMxBlock && K % kMxBlock == 0 && K <= kMxMaxValues, "a row's values must be a multiple of 32, 32 .. 65536"); }
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+MOE_API uint32_t moe_mx4_scale_row_bytes(uint32_t K) { return mx_scale_row_bytes(K); }
+
+MOE_API moe_status moe_mx4_quantize_rows_device(const void *x_dev, uint32_t type, uint64_t stride, uint32_t T, uint32_t K, const int32_t *inv_dev,
+                                                uint32_t n_used, uint32_t R, void *codes_dev, void *scales_dev, void *stream) {
+  return ops_call([&] {
+    const uint32_t size = row_type_bytes(type);
+    need(size != 0, "type must be MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need_mx_row(K);
+    need(stride == 0 || (stride >= K && stride < 1ull << 32 && stride * size % 16 == 0), "stride must be 0, or K at least with rows 16-byte aligned");
+    need(inv_dev ? n_used >= 1 && n_used <= kRowsMaxUsed : R == T, "n_used must be 1 .. 16 with inv, and R be T without");
+    need(T < 1u << 31 && R < 1u << 31, "T and R must be below 2^31");
+    if (T == 0 || R == 0) return;
+    need_device({{x_dev, "x", 16}, {inv_dev, "inv", 4, true}, {codes_dev, "codes", 16}, {scales_dev, "scales", 4}});
+    const uint64_t s = stride ? stride : K;
+    uint8_t *codes = (uint8_t *)codes_dev, *scales = (uint8_t *)scales_dev;
+    // A piece more than the codes need where the scales' filling lies past the last thread.
+    const dim3 grid = rows_grid(T, mx_scale_row_bytes(K) * 4), block(256);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (type == MOE_TYPE_F32)
+      CUDA_OK(launch_kernel(true, k_mx4_quantize<float>, grid, block, 0, st, (const float *)x_dev, s, K, inv_dev, n_used, R, codes, scales));
+    else if (type == MOE_TYPE_F16)
+      CUDA_OK(launch_kernel(true, k_mx4_quantize<__half>, grid, block, 0, st, (const __half *)x_dev, s, K, inv_dev, n_used, R, codes, scales));
+    else
+      CUDA_OK(launch_kernel(true, k_mx4_quantize<__nv_bfloat16>, grid, block, 0, st, (const __nv_bfloat16 *)x_dev, s, K, inv_dev, n_used, R, codes, scales));
+  });
+}
+
+MOE_API moe_status moe_mx4_dequantize_rows_device(const void *codes_dev, const void *scales_dev, uint32_t R, uint32_t K, void *out_dev,
+                                                  uint32_t type, void *stream) {
+  return ops_call([&] {
+    need(row_type_bytes(type) != 0, "type must be MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need_mx_row(K);
+    need(R < 1u << 31, "R must be below 2^31");
+    if (R == 0) return;
+    need_device({{codes_dev, "codes", 16}, {scales_dev, "scales", 4}, {out_dev, "out", 16}});
+    const uint8_t *codes = (const uint8_t *)codes_dev, *scales = (const uint8_t *)scales_dev;
+    const dim3 grid = rows_grid(R, K / 8), block(256);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (type == MOE_TYPE_F32)
+      CUDA_OK(launch_kernel(true, k_mx4_dequantize<float>, grid, block, 0, st, codes, scales, K, (float *)out_dev));
+    else if (type == MOE_TYPE_F16)
+      CUDA_OK(launch_kernel(true, k_mx4_dequantize<__half>, grid, block, 0, st, codes, scales, K, (__half *)out_dev));
+    else
+      CUDA_OK(launch_kernel(true, k_mx4_dequantize<__nv_bfloat16>, grid, block, 0, st, codes, scales, K, (__nv_bfloat16 *)out_dev));
+  });
+}
+
+MOE_API moe_status moe_mx4_from_blocks_device(const void *blocks_dev, uint32_t R, uint32_t K, void *codes_dev, void *scales_dev, void *stream) {
+  return ops_call([&] {
+    need_mx_row(K);
+    need(R < 1u << 31, "R must be below 2^31");
+    if (R == 0) return;
+    need_device({{blocks_dev, "blocks", 1}, {codes_dev, "codes", 16}, {scales_dev, "scales", 4}});
+    CUDA_OK(launch_kernel(true, k_mx4_from_blocks, rows_grid(R, mx_scale_row_bytes(K)), dim3(256), 0, (cudaStream_t)stream, (const uint8_t *)blocks_dev, K,
+                          (uint8_t *)codes_dev, (uint8_t *)scales_dev));
+  });
+}
+
+MOE_API moe_status moe_combine_rows_device(const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev, const float *w_dev, uint32_t T,
+                                           uint32_t n_used, uint32_t n_embd, const float *residual_dev, float *out_dev, void *stream) {
+  return ops_call([&] {
+    need(row_type_bytes(y_type) != 0, "y_type must be MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need(n_used >= 1 && n_used <= kRowsMaxUsed, "n_used must be 1 .. 16");
+    need(n_embd >= 8 && n_embd % 8 == 0 && n_embd <= 1u << 24, "n_embd must be a multiple of 8, at most 2^24");
+    need(T < 1u << 31 && R < 1u << 31, "T and R must be below 2^31");
+    if (T == 0) return;
+    // With R 0 no row of y is read: it may be null then.
+    need_device({{y_dev, "y", 16, R == 0}, {inv_dev, "inv", 4}, {w_dev, "w", 4}, {residual_dev, "residual", 16, true}, {out_dev, "out", 16}});
+    const dim3 grid = rows_grid(T, n_embd / 8), block(256);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (y_type == MOE_TYPE_F32)
+      CUDA_OK(launch_kernel(true, k_combine_rows<float>, grid, block, 0, st, (const float *)y_dev, R, inv_dev, w_dev, n_used, n_embd, residual_dev, out_dev));
+    else if (y_type == MOE_TYPE_F16)
+      CUDA_OK(launch_kernel(true, k_combine_rows<__half>, grid, block, 0, st, (const __half *)y_dev, R, inv_dev, w_dev, n_used, n_embd, residual_dev, out_dev));
+    else
+      CUDA_OK(launch_kernel(true, k_combine_rows<__nv_bfloat16>, grid, block, 0, st, (const __nv_bfloat16 *)y_dev, R, inv_dev, w_dev, n_used, n_embd, residual_dev,
+                            out_dev));
+  });
+}
+
+}  // extern "C"

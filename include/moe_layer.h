@@ -23,7 +23,7 @@ extern "C" {
 #define MOE_API
 #endif
 
-#define MOE_API_VERSION 2
+#define MOE_API_VERSION 3
 
 /* engine_status's values (include/engine_api.h:28-34). */
 typedef enum {
@@ -44,6 +44,11 @@ typedef enum {
 #define MOE_TYPE_IQ2_S 22
 #define MOE_TYPE_IQ4_XS 23
 #define MOE_TYPE_Q2_0 42 /* the reference's fork of ggml (shared/quant.h:33) */
+
+/* Types of the rows that the operators without a layer take, ggml's numbers too. */
+#define MOE_TYPE_F32 0
+#define MOE_TYPE_F16 1
+#define MOE_TYPE_BF16 30
 
 typedef struct moe_layer moe_layer;
 
@@ -305,6 +310,97 @@ MOE_API moe_status moe_route_rows_static(const float *x_dev, uint32_t T, uint32_
                                          const float *bias_dev, uint32_t n_experts, uint32_t n_used, int32_t *ids_dev,
                                          float *w_dev, float *gate_dev, void *stream);
 MOE_API const char *moe_route_rows_static_error(void);
+
+/* Operators without a layer: a MoE block whose router is not a plain softmax, or whose experts are in microscaled 4-bit
+ * floating point, put together by the caller. No counterpart in the reference. In the order a step uses them:
+ *
+ *   moe_route_logits_device (ids, w, offsets, inv) -> moe_mx4_quantize_rows_device (rows into expert order by inv) ->
+ *   moe_mx4_gate_up_device -> moe_mx4_product_device -> moe_combine_rows_device.
+ *
+ * They keep nothing between calls and allocate nothing: every buffer is the caller's, a DEVICE pointer of the current
+ * device (a host pointer or another device's is refused), and every call queues on stream (a cudaStream_t; null: the
+ * default stream) without waiting, so a call can be captured into a graph. The first call of each on a device sets
+ * kernel attributes; that may happen during a capture too. Calls with different buffers may overlap. T or R of 0 is a
+ * call with nothing to do (offsets become 0). moe_ops_error: the calling thread's last message from any of them.
+ *
+ * MX rows: values in blocks of 32 along the row, a value an e2m1 code (sign, 0 0.5 1 1.5 2 3 4 6), a block one e8m0 scale
+ * byte (2^(byte - 127); 255: the block is NaN). codes [rows][K / 2]: value 2i in the low half of byte i, 2i + 1 in the high
+ * half. scales [rows][moe_mx4_scale_row_bytes(K)]: K / 32 bytes, then zeros up to whole words of four (never read). K is a
+ * multiple of 32, at most 65,536; codes pointers are 16-byte aligned, scales pointers 4-byte. */
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
+
+typedef struct {
+  uint32_t n_experts;     /* 1 .. 512 */
+  uint32_t n_used;        /* experts per row, 1 .. 16, at most n_experts */
+  uint32_t score;         /* MOE_SCORE_* */
+  uint32_t n_groups;      /* 0 or 1: none; else groups of n_experts / n_groups neighbouring experts, at most 32 */
+  uint32_t n_groups_used; /* with groups: the groups a row's experts may come from, 1 .. n_groups, that hold n_used experts at
+                             least */
+  uint32_t no_renorm;     /* 0: a row's weights are divided by their sum; 1: they are the scores */
+  float scale;            /* the weights' factor; 0: 1 */
+  uint32_t logits_type;   /* MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16 */
+} moe_route_config;
+
+/* A step's routing from its logits, [T] rows of n_experts values, stride values apart (0: n_experts). A row's scores s are
+ * the softmax of its logits or their sigmoids; an expert's key is s + bias_dev[expert] (null: the score). With groups, the
+ * n_groups_used groups whose two best keys have the largest sums stay (of one expert: its key). ids_dev [T][n_used] are the
+ * largest keys' experts, best first; w_dev [T][n_used] their scores (without the bias), renormalised, times scale. Ties go to
+ * the lower expert, or group. Which experts are chosen is decided as in 64-bit arithmetic on the given logits and bias.
+ * An expert whose logit or bias is -infinity or NaN is out: it takes no part in softmax and is never chosen; a row with too few
+ * others has id -1 and weight 0 in its last places.
+ * offsets_dev (null: no lists; then inv_dev is null too): [n_experts + 1], expert e's rows in expert order are offsets[e] ..
+ * offsets[e + 1]; inv_dev [T][n_used], each assignment's row there, assignments in ascending order within an expert, -1 for
+ * id -1. Rows of more than one launch need work_dev: moe_route_work_bytes(T, n_experts) bytes, 4-byte aligned, whose contents do
+ * not matter and are not kept. T at most 2^24. */
+MOE_API uint64_t moe_route_work_bytes(uint32_t T, uint32_t n_experts);
+MOE_API moe_status moe_route_logits_device(const moe_route_config *config, const void *logits_dev, uint64_t stride, const float *bias_dev,
+                                           uint32_t T, int32_t *ids_dev, float *w_dev, int32_t *offsets_dev, int32_t *inv_dev,
+                                           void *work_dev, uint64_t work_bytes, void *stream);
+
+/* Rows of K values (type MOE_TYPE_F32, F16 or BF16; stride values apart, 0: K; rows 16-byte aligned) to MX rows. A block's
+ * scale is 2^(floor(log2 of its largest magnitude) - 2), at least 2^-127; codes are the nearest values, ties to even, beyond 6
+ * to 6. A block with an infinity or NaN gets scale 255 and codes 0. inv_dev null: row t to row t of R = T rows. Else [T][n_used], and
+ * row t goes to each row inv_dev[t][k] of the R (one outside 0 .. R - 1 is skipped); a row no entry names is left as it was.
+ * dequantize: what R MX rows stand for, rounded to type where that has fewer bits or less range; [R][K], 16-byte aligned.
+ * from_blocks: rows of a GGUF tensor of ggml type 39 (17-byte blocks: the scale, then 16 bytes whose low halves are values 0 .. 15
+ * and high halves 16 .. 31) to MX rows, which is how the experts' matrices of a file get into the form below. */
+MOE_API uint32_t moe_mx4_scale_row_bytes(uint32_t K);
+MOE_API moe_status moe_mx4_quantize_rows_device(const void *x_dev, uint32_t type, uint64_t stride, uint32_t T, uint32_t K, const int32_t *inv_dev,
+                                                uint32_t n_used, uint32_t R, void *codes_dev, void *scales_dev, void *stream);
+MOE_API moe_status moe_mx4_dequantize_rows_device(const void *codes_dev, const void *scales_dev, uint32_t R, uint32_t K, void *out_dev,
+                                                  uint32_t type, void *stream);
+MOE_API moe_status moe_mx4_from_blocks_device(const void *blocks_dev, uint32_t R, uint32_t K, void *codes_dev, void *scales_dev, void *stream);
+
+/* Matrices in MX rows, on the device: n_experts (1 .. 512) of n_out rows of n_in values, one after another. n_out and n_in are
+ * multiples of 32, at most 65,536. */
+typedef struct {
+  uint32_t n_experts;
+  uint32_t n_out;
+  uint32_t n_in;
+  uint32_t reserved;      /* 0 */
+  const void *codes_dev;  /* [n_experts][n_out][n_in / 2] */
+  const void *scales_dev; /* [n_experts][n_out][moe_mx4_scale_row_bytes(n_in)] */
+} moe_mx4_weights;
+
+/* Products of R MX rows in expert order with their experts' matrices, each row with its own expert's: rows offsets_dev[e] ..
+ * offsets_dev[e + 1] with expert e's (ascending, as moe_route_logits_device leaves them; n_experts + 1 of them; what they say past
+ * R is cut off; null: one expert has all R). Rows of no expert are left as they were. Sums are f32.
+ *   product: y_dev [R][n_out], f16 or bf16 (MOE_TYPE_F16, MOE_TYPE_BF16), 16-byte aligned: the products, rounded once.
+ *   gate_up: w's rows are n_out / 2 gate rows and then as many up rows, n_out a multiple of 64; h = g / (1 + exp(-g)) * u,
+ *            with limit > 0 of min(g, limit) and of u held to [-limit, limit], to MX rows of n_out / 2 values.
+ * R at most 2^24. */
+MOE_API moe_status moe_mx4_product_device(const moe_mx4_weights *w, const void *codes_dev, const void *scales_dev, uint32_t R,
+                                          const int32_t *offsets_dev, void *y_dev, uint32_t y_type, void *stream);
+MOE_API moe_status moe_mx4_gate_up_device(const moe_mx4_weights *w, const void *codes_dev, const void *scales_dev, uint32_t R,
+                                          const int32_t *offsets_dev, float swiglu_limit, void *h_codes_dev, void *h_scales_dev, void *stream);
+
+/* out[t] = (residual[t] +) sum over k, in rank order, of w[t][k] * y[inv[t][k]], in f32; an inv outside 0 .. R - 1 adds nothing. y_dev [R][n_embd]
+ * f32, f16 or bf16, residual_dev (or null) and out_dev [T][n_embd] f32; n_embd a multiple of 8; all three 16-byte aligned.
+ * n_used 1 .. 16. out_dev may be residual_dev. */
+MOE_API moe_status moe_combine_rows_device(const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev, const float *w_dev, uint32_t T,
+                                           uint32_t n_used, uint32_t n_embd, const float *residual_dev, float *out_dev, void *stream);
+MOE_API const char *moe_ops_error(void);
 
 /* The layout the GPU holds a slice of nblocks blocks in: one run per field of the block, quants first, as the
  * reference's to_runs and from_runs make it (core/load/runs.cpp:12-41; shared/quant.h:172-176). Host only: a

@@ -1,0 +1,422 @@
+"""On a B200: rows to and from microscaled 4-bit floating point, the experts' products over them and the combine, against the
+definitions in 64 bits."""
+import numpy as np
+import pytest
+
+import ops_common as R
+from c0ven_b200 import MoEError, _lib, ops
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": ops.F32, "f16": ops.F16, "bf16": ops.BF16}
+
+
+def dtype(name):
+    import torch
+
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def dev(a, type=None):
+    import torch
+
+    t = torch.from_numpy(np.ascontiguousarray(a))
+    return (t if type is None else t.to(dtype(type))).cuda()
+
+
+def mx_buffers(rows, K, fill=0xEE):
+    import torch
+
+    return (torch.full((rows, K // 2), fill, dtype=torch.uint8, device="cuda"), torch.full((rows, R.scale_row_bytes(K)), fill, dtype=torch.uint8, device="cuda"))
+
+
+def rows_of(rng, T, K):
+    """Rows with all the sizes a type has room for, zeros, signed zeros and values on the borders between codes."""
+    x = rng.standard_normal((T, K)) * np.exp2(rng.integers(-12, 13, (T, K // 32)).repeat(32, 1).astype(np.float64))
+    b = x.reshape(T, -1, 32)
+    b[0, 0] = 0
+    b[-1, -1] = -0.0
+    borders = np.array([4, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5, 6, 7, -7.5, 7.99, 0.2499, 0.2501, 2.4999, 2.5001, 4.999, 5.001, 0.125, -0.1])
+    b[0, -1, :len(borders)] = borders * 0.125
+    return x
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T, K", [(1, 32), (3, 96), (5, 2048), (2, 2080), (33, 2880), (1, 65536), (700, 160)])
+def test_quantize_rows_bit_for_bit(type, T, K):
+    import torch
+
+    rng = np.random.default_rng(T + K)
+    x = dev(rows_of(rng, T, K).astype(np.float32), type)
+    code, byte = R.quantize(x.double().cpu().numpy())
+    codes, scales = mx_buffers(T + 1, K)
+    ops.mx4_quantize_rows_device(x.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), T)
+    torch.cuda.synchronize()
+    want = R.pack(code, byte)
+    assert np.array_equal(codes[:T].cpu().numpy(), want[0]) and np.array_equal(scales[:T].cpu().numpy(), want[1])
+    assert (codes[T] == 0xEE).all() and (scales[T] == 0xEE).all()
+    for out_type in ("f32", "bf16", "f16"):
+        out = torch.empty((T, K), dtype=dtype(out_type), device="cuda")
+        ops.mx4_dequantize_rows_device(codes.data_ptr(), scales.data_ptr(), T, K, out.data_ptr(), TYPES[out_type])
+        v = R.values(code, byte)
+        exact = torch.from_numpy(v).to(dtype(out_type)).double().numpy()  # rounded once; f32 and bf16 hold every value here
+        assert np.array_equal(out.double().cpu().numpy(), exact)
+        if out_type != "f16":
+            assert np.array_equal(exact, v)
+
+
+def test_quantize_extremes():
+    """The largest and smallest scales, blocks with an infinity or NaN, denormals."""
+    import torch
+
+    rng = np.random.default_rng(1)
+    x = rng.uniform(1, 2, (9, 64)).astype(np.float32)
+    x[0] = np.finfo(np.float32).max
+    x[1] = 2.0 ** -126 * x[1]
+    x[2] = 2.0 ** -140
+    x[3] = np.float32(2.0 ** -149)
+    x[4, 3], x[4, 40] = np.inf, -np.inf
+    x[5, 63] = np.nan
+    x[6] *= np.float32(2.0 ** -125)
+    x[7, :32] = 2.0 ** 120
+    x[8] *= -1
+    codes, scales = mx_buffers(9, 64)
+    xd = dev(x)
+    ops.mx4_quantize_rows_device(xd.data_ptr(), ops.F32, 9, 64, codes.data_ptr(), scales.data_ptr(), 9)
+    code, byte = R.quantize(x)
+    want = R.pack(code, byte)
+    assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
+    assert byte[4, 0] == 255 and byte[4, 1] == 255 and byte[5, 0] != 255 and byte[5, 1] == 255 and byte[0, 0] == 252 and byte[3, 0] == 0
+    out = torch.empty((9, 64), device="cuda")
+    ops.mx4_dequantize_rows_device(codes.data_ptr(), scales.data_ptr(), 9, 64, out.data_ptr(), ops.F32)
+    assert np.array_equal(out.cpu().numpy().astype(np.float64), R.values(code, byte), equal_nan=True)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_quantize_scatters_strided_rows(type):
+    """Every row to the places its assignments have; places of none and rows past R are left as they were."""
+    import torch
+
+    rng = np.random.default_rng(2)
+    T, K, n, rows = 21, 224, 5, 90
+    full = dev(rng.standard_normal((T, 256)).astype(np.float32), type)
+    inv = rng.permutation(120)[:T * n].reshape(T, n).astype(np.int32)  # some at rows and past
+    inv[3, 2], inv[4, :] = -1, -1
+    codes, scales = mx_buffers(rows + 2, K)
+    di = dev(inv)
+    ops.mx4_quantize_rows_device(full.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), rows, stride=256, inv_ptr=di.data_ptr(), n_used=n)
+    torch.cuda.synchronize()
+    c, s = R.pack(*R.quantize(full.double().cpu().numpy()[:, :K]))
+    want_c, want_s = np.full((rows + 2, K // 2), 0xEE, np.uint8), np.full((rows + 2, R.scale_row_bytes(K)), 0xEE, np.uint8)
+    for t in range(T):
+        for r in inv[t]:
+            if 0 <= r < rows:
+                want_c[r], want_s[r] = c[t], s[t]
+    assert np.array_equal(codes.cpu().numpy(), want_c) and np.array_equal(scales.cpu().numpy(), want_s)
+
+
+def test_rows_of_a_files_blocks():
+    import torch
+
+    rng = np.random.default_rng(3)
+    for rows, K in ((1, 32), (5, 160), (3, 9600)):
+        code, byte = rng.integers(0, 16, (rows, K), dtype=np.uint8), rng.integers(0, 255, (rows, K // 32), dtype=np.uint8)
+        b = code.reshape(rows, -1, 2, 16)
+        blocks = np.concatenate([byte[..., None], b[:, :, 0] | b[:, :, 1] << 4], -1)  # the scale; low halves values 0 .. 15, high halves 16 .. 31
+        codes, scales = mx_buffers(rows, K)
+        bd = dev(blocks)
+        ops.mx4_from_blocks_device(bd.data_ptr(), rows, K, codes.data_ptr(), scales.data_ptr())
+        torch.cuda.synchronize()
+        want = R.pack(code, byte)
+        assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
+
+
+def product_case(rng, E, N, K, offsets, rows):
+    """Weights and rows with their values: w (codes, scales) [E][N], x [rows]."""
+    (wc, ws), w = R.random_mx(rng, (E, N, K))
+    (xc, xs), x = R.random_mx(rng, (rows, K), 125, 129)
+    # Bytes that fill a row's scales up are never read.
+    ws[..., K // 32:] = 255
+    xs[..., K // 32:] = 255
+    return dev(wc), dev(ws), w, dev(xc), dev(xs), x
+
+
+def by_expert(x, w, offsets, rows, absolute=False):
+    out = np.zeros((rows, w.shape[1]))
+    if absolute:
+        x, w = np.abs(x), np.abs(w)
+    for e in range(w.shape[0]):
+        a, b = offsets[e], min(offsets[e + 1], rows)
+        out[a:b] = x[a:b] @ w[e].T
+    return out
+
+
+def sum_bound(magnitude, K):
+    """What an f32 sum of K products (exact themselves: two-bit significands) may be off by: a step of 2^-23 of the running sum a product,
+    however the hardware orders or cuts them."""
+    return K * 2.0 ** -23 * magnitude
+
+
+SHAPES = [(1, 32, 32, [5]), (1, 64, 96, [1]), (1, 160, 256, [300]), (3, 128, 64, [0, 7, 130]), (8, 96, 544, [1, 0, 2, 64, 65, 0, 17, 1]),
+          (5, 288, 2880, [16, 15, 0, 33, 1]), (2, 2080, 160, [129, 257]), (70, 64, 128, [1] * 70), (4, 32, 4096, [0, 0, 0, 3]), (512, 32, 32, [0, 1] * 256)]
+
+
+@pytest.mark.parametrize("y_type", ["f16", "bf16"])
+@pytest.mark.parametrize("E, N, K, counts", SHAPES)
+def test_products(E, N, K, counts, y_type):
+    import torch
+
+    rng = np.random.default_rng(N + K)
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    used = int(offsets[-1])
+    rows = used + 3  # rows of no expert behind the last
+    wc, ws, w, xc, xs, x = product_case(rng, E, N, K, offsets, rows)
+    y = torch.full((rows + 1, N), 7.0, dtype=dtype(y_type), device="cuda")
+    od = dev(offsets)
+    for at in (od.data_ptr(),) + ((None,) if E == 1 else ()):
+        y[:] = 7.0
+        r = rows if at else used
+        ops.mx4_product_device(ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), r, at, y.data_ptr(), TYPES[y_type])
+        torch.cuda.synchronize()
+        got, want, size = y.double().cpu().numpy(), by_expert(x, w, offsets, rows), by_expert(x, w, offsets, rows, True)
+        assert (got[used:] == 7.0).all()
+        off = np.abs(got[:used] - want[:used])
+        assert (off <= HALF(y_type) * np.abs(want[:used]) + sum_bound(size[:used], K) * (1 + HALF(y_type)) + 2.0 ** -25).all(), off.max()
+        # Taken together the roundings spread: no more than half a step, and the sums' own error is far below it.
+        assert np.linalg.norm(off) <= (HALF(y_type) + 1e-5) * np.linalg.norm(want[:used])
+
+
+def HALF(y_type):
+    return R.HALF_STEP[y_type]
+
+
+def test_offsets_that_say_too_much_are_cut_off():
+    """Offsets past R, below 0 or falling: no row outside 0 .. R - 1 is read or written."""
+    import torch
+
+    rng = np.random.default_rng(11)
+    E, N, K, rows = 4, 64, 64, 40
+    wc, ws, w, xc, xs, x = product_case(rng, E, N, K, None, rows)
+    y = torch.full((rows + 8, N), 7.0, dtype=torch.float16, device="cuda")
+    for offsets, sound in (([0, 10, 20, 30, 1000], [0, 10, 20, 30, 40]), ([-5, 10, 20, 20, 2 ** 31 - 1], [0, 10, 20, 20, 40])):
+        y[:] = 7.0
+        od = dev(np.array(offsets, np.int32))
+        ops.mx4_product_device(ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), y.data_ptr(), ops.F16)
+        torch.cuda.synchronize()
+        want = by_expert(x, w, np.array(sound), rows)
+        got = y.double().cpu().numpy()
+        assert (got[rows:] == 7.0).all()
+        assert np.linalg.norm(got[:rows] - want) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(want)
+    od = dev(np.array([30, 20, 35, 10, 5], np.int32))
+    ops.mx4_product_device(ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), y.data_ptr(), ops.F16)
+    torch.cuda.synchronize()
+    assert (y[rows:] == 7.0).all()
+
+
+def test_nan_scales_reach_their_rows_alone():
+    import torch
+
+    rng = np.random.default_rng(12)
+    E, N, K, rows = 2, 64, 320, 50
+    wc, ws, w, xc, xs, x = product_case(rng, E, N, K, None, rows)
+    xs[17, 3] = 255
+    ws[1, 40, 9] = 255
+    offsets = dev(np.array([0, 20, 50], np.int32))
+    y = torch.empty((rows, N), dtype=torch.bfloat16, device="cuda")
+    ops.mx4_product_device(ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, offsets.data_ptr(), y.data_ptr(), ops.BF16)
+    bad = torch.isnan(y).cpu().numpy()
+    want = np.zeros((rows, N), bool)
+    want[17] = True
+    want[20:, 40] = True
+    assert np.array_equal(bad, want)
+
+
+@pytest.mark.parametrize("limit", [0.0, 2.0])
+@pytest.mark.parametrize("E, F, K, counts", [(1, 32, 32, [5]), (3, 64, 96, [0, 7, 130]), (6, 96, 2880, [1, 0, 33, 64, 2, 0]), (2, 224, 256, [129, 257]), (1, 640, 544, [300])])
+def test_gate_up(E, F, K, counts, limit):
+    import torch
+
+    rng = np.random.default_rng(F + K)
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    used = int(offsets[-1])
+    rows = used + 3
+    wc, ws, w, xc, xs, x = product_case(rng, E, 2 * F, K, offsets, rows)
+    hc, hs = mx_buffers(rows, F)
+    od = dev(offsets)
+    ops.mx4_gate_up_device(ops.Mx4Weights(E, 2 * F, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), hc.data_ptr(),
+                           hs.data_ptr(), swiglu_limit=limit)
+    torch.cuda.synchronize()
+    assert (hc[used:] == 0xEE).all() and (hs[used:] == 0xEE).all()
+    assert (hs[:used, F // 32:] == 0).all()
+    code, byte = R.unpack(hc[:used].cpu().numpy(), hs[:used].cpu().numpy())
+    v, size = by_expert(x, w, offsets, rows)[:used], by_expert(x, w, offsets, rows, True)[:used]
+    g, u = v[:, :F], v[:, F:]
+    h = R.swiglu(g, u, limit)
+    # What h may be off by before it is rounded: the sums' errors through a function whose slopes are at most 1.1 |u| and |silu(g)|, at most g above
+    # zero and 0.28 below, both of what the limit leaves; and the exponential and division, 2^-20 of it.
+    e = sum_bound(size, K)
+    eg, eu, top = e[:, :F], e[:, F:], limit or np.inf
+    err = 1.1 * np.minimum(np.abs(u) + eu, top) * eg + np.clip(g + eg, 0.28, max(top, 0.28)) * eu + 2.0 ** -20 * np.abs(h) + 1e-38
+    # A block's scale is the largest magnitude's, or a neighbour's where that lies within its error of a power of two.
+    hb, eb = np.abs(h).reshape(used, -1, 32), err.reshape(used, -1, 32)
+    lo, hi = ((hb - eb).clip(0).max(2), (hb + eb).max(2))
+    blo, bhi = (np.where(m > 0, np.maximum(np.frexp(np.where(m > 0, m, 1))[1] - 3, -127) + 127, 0) for m in (lo, hi))
+    assert ((byte >= blo) & (byte <= bhi)).all()
+    # Each code is right for some value within the error: between the codes of the error's two ends.
+    s = np.repeat(np.exp2(byte.astype(np.float64) - 127), 32, axis=1)
+    nearest = lambda a: np.sign(a) * R.E2M1[np.searchsorted([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.abs(a))]  # noqa: E731
+    down, up = (h - err) / s, (h + err) / s
+    got = R.E2M1[code & 7] * np.where(code & 8, -1.0, 1.0)
+    tie = 1e-9
+    assert ((got >= nearest(down - tie)) & (got <= nearest(up + tie))).all()
+    # That bound is the worst case's. Roundings spread: a sum is off by some 2^-23 of its terms' magnitudes, h by a K-th of err then, and a code
+    # differs from h's own where a border lies that near: borders are half a scale apart or more, so of all codes 4 err / (K s) at most, which
+    # is under two thousandths in each of these cases; five times that is allowed.
+    assert 4 * (err / s).mean() / K < 2e-3
+    assert (got == nearest(h / s)).mean() > 0.99
+
+
+def test_products_on_a_stream_and_in_a_graph():
+    import torch
+
+    rng = np.random.default_rng(13)
+    E, N, K, rows = 6, 128, 288, 100
+    offsets = np.array([0, 3, 3, 40, 41, 90, 100], np.int32)
+    wc, ws, w, xc, xs, x = product_case(rng, E, N, K, offsets, rows)
+    od = dev(offsets)
+    y, z = (torch.zeros((rows, N), dtype=torch.float16, device="cuda") for _ in range(2))
+    weights = ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr())
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    ops.mx4_product_device(weights, xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), y.data_ptr(), ops.F16, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    want = by_expert(x, w, offsets, rows)
+    assert np.linalg.norm(y.double().cpu().numpy() - want) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.mx4_product_device(weights, xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), z.data_ptr(), ops.F16, stream=torch.cuda.current_stream().cuda_stream)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
+    # Other rows and another split through the same graph.
+    (c2, s2), x2 = R.random_mx(rng, (rows, K), 125, 129)
+    s2[:, K // 32:] = 255
+    xc.copy_(dev(c2)), xs.copy_(dev(s2)), od.copy_(dev(np.array([0, 0, 64, 64, 65, 66, 99], np.int32)))
+    z.fill_(7)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = by_expert(x2, w, [0, 0, 64, 64, 65, 66, 99], rows)
+    assert (z[99] == 7).all()
+    assert np.linalg.norm(z[:99].double().cpu().numpy() - want[:99]) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("y_type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T, n, D", [(1, 1, 8), (1, 16, 2560), (7, 3, 4104), (300, 10, 64)])
+def test_combine(T, n, D, y_type):
+    import torch
+
+    rng = np.random.default_rng(T + n + D)
+    rows = T * n
+    y = dev(rng.standard_normal((rows + 1, D)).astype(np.float32), y_type)
+    y[rows] = float("nan")
+    inv = rng.permutation(rows).reshape(T, n).astype(np.int32)
+    if n > 2:
+        inv[0, 1], inv[-1, 2] = -1, rows  # no expert, and past the end
+        inv[T // 2, :] = -1
+    w, res = rng.random((T, n)).astype(np.float32), rng.standard_normal((T, D)).astype(np.float32)
+    yd, there = y.double().cpu().numpy(), (inv >= 0) & (inv < rows)
+    terms = np.where(there, w, 0)[..., None].astype(np.float64) * yd[np.where(there, inv, 0)]
+    want, size = terms.sum(1), np.abs(terms).sum(1)
+    out = torch.full((T + 1, D), 7.0, device="cuda")
+    di, dw, dr = dev(inv), dev(w), dev(res)
+    ops.combine_rows_device(y.data_ptr(), TYPES[y_type], rows, di.data_ptr(), dw.data_ptr(), T, n, D, out.data_ptr())
+    assert (out[T] == 7.0).all()
+    bound = (n + 2) * 2.0 ** -24  # a rounding a term
+    assert (np.abs(out[:T].double().cpu().numpy() - want) <= bound * size).all()
+    ops.combine_rows_device(y.data_ptr(), TYPES[y_type], rows, di.data_ptr(), dw.data_ptr(), T, n, D, dr.data_ptr(), residual_ptr=dr.data_ptr())
+    assert (np.abs(dr.double().cpu().numpy() - want - res) <= bound * (size + np.abs(res))).all()
+
+
+def test_combine_of_no_results():
+    import torch
+
+    inv, w, res, out = torch.full((3, 2), -1, dtype=torch.int32, device="cuda"), torch.ones((3, 2), device="cuda"), torch.ones((3, 64), device="cuda"), torch.zeros((3, 64), device="cuda")
+    ops.combine_rows_device(None, ops.F16, 0, inv.data_ptr(), w.data_ptr(), 3, 2, 64, out.data_ptr(), residual_ptr=res.data_ptr())
+    assert (out == 1).all()
+
+
+def test_memory_refused():
+    import torch
+
+    d, h = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda"), torch.zeros(1 << 16, dtype=torch.uint8)
+    p, q = d.data_ptr(), h.data_ptr()
+    for call, word in ((lambda: ops.mx4_quantize_rows_device(q, ops.F32, 4, 64, p, p, 4), "x is not device memory"),
+                       (lambda: ops.mx4_quantize_rows_device(p + 4, ops.F32, 4, 64, p, p, 4), "x must be 16-byte aligned"),
+                       (lambda: ops.mx4_quantize_rows_device(p, ops.F32, 4, 64, p, p + 2, 4), "scales must be 4-byte aligned"),
+                       (lambda: ops.mx4_product_device(ops.Mx4Weights(2, 64, 64, p, q), p, p, 4, p, p, ops.F16), "weight scales is not device memory"),
+                       (lambda: ops.mx4_product_device(ops.Mx4Weights(2, 64, 64, p, p), p, p, 4, p, p + 8, ops.F16), "y must be 16-byte aligned"),
+                       (lambda: ops.mx4_gate_up_device(ops.Mx4Weights(2, 64, 64, p, p), p, p, 4, p, p, None), "h scales is required"),
+                       (lambda: ops.combine_rows_device(p, ops.F16, 4, p, p, 2, 2, 64, q), "out is not device memory"),
+                       (lambda: ops.mx4_from_blocks_device(q, 4, 64, p, p), "blocks is not device memory")):
+        with pytest.raises(MoEError) as e:
+            call()
+        assert e.value.status == _lib.MOE_BAD_ARGUMENT and word in str(e.value)
+
+
+@pytest.mark.parametrize("T", [1, 50, 700])
+def test_a_block_put_together(T):
+    """Router logits to the block's output by all the operators in their order, on one stream, twice from one graph: against the definition in
+    64 bits on the same quantised rows."""
+    import torch
+
+    rng = np.random.default_rng(T)
+    E, k, D, F = 16, 3, 160, 96
+    logits, bias = rng.standard_normal((T, E)).astype(np.float32), (0.1 * rng.standard_normal(E)).astype(np.float32)
+    x = rng.standard_normal((T, D)).astype(np.float32)
+    w1c, w1s, w1, _, _, _ = product_case(rng, E, 2 * F, D, None, 1)
+    w2c, w2s, w2, _, _, _ = product_case(rng, E, D, F, None, 1)
+    rows = T * k
+    ids, w = torch.empty((T, k), dtype=torch.int32, device="cuda"), torch.empty((T, k), device="cuda")
+    offsets, inv = torch.empty(E + 1, dtype=torch.int32, device="cuda"), torch.empty((T, k), dtype=torch.int32, device="cuda")
+    work = torch.empty(ops.route_work_bytes(T, E), dtype=torch.uint8, device="cuda")
+    (xc, xs), (hc, hs) = mx_buffers(rows, D), mx_buffers(rows, F)
+    y, out = torch.empty((rows, D), dtype=torch.float16, device="cuda"), torch.empty((T, D), device="cuda")
+    dl, db, dx = dev(logits), dev(bias), dev(x)
+    up, down = ops.Mx4Weights(E, 2 * F, D, w1c.data_ptr(), w1s.data_ptr()), ops.Mx4Weights(E, D, F, w2c.data_ptr(), w2s.data_ptr())
+
+    def block(st):
+        ops.route_logits_device(dl.data_ptr(), ops.F32, T, E, k, ids.data_ptr(), w.data_ptr(), score=ops.SIGMOID, bias_ptr=db.data_ptr(), n_groups=4,
+                                n_groups_used=2, scale=1.5, offsets_ptr=offsets.data_ptr(), inv_ptr=inv.data_ptr(), work_ptr=work.data_ptr(),
+                                work_bytes=work.numel(), stream=st)
+        ops.mx4_quantize_rows_device(dx.data_ptr(), ops.F32, T, D, xc.data_ptr(), xs.data_ptr(), rows, inv_ptr=inv.data_ptr(), n_used=k, stream=st)
+        ops.mx4_gate_up_device(up, xc.data_ptr(), xs.data_ptr(), rows, offsets.data_ptr(), hc.data_ptr(), hs.data_ptr(), swiglu_limit=7.0, stream=st)
+        ops.mx4_product_device(down, hc.data_ptr(), hs.data_ptr(), rows, offsets.data_ptr(), y.data_ptr(), ops.F16, stream=st)
+        ops.combine_rows_device(y.data_ptr(), ops.F16, rows, inv.data_ptr(), w.data_ptr(), T, k, D, out.data_ptr(), residual_ptr=dx.data_ptr(), stream=st)
+
+    def want(l, x):
+        i, wt, off, place = R.route(l.astype(np.float64), k, "sigmoid", bias, 4, 2, True, 1.5)
+        xe = np.empty((rows, D))
+        xe[place.reshape(-1)] = np.repeat(R.values(*R.quantize(x)), k, 0)
+        v = by_expert(xe, w1, off, rows)
+        h = R.values(*R.quantize(R.swiglu(v[:, :F], v[:, F:], 7.0)))
+        ye = by_expert(h, w2, off, rows)
+        return x + (wt[..., None] * ye[place]).sum(1)
+
+    block(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    first = out.clone()
+    # y's rounding to f16, and the few values of h within an f32 sum's error of a border between two codes (a code further off: some 1e-6 of them
+    # by a fifth of a block's size): a part in two thousand of the block's result, which the residual is no smaller than.
+    assert np.linalg.norm(first.double().cpu().numpy() - want(logits, x)) <= 2e-3 * np.linalg.norm(want(logits, x))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        block(torch.cuda.current_stream().cuda_stream)
+    for seed in (None, 1, 2):
+        if seed is not None:
+            g = np.random.default_rng(seed)
+            logits, x = g.standard_normal((T, E)).astype(np.float32), g.standard_normal((T, D)).astype(np.float32)
+            dl.copy_(dev(logits)), dx.copy_(dev(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        if seed is None:
+            assert torch.equal(out, first)  # the same bits, captured or not
+        assert np.linalg.norm(out.double().cpu().numpy() - want(logits, x)) <= 2e-3 * np.linalg.norm(want(logits, x))
