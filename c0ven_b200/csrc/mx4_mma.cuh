@@ -1,0 +1,52 @@
+// The tensor core's block-scaled 4-bit product (tcgen05.mma kind::mxf4): A and B e2m1 codes in shared memory, K-major with the 128-byte
+// swizzle, 64 values of the contraction an instruction (32 bytes of a row); their scales, a byte per 32 values, in tensor memory.
+//
+// Scales reach tensor memory by tcgen05.cp from shared memory, 512 bytes a copy: 128 rows' words of four scales (128 values). Row r's word
+// lies at 16 (r % 32) + 4 (r / 32) of the piece, and lands in lane r % 32 (of every warp's quarter) of column r / 32. An instruction takes bytes
+// 0, 1 or 2, 3 of the words, named by its descriptor's scale ids 0 or 2.
+#pragma once
+
+#include <cstdint>
+
+#include "expert_tiles.cuh"
+
+namespace moe {
+namespace tc {
+
+// 32 rows of 16 bytes, no swizzle: 8 rows 128 bytes on.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void copy_scales(uint32_t leader, uint32_t taddr, uint32_t smem_addr) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr),
+      "l"(smem_desc_scales(smem_addr)), "r"(leader)
+      : "memory");
+}
+// kind::mxf4 instruction descriptor: A and B e2m1, e8m0 scales, M m, N n, both operands' scale ids id (0 or 2).
+__device__ __forceinline__ uint32_t mx4_instr_desc(uint32_t n, uint32_t m, uint32_t id) {
+  return (id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) | (id << 29);
+}
+// D[tmem] (+)= A[128 rows] * B[n rows]^T over 64 values.
+__device__ __forceinline__ void mma_mx4(uint32_t leader, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scales_a, uint32_t scales_b,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scales_a), "r"(scales_b), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+// Four bytes into shared memory, the first n of them from memory and zeros behind (n 0: nothing is read).
+__device__ __forceinline__ void copy_word(uint32_t dst, const void *src, uint32_t n) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_words_wait() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+}
+
+}  // namespace tc
+}  // namespace moe

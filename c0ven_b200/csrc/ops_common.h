@@ -55,6 +55,12 @@ inline moe_status ops_call(Body &&body) noexcept {
     } catch (...) {
     }
     return MOE_BAD_ARGUMENT;
+  } catch (const Timeout &e) {
+    try {
+      ops_error() = e.what();
+    } catch (...) {
+    }
+    return MOE_TIMEOUT;
   } catch (const std::exception &e) {
     try {
       ops_error() = e.what();

@@ -84,3 +84,8 @@ def combine_rows_device(y_ptr: int, y_type: int, R: int, inv_ptr: int, w_ptr: in
                         residual_ptr: int | None = None, stream: int | None = None):
     """out [T][n_embd] f32: each row's results, weighted and summed in rank order, and its residual."""
     _check(_lib.lib().moe_combine_rows_device(y_ptr, y_type, R, inv_ptr, w_ptr, T, n_used, n_embd, residual_ptr, out_ptr, stream))
+
+
+def status(stream: int | None = None, timeout_ms: int = 0):
+    """Waits for stream; raises MoEError where that runs out, or where a product gave up one of its own waits since this was last asked."""
+    _check(_lib.lib().moe_ops_status(timeout_ms, stream))

@@ -103,6 +103,7 @@ def test_quantize_scatters_strided_rows(type):
     inv[3, 2], inv[4, :] = -1, -1
     codes, scales = mx_buffers(rows + 2, K)
     di = dev(inv)
+    ops.status()
     ops.mx4_quantize_rows_device(full.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), rows, stride=256, inv_ptr=di.data_ptr(), n_used=n)
     torch.cuda.synchronize()
     c, s = R.pack(*R.quantize(full.double().cpu().numpy()[:, :K]))
@@ -176,7 +177,7 @@ def test_products(E, N, K, counts, y_type):
         y[:] = 7.0
         r = rows if at else used
         ops.mx4_product_device(ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), r, at, y.data_ptr(), TYPES[y_type])
-        torch.cuda.synchronize()
+        ops.status()
         got, want, size = y.double().cpu().numpy(), by_expert(x, w, offsets, rows), by_expert(x, w, offsets, rows, True)
         assert (got[used:] == 7.0).all()
         off = np.abs(got[:used] - want[:used])
@@ -244,7 +245,7 @@ def test_gate_up(E, F, K, counts, limit):
     od = dev(offsets)
     ops.mx4_gate_up_device(ops.Mx4Weights(E, 2 * F, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), hc.data_ptr(),
                            hs.data_ptr(), swiglu_limit=limit)
-    torch.cuda.synchronize()
+    ops.status()
     assert (hc[used:] == 0xEE).all() and (hs[used:] == 0xEE).all()
     assert (hs[:used, F // 32:] == 0).all()
     code, byte = R.unpack(hc[:used].cpu().numpy(), hs[:used].cpu().numpy())
