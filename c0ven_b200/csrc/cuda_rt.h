@@ -78,6 +78,31 @@ inline cudaError_t ensure_dynamic_smem(Kernel kernel, size_t bytes, std::atomic<
   return e;
 }
 
+#if defined(__CUDACC__)
+// Pairs of CTAs the GPU runs at once for kernel (one CTA an SM, so at most one pair a TPC), asked once per device. The kernel is
+// the template's own argument, for the answer is kept beside it: kernels of one type (the tile kernels of gate and up and of down) differ in
+// their blocks.
+template <auto kernel>
+static cudaError_t max_pairs(uint32_t threads, size_t smem, int device, uint32_t &pairs) {
+  static std::atomic<uint32_t> known[64];
+  if (device < 0 || device >= 64) return cudaErrorInvalidValue;
+  pairs = known[device].load(std::memory_order_acquire);
+  if (pairs) return cudaSuccess;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = 2, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.attrs = &at, cfg.numAttrs = 1;
+  int n = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  if (e != cudaSuccess) return e;
+  if (n <= 0) return cudaErrorInvalidConfiguration;
+  pairs = (uint32_t)n;
+  known[device].store(pairs, std::memory_order_release);
+  return cudaSuccess;
+}
+#endif
+
 // Device memory of n elements of T, freed with its owner.
 template <class T>
 class DeviceBuffer {

@@ -1,14 +1,15 @@
 // Products of MX rows in expert order with their experts' MX matrices (include/moe_layer.h: moe_mx4_product_device, moe_mx4_gate_up_device),
 // on the tensor core's own 4-bit product: nothing is decoded.
 //
-// A work item is 128 rows of one expert's matrix (for gate_up 64 gate rows and the 64 up rows of the same features) times up to kTokens of
-// the expert's rows. The matrix is the instruction's M side and the rows its N side, so a few rows cost a short instruction and what an item
-// costs is bringing the matrix. Persistent CTAs, one an SM, take items in turn; items of one expert are neighbours.
+// A work item is 128 rows of one expert's matrix for each CTA that works on it (for gate_up 64 gate rows and the 64 up rows of the same
+// features) times up to NT of the expert's rows. The matrix is the instruction's M side and the rows its N side, so a few rows cost a
+// short instruction and what an item costs is bringing the matrix. Persistent units (a CTA, or a pair of CTAs on two SMs that share the rows:
+// tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
 //
-// Roles of a CTA's ten warps: one thread brings codes by bulk-tensor copies, 256 values of the contraction a stage; four warps bring the scales,
+// Roles of a CTA's warps: one thread brings codes by bulk-tensor copies, 256 values of the contraction a stage; four warps bring the scales,
 // four stages (1,024 values: a sector of a row's scales) at a time in turn, word by word into the layout that the tensor core's copy reads
-// (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance); one lane issues scale copies and MMAs; four warps
-// turn accumulators, of which there are two sets, into results.
+// (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance); one lane (of a pair's first CTA) issues scale copies and
+// MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
 //
 // Every wait on an mbarrier is bounded: one that runs out raises the CTA's abort flag and the device's error word (moe_ops_status), the other
 // waits return at once, and the CTA frees its tensor memory before it exits.
@@ -27,24 +28,24 @@ namespace moe {
 namespace {
 
 constexpr uint32_t kMaxExperts = 512;
-constexpr uint32_t kRowsM = 128;        // matrix rows of an item
+constexpr uint32_t kRowsM = 128;        // matrix rows a CTA takes
 constexpr uint32_t kStageK = 256;       // values of the contraction a stage holds: 128 bytes of a row
 constexpr uint32_t kScaleStages = 4;    // stages that one slot of scales covers
-constexpr uint32_t kScaleSlots = 4;     // and as many warps fill them
 constexpr uint32_t kBoxRows = 16;       // rows one copy of the rows' codes brings
+constexpr uint32_t kChunk = 16;         // rows an epilogue warp turns at a time
 
-// Barriers of the four epilogue warps alone. The second tells every one of them whether ok holds for all: they leave their loop together
+// Barriers of a group of four epilogue warps alone. The second tells every one of them whether ok holds for all: they leave their loop together
 // or not at all, so that none waits here for one that has left.
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool epilogue_all(bool ok) {
+__device__ __forceinline__ void group_sync(uint32_t group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
+__device__ __forceinline__ bool group_all(uint32_t group, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, 1, 128, p;\n\t"
+      "bar.red.and.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)ok)
+      : "r"((uint32_t)ok), "r"(1 + group)
       : "memory");
   return r != 0;
 }
@@ -62,60 +63,79 @@ struct Mx4Args {
   uint8_t *hc, *hs;
 };
 
-// Shared memory of a CTA, for tiles of at most NT rows. Stages of codes; slots of scales, the matrix's and then the rows', eight pieces of 512
-// bytes each; for gate_up the accumulators on their way to the quantiser; barriers; the experts' first rows and tiles.
-template <bool GU, uint32_t NT>
-struct Mx4Smem {
-  static constexpr uint32_t kStages = 8;
-  static constexpr uint32_t kStageBytes = (kRowsM + NT) * 128;
+// A form of the kernel: CTAs a unit has, and the most rows of a tile. Its shared memory: stages of codes; slots of scales, the matrix's and then
+// the rows', eight words of every row each; for gate_up the accumulators on their way to the quantiser, two chunks a group; barriers; the
+// experts' first and last rows and first tiles.
+template <bool GU, uint32_t CTAS, uint32_t NT>
+struct Mx4Form {
+  static constexpr uint32_t kGroups = CTAS;  // of four epilogue warps
+  static constexpr uint32_t kThreads = 32 * (6 + 4 * kGroups);
+  static constexpr uint32_t kStages = CTAS == 2 ? 5 : 8;
+  static constexpr uint32_t kStageBytes = (kRowsM + NT / CTAS) * 128;
+  static constexpr uint32_t kScaleSlots = CTAS == 2 ? 3 : 4;
+  static constexpr uint32_t kRowPieces = (NT + 127) / 128;  // 512-byte pieces a word of the rows' scales takes
   static constexpr uint32_t kScales = kStages * kStageBytes;
-  static constexpr uint32_t kSlotBytes = 2 * 8 * 512;
+  static constexpr uint32_t kSlotBytes = (1 + kRowPieces) * 8 * 512;
   static constexpr uint32_t kStaging = kScales + kScaleSlots * kSlotBytes;
-  static constexpr uint32_t kStagingRow = kRowsM + 4;  // floats of a row of the tile, padded
-  static constexpr uint32_t kBarriers = kStaging + (GU ? NT * kStagingRow * 4 : 0);
+  static constexpr uint32_t kStagingRow = kRowsM + 4;  // floats of a row of a chunk, padded
+  static constexpr uint32_t kStagingBytes = kChunk * kStagingRow * 4;
+  static constexpr uint32_t kBarriers = kStaging + (GU ? 2 * kGroups * kStagingBytes : 0);
   static constexpr uint32_t kTables = kBarriers + 256;
   static constexpr uint32_t kBytes = kTables + 3 * (kMaxExperts + 1) * 4 + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
-  static_assert(NT <= 128, "the rows' scales are one piece a word");
+  // Tensor memory: two accumulators, then the scales of kScaleRing stages.
+  static constexpr uint32_t kScaleCols = 8 + 8 * kRowPieces;
+  static constexpr uint32_t kScaleRing = CTAS == 2 ? 2 : kStages;
+  static constexpr uint32_t kUsedCols = 2 * NT + kScaleRing * kScaleCols;
+  static constexpr uint32_t kCols = kUsedCols <= 256 ? 256 : 512;
+  static_assert(kUsedCols <= kCols, "tensor memory");
 };
 
-constexpr uint32_t kThreads = 320;
 enum : uint32_t { kCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kEpilogueWarp = 6 };
 
-template <bool GU, uint32_t NT>
-__global__ void __launch_bounds__(kThreads, 1) k_mx4_product(const __grid_constant__ Mx4Args a, const __grid_constant__ CUtensorMap wmap,
-                                                             const __grid_constant__ CUtensorMap xmap) {
+// Rows a tile of an expert's n rows has: the tiles of a few share them evenly (which 16 rows a tile can be off by leaves no tile empty up to
+// eight tiles of 224).
+template <uint32_t NT>
+__device__ __forceinline__ uint32_t tile_rows(uint32_t n) {
+  const uint32_t tiles = (n + NT - 1) / NT;
+  return NT >= 128 && tiles > 1 && tiles <= 8 ? ((n + tiles - 1) / tiles + 15) & ~15u : NT;
+}
+
+template <bool GU, uint32_t CTAS, uint32_t NT>
+__global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_product(const __grid_constant__ Mx4Args a, const __grid_constant__ CUtensorMap wmap,
+                                                                                    const __grid_constant__ CUtensorMap xmap) {
   using namespace tc;
-  using SM = Mx4Smem<GU, NT>;
-  constexpr uint32_t S = SM::kStages;
-  constexpr uint32_t kScaleCols = 2 * NT;          // columns of the scales: 8 of the matrix's and 8 of the rows' a stage
-  constexpr uint32_t kCols = kScaleCols + 16 * S <= 256 ? 256 : 512;
-  static_assert(kScaleCols + 16 * S <= kCols, "tensor memory");
+  using SM = Mx4Form<GU, CTAS, NT>;
+  constexpr uint32_t S = SM::kStages, SL = SM::kScaleSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0, unit = blockIdx.x / CTAS, nunits = gridDim.x / CTAS;
   uint64_t *bars = (uint64_t *)(smem + SM::kBarriers);
+  // Barriers: stages full, empty; scales full, empty; accumulators full, empty. Of a pair the first CTA's "full" of stages and scales and "empty"
+  // of accumulators take both CTAs' arrivals.
+  constexpr uint32_t kEmpty = S, kScFull = 2 * S, kScEmpty = kScFull + SL, kAccFull = kScEmpty + SL, kAccEmpty = kAccFull + 2, kBars = kAccEmpty + 2;
+  static_assert(8 * kBars + 8 <= 256, "the barriers' room");
   const uint32_t bar0 = smem_u32(bars);
-  auto full_bar = [&](uint32_t s) { return bar0 + 8 * s; };
-  auto empty_bar = [&](uint32_t s) { return bar0 + 8 * (S + s); };
-  auto scales_full = [&](uint32_t s) { return bar0 + 8 * (2 * S + s); };
-  auto scales_empty = [&](uint32_t s) { return bar0 + 8 * (2 * S + kScaleSlots + s); };
-  auto acc_full = [&](uint32_t b) { return bar0 + 8 * (2 * S + 2 * kScaleSlots + b); };
-  auto acc_empty = [&](uint32_t b) { return bar0 + 8 * (2 * S + 2 * kScaleSlots + 2 + b); };
-  static_assert(8 * (2 * S + 2 * kScaleSlots + 4) + 8 <= 256, "the barriers' room");
-  uint32_t *tmem_slot = (uint32_t *)(bars + 2 * S + 2 * kScaleSlots + 4);
+  auto bar = [&](uint32_t i) { return bar0 + 8 * i; };
+  uint32_t *tmem_slot = (uint32_t *)(bars + kBars);
   volatile uint32_t *abort = tmem_slot + 1;
   uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *end_row = first_row + kMaxExperts + 1, *first_tile = end_row + kMaxExperts + 1;
   uint32_t *error = &g_gave_up;
 
   if (tid == 0) {
-    for (uint32_t s = 0; s < S; s++) mbar_init(full_bar(s), 1), mbar_init(empty_bar(s), 1);
-    for (uint32_t s = 0; s < kScaleSlots; s++) mbar_init(scales_full(s), 1), mbar_init(scales_empty(s), 1);
-    for (uint32_t b = 0; b < 2; b++) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 4);
+    for (uint32_t s = 0; s < S; s++) mbar_init(bar(s), CTAS), mbar_init(bar(kEmpty + s), 1);
+    for (uint32_t s = 0; s < SL; s++) mbar_init(bar(kScFull + s), CTAS), mbar_init(bar(kScEmpty + s), 1);
+    for (uint32_t b = 0; b < 2; b++) mbar_init(bar(kAccFull + b), 1), mbar_init(bar(kAccEmpty + b), CTAS * 4 * SM::kGroups);
     *abort = 0;
     fence_barrier_init();
   }
-  if (warp == kMmaWarp) tmem_alloc(smem_u32(tmem_slot), kCols);
+  if (warp == kMmaWarp) {
+    if constexpr (CTAS == 2)
+      tmem_alloc_pair(smem_u32(tmem_slot), SM::kCols);
+    else
+      tmem_alloc(smem_u32(tmem_slot), SM::kCols);
+  }
   dependents_may_launch(), wait_for_predecessors();
   // The experts' rows and tiles, summed up by one warp, 16 experts a lane. Offsets are held to 0 .. R and to their order.
   if (warp == kEpilogueWarp) {
@@ -142,14 +162,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_mx4_product(const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK;
   const uint32_t nitems = first_tile[a.E] * M;  // 2^24 / 32 + 512 tiles of 1,024 at most
+  const uint32_t lead0 = CTAS == 2 ? map_to_cta(bar0, 0) : bar0;  // the first CTA's barriers as this CTA names them
+  auto lead = [&](uint32_t i) { return lead0 + 8 * i; };
+  auto arrive_lead = [&](uint32_t i) {
+    if constexpr (CTAS == 2)
+      mbar_arrive_cluster(lead(i));
+    else
+      mbar_arrive(lead(i));
+  };
   bool ok = true;
 
+  // row0: the first of this CTA's matrix rows, or of its features.
   struct Tile {
-    uint32_t expert, start, count, m;
+    uint32_t expert, start, count, row0;
   };
   // Item i: tile i / M of the experts' tiles in order, and which of its M pieces of the matrix.
   auto tile_at = [&](uint32_t i) {
@@ -162,29 +192,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_mx4_product(const __grid_consta
       else
         hi = mid;
     }
-    const uint32_t start = first_row[lo] + (t - first_tile[lo]) * NT;
-    return Tile{lo, start, min(NT, end_row[lo] - start), i - t * M};
+    const uint32_t per = tile_rows<NT>(end_row[lo] - first_row[lo]), start = first_row[lo] + (t - first_tile[lo]) * per;
+    return Tile{lo, start, min(per, end_row[lo] - start), ((i - t * M) * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
   };
 
   if (warp == kCopyWarp) {
     if (lane == 0) {
-      uint32_t g = 0;  // stages used so far
-      for (uint32_t i = blockIdx.x; i < nitems && ok; i += gridDim.x) {
+      uint32_t s = 0, phase = 1;  // of the stage's "empty": the first round finds it so
+      for (uint32_t i = unit; i < nitems && ok; i += nunits) {
         const Tile t = tile_at(i);
-        const uint32_t boxes = (t.count + kBoxRows - 1) / kBoxRows;
-        for (uint32_t it = 0; it < KT && ok; it++, g++) {
-          const uint32_t s = g % S, use = g / S;
-          if (use > 0) ok = mbar_wait(empty_bar(s), (use - 1) & 1, abort, error);
+        // A CTA of a pair brings its half of the rows the instruction takes, which are rounded up to 16.
+        const uint32_t half = ((t.count + 15) & ~15u) / CTAS, x_row = t.start + rank * half, boxes = (half + kBoxRows - 1) / kBoxRows;
+        for (uint32_t it = 0; it < KT && ok; it++) {
+          ok = mbar_wait(bar(kEmpty + s), phase, abort, error);
           if (!ok) break;
           const uint32_t at = smem_u32(smem + s * SM::kStageBytes), x0 = it * (kStageK / 2);
-          mbar_arrive_expect(full_bar(s), kRowsM * 128 + boxes * kBoxRows * 128);
-          if constexpr (GU) {
-            tma_load_quants(at, &wmap, x0, t.m * 64, t.expert, full_bar(s));
-            tma_load_quants(at + 64 * 128, &wmap, x0, F + t.m * 64, t.expert, full_bar(s));
-          } else {
-            tma_load_quants(at, &wmap, x0, t.m * kRowsM, t.expert, full_bar(s));
-          }
-          for (uint32_t b = 0; b < boxes; b++) tma_load_quants(at + (kRowsM + b * kBoxRows) * 128, &xmap, x0, t.start + b * kBoxRows, 0, full_bar(s));
+          auto copy = [&](uint32_t dst, const CUtensorMap *map, uint32_t y, uint32_t z) {
+            if constexpr (CTAS == 2)
+              tma_load_codes_pair(dst, map, x0, y, z, lead(s));
+            else
+              tma_load_quants(dst, map, x0, y, z, lead(s));
+          };
+          if constexpr (CTAS == 2)
+            mbar_arrive_expect_cluster(lead(s), kRowsM * 128 + boxes * kBoxRows * 128);
+          else
+            mbar_arrive_expect(lead(s), kRowsM * 128 + boxes * kBoxRows * 128);
+          copy(at, &wmap, t.row0, t.expert);
+          if constexpr (GU) copy(at + 64 * 128, &wmap, F + t.row0, t.expert);
+          for (uint32_t b = 0; b < boxes; b++) copy(at + (kRowsM + b * kBoxRows) * 128, &xmap, x_row + b * kBoxRows, 0);
+          if (++s == S) s = 0, phase ^= 1;
         }
       }
       if (!ok) {
@@ -194,78 +230,102 @@ __global__ void __launch_bounds__(kThreads, 1) k_mx4_product(const __grid_consta
         }
       }
     }
-  } else if (warp >= kScaleWarp && warp < kScaleWarp + kScaleSlots) {
+  } else if (warp >= kScaleWarp && warp < kScaleWarp + SL) {
     // A slot of scales by a warp: four rows' eight words an instruction, so that a row's 32 bytes are one request.
     const uint32_t mine = warp - kScaleWarp, srow = mx_scale_row_bytes(K), nb = K / kMxBlock, slots = (KT + kScaleStages - 1) / kScaleStages;
-    const uint32_t word = lane % 8, at = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes) + word * 512;
-    uint32_t g = 0;  // slots filled so far, by all
-    for (uint32_t i = blockIdx.x; i < nitems && ok; i += gridDim.x) {
+    const uint32_t word = lane % 8, slot = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes);
+    const uint32_t at = slot + word * 512, x_at = slot + 8 * 512 + word * SM::kRowPieces * 512;
+    uint32_t turn = 0, phase = 1;  // whose turn the next slot is
+    for (uint32_t i = unit; i < nitems && ok; i += nunits) {
       const Tile t = tile_at(i);
-      for (uint32_t j = 0; j < slots && ok; j++, g++) {
-        if (g % kScaleSlots != mine) continue;
-        const uint32_t use = g / kScaleSlots;
-        if (use > 0) ok = mbar_wait_warp(scales_empty(mine), (use - 1) & 1, abort, error);
+      for (uint32_t j = 0; j < slots && ok; j++, turn = turn == SL - 1 ? 0 : turn + 1) {
+        if (turn != mine) continue;
+        ok = mbar_wait_warp(bar(kScEmpty + mine), phase, abort, error);
         if (!ok) break;
+        phase ^= 1;
         const uint32_t b0 = j * (kScaleStages * kStageK / kMxBlock) + 4 * word, n = b0 < nb ? min(4u, nb - b0) : 0u;
         for (uint32_t r = lane / 8; r < kRowsM; r += 4) {
-          uint32_t row = GU ? (r < 64 ? t.m * 64 + r : F + t.m * 64 + r - 64) : t.m * kRowsM + r;
-          const uint32_t have = row < a.N ? n : 0;
+          const uint32_t row = GU ? (r < 64 ? t.row0 + r : F + t.row0 + r - 64) : t.row0 + r, have = row < a.N ? n : 0;
           copy_word(at + 16 * (r % 32) + 4 * (r / 32), have ? a.ws + ((uint64_t)t.expert * a.N + row) * srow + b0 : a.ws, have);
         }
         for (uint32_t r = lane / 8; r < ((t.count + 3) & ~3u); r += 4) {
           const uint32_t have = r < t.count ? n : 0;
-          copy_word(at + 8 * 512 + 16 * (r % 32) + 4 * (r / 32), have ? a.xs + (uint64_t)(t.start + r) * srow + b0 : a.xs, have);
+          copy_word(x_at + r / 128 * 512 + 16 * (r % 32) + 4 * (r / 32 % 4), have ? a.xs + (uint64_t)(t.start + r) * srow + b0 : a.xs, have);
         }
         copy_words_wait();
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(scales_full(mine));
+        if (lane == 0) arrive_lead(kScFull + mine);
       }
     }
   } else if (warp == kMmaWarp) {
-    const uint32_t leader = elect_leader();
-    uint32_t g = 0, gs = 0, li = 0;
-    for (uint32_t i = blockIdx.x; i < nitems && ok; i += gridDim.x, li++) {
-      const Tile t = tile_at(i);
-      const uint32_t n = (t.count + 15) & ~15u, b = li & 1, acc = tmem_base + b * NT;
-      const uint32_t d0 = mx4_instr_desc(n, kRowsM, 0), d2 = mx4_instr_desc(n, kRowsM, 2);
-      if (li > 1) ok = mbar_wait_warp(acc_empty(b), (li / 2 - 1) & 1, abort, error);
-      for (uint32_t it = 0; it < KT && ok; it++, g++) {
-        const uint32_t s = g % S, slot = gs % kScaleSlots, sub = it % kScaleStages;
-        if (sub == 0) ok = mbar_wait_warp(scales_full(slot), (gs / kScaleSlots) & 1, abort, error);
-        if (ok) ok = mbar_wait_warp(full_bar(s), (g / S) & 1, abort, error);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t stage = smem_u32(smem + s * SM::kStageBytes), rows = stage + kRowsM * 128;
-        const uint32_t sc = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes) + 2 * sub * 512, ta = tmem_base + kScaleCols + 16 * s, tb = ta + 8;
-        // The stage's columns of scales are its own: the MMAs that read them last are done, for the stage was empty again.
-        copy_scales(leader, ta, sc), copy_scales(leader, ta + 4, sc + 512);
-        copy_scales(leader, tb, sc + 8 * 512), copy_scales(leader, tb + 4, sc + 9 * 512);
-        const uint32_t steps = min(4u, (K - it * kStageK + 63) / 64);
+    if (rank == 0) {
+      const uint32_t leader = elect_leader();
+      auto commit = [&](uint32_t i) {
+        if constexpr (CTAS == 2)
+          mma_commit_pair(leader, bar(i), 3);
+        else
+          mma_commit(leader, bar(i));
+      };
+      uint32_t s = 0, phase = 0, slot = 0, slot_phase = 0, ring = 0, b = 0, acc_phase = 1;
+      uint32_t old = S - SM::kScaleRing % S, old_phase = 1;  // the stage whose scales the ring's next columns held, kScaleRing stages ago
+      for (uint32_t i = unit; i < nitems && ok; i += nunits) {
+        const Tile t = tile_at(i);
+        const uint32_t n = (t.count + 15) & ~15u, acc = tmem_base + b * NT;
+        const uint32_t d0 = mx4_instr_desc(n, CTAS * kRowsM, 0), d2 = mx4_instr_desc(n, CTAS * kRowsM, 2);
+        ok = mbar_wait_warp(bar(kAccEmpty + b), acc_phase, abort, error);
+        for (uint32_t it = 0; it < KT && ok; it++) {
+          const uint32_t sub = it % kScaleStages;
+          if (sub == 0) ok = mbar_wait_warp(bar(kScFull + slot), slot_phase, abort, error);
+          if (ok) ok = mbar_wait_warp(bar(s), phase, abort, error);
+          // The columns this stage's scales go to are free when the MMAs that read them are done: with as many columns as stages they are,
+          // for the stage was empty again; else the commit after those MMAs says so.
+          if constexpr (SM::kScaleRing < S)
+            if (ok) ok = mbar_wait_warp(bar(kEmpty + old % S), old_phase, abort, error);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t stage = smem_u32(smem + s * SM::kStageBytes), rows = stage + kRowsM * 128;
+          const uint32_t sc = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes) + 2 * sub * 512;
+          const uint32_t sx = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes) + 8 * 512 + 2 * sub * SM::kRowPieces * 512;
+          const uint32_t ta = tmem_base + 2 * NT + ring * SM::kScaleCols, tb = ta + 8;
+          copy_scales<CTAS>(leader, ta, sc), copy_scales<CTAS>(leader, ta + 4, sc + 512);
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++)
-          if (k < steps)
-            mma_mx4(leader, acc, smem_desc_sw128(stage + 32 * k), smem_desc_sw128(rows + 32 * k), k % 2 ? d2 : d0, ta + 4 * (k / 2), tb + 4 * (k / 2), (it | k) != 0);
-        mma_commit(leader, empty_bar(s));
-        if (sub == kScaleStages - 1 || it == KT - 1) mma_commit(leader, scales_empty(slot)), gs++;
+          for (uint32_t p = 0; p < 2 * SM::kRowPieces; p++) copy_scales<CTAS>(leader, tb + 4 * p, sx + 512 * p);
+          const uint32_t steps = min(4u, (K - it * kStageK + 63) / 64);
+#pragma unroll
+          for (uint32_t k = 0; k < 4; k++)
+            if (k < steps)
+              mma_mx4<CTAS>(leader, acc, smem_desc_sw128(stage + 32 * k), smem_desc_sw128(rows + 32 * k), k % 2 ? d2 : d0, ta + 4 * (k / 2),
+                            tb + 4 * SM::kRowPieces * (k / 2), (it | k) != 0);
+          commit(kEmpty + s);
+          if (sub == kScaleStages - 1 || it == KT - 1) {
+            commit(kScEmpty + slot);
+            if (++slot == SL) slot = 0, slot_phase ^= 1;
+          }
+          if (++s == S) s = 0, phase ^= 1;
+          if (++ring == SM::kScaleRing) ring = 0;
+          if (++old == S) old = 0, old_phase ^= 1;
+        }
+        if (!ok) break;
+        commit(kAccFull + b);
+        acc_phase ^= b, b ^= 1;
       }
-      if (!ok) break;
-      mma_commit(leader, acc_full(b));
     }
   } else if (warp >= kEpilogueWarp) {
-    // Warp w reads tensor memory's lanes 32 (w % 4) ...
-    const uint32_t q = warp % 4;
-    uint32_t li = 0;
-    for (uint32_t i = blockIdx.x; i < nitems && ok; i += gridDim.x, li++) {
+    // Warp w reads tensor memory's lanes 32 (w % 4) ...; the groups take chunks of 16 rows in turn.
+    const uint32_t q = warp % 4, group = (warp - kEpilogueWarp) / 4;
+    uint32_t b = 0, phase = 0;
+    [[maybe_unused]] uint32_t turn = 0;
+    for (uint32_t i = unit; i < nitems && ok; i += nunits) {
       const Tile t = tile_at(i);
-      const uint32_t b = li & 1, from = tmem_base + ((32 * q) << 16) + b * NT;
-      ok = mbar_wait_warp(acc_full(b), (li / 2) & 1, abort, error);
-      if constexpr (GU) ok = epilogue_all(ok);  // the staging room's item before has been read, too
+      const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT;
+      ok = mbar_wait_warp(bar(kAccFull + b), phase, abort, error);
+      if constexpr (GU) ok = group_all(group, ok);
       if (!ok) break;
       tc_fence_after();
       if constexpr (!GU) {
-        const uint32_t n = t.m * kRowsM + 32 * q + lane;
-        for (uint32_t c = 0; c < t.count; c += 16) {
+        const uint32_t n = t.row0 + 32 * q + lane;
+        for (uint32_t c = group * kChunk; c < t.count; c += SM::kGroups * kChunk) {
           uint32_t v[16];
           tmem_ld16(from + c, v);
           tmem_ld_wait16(v);
@@ -279,31 +339,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_mx4_product(const __grid_consta
               ((__half *)a.y)[at + (uint64_t)j * a.N] = __float2half_rn(__uint_as_float(v[j]));
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty(b));
       } else {
-        // Through shared memory, a row of the tile its 64 gate and 64 up products, to threads of eight features each.
-        float *st = (float *)(smem + SM::kStaging);
-        for (uint32_t c = 0; c < t.count; c += 16) {
+        // Through shared memory, a row of the chunk its 64 gate and 64 up products, to threads of eight features each. Of a group's two
+        // chunks there the one is written while another warp may still read the other; past the barrier all have left it.
+        const uint32_t f = (tid % 8) * 8, hrow = mx_scale_row_bytes(F), at = t.row0 + f, r = (tid / 8) % 16;
+        for (uint32_t c = group * kChunk; c < t.count; c += SM::kGroups * kChunk, turn ^= 1) {
+          float *st = (float *)(smem + SM::kStaging + (2 * group + turn) * SM::kStagingBytes);
           uint32_t v[16];
           tmem_ld16(from + c, v);
           tmem_ld_wait16(v);
 #pragma unroll
-          for (uint32_t j = 0; j < 16; j++) st[(c + j) * SM::kStagingRow + 32 * q + lane] = __uint_as_float(v[j]);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty(b));
-        epilogue_sync();
-        const uint32_t f = (tid % 8) * 8, hrow = mx_scale_row_bytes(F), at = t.m * 64 + f;
-        for (uint32_t r0 = 0; r0 < t.count; r0 += 16) {
-          const uint32_t r = r0 + (tid - 32 * kEpilogueWarp) / 8;
+          for (uint32_t j = 0; j < 16; j++) st[j * SM::kStagingRow + 32 * q + lane] = __uint_as_float(v[j]);
+          group_sync(group);
           float h[8];
           uint32_t m = 0;
 #pragma unroll
           for (int j = 0; j < 8; j++) {
-            const float *p = st + min(r, NT - 1) * SM::kStagingRow + f + j;
+            const float *p = st + r * SM::kStagingRow + f + j;
             h[j] = swiglu(p[0], p[64], a.limit);
             m = max(m, __float_as_uint(h[j]) & 0x7FFFFFFFu);
           }
@@ -313,39 +365,71 @@ __global__ void __launch_bounds__(kThreads, 1) k_mx4_product(const __grid_consta
           const float inv = mx_inverse(scale);
 #pragma unroll
           for (int j = 0; j < 8; j++) h[j] *= inv;
-          if (r >= t.count || at >= F) continue;
-          const uint64_t row = t.start + r;
+          if (c + r >= t.count || at >= F) continue;
+          const uint64_t row = t.start + c + r;
           *(uint32_t *)(a.hc + row * (F / 2) + at / 2) = scale == 255 ? 0u : mx_codes8(h);
           if (tid % 4 == 0) a.hs[row * hrow + at / kMxBlock] = (uint8_t)scale;
           if (tid % 4 == 0 && at + kMxBlock == F)
             for (uint32_t s = F / kMxBlock; s < hrow; s++) a.hs[row * hrow + s] = 0;
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_lead(kAccEmpty + b);
+      phase ^= b, b ^= 1;
     }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();  // neither CTA leaves while the other may still read its shared memory or write its tensor memory
   if (warp == kMmaWarp) {
     __syncwarp();
     tc_fence_after();
-    tmem_free(tmem_base, kCols);
+    if constexpr (CTAS == 2)
+      tmem_free_pair(tmem_base, SM::kCols);
+    else
+      tmem_free(tmem_base, SM::kCols);
   }
 }
 
-template <bool GU, uint32_t NT>
-void launch_product(const Mx4Args &args, const uint8_t *wc, const uint8_t *xc, cudaStream_t st) {
+template <bool GU, uint32_t CTAS, uint32_t NT>
+void launch_product(const Mx4Args &args, const void *wc, const void *xc, cudaStream_t st) {
+  using Form = Mx4Form<GU, CTAS, NT>;
+  constexpr auto kernel = k_mx4_product<GU, CTAS, NT>;
   Mx4Args a = args;
   int device = 0;
   CUDA_OK(cudaGetDevice(&device));
-  constexpr size_t smem = Mx4Smem<GU, NT>::kBytes;
+  constexpr size_t smem = Form::kBytes;
   static std::atomic<uint32_t> done{0};
-  CUDA_OK(ensure_dynamic_smem(k_mx4_product<GU, NT>, smem, done, device));
-  int sms = 0;
-  CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-  a.items_per_tile = GU ? (a.N / 2 + 63) / 64 : (a.N + kRowsM - 1) / kRowsM;
+  CUDA_OK(ensure_dynamic_smem(kernel, smem, done, device));
+  uint32_t units = 0;
+  if constexpr (CTAS == 2) {
+    CUDA_OK(max_pairs<kernel>(Form::kThreads, smem, device, units));
+  } else {
+    int sms = 0;
+    CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    units = (uint32_t)sms;
+  }
+  const uint32_t rows = CTAS * (GU ? kRowsM / 2 : kRowsM), all = GU ? a.N / 2 : a.N;
+  a.items_per_tile = (all + rows - 1) / rows;
   const uint64_t most = ((uint64_t)a.R / NT + std::min(a.E, a.R)) * a.items_per_tile;  // items there can be
   const CUtensorMap wmap = make_codes_map(wc, a.K / 2, a.N, a.E, GU ? 64 : kRowsM), xmap = make_codes_map(xc, a.K / 2, a.R, 1, kBoxRows);
-  CUDA_OK(launch_kernel(true, k_mx4_product<GU, NT>, dim3((unsigned)std::min<uint64_t>(most, (uint64_t)sms)), dim3(kThreads), smem, st, a, wmap, xmap));
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension, at[1].val.clusterDim = {CTAS, 1, 1};
+  cfg.gridDim = dim3(CTAS * (unsigned)std::min<uint64_t>(most, units)), cfg.blockDim = dim3(Form::kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cfg.attrs = at, cfg.numAttrs = CTAS;  // a single CTA is no cluster
+  CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, wmap, xmap));
+}
+
+// Tiles of 224 rows by pairs of CTAs, or of 32 by single ones.
+template <bool GU>
+void launch(const Mx4Args &a, const void *wc, const void *xc, cudaStream_t st) {
+  if (a.R > 32ull * a.E)
+    launch_product<GU, 2, 224>(a, wc, xc, st);
+  else
+    launch_product<GU, 1, 32>(a, wc, xc, st);
 }
 
 Mx4Args arguments(const moe_mx4_weights *w, const void *scales, uint32_t R, const int32_t *offsets) {
@@ -377,7 +461,7 @@ MOE_API moe_status moe_mx4_product_device(const moe_mx4_weights *w, const void *
     if (R == 0) return;
     need_device({{w->codes_dev, "weight codes", 16}, {a.ws, "weight scales", 4}, {codes_dev, "codes", 16}, {a.xs, "scales", 4}, {a.offsets, "offsets", 4, true}, {y_dev, "y", 16}});
     a.y = y_dev, a.bf16 = y_type == MOE_TYPE_BF16;
-    launch_product<false, 32>(a, (const uint8_t *)w->codes_dev, (const uint8_t *)codes_dev, (cudaStream_t)stream);
+    launch<false>(a, w->codes_dev, codes_dev, (cudaStream_t)stream);
   });
 }
 
@@ -391,7 +475,7 @@ MOE_API moe_status moe_mx4_gate_up_device(const moe_mx4_weights *w, const void *
     need_device({{w->codes_dev, "weight codes", 16}, {a.ws, "weight scales", 4}, {codes_dev, "codes", 16}, {a.xs, "scales", 4}, {a.offsets, "offsets", 4, true},
                  {h_codes_dev, "h codes", 16}, {h_scales_dev, "h scales", 4}});
     a.limit = swiglu_limit, a.hc = (uint8_t *)h_codes_dev, a.hs = (uint8_t *)h_scales_dev;
-    launch_product<true, 32>(a, (const uint8_t *)w->codes_dev, (const uint8_t *)codes_dev, (cudaStream_t)stream);
+    launch<true>(a, w->codes_dev, codes_dev, (cudaStream_t)stream);
   });
 }
 

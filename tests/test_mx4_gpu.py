@@ -158,7 +158,8 @@ def sum_bound(magnitude, K):
 
 
 SHAPES = [(1, 32, 32, [5]), (1, 64, 96, [1]), (1, 160, 256, [300]), (3, 128, 64, [0, 7, 130]), (8, 96, 544, [1, 0, 2, 64, 65, 0, 17, 1]),
-          (5, 288, 2880, [16, 15, 0, 33, 1]), (2, 2080, 160, [129, 257]), (70, 64, 128, [1] * 70), (4, 32, 4096, [0, 0, 0, 3]), (512, 32, 32, [0, 1] * 256)]
+          (5, 288, 2880, [16, 15, 0, 33, 1]), (2, 2080, 160, [129, 257]), (70, 64, 128, [1] * 70), (4, 32, 4096, [0, 0, 0, 3]), (512, 32, 32, [0, 1] * 256),
+          (2, 256, 2880, [225, 33]), (1, 288, 1312, [1793]), (7, 544, 4128, [0, 448, 449, 1, 100, 17, 224])]
 
 
 @pytest.mark.parametrize("y_type", ["f16", "bf16"])
@@ -232,7 +233,8 @@ def test_nan_scales_reach_their_rows_alone():
 
 
 @pytest.mark.parametrize("limit", [0.0, 2.0])
-@pytest.mark.parametrize("E, F, K, counts", [(1, 32, 32, [5]), (3, 64, 96, [0, 7, 130]), (6, 96, 2880, [1, 0, 33, 64, 2, 0]), (2, 224, 256, [129, 257]), (1, 640, 544, [300])])
+@pytest.mark.parametrize("E, F, K, counts", [(1, 32, 32, [5]), (3, 64, 96, [0, 7, 130]), (6, 96, 2880, [1, 0, 33, 64, 2, 0]), (2, 224, 256, [129, 257]), (1, 640, 544, [300]),
+                                           (3, 288, 1312, [225, 0, 500]), (2, 160, 2880, [100, 40])])
 def test_gate_up(E, F, K, counts, limit):
     import torch
 
