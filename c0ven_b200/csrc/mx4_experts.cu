@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
@@ -31,7 +32,7 @@ constexpr uint32_t kMaxExperts = 512;
 constexpr uint32_t kRowsM = 128;        // matrix rows a CTA takes
 constexpr uint32_t kStageK = 256;       // values of the contraction a stage holds: 128 bytes of a row
 constexpr uint32_t kScaleStages = 4;    // stages that one slot of scales covers
-constexpr uint32_t kBoxRows = 16;       // rows one copy of the rows' codes brings
+constexpr uint32_t kTileTable = 1024;   // tiles whose expert is looked up in a table
 constexpr uint32_t kChunk = 16;         // rows an epilogue warp turns at a time
 
 // Barriers of a group of four epilogue warps alone. The second tells every one of them whether ok holds for all: they leave their loop together
@@ -59,34 +60,49 @@ struct Mx4Args {
   uint32_t items_per_tile;  // items that share a tile of rows
   float limit;
   void *y;
-  uint32_t bf16;
   uint8_t *hc, *hs;
 };
 
-// A form of the kernel: CTAs a unit has, and the most rows of a tile. Its shared memory: stages of codes; slots of scales, the matrix's and then
-// the rows', eight words of every row each; for gate_up the accumulators on their way to the quantiser, two chunks a group; barriers; the
-// experts' first and last rows and first tiles.
-template <bool GU, uint32_t CTAS, uint32_t NT>
+// Maps over the codes of the matrices and, in boxes of 16, 32, 64 and 112 rows, of the rows.
+constexpr uint32_t kBoxes = 4;
+__host__ __device__ constexpr uint32_t box_rows(uint32_t i) { return i == 3 ? 112u : 16u << i; }
+struct Mx4Maps {
+  CUtensorMap w, x[kBoxes];
+};
+
+// What a form of the kernel makes: h as MX rows of swiglu(gate, up), or the products in Y.
+struct GateUp {};
+
+// A form of the kernel: what it makes, CTAs a unit has, and the most rows of a tile. Its shared memory: stages of codes; slots of scales, the matrix's
+// and then the rows', eight words of every row each; for gate_up the accumulators on their way to the quantiser, two chunks a group;
+// barriers; the experts' first rows and first tiles; the tiles' experts.
+template <class Out, uint32_t CTAS, uint32_t NT>
 struct Mx4Form {
+  static constexpr bool GU = std::is_same<Out, GateUp>::value;
   static constexpr uint32_t kGroups = CTAS;  // of four epilogue warps
   static constexpr uint32_t kThreads = 32 * (6 + 4 * kGroups);
   static constexpr uint32_t kStages = CTAS == 2 ? 5 : 8;
   static constexpr uint32_t kStageBytes = (kRowsM + NT / CTAS) * 128;
   static constexpr uint32_t kScaleSlots = CTAS == 2 ? 3 : 4;
-  static constexpr uint32_t kRowPieces = (NT + 127) / 128;  // 512-byte pieces a word of the rows' scales takes
+  // A word of 128 rows' scales is a piece of 512 bytes and four columns of tensor memory, even where there are fewer rows: an instruction's scales
+  // begin at a multiple of four columns.
+  static constexpr uint32_t kRowPieces = (NT + 127) / 128;
   static constexpr uint32_t kScales = kStages * kStageBytes;
-  static constexpr uint32_t kSlotBytes = (1 + kRowPieces) * 8 * 512;
+  static constexpr uint32_t kSlotBytes = (8 + 8 * kRowPieces) * 512;
   static constexpr uint32_t kStaging = kScales + kScaleSlots * kSlotBytes;
   static constexpr uint32_t kStagingRow = kRowsM + 4;  // floats of a row of a chunk, padded
   static constexpr uint32_t kStagingBytes = kChunk * kStagingRow * 4;
   static constexpr uint32_t kBarriers = kStaging + (GU ? 2 * kGroups * kStagingBytes : 0);
   static constexpr uint32_t kTables = kBarriers + 256;
-  static constexpr uint32_t kBytes = kTables + 3 * (kMaxExperts + 1) * 4 + 1024;  // and room to align the base to 1024
+  static constexpr uint32_t kTileExperts = kTables + 2 * (kMaxExperts + 1) * 4;
+  static constexpr uint32_t kBytes = kTileExperts + 2 * kTileTable + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
-  // Tensor memory: two accumulators, then the scales of kScaleRing stages.
-  static constexpr uint32_t kScaleCols = 8 + 8 * kRowPieces;
-  static constexpr uint32_t kScaleRing = CTAS == 2 ? 2 : kStages;
-  static constexpr uint32_t kUsedCols = 2 * NT + kScaleRing * kScaleCols;
+  // Tensor memory: two accumulators, then two sets of columns for scales, which are copied there for kScaleStages stages at once where they have the
+  // room (a copy and the products after it wait for one another), else for one.
+  static constexpr uint32_t kStageCols = 2 * 4 * (1 + kRowPieces);
+  static constexpr uint32_t kUnitStages = 2 * NT + 2 * kScaleStages * kStageCols <= 512 ? kScaleStages : 1;
+  static constexpr uint32_t kUnitCols = kUnitStages * kStageCols;
+  static constexpr uint32_t kUsedCols = 2 * NT + 2 * kUnitCols;
   static constexpr uint32_t kCols = kUsedCols <= 256 ? 256 : 512;
   static_assert(kUsedCols <= kCols, "tensor memory");
 };
@@ -101,11 +117,11 @@ __device__ __forceinline__ uint32_t tile_rows(uint32_t n) {
   return NT >= 128 && tiles > 1 && tiles <= 8 ? ((n + tiles - 1) / tiles + 15) & ~15u : NT;
 }
 
-template <bool GU, uint32_t CTAS, uint32_t NT>
-__global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_product(const __grid_constant__ Mx4Args a, const __grid_constant__ CUtensorMap wmap,
-                                                                                    const __grid_constant__ CUtensorMap xmap) {
+template <class Out, uint32_t CTAS, uint32_t NT>
+__global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_product(const __grid_constant__ Mx4Args a, const __grid_constant__ Mx4Maps maps) {
   using namespace tc;
-  using SM = Mx4Form<GU, CTAS, NT>;
+  using SM = Mx4Form<Out, CTAS, NT>;
+  constexpr bool GU = SM::GU;
   constexpr uint32_t S = SM::kStages, SL = SM::kScaleSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -120,7 +136,8 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
   auto bar = [&](uint32_t i) { return bar0 + 8 * i; };
   uint32_t *tmem_slot = (uint32_t *)(bars + kBars);
   volatile uint32_t *abort = tmem_slot + 1;
-  uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *end_row = first_row + kMaxExperts + 1, *first_tile = end_row + kMaxExperts + 1;
+  uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *first_tile = first_row + kMaxExperts + 1;  // [E + 1] each
+  uint16_t *tile_expert = (uint16_t *)(smem + SM::kTileExperts);
   uint32_t *error = &g_gave_up;
 
   if (tid == 0) {
@@ -137,16 +154,26 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
       tmem_alloc(smem_u32(tmem_slot), SM::kCols);
   }
   dependents_may_launch(), wait_for_predecessors();
-  // The experts' rows and tiles, summed up by one warp, 16 experts a lane. Offsets are held to 0 .. R and to their order.
+  // The experts' first rows and tiles by one warp, 16 experts a lane. Offsets are held to 0 .. R, and to rise: each to the largest before it.
   if (warp == kEpilogueWarp) {
-    const uint32_t per = (a.E + 31) / 32, e0 = min(a.E, lane * per), e1 = min(a.E, e0 + per);
-    auto row_of = [&](uint32_t e) { return a.offsets ? min((uint32_t)max(a.offsets[e], 0), a.R) : e ? a.R : 0u; };
-    uint32_t sum = 0;
+    const uint32_t per = (a.E + 32) / 32, e0 = min(a.E + 1, lane * per), e1 = min(a.E + 1, e0 + per);
+    uint32_t top = 0;
     for (uint32_t e = e0; e < e1; e++) {
-      const uint32_t lo = row_of(e), hi = row_of(e + 1), n = hi > lo ? hi - lo : 0;
-      first_row[e] = lo, end_row[e] = lo + n;
-      sum += (n + NT - 1) / NT;
+      top = max(top, a.offsets ? min((uint32_t)max(a.offsets[e], 0), a.R) : e ? a.R : 0u);
+      first_row[e] = top;
     }
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, top, off);
+      if (lane >= (uint32_t)off) top = max(top, o);
+    }
+    top = __shfl_up_sync(0xffffffffu, top, 1);  // the largest of the lanes before
+    if (lane > 0)
+      for (uint32_t e = e0; e < e1; e++) first_row[e] = max(first_row[e], top);
+    __syncwarp();
+    auto tiles_of = [&](uint32_t e) { return e < a.E ? (first_row[e + 1] - first_row[e] + NT - 1) / NT : 0u; };
+    uint32_t sum = 0;
+    for (uint32_t e = e0; e < e1; e++) sum += tiles_of(e);
     uint32_t before = sum;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -156,17 +183,28 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
     before -= sum;
     for (uint32_t e = e0; e < e1; e++) {
       first_tile[e] = before;
-      before += (end_row[e] - first_row[e] + NT - 1) / NT;
+      before += tiles_of(e);
     }
-    if (lane == 31) first_tile[a.E] = before;
   }
+  __syncthreads();
+  const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK, ntiles = first_tile[a.E];
+  auto expert_at = [&](uint32_t t) {  // the last expert whose first tile is at most t
+    uint32_t lo = 0, hi = a.E;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (first_tile[mid] <= t)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  };
+  for (uint32_t t = tid; t < min(ntiles, kTileTable); t += SM::kThreads) tile_expert[t] = (uint16_t)expert_at(t);
   tc_fence_before();
   __syncthreads();
   if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK;
-  const uint32_t nitems = first_tile[a.E] * M;  // 2^24 / 32 + 512 tiles of 1,024 at most
   const uint32_t lead0 = CTAS == 2 ? map_to_cta(bar0, 0) : bar0;  // the first CTA's barriers as this CTA names them
   auto lead = [&](uint32_t i) { return lead0 + 8 * i; };
   auto arrive_lead = [&](uint32_t i) {
@@ -177,49 +215,48 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
   };
   bool ok = true;
 
+  // Item i is piece m = i % M of the matrix for tile t = i / M of the experts' tiles in order; a unit steps by nunits items.
+  struct Item {
+    uint32_t t, m;
+  };
+  const uint32_t step_t = nunits / M, step_m = nunits - step_t * M;
+  const Item first{unit / M, unit % M};
+  auto step = [&](Item &i) {
+    i.t += step_t, i.m += step_m;
+    if (i.m >= M) i.m -= M, i.t++;
+  };
   // row0: the first of this CTA's matrix rows, or of its features.
   struct Tile {
     uint32_t expert, start, count, row0;
   };
-  // Item i: tile i / M of the experts' tiles in order, and which of its M pieces of the matrix.
-  auto tile_at = [&](uint32_t i) {
-    const uint32_t t = i / M;
-    uint32_t lo = 0, hi = a.E;  // the last expert whose first tile is at most t
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (first_tile[mid] <= t)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    const uint32_t per = tile_rows<NT>(end_row[lo] - first_row[lo]), start = first_row[lo] + (t - first_tile[lo]) * per;
-    return Tile{lo, start, min(per, end_row[lo] - start), ((i - t * M) * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
+  auto tile_at = [&](const Item &i) {
+    const uint32_t e = i.t < kTileTable ? tile_expert[i.t] : expert_at(i.t);
+    const uint32_t r0 = first_row[e], r1 = first_row[e + 1], per = tile_rows<NT>(r1 - r0), start = r0 + (i.t - first_tile[e]) * per;
+    return Tile{e, start, min(per, r1 - start), (i.m * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
   };
 
   if (warp == kCopyWarp) {
     if (lane == 0) {
       uint32_t s = 0, phase = 1;  // of the stage's "empty": the first round finds it so
-      for (uint32_t i = unit; i < nitems && ok; i += nunits) {
+      for (Item i = first; i.t < ntiles && ok; step(i)) {
         const Tile t = tile_at(i);
-        // A CTA of a pair brings its half of the rows the instruction takes, which are rounded up to 16.
-        const uint32_t half = ((t.count + 15) & ~15u) / CTAS, x_row = t.start + rank * half, boxes = (half + kBoxRows - 1) / kBoxRows;
+        // A CTA of a pair brings its half of the rows the instruction takes, which are rounded up to 16: by one copy, or two. A copy may run past
+        // the tile's rows; what it brings then goes into columns nobody reads. (Copies of 16 rows, seven a stage for a full tile, took 260 us
+        // of a step whose copies take 141 so.)
+        const uint32_t half = ((t.count + 15) & ~15u) / CTAS, x_row = t.start + rank * half;
+        const uint32_t b0 = half > 80 ? 3 : half > 48 ? 2 : half > 16 ? 1 : 0, rest = half > box_rows(b0) ? box_rows(0) : 0;
+        const uint32_t bytes = (kRowsM + box_rows(b0) + rest) * 128;
         for (uint32_t it = 0; it < KT && ok; it++) {
           ok = mbar_wait(bar(kEmpty + s), phase, abort, error);
           if (!ok) break;
           const uint32_t at = smem_u32(smem + s * SM::kStageBytes), x0 = it * (kStageK / 2);
-          auto copy = [&](uint32_t dst, const CUtensorMap *map, uint32_t y, uint32_t z) {
-            if constexpr (CTAS == 2)
-              tma_load_codes_pair(dst, map, x0, y, z, lead(s));
-            else
-              tma_load_quants(dst, map, x0, y, z, lead(s));
-          };
           if constexpr (CTAS == 2)
-            mbar_arrive_expect_cluster(lead(s), kRowsM * 128 + boxes * kBoxRows * 128);
+            mbar_arrive_expect_cluster(lead(s), bytes);
           else
-            mbar_arrive_expect(lead(s), kRowsM * 128 + boxes * kBoxRows * 128);
-          copy(at, &wmap, t.row0, t.expert);
-          if constexpr (GU) copy(at + 64 * 128, &wmap, F + t.row0, t.expert);
-          for (uint32_t b = 0; b < boxes; b++) copy(at + (kRowsM + b * kBoxRows) * 128, &xmap, x_row + b * kBoxRows, 0);
+            mbar_arrive_expect(lead(s), bytes);
+          tma_load_codes<CTAS>(at, &maps.w, x0, t.row0, t.expert, lead(s));
+          tma_load_codes<CTAS>(at + kRowsM * 128, &maps.x[b0], x0, x_row, 0, lead(s));
+          if (rest) tma_load_codes<CTAS>(at + (kRowsM + box_rows(b0)) * 128, &maps.x[0], x0, x_row + box_rows(b0), 0, lead(s));
           if (++s == S) s = 0, phase ^= 1;
         }
       }
@@ -236,7 +273,7 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
     const uint32_t word = lane % 8, slot = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes);
     const uint32_t at = slot + word * 512, x_at = slot + 8 * 512 + word * SM::kRowPieces * 512;
     uint32_t turn = 0, phase = 1;  // whose turn the next slot is
-    for (uint32_t i = unit; i < nitems && ok; i += nunits) {
+    for (Item i = first; i.t < ntiles && ok; step(i)) {
       const Tile t = tile_at(i);
       for (uint32_t j = 0; j < slots && ok; j++, turn = turn == SL - 1 ? 0 : turn + 1) {
         if (turn != mine) continue;
@@ -267,44 +304,54 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
         else
           mma_commit(leader, bar(i));
       };
-      uint32_t s = 0, phase = 0, slot = 0, slot_phase = 0, ring = 0, b = 0, acc_phase = 1;
-      uint32_t old = S - SM::kScaleRing % S, old_phase = 1;  // the stage whose scales the ring's next columns held, kScaleRing stages ago
-      for (uint32_t i = unit; i < nitems && ok; i += nunits) {
+      uint32_t s = 0, phase = 0, slot = 0, slot_phase = 0, set = 0, b = 0, acc_phase = 1;
+      // The barrier that says the MMAs of two units ago, which read the columns the next scales go to, are done: a stage's or a slot's "empty".
+      constexpr uint32_t kRing = SM::kUnitStages == 1 ? S : SL, kDone = SM::kUnitStages == 1 ? kEmpty : kScEmpty;
+      uint32_t old = kRing - 2, old_phase = 1;
+      for (Item i = first; i.t < ntiles && ok; step(i)) {
         const Tile t = tile_at(i);
         const uint32_t n = (t.count + 15) & ~15u, acc = tmem_base + b * NT;
         const uint32_t d0 = mx4_instr_desc(n, CTAS * kRowsM, 0), d2 = mx4_instr_desc(n, CTAS * kRowsM, 2);
+        uint32_t ta = 0, tb = 0;
         ok = mbar_wait_warp(bar(kAccEmpty + b), acc_phase, abort, error);
         for (uint32_t it = 0; it < KT && ok; it++) {
-          const uint32_t sub = it % kScaleStages;
+          const uint32_t sub = it % kScaleStages, in_unit = it % SM::kUnitStages;
           if (sub == 0) ok = mbar_wait_warp(bar(kScFull + slot), slot_phase, abort, error);
+          if (in_unit == 0) {
+            if (ok) ok = mbar_wait_warp(bar(kDone + old), old_phase, abort, error);
+            if (!ok) break;
+            if (++old == kRing) old = 0, old_phase ^= 1;
+            tc_fence_after();
+            ta = tmem_base + 2 * NT + set * SM::kUnitCols, tb = ta + 8 * SM::kUnitStages, set ^= 1;
+            const uint32_t from = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes);
+            const uint32_t words = min(2 * SM::kUnitStages, (K - it * kStageK + 127) / 128);
+#pragma unroll
+            for (uint32_t w = 0; w < 2 * SM::kUnitStages; w++) {
+              if (w >= words) continue;
+              copy_scales<CTAS>(leader, ta + 4 * w, from + (2 * sub + w) * 512);
+#pragma unroll
+              for (uint32_t p = 0; p < SM::kRowPieces; p++)
+                copy_scales<CTAS>(leader, tb + 4 * (w * SM::kRowPieces + p), from + (8 + (2 * sub + w) * SM::kRowPieces + p) * 512);
+            }
+          }
           if (ok) ok = mbar_wait_warp(bar(s), phase, abort, error);
-          // The columns this stage's scales go to are free when the MMAs that read them are done: with as many columns as stages they are,
-          // for the stage was empty again; else the commit after those MMAs says so.
-          if constexpr (SM::kScaleRing < S)
-            if (ok) ok = mbar_wait_warp(bar(kEmpty + old % S), old_phase, abort, error);
           if (!ok) break;
           tc_fence_after();
           const uint32_t stage = smem_u32(smem + s * SM::kStageBytes), rows = stage + kRowsM * 128;
-          const uint32_t sc = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes) + 2 * sub * 512;
-          const uint32_t sx = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes) + 8 * 512 + 2 * sub * SM::kRowPieces * 512;
-          const uint32_t ta = tmem_base + 2 * NT + ring * SM::kScaleCols, tb = ta + 8;
-          copy_scales<CTAS>(leader, ta, sc), copy_scales<CTAS>(leader, ta + 4, sc + 512);
-#pragma unroll
-          for (uint32_t p = 0; p < 2 * SM::kRowPieces; p++) copy_scales<CTAS>(leader, tb + 4 * p, sx + 512 * p);
           const uint32_t steps = min(4u, (K - it * kStageK + 63) / 64);
 #pragma unroll
-          for (uint32_t k = 0; k < 4; k++)
+          for (uint32_t k = 0; k < 4; k++) {
+            const uint32_t w = 2 * in_unit + k / 2;
             if (k < steps)
-              mma_mx4<CTAS>(leader, acc, smem_desc_sw128(stage + 32 * k), smem_desc_sw128(rows + 32 * k), k % 2 ? d2 : d0, ta + 4 * (k / 2),
-                            tb + 4 * SM::kRowPieces * (k / 2), (it | k) != 0);
+              mma_mx4<CTAS>(leader, acc, smem_desc_sw128(stage + 32 * k), smem_desc_sw128(rows + 32 * k), k % 2 ? d2 : d0, ta + 4 * w,
+                            tb + 4 * SM::kRowPieces * w, (it | k) != 0);
+          }
           commit(kEmpty + s);
           if (sub == kScaleStages - 1 || it == KT - 1) {
             commit(kScEmpty + slot);
             if (++slot == SL) slot = 0, slot_phase ^= 1;
           }
           if (++s == S) s = 0, phase ^= 1;
-          if (++ring == SM::kScaleRing) ring = 0;
-          if (++old == S) old = 0, old_phase ^= 1;
         }
         if (!ok) break;
         commit(kAccFull + b);
@@ -315,48 +362,65 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
     // Warp w reads tensor memory's lanes 32 (w % 4) ...; the groups take chunks of 16 rows in turn.
     const uint32_t q = warp % 4, group = (warp - kEpilogueWarp) / 4;
     uint32_t b = 0, phase = 0;
-    [[maybe_unused]] uint32_t turn = 0;
-    for (uint32_t i = unit; i < nitems && ok; i += nunits) {
+    for (Item i = first; i.t < ntiles && ok; step(i)) {
       const Tile t = tile_at(i);
       const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT;
       ok = mbar_wait_warp(bar(kAccFull + b), phase, abort, error);
       if constexpr (GU) ok = group_all(group, ok);
       if (!ok) break;
       tc_fence_after();
+      const uint32_t c0 = group * kChunk, dc = SM::kGroups * kChunk;
       if constexpr (!GU) {
-        const uint32_t n = t.row0 + 32 * q + lane;
-        for (uint32_t c = group * kChunk; c < t.count; c += SM::kGroups * kChunk) {
-          uint32_t v[16];
-          tmem_ld16(from + c, v);
-          tmem_ld_wait16(v);
-          const uint64_t at = (uint64_t)(t.start + c) * a.N + n;
+        // A lane holds one feature of 16 rows. Two lanes with neighbouring features share out two rows: the even one stores both features of the
+        // first, the odd one of the second. A chunk's values are on their way from tensor memory while the one before is stored.
+        const uint32_t odd = lane & 1, sel = odd ? 0x3276u : 0x5410u;
+        auto store = [&](uint32_t c, const uint32_t *v) {
+          Out *p = (Out *)a.y + (uint64_t)(t.start + c + odd) * a.N + (t.row0 + 32 * q + lane - odd);
+          const uint32_t left = t.count - c;
 #pragma unroll
-          for (uint32_t j = 0; j < 16; j++) {
-            if (c + j >= t.count || n >= a.N) continue;
-            if (a.bf16)
-              ((__nv_bfloat16 *)a.y)[at + (uint64_t)j * a.N] = __float2bfloat16_rn(__uint_as_float(v[j]));
-            else
-              ((__half *)a.y)[at + (uint64_t)j * a.N] = __float2half_rn(__uint_as_float(v[j]));
+          for (uint32_t j = 0; j < 16; j += 2, p += 2 * a.N) {
+            const uint32_t mine = pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), (const Out *)nullptr), theirs = __shfl_xor_sync(0xffffffffu, mine, 1);
+            if (j + odd < left) *(uint32_t *)p = __byte_perm(mine, theirs, sel);
+          }
+        };
+        if (t.row0 + 32 * q < a.N) {  // features come 32 together
+          uint32_t v[16], u[16];
+          if (c0 < t.count) tmem_ld16(from + c0, v);
+          for (uint32_t c = c0; c < t.count; c += 2 * dc) {
+            tmem_ld_wait16(v);
+            if (c + dc < t.count) tmem_ld16(from + c + dc, u);
+            store(c, v);
+            if (c + dc >= t.count) break;
+            tmem_ld_wait16(u);
+            if (c + 2 * dc < t.count) tmem_ld16(from + c + 2 * dc, v);
+            store(c + dc, u);
           }
         }
       } else {
-        // Through shared memory, a row of the chunk its 64 gate and 64 up products, to threads of eight features each. Of a group's two
-        // chunks there the one is written while another warp may still read the other; past the barrier all have left it.
+        // Through shared memory, a row of the chunk its 64 gate and 64 up products, to threads of eight features each. A group has two chunks
+        // there: the next one's values come from tensor memory while this one is worked on, and are put where the one before was, which every
+        // thread of the group left before the barrier this chunk came by.
         const uint32_t f = (tid % 8) * 8, hrow = mx_scale_row_bytes(F), at = t.row0 + f, r = (tid / 8) % 16;
-        for (uint32_t c = group * kChunk; c < t.count; c += SM::kGroups * kChunk, turn ^= 1) {
-          float *st = (float *)(smem + SM::kStaging + (2 * group + turn) * SM::kStagingBytes);
-          uint32_t v[16];
-          tmem_ld16(from + c, v);
+        auto room = [&](uint32_t n) { return (float *)(smem + SM::kStaging + (2 * group + n) * SM::kStagingBytes); };
+        uint32_t v[16];
+        auto put = [&](float *st) {
           tmem_ld_wait16(v);
 #pragma unroll
           for (uint32_t j = 0; j < 16; j++) st[j * SM::kStagingRow + 32 * q + lane] = __uint_as_float(v[j]);
           group_sync(group);
-          float h[8];
+        };
+        if (c0 < t.count) tmem_ld16(from + c0, v), put(room(0));
+        uint32_t turn = 0;
+        for (uint32_t c = c0; c < t.count; c += dc, turn ^= 1) {
+          const bool more = c + dc < t.count;
+          if (more) tmem_ld16(from + c + dc, v);
+          const float *p = room(turn) + r * SM::kStagingRow + f;
+          float g[8], u[8], h[8];
+          load8(p, g), load8(p + 64, u);
           uint32_t m = 0;
 #pragma unroll
           for (int j = 0; j < 8; j++) {
-            const float *p = st + r * SM::kStagingRow + f + j;
-            h[j] = swiglu(p[0], p[64], a.limit);
+            h[j] = swiglu_fast(g[j], u[j], a.limit);  // two significant bits of it stay
             m = max(m, __float_as_uint(h[j]) & 0x7FFFFFFFu);
           }
           m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
@@ -365,12 +429,14 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
           const float inv = mx_inverse(scale);
 #pragma unroll
           for (int j = 0; j < 8; j++) h[j] *= inv;
-          if (c + r >= t.count || at >= F) continue;
-          const uint64_t row = t.start + c + r;
-          *(uint32_t *)(a.hc + row * (F / 2) + at / 2) = scale == 255 ? 0u : mx_codes8(h);
-          if (tid % 4 == 0) a.hs[row * hrow + at / kMxBlock] = (uint8_t)scale;
-          if (tid % 4 == 0 && at + kMxBlock == F)
-            for (uint32_t s = F / kMxBlock; s < hrow; s++) a.hs[row * hrow + s] = 0;
+          if (c + r < t.count && at < F) {
+            const uint64_t row = t.start + c + r;
+            *(uint32_t *)(a.hc + row * (F / 2) + at / 2) = scale == 255 ? 0u : mx_codes8(h);
+            if (tid % 4 == 0) a.hs[row * hrow + at / kMxBlock] = (uint8_t)scale;
+            if (tid % 4 == 0 && at + kMxBlock == F)
+              for (uint32_t s = F / kMxBlock; s < hrow; s++) a.hs[row * hrow + s] = 0;
+          }
+          if (more) put(room(turn ^ 1));
         }
       }
       tc_fence_before();
@@ -392,10 +458,11 @@ __global__ void __launch_bounds__(Mx4Form<GU, CTAS, NT>::kThreads, 1) k_mx4_prod
   }
 }
 
-template <bool GU, uint32_t CTAS, uint32_t NT>
+template <class Out, uint32_t CTAS, uint32_t NT>
 void launch_product(const Mx4Args &args, const void *wc, const void *xc, cudaStream_t st) {
-  using Form = Mx4Form<GU, CTAS, NT>;
-  constexpr auto kernel = k_mx4_product<GU, CTAS, NT>;
+  using Form = Mx4Form<Out, CTAS, NT>;
+  constexpr auto kernel = k_mx4_product<Out, CTAS, NT>;
+  constexpr bool GU = Form::GU;
   Mx4Args a = args;
   int device = 0;
   CUDA_OK(cudaGetDevice(&device));
@@ -413,23 +480,25 @@ void launch_product(const Mx4Args &args, const void *wc, const void *xc, cudaStr
   const uint32_t rows = CTAS * (GU ? kRowsM / 2 : kRowsM), all = GU ? a.N / 2 : a.N;
   a.items_per_tile = (all + rows - 1) / rows;
   const uint64_t most = ((uint64_t)a.R / NT + std::min(a.E, a.R)) * a.items_per_tile;  // items there can be
-  const CUtensorMap wmap = make_codes_map(wc, a.K / 2, a.N, a.E, GU ? 64 : kRowsM), xmap = make_codes_map(xc, a.K / 2, a.R, 1, kBoxRows);
+  Mx4Maps maps;
+  maps.w = make_codes_map(wc, a.K / 2, all, GU ? 2 : 1, a.E, GU ? kRowsM / 2 : kRowsM);
+  for (uint32_t i = 0; i < kBoxes; i++) maps.x[i] = make_codes_map(xc, a.K / 2, a.R, 1, 1, box_rows(i));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2]{};
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension, at[1].val.clusterDim = {CTAS, 1, 1};
   cfg.gridDim = dim3(CTAS * (unsigned)std::min<uint64_t>(most, units)), cfg.blockDim = dim3(Form::kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cfg.attrs = at, cfg.numAttrs = CTAS;  // a single CTA is no cluster
-  CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, wmap, xmap));
+  CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, maps));
 }
 
 // Tiles of 224 rows by pairs of CTAs, or of 32 by single ones.
-template <bool GU>
+template <class Out>
 void launch(const Mx4Args &a, const void *wc, const void *xc, cudaStream_t st) {
   if (a.R > 32ull * a.E)
-    launch_product<GU, 2, 224>(a, wc, xc, st);
+    launch_product<Out, 2, 224>(a, wc, xc, st);
   else
-    launch_product<GU, 1, 32>(a, wc, xc, st);
+    launch_product<Out, 1, 32>(a, wc, xc, st);
 }
 
 Mx4Args arguments(const moe_mx4_weights *w, const void *scales, uint32_t R, const int32_t *offsets) {
@@ -460,8 +529,11 @@ MOE_API moe_status moe_mx4_product_device(const moe_mx4_weights *w, const void *
     Mx4Args a = arguments(w, scales_dev, R, offsets_dev);
     if (R == 0) return;
     need_device({{w->codes_dev, "weight codes", 16}, {a.ws, "weight scales", 4}, {codes_dev, "codes", 16}, {a.xs, "scales", 4}, {a.offsets, "offsets", 4, true}, {y_dev, "y", 16}});
-    a.y = y_dev, a.bf16 = y_type == MOE_TYPE_BF16;
-    launch<false>(a, w->codes_dev, codes_dev, (cudaStream_t)stream);
+    a.y = y_dev;
+    if (y_type == MOE_TYPE_BF16)
+      launch<__nv_bfloat16>(a, w->codes_dev, codes_dev, (cudaStream_t)stream);
+    else
+      launch<__half>(a, w->codes_dev, codes_dev, (cudaStream_t)stream);
   });
 }
 
@@ -475,7 +547,7 @@ MOE_API moe_status moe_mx4_gate_up_device(const moe_mx4_weights *w, const void *
     need_device({{w->codes_dev, "weight codes", 16}, {a.ws, "weight scales", 4}, {codes_dev, "codes", 16}, {a.xs, "scales", 4}, {a.offsets, "offsets", 4, true},
                  {h_codes_dev, "h codes", 16}, {h_scales_dev, "h scales", 4}});
     a.limit = swiglu_limit, a.hc = (uint8_t *)h_codes_dev, a.hs = (uint8_t *)h_scales_dev;
-    launch<true>(a, w->codes_dev, codes_dev, (cudaStream_t)stream);
+    launch<GateUp>(a, w->codes_dev, codes_dev, (cudaStream_t)stream);
   });
 }
 

@@ -3,7 +3,8 @@
 //
 // Scales reach tensor memory by tcgen05.cp from shared memory, 512 bytes a copy: 128 rows' words of four scales (128 values). Row r's word
 // lies at 16 (r % 32) + 4 (r / 32) of the piece, and lands in lane r % 32 (of every warp's quarter) of column r / 32. An instruction takes bytes
-// 0, 1 or 2, 3 of the words, named by its descriptor's scale ids 0 or 2.
+// 0, 1 or 2, 3 of the words, named by its descriptor's scale ids 0 or 2. Its scales' first columns are multiples of four: with another one it
+// faults.
 #pragma once
 
 #include <cstdint>
@@ -61,12 +62,18 @@ __device__ __forceinline__ void mma_mx4(uint32_t leader, uint32_t tmem_d, uint64
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scales_a), "r"(scales_b), "r"(accumulate), "r"(leader)
         : "memory");
 }
-// A box of 128 bytes' width of the map's tensor, by a CTA of a pair: into its own shared memory, the bytes counted on a barrier that may be the
-// other CTA's. x is a multiple of 16.
-__device__ __forceinline__ void tma_load_codes_pair(uint32_t dst_smem, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(dst_smem), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
-               : "memory");
+// A box of the map's tensor of codes (tensor_map.h, make_codes_map): 128 bytes from byte x (a multiple of 16) of the rows from y on, of all parts of
+// matrix z. CTAS 2: by a CTA of a pair, into its own shared memory, the bytes counted on a barrier that may be the other CTA's.
+template <uint32_t CTAS>
+__device__ __forceinline__ void tma_load_codes(uint32_t dst_smem, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z, uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst_smem), "l"((uint64_t)map), "r"(x), "r"(y), "r"(0), "r"(z), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst_smem), "l"((uint64_t)map), "r"(x), "r"(y), "r"(0), "r"(z), "r"(bar)
+                 : "memory");
 }
 // Four bytes into shared memory, the first n of them from memory and zeros behind (n 0: nothing is read).
 __device__ __forceinline__ void copy_word(uint32_t dst, const void *src, uint32_t n) {

@@ -49,13 +49,14 @@ CUtensorMap make_rows_map(const void *base, uint64_t rows, uint32_t K, uint32_t 
   return m;
 }
 
-CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t matrices, uint32_t box_rows) {
+CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows) {
   CUtensorMap m{};
-  const cuuint64_t dims[3] = {row_bytes, rows, matrices};
-  const cuuint64_t strides[2] = {row_bytes, (cuuint64_t)row_bytes * rows};
-  const cuuint32_t box[3] = {128, box_rows, 1};
-  const cuuint32_t elem[3] = {1, 1, 1};
-  const CUresult r = tensor_map_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, elem,
+  const cuuint64_t part = (cuuint64_t)row_bytes * rows;
+  const cuuint64_t dims[4] = {row_bytes, rows, parts, matrices};
+  const cuuint64_t strides[3] = {row_bytes, part, part * parts};
+  const cuuint32_t box[4] = {128, box_rows, parts, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  const CUresult r = tensor_map_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, box, elem,
                                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw CudaFailure(cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed with driver error " + std::to_string((int)r));

@@ -21,9 +21,9 @@ CUtensorMap make_rows_map(const void *base, uint64_t rows, uint32_t K, uint32_t 
 // of neighbouring rows fall on different banks.
 CUtensorMap make_quants_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t nslots, uint64_t slice_bytes, uint32_t box_bytes);
 
-// A map over matrices of 4-bit codes two a byte, [matrices][rows][row_bytes] one after another (base 16-byte aligned, row_bytes a multiple of
-// 16), whose copies bring 128 bytes (256 values) of box_rows rows of one of them with the 128-byte swizzle. What lies past a row's
-// end or past a matrix's rows reads as zero.
-CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t matrices, uint32_t box_rows);
+// A map over matrices of 4-bit codes two a byte, [matrices][parts][rows][row_bytes] one after another (base 16-byte aligned, row_bytes a
+// multiple of 16), whose copies bring 128 bytes (256 values) of box_rows rows of every part of one matrix, part after part, with the 128-byte
+// swizzle. What lies past a row's end or past a part's rows reads as zero.
+CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows);
 
 }  // namespace moe

@@ -384,8 +384,8 @@ typedef struct {
 } moe_mx4_weights;
 
 /* Products of R MX rows in expert order with their experts' matrices, each row with its own expert's: rows offsets_dev[e] ..
- * offsets_dev[e + 1] with expert e's (ascending, as moe_route_logits_device leaves them; n_experts + 1 of them; what they say past
- * R is cut off; null: one expert has all R). Rows of no expert are left as they were. Sums are f32.
+ * offsets_dev[e + 1] with expert e's (ascending, as moe_route_logits_device leaves them; n_experts + 1 of them; one past
+ * R counts as R, one below 0 or one before it as that; null: one expert has all R). Rows of no expert are left as they were. Sums are f32.
  *   product: y_dev [R][n_out], f16 or bf16 (MOE_TYPE_F16, MOE_TYPE_BF16), 16-byte aligned: the products, rounded once.
  *   gate_up: w's rows are n_out / 2 gate rows and then as many up rows, n_out a multiple of 64; h = g / (1 + exp(-g)) * u,
  *            with limit > 0 of min(g, limit) and of u held to [-limit, limit], to MX rows of n_out / 2 values.
