@@ -6,10 +6,10 @@
 // short instruction and what an item costs is bringing the matrix. Persistent units (a CTA, or a pair of CTAs on two SMs that share the rows:
 // tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
 //
-// Roles of a CTA's warps: one thread brings codes by bulk-tensor copies, 256 values of the contraction a stage; four warps bring the scales,
+// Roles of a CTA's warps: one thread brings codes by bulk-tensor copies, 256 values of the contraction a stage; three warps bring the scales,
 // four stages (1,024 values: a sector of a row's scales) at a time in turn, word by word into the layout that the tensor core's copy reads
-// (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance); one lane (of a pair's first CTA) issues scale copies and
-// MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
+// (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance); one lane (of a pair's first CTA) issues the copies of
+// scales to tensor memory, and one the MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
 //
 // Every wait on an mbarrier is bounded: one that runs out raises the CTA's abort flag and the device's error word (moe_ops_status), the other
 // waits return at once, and the CTA frees its tensor memory before it exits.
@@ -34,21 +34,32 @@ constexpr uint32_t kStageK = 256;       // values of the contraction a stage hol
 constexpr uint32_t kScaleStages = 4;    // stages that one slot of scales covers
 constexpr uint32_t kTileTable = 1024;   // tiles whose expert is looked up in a table
 constexpr uint32_t kChunk = 16;         // rows an epilogue warp turns at a time
+constexpr uint32_t kPiece = 528;        // bytes from a piece of 512 bytes of scales to the next: the eight words of a row fall on different banks
 
-// Barriers of a group of four epilogue warps alone. The second tells every one of them whether ok holds for all: they leave their loop together
-// or not at all, so that none waits here for one that has left.
-__device__ __forceinline__ void group_sync(uint32_t group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
-__device__ __forceinline__ bool group_all(uint32_t group, bool ok) {
+// Barriers of two epilogue warps alone. The second tells both whether ok holds for both: they leave their loop together or not at all, so
+// that neither waits here for one that has left.
+__device__ __forceinline__ void two_warps_sync(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(1 + id) : "memory"); }
+__device__ __forceinline__ bool two_warps_all(uint32_t id, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, %2, 128, p;\n\t"
+      "bar.red.and.pred q, %2, 64, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)ok), "r"(1 + group)
+      : "r"((uint32_t)ok), "r"(1 + id)
       : "memory");
   return r != 0;
+}
+
+// Eight lanes hold eight 4-bit codes each, code j of lane i becomes code i of lane j: three exchanges of the half a lane does not keep.
+__device__ __forceinline__ uint32_t transpose_codes(uint32_t v, uint32_t lane) {
+  const uint32_t a = __shfl_xor_sync(0xffffffffu, v, 4);
+  v = lane & 4 ? (v & 0xFFFF0000u) | a >> 16 : (v & 0x0000FFFFu) | a << 16;
+  const uint32_t b = __shfl_xor_sync(0xffffffffu, v, 2);
+  v = lane & 2 ? (v & 0xFF00FF00u) | (b >> 8 & 0x00FF00FFu) : (v & 0x00FF00FFu) | (b << 8 & 0xFF00FF00u);
+  const uint32_t c = __shfl_xor_sync(0xffffffffu, v, 1);
+  return lane & 1 ? (v & 0xF0F0F0F0u) | (c >> 4 & 0x0F0F0F0Fu) : (v & 0x0F0F0F0Fu) | (c << 4 & 0xF0F0F0F0u);
 }
 
 __device__ uint32_t g_gave_up;  // a wait ran out since moe_ops_status last asked
@@ -74,8 +85,7 @@ struct Mx4Maps {
 struct GateUp {};
 
 // A form of the kernel: what it makes, CTAs a unit has, and the most rows of a tile. Its shared memory: stages of codes; slots of scales, the matrix's
-// and then the rows', eight words of every row each; for gate_up the accumulators on their way to the quantiser, two chunks a group;
-// barriers; the experts' first rows and first tiles; the tiles' experts.
+// and then the rows', eight words of every row each; for gate_up the accumulators that two warps exchange, twice 1 KB a warp; barriers; the experts' first rows and first tiles; the tiles' experts.
 template <class Out, uint32_t CTAS, uint32_t NT>
 struct Mx4Form {
   static constexpr bool GU = std::is_same<Out, GateUp>::value;
@@ -83,22 +93,19 @@ struct Mx4Form {
   static constexpr uint32_t kThreads = 32 * (6 + 4 * kGroups);
   static constexpr uint32_t kStages = CTAS == 2 ? 5 : 8;
   static constexpr uint32_t kStageBytes = (kRowsM + NT / CTAS) * 128;
-  static constexpr uint32_t kScaleSlots = CTAS == 2 ? 3 : 4;
+  static constexpr uint32_t kScaleSlots = 3;  // and as many warps to fill them
   // A word of 128 rows' scales is a piece of 512 bytes and four columns of tensor memory, even where there are fewer rows: an instruction's scales
   // begin at a multiple of four columns.
   static constexpr uint32_t kRowPieces = (NT + 127) / 128;
   static constexpr uint32_t kScales = kStages * kStageBytes;
-  static constexpr uint32_t kSlotBytes = (8 + 8 * kRowPieces) * 512;
+  static constexpr uint32_t kSlotBytes = 8 * (1 + kRowPieces) * kPiece;
   static constexpr uint32_t kStaging = kScales + kScaleSlots * kSlotBytes;
-  static constexpr uint32_t kStagingRow = kRowsM + 4;  // floats of a row of a chunk, padded
-  static constexpr uint32_t kStagingBytes = kChunk * kStagingRow * 4;
-  static constexpr uint32_t kBarriers = kStaging + (GU ? 2 * kGroups * kStagingBytes : 0);
+  static constexpr uint32_t kBarriers = kStaging + (GU ? 4 * kGroups * 2048 : 0);
   static constexpr uint32_t kTables = kBarriers + 256;
   static constexpr uint32_t kTileExperts = kTables + 2 * (kMaxExperts + 1) * 4;
   static constexpr uint32_t kBytes = kTileExperts + 2 * kTileTable + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
-  // Tensor memory: two accumulators, then two sets of columns for scales, which are copied there for kScaleStages stages at once where they have the
-  // room (a copy and the products after it wait for one another), else for one.
+  // Tensor memory: two accumulators, then two sets of columns for scales, of kScaleStages stages where they have the room, else of one.
   static constexpr uint32_t kStageCols = 2 * 4 * (1 + kRowPieces);
   static constexpr uint32_t kUnitStages = 2 * NT + 2 * kScaleStages * kStageCols <= 512 ? kScaleStages : 1;
   static constexpr uint32_t kUnitCols = kUnitStages * kStageCols;
@@ -107,7 +114,7 @@ struct Mx4Form {
   static_assert(kUsedCols <= kCols, "tensor memory");
 };
 
-enum : uint32_t { kCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kEpilogueWarp = 6 };
+enum : uint32_t { kCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kScaleCopyWarp = 5, kEpilogueWarp = 6 };
 
 // Rows a tile of an expert's n rows has: the tiles of a few share them evenly (which 16 rows a tile can be off by leaves no tile empty up to
 // eight tiles of 224).
@@ -128,9 +135,10 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0, unit = blockIdx.x / CTAS, nunits = gridDim.x / CTAS;
   uint64_t *bars = (uint64_t *)(smem + SM::kBarriers);
-  // Barriers: stages full, empty; scales full, empty; accumulators full, empty. Of a pair the first CTA's "full" of stages and scales and "empty"
+  // Barriers: stages full, empty; scales full, empty; accumulators full, empty; sets of scales in tensor memory full, empty. Of a pair the first CTA's "full" of stages and scales and "empty"
   // of accumulators take both CTAs' arrivals.
-  constexpr uint32_t kEmpty = S, kScFull = 2 * S, kScEmpty = kScFull + SL, kAccFull = kScEmpty + SL, kAccEmpty = kAccFull + 2, kBars = kAccEmpty + 2;
+  constexpr uint32_t kEmpty = S, kScFull = 2 * S, kScEmpty = kScFull + SL, kAccFull = kScEmpty + SL, kAccEmpty = kAccFull + 2, kSetFull = kAccEmpty + 2,
+                     kSetEmpty = kSetFull + 2, kBars = kSetEmpty + 2;
   static_assert(8 * kBars + 8 <= 256, "the barriers' room");
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](uint32_t i) { return bar0 + 8 * i; };
@@ -144,6 +152,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     for (uint32_t s = 0; s < S; s++) mbar_init(bar(s), CTAS), mbar_init(bar(kEmpty + s), 1);
     for (uint32_t s = 0; s < SL; s++) mbar_init(bar(kScFull + s), CTAS), mbar_init(bar(kScEmpty + s), 1);
     for (uint32_t b = 0; b < 2; b++) mbar_init(bar(kAccFull + b), 1), mbar_init(bar(kAccEmpty + b), CTAS * 4 * SM::kGroups);
+    for (uint32_t b = 0; b < 2; b++) mbar_init(bar(kSetFull + b), 1), mbar_init(bar(kSetEmpty + b), 1);
     *abort = 0;
     fence_barrier_init();
   }
@@ -268,10 +277,12 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
       }
     }
   } else if (warp >= kScaleWarp && warp < kScaleWarp + SL) {
-    // A slot of scales by a warp: four rows' eight words an instruction, so that a row's 32 bytes are one request.
+    // A slot of scales by a warp: eight words of rows i, i + 32, i + 64 and i + 96 an instruction, so that a row's 32 bytes are one request and the
+    // 32 words, at 16 i + 4 (row / 32) of pieces 528 bytes apart, fall on 32 banks. (Of four neighbouring rows into pieces 512 bytes apart,
+    // eight words to a bank, this took a third of shared memory's cycles.)
     const uint32_t mine = warp - kScaleWarp, srow = mx_scale_row_bytes(K), nb = K / kMxBlock, slots = (KT + kScaleStages - 1) / kScaleStages;
     const uint32_t word = lane % 8, slot = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes);
-    const uint32_t at = slot + word * 512, x_at = slot + 8 * 512 + word * SM::kRowPieces * 512;
+    const uint32_t quarter = lane / 8, at = slot + word * kPiece + 4 * quarter, x_at = at + 8 * kPiece;
     uint32_t turn = 0, phase = 1;  // whose turn the next slot is
     for (Item i = first; i.t < ntiles && ok; step(i)) {
       const Tile t = tile_at(i);
@@ -281,13 +292,30 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
         if (!ok) break;
         phase ^= 1;
         const uint32_t b0 = j * (kScaleStages * kStageK / kMxBlock) + 4 * word, n = b0 < nb ? min(4u, nb - b0) : 0u;
-        for (uint32_t r = lane / 8; r < kRowsM; r += 4) {
-          const uint32_t row = GU ? (r < 64 ? t.row0 + r : F + t.row0 + r - 64) : t.row0 + r, have = row < a.N ? n : 0;
-          copy_word(at + 16 * (r % 32) + 4 * (r / 32), have ? a.ws + ((uint64_t)t.expert * a.N + row) * srow + b0 : a.ws, have);
+        {
+          // This lane's 32 rows of the matrix follow one another.
+          const uint32_t r = 32 * quarter, row = GU ? (r < 64 ? t.row0 + r : F + t.row0 + r - 64) : t.row0 + r;
+          const uint8_t *src = a.ws + ((uint64_t)t.expert * a.N + row) * srow + b0;
+#pragma unroll 8
+          for (uint32_t k = 0; k < 32; k++, src += srow) {
+            const uint32_t have = row + k < a.N ? n : 0;
+            copy_word(at + 16 * k, have ? src : a.ws, have);
+          }
         }
-        for (uint32_t r = lane / 8; r < ((t.count + 3) & ~3u); r += 4) {
-          const uint32_t have = r < t.count ? n : 0;
-          copy_word(x_at + r / 128 * 512 + 16 * (r % 32) + 4 * (r / 32 % 4), have ? a.xs + (uint64_t)(t.start + r) * srow + b0 : a.xs, have);
+        if constexpr (NT <= 32) {
+          // Up to 32 rows, which lie in the first column of a piece: four neighbours an instruction.
+          for (uint32_t r = quarter; r < t.count; r += 4) copy_word(x_at - 4 * quarter + 16 * r, a.xs + (n ? (uint64_t)(t.start + r) * srow + b0 : 0), n);
+        } else {
+#pragma unroll
+          for (uint32_t p = 0; p < SM::kRowPieces; p++) {
+            const uint32_t r0 = 128 * p + 32 * quarter, left = t.count > 128 * p ? min(32u, t.count - 128 * p) : 0;
+            const uint8_t *src = a.xs + (uint64_t)(t.start + r0) * srow + b0;
+#pragma unroll 8
+            for (uint32_t k = 0; k < left; k++, src += srow) {
+              const uint32_t have = r0 + k < t.count ? n : 0;
+              copy_word(x_at + p * 8 * kPiece + 16 * k, have ? src : a.xs, have);
+            }
+          }
         }
         copy_words_wait();
         fence_async_smem();
@@ -295,45 +323,64 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
         if (lane == 0) arrive_lead(kScFull + mine);
       }
     }
+  } else if (warp == kScaleCopyWarp) {
+    // Scales to tensor memory, a unit of stages at a time, while the MMAs of the unit before run: an MMA waits for every copy that the same thread
+    // issued before it, which cost a stage of a full tile a third of its time.
+    if (rank == 0) {
+      constexpr uint32_t U = SM::kUnitStages;
+      const uint32_t leader = elect_leader();
+      uint32_t slot = 0, slot_phase = 0, set = 0, set_phase = 1;
+      for (Item i = first; i.t < ntiles && ok; step(i)) {
+        for (uint32_t it = 0; it < KT && ok; it += U) {
+          const uint32_t sub = it % kScaleStages;
+          if (sub == 0) ok = mbar_wait_warp(bar(kScFull + slot), slot_phase, abort, error);
+          if (ok) ok = mbar_wait_warp(bar(kSetEmpty + set), set_phase, abort, error);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t to = tmem_base + 2 * NT + set * SM::kUnitCols, to_rows = to + 8 * U, from = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes);
+          const uint32_t words = min(2 * U, (K - it * kStageK + 127) / 128);
+#pragma unroll
+          for (uint32_t w = 0; w < 2 * U; w++) {
+            if (w >= words) continue;
+            copy_scales<CTAS>(leader, to + 4 * w, from + (2 * sub + w) * kPiece);
+#pragma unroll
+            for (uint32_t p = 0; p < SM::kRowPieces; p++)
+              copy_scales<CTAS>(leader, to_rows + 4 * (w * SM::kRowPieces + p), from + (8 * (1 + p) + 2 * sub + w) * kPiece);
+          }
+          if constexpr (CTAS == 2)
+            mma_commit_pair(leader, bar(kSetFull + set), 1);
+          else
+            mma_commit(leader, bar(kSetFull + set));
+          if (sub + U == kScaleStages || it + U >= KT) {
+            if constexpr (CTAS == 2)
+              mma_commit_pair(leader, bar(kScEmpty + slot), 3);
+            else
+              mma_commit(leader, bar(kScEmpty + slot));
+            if (++slot == SL) slot = 0, slot_phase ^= 1;
+          }
+          set_phase ^= set, set ^= 1;
+        }
+      }
+    }
   } else if (warp == kMmaWarp) {
     if (rank == 0) {
+      constexpr uint32_t U = SM::kUnitStages;
       const uint32_t leader = elect_leader();
-      auto commit = [&](uint32_t i) {
+      auto commit = [&](uint32_t i, uint32_t ctas) {
         if constexpr (CTAS == 2)
-          mma_commit_pair(leader, bar(i), 3);
+          mma_commit_pair(leader, bar(i), ctas);
         else
           mma_commit(leader, bar(i));
       };
-      uint32_t s = 0, phase = 0, slot = 0, slot_phase = 0, set = 0, b = 0, acc_phase = 1;
-      // The barrier that says the MMAs of two units ago, which read the columns the next scales go to, are done: a stage's or a slot's "empty".
-      constexpr uint32_t kRing = SM::kUnitStages == 1 ? S : SL, kDone = SM::kUnitStages == 1 ? kEmpty : kScEmpty;
-      uint32_t old = kRing - 2, old_phase = 1;
+      uint32_t s = 0, phase = 0, set = 0, set_phase = 0, b = 0, acc_phase = 1;
       for (Item i = first; i.t < ntiles && ok; step(i)) {
         const Tile t = tile_at(i);
         const uint32_t n = (t.count + 15) & ~15u, acc = tmem_base + b * NT;
         const uint32_t d0 = mx4_instr_desc(n, CTAS * kRowsM, 0), d2 = mx4_instr_desc(n, CTAS * kRowsM, 2);
-        uint32_t ta = 0, tb = 0;
         ok = mbar_wait_warp(bar(kAccEmpty + b), acc_phase, abort, error);
         for (uint32_t it = 0; it < KT && ok; it++) {
-          const uint32_t sub = it % kScaleStages, in_unit = it % SM::kUnitStages;
-          if (sub == 0) ok = mbar_wait_warp(bar(kScFull + slot), slot_phase, abort, error);
-          if (in_unit == 0) {
-            if (ok) ok = mbar_wait_warp(bar(kDone + old), old_phase, abort, error);
-            if (!ok) break;
-            if (++old == kRing) old = 0, old_phase ^= 1;
-            tc_fence_after();
-            ta = tmem_base + 2 * NT + set * SM::kUnitCols, tb = ta + 8 * SM::kUnitStages, set ^= 1;
-            const uint32_t from = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes);
-            const uint32_t words = min(2 * SM::kUnitStages, (K - it * kStageK + 127) / 128);
-#pragma unroll
-            for (uint32_t w = 0; w < 2 * SM::kUnitStages; w++) {
-              if (w >= words) continue;
-              copy_scales<CTAS>(leader, ta + 4 * w, from + (2 * sub + w) * 512);
-#pragma unroll
-              for (uint32_t p = 0; p < SM::kRowPieces; p++)
-                copy_scales<CTAS>(leader, tb + 4 * (w * SM::kRowPieces + p), from + (8 + (2 * sub + w) * SM::kRowPieces + p) * 512);
-            }
-          }
+          const uint32_t in_unit = it % U, ta = tmem_base + 2 * NT + set * SM::kUnitCols, tb = ta + 8 * U;
+          if (in_unit == 0) ok = mbar_wait_warp(bar(kSetFull + set), set_phase, abort, error);
           if (ok) ok = mbar_wait_warp(bar(s), phase, abort, error);
           if (!ok) break;
           tc_fence_after();
@@ -346,15 +393,15 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
               mma_mx4<CTAS>(leader, acc, smem_desc_sw128(stage + 32 * k), smem_desc_sw128(rows + 32 * k), k % 2 ? d2 : d0, ta + 4 * w,
                             tb + 4 * SM::kRowPieces * w, (it | k) != 0);
           }
-          commit(kEmpty + s);
-          if (sub == kScaleStages - 1 || it == KT - 1) {
-            commit(kScEmpty + slot);
-            if (++slot == SL) slot = 0, slot_phase ^= 1;
-          }
+          commit(kEmpty + s, 3);
           if (++s == S) s = 0, phase ^= 1;
+          if (in_unit == U - 1 || it == KT - 1) {
+            commit(kSetEmpty + set, 1);
+            set_phase ^= set, set ^= 1;
+          }
         }
         if (!ok) break;
-        commit(kAccFull + b);
+        commit(kAccFull + b, 3);
         acc_phase ^= b, b ^= 1;
       }
     }
@@ -366,7 +413,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
       const Tile t = tile_at(i);
       const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT;
       ok = mbar_wait_warp(bar(kAccFull + b), phase, abort, error);
-      if constexpr (GU) ok = group_all(group, ok);
+      if constexpr (GU) ok = two_warps_all(2 * group + q % 2, ok);
       if (!ok) break;
       tc_fence_after();
       const uint32_t c0 = group * kChunk, dc = SM::kGroups * kChunk;
@@ -397,46 +444,43 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
           }
         }
       } else {
-        // Through shared memory, a row of the chunk its 64 gate and 64 up products, to threads of eight features each. A group has two chunks
-        // there: the next one's values come from tensor memory while this one is worked on, and are put where the one before was, which every
-        // thread of the group left before the barrier this chunk came by.
-        const uint32_t f = (tid % 8) * 8, hrow = mx_scale_row_bytes(F), at = t.row0 + f, r = (tid / 8) % 16;
-        auto room = [&](uint32_t n) { return (float *)(smem + SM::kStaging + (2 * group + n) * SM::kStagingBytes); };
-        uint32_t v[16];
-        auto put = [&](float *st) {
+        // Warps q and q + 2 hold gate and up of the same 32 features, a lane's one feature of 16 rows. They exchange: the first takes both of the
+        // chunk's first eight rows, the other of its last eight. A block of h is then a row's 32 lanes. The exchange has two places, by turns:
+        // when one is written again both warps have passed the barrier that came after its reading.
+        const uint32_t up = q / 2, at = t.row0 + 32 * (q % 2), hrow = mx_scale_row_bytes(F);
+        float *mine = (float *)(smem + SM::kStaging) + (4 * group + q) * 512 + lane, *theirs = (float *)(smem + SM::kStaging) + (4 * group + (q ^ 2)) * 512 + lane;
+        const uint32_t own = 8 * up;  // the first of the rows this warp keeps
+        uint32_t v[16], turn = 0;
+        if (c0 < t.count) tmem_ld16(from + c0, v);
+        for (uint32_t c = c0; c < t.count; c += dc, turn ^= 256) {
           tmem_ld_wait16(v);
+          float keep[8];
 #pragma unroll
-          for (uint32_t j = 0; j < 16; j++) st[j * SM::kStagingRow + 32 * q + lane] = __uint_as_float(v[j]);
-          group_sync(group);
-        };
-        if (c0 < t.count) tmem_ld16(from + c0, v), put(room(0));
-        uint32_t turn = 0;
-        for (uint32_t c = c0; c < t.count; c += dc, turn ^= 1) {
-          const bool more = c + dc < t.count;
-          if (more) tmem_ld16(from + c + dc, v);
-          const float *p = room(turn) + r * SM::kStagingRow + f;
-          float g[8], u[8], h[8];
-          load8(p, g), load8(p + 64, u);
-          uint32_t m = 0;
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            h[j] = swiglu_fast(g[j], u[j], a.limit);  // two significant bits of it stay
-            m = max(m, __float_as_uint(h[j]) & 0x7FFFFFFFu);
+          for (uint32_t j = 0; j < 8; j++) {
+            keep[j] = __uint_as_float(up ? v[8 + j] : v[j]);
+            mine[turn + 32 * j] = __uint_as_float(up ? v[j] : v[8 + j]);
           }
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          const uint32_t scale = mx_scale_of(m);
-          const float inv = mx_inverse(scale);
+          if (c + dc < t.count) tmem_ld16(from + c + dc, v);
+          two_warps_sync(2 * group + q % 2);
+          uint32_t scale_of = 0;  // lane j's: of the warp's row j
+          float h[8];
 #pragma unroll
-          for (int j = 0; j < 8; j++) h[j] *= inv;
-          if (c + r < t.count && at < F) {
-            const uint64_t row = t.start + c + r;
-            *(uint32_t *)(a.hc + row * (F / 2) + at / 2) = scale == 255 ? 0u : mx_codes8(h);
-            if (tid % 4 == 0) a.hs[row * hrow + at / kMxBlock] = (uint8_t)scale;
-            if (tid % 4 == 0 && at + kMxBlock == F)
-              for (uint32_t s = F / kMxBlock; s < hrow; s++) a.hs[row * hrow + s] = 0;
+          for (uint32_t j = 0; j < 8; j++) {
+            const float got = theirs[turn + 32 * j];
+            h[j] = up ? swiglu_fast(got, keep[j], a.limit) : swiglu_fast(keep[j], got, a.limit);  // two significant bits of it stay
+            const uint32_t scale = mx_scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(h[j]) & 0x7FFFFFFFu));
+            h[j] = scale == 255 ? 0.0f : h[j] * mx_inverse(scale);
+            if (lane == j) scale_of = scale;
           }
-          if (more) put(room(turn ^ 1));
+          // The warp's eight rows by eight features: lane j of each eight gets row j's codes of those features.
+          const uint32_t codes = transpose_codes(mx_codes8(h), lane), r = c + own + lane % 8;
+          if (r < t.count && at < F) *(uint32_t *)(a.hc + (uint64_t)(t.start + r) * (F / 2) + at / 2 + 4 * (lane / 8)) = codes;
+          if (lane < 8 && r < t.count && at < F) {
+            uint8_t *hs = a.hs + (uint64_t)(t.start + r) * hrow;
+            hs[at / kMxBlock] = (uint8_t)scale_of;
+            if (at + kMxBlock == F)
+              for (uint32_t z = F / kMxBlock; z < hrow; z++) hs[z] = 0;
+          }
         }
       }
       tc_fence_before();
