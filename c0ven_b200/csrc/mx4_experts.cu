@@ -329,13 +329,15 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     if (rank == 0) {
       constexpr uint32_t U = SM::kUnitStages;
       const uint32_t leader = elect_leader();
-      uint32_t slot = 0, slot_phase = 0, set = 0, set_phase = 1;
+      // The MMAs of two units ago, which read the set's columns, are done: a unit of one stage has that stage's "empty" say so.
+      uint32_t slot = 0, slot_phase = 0, set = 0, done = U == 1 ? S - 2 : 0, done_phase = 1;
       for (Item i = first; i.t < ntiles && ok; step(i)) {
         for (uint32_t it = 0; it < KT && ok; it += U) {
           const uint32_t sub = it % kScaleStages;
           if (sub == 0) ok = mbar_wait_warp(bar(kScFull + slot), slot_phase, abort, error);
-          if (ok) ok = mbar_wait_warp(bar(kSetEmpty + set), set_phase, abort, error);
+          if (ok) ok = mbar_wait_warp(bar((U == 1 ? kEmpty : kSetEmpty) + done), done_phase, abort, error);
           if (!ok) break;
+          if (++done == (U == 1 ? S : 2)) done = 0, done_phase ^= 1;
           tc_fence_after();
           const uint32_t to = tmem_base + 2 * NT + set * SM::kUnitCols, to_rows = to + 8 * U, from = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes);
           const uint32_t words = min(2 * U, (K - it * kStageK + 127) / 128);
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
               mma_commit(leader, bar(kScEmpty + slot));
             if (++slot == SL) slot = 0, slot_phase ^= 1;
           }
-          set_phase ^= set, set ^= 1;
+          set ^= 1;
         }
       }
     }
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
           commit(kEmpty + s, 3);
           if (++s == S) s = 0, phase ^= 1;
           if (in_unit == U - 1 || it == KT - 1) {
-            commit(kSetEmpty + set, 1);
+            if constexpr (U > 1) commit(kSetEmpty + set, 1);
             set_phase ^= set, set ^= 1;
           }
         }
