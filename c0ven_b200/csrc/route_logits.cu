@@ -1,15 +1,17 @@
 // Routing of a step's logits without a layer: softmax or sigmoid scores, a bias that chooses but does not weigh, groups of
 // experts, the top n_used, and the lists of expert order (moe_route_logits_device).
 //
-// A warp takes a row; lane l holds experts l, l + 32, .... Keys (score + bias) are first worked out in f32, with the fast exponential and
-// division, and the largest are taken off one at a time by a warp-wide maximum of order-preserving integers. That decides the row
-// when every two neighbours among the keys taken, and the last taken and the first left, are further apart than the f32 keys'
-// error (key_error): the order is then that of the exact keys. Else (two keys in some ten thousand rows of distinct logits) the warp
-// takes the row again with keys in f64. Without bias and groups the scores' order is the logits' own, which are exact. The weights come from
-// the chosen logits alone, by the accurate exponential, relative to the largest of them, so that they neither overflow nor
-// vanish together.
+// A warp takes a row; lane l holds experts l, l + 32, .... Keys (score + bias) are first worked out in f32 with the fast exponential and
+// reciprocal. The n_used-th largest of the lanes' own largest keys bounds the n_used-th largest key from below: the few keys not under it
+// (some 13 for 10 of 512) are gathered, one a lane, and each finds its rank by looking at the others. That decides the row when every two
+// neighbours among the first n_used + 1 are further apart than the f32 keys' error (key_error): the order is then that of the exact
+// keys. Else (a row in a few hundred for a bias and 512 experts), and where ties leave more than 32 keys, the warp takes the row again with
+// keys in f64. Without bias and groups the scores' order is the logits' own, which are exact. The weights come from the chosen
+// logits alone, by the accurate exponential, relative to the largest of them, so that they neither overflow nor vanish together.
 //
-// What bounds it: 32,768 rows of 512 f32 logits are 67 MB, 10 us of HBM; the selection's instructions take longer.
+// The lists: rows are counted by chunks of 32, an expert's rows of a chunk a bit each of a word in shared memory, so that a row's place
+// among them is a population count. A scan over the chunks' counts and a pass over the assignments follow; short steps are one CTA's.
+//
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -29,9 +31,11 @@ std::string &ops_error() {
 namespace {
 
 constexpr uint32_t kRouteMaxExperts = 512, kRouteMaxUsed = 16, kRouteMaxGroups = 32;
-constexpr uint32_t kRouteChunk = 32;     // rows whose experts are counted together
-constexpr uint32_t kRouteWarps = 8;      // of a CTA that takes a chunk
-constexpr uint32_t kRouteOneCta = 64;    // rows that one CTA of 32 warps routes and lists by itself
+constexpr uint32_t kRouteChunk = 32;       // rows whose experts are counted together
+constexpr uint32_t kRouteWarps = 8;        // of a CTA that takes a chunk, or a step of up to kRouteFewRows rows
+constexpr uint32_t kRouteFewRows = 16;
+constexpr uint32_t kRouteOneCta = 64;      // rows that one CTA of 32 warps routes and lists by itself
+constexpr uint32_t kRoutePlaces = 2048;    // assignments a CTA of the last pass takes
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
 struct RouteArgs {
@@ -56,24 +60,30 @@ __device__ __forceinline__ float logit_of(const RouteArgs &a, uint64_t t, uint32
 
 // f32 as an integer of the same order.
 __device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 is 0
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u); }
 
 // Arithmetic of the keys by type. f32: the fast forms, whose errors key_error bounds. f64: what decides.
-__device__ __forceinline__ float key_exp(float x) { return __expf(x); }
+__device__ __forceinline__ float key_exp(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
 __device__ __forceinline__ double key_exp(double x) { return exp(x); }
-__device__ __forceinline__ float key_div(float a, float b) { return __fdividef(a, b); }
-__device__ __forceinline__ double key_div(double a, double b) { return a / b; }
 template <class T>
 __device__ __forceinline__ T minus_inf() {
   return (T)(-INFINITY);
 }
-template <class T>
-__device__ __forceinline__ T sigmoid_key(T l) {
-  const T e = key_exp(l < 0 ? l : -l);  // at most 1
-  return key_div(l < 0 ? e : (T)1, (T)1 + e);
+__device__ __forceinline__ float sigmoid_key(float l) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + key_exp(-l)));
+  return r;
+}
+__device__ __forceinline__ double sigmoid_key(double l) {
+  const double e = exp(l < 0 ? l : -l);  // at most 1
+  return (l < 0 ? e : 1.0) / (1.0 + e);
 }
 // e^(l - largest), the largest's own 1 even where it is infinite.
 template <class T>
@@ -104,10 +114,11 @@ __device__ __forceinline__ void warp_best(double &v, uint32_t &e) {
   }
 }
 
-// What the f32 score of any of a row's experts may be off by. CUDA's documented bounds: the fast exponential of x is within 2 + 1.173 |x| ulp,
-// the fast division within 2. A sigmoid is made of e^-|l| <= 1 with |l| e^-|l| < 0.37: 2^-20 covers it. A softmax score e^-d / sum is
-// within (4 + d) 2^-22 of itself, the rounding of l - largest with it, so within 2^-20 of the largest score; and its sum, the mean of (4 + d) over
-// 512 experts by their e^-d being 8 at most, within 2^-19: 2^-18 of the largest score covers both.
+// What the f32 score of any of a row's experts may be off by. By PTX's bounds the approximate power of two is within 2^-22 of itself and the
+// reciprocal within 2^-23; the exponent x log2(e) is rounded twice, by 2^-23 |x| in all, and l - largest once more. A sigmoid s = 1 / (1 + e)
+// moves by s (1 - s) times e's relative error, (1 + |l|) 2^-22 at most, and s (1 - s) (1 + |l|) < 0.5: 2^-20 covers it, the reciprocal and the sum. A softmax
+// score e^-d / sum is within (4 + d) 2^-22 of itself, so within 2^-20 of the largest score; and its sum, the mean of (4 + d) over 512
+// experts by their e^-d being 8 at most, within 2^-19: 2^-18 of the largest score covers both.
 __device__ __forceinline__ float key_error(bool sigmoid, float largest_score) { return sigmoid ? 9.5367432e-7f : 3.8146973e-6f * largest_score; }
 
 // Groups, on the warp's E keys in shared memory: each ranked by the sum of its two best; the keys of all but the best a.used become
@@ -167,7 +178,7 @@ __device__ __noinline__ uint32_t choose_f64(const RouteArgs &a, uint64_t t, uint
   double sum = 0;
   for (uint32_t e = lane; e < a.E; e += 32) {
     const float l = logit_of<L>(a, t, e);
-    sk[e] = l == -INFINITY ? -INFINITY : a.sigmoid ? sigmoid_key<double>(l) : softmax_part<double>(l, largest);
+    sk[e] = l == -INFINITY ? -INFINITY : a.sigmoid ? sigmoid_key((double)l) : softmax_part<double>(l, largest);
     if (l > -INFINITY) sum += sk[e];
   }
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -198,74 +209,123 @@ __device__ __noinline__ uint32_t choose_f64(const RouteArgs &a, uint64_t t, uint
   return id;
 }
 
-// One row, by a warp, with E doubles of shared memory of its own. Lane j < k returns the j-th expert (kNone: none) after writing ids and w.
+// The bias of the lane's experts, as every row of the warp takes it: NaN is out like -infinity.
+template <int V>
+__device__ __forceinline__ void load_bias(const RouteArgs &a, uint32_t lane, float (&bias)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    bias[i] = a.bias && lane + 32 * i < a.E ? a.bias[lane + 32 * i] : 0.0f;
+    if (!(bias[i] > -INFINITY)) bias[i] = -INFINITY;
+  }
+}
+
+// One row, by a warp, with 32 V doubles of shared memory of its own. Lane j < k returns the j-th expert (kNone: none) after writing ids and w.
 template <class L, int V>
-__device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, uint32_t lane, double *sk) {
-  float key[V], largest = -INFINITY;  // the logits, then the keys
+__device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, uint32_t lane, const float (&bias)[V], double *sk) {
+  float key[V];  // the logits, then the keys
+  const L *row = (const L *)a.logits + t * a.stride;
 #pragma unroll
-  for (int i = 0; i < V; i++) key[i] = lane + 32 * i < a.E ? logit_of<L>(a, t, lane + 32 * i) : -INFINITY;
+  for (int i = 0; i < V; i++) key[i] = lane + 32 * i < a.E ? (float)row[lane + 32 * i] : -INFINITY;
+  const bool scored = a.bias || a.G > 1;
+  float largest = -INFINITY, score_max = 1.0f;
+  if (!a.sigmoid && (scored || !a.renorm)) {
 #pragma unroll
-  for (int i = 0; i < V; i++) largest = fmaxf(largest, key[i]);
-  largest = unordered(__reduce_max_sync(0xffffffffu, ordered(largest)));
-  uint32_t id = kNone;
-  float score_max = 1.0f;
-  if (largest > -INFINITY) {
-    const bool scored = a.bias || a.G > 1;
-    if (!a.sigmoid && (scored || !a.renorm)) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < V; i++) sum += key[i] == -INFINITY ? 0.0f : softmax_part<float>(key[i], largest);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      score_max = 1.0f / sum;
+    for (int i = 0; i < V; i++) {
+      if (!(key[i] > -INFINITY) || bias[i] == -INFINITY) key[i] = -INFINITY;
+      largest = fmaxf(largest, key[i]);
     }
-    const float err = key_error(a.sigmoid, score_max);
-    bool sure = true;
-    if (scored) {
-      float *fk = (float *)sk, top = 0.0f;
+    largest = unordered(__reduce_max_sync(0xffffffffu, ordered(largest)));
+    float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        const uint32_t e = lane + 32 * i;
-        if (key[i] == -INFINITY) {
-          if (a.G > 1 && e < a.E) fk[e] = -INFINITY;
-          continue;
-        }
-        float v = a.sigmoid ? sigmoid_key(key[i]) : softmax_part<float>(key[i], largest) * score_max;
-        if (a.bias) key[i] = v += a.bias[e];
-        if (a.G > 1) fk[e] = v, top = fmaxf(top, fabsf(v));
-      }
-      if (a.G > 1) {
-        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-        __syncwarp();
-        // Two sums of two keys, each with its own rounding, and theirs.
-        sure = keep_groups<float>(fk, a, lane, true, 4 * err + 4.7683716e-7f * top);
+    for (int i = 0; i < V; i++) sum += key[i] == -INFINITY ? 0.0f : softmax_part<float>(key[i], largest);
 #pragma unroll
-        for (int i = 0; i < V; i++)
-          if (lane + 32 * i < a.E && fk[lane + 32 * i] == -INFINITY) key[i] = -INFINITY;
-        __syncwarp();
-      }
-    }
-    // The largest keys, one at a time. With a bias no two neighbours among them, the first one left out with them, may lie within
-    // what their scores and their sums' roundings may be off by (rounding keeps an order, so neighbours are all that has to be looked at).
-    // Without one the keys are the logits, as they are.
-    const uint32_t rounds = a.k + (a.bias ? 1 : 0);
-    float last = 0.0f;
-    for (uint32_t j = 0; j < rounds && sure; j++) {
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    score_max = largest == -INFINITY ? 0.0f : 1.0f / sum;
+  }
+  const float err = key_error(a.sigmoid, score_max);
+  bool sure = true;
+  if (a.G > 1) {
+    float *fk = (float *)sk, top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const uint32_t e = lane + 32 * i;
       float v = -INFINITY;
-      uint32_t e = kNone;
-#pragma unroll
-      for (int i = 0; i < V; i++)
-        if (key[i] > v) v = key[i], e = lane + 32 * i;
-      warp_best(v, e);
-      if (e == kNone) break;  // no expert is left
-      if (a.bias && j > 0) sure = last - v > 2 * err + 2.3841858e-7f * fmaxf(fabsf(last), fabsf(v));
-      last = v;
-      if (lane == j && j < a.k) id = e;
-#pragma unroll
-      for (int i = 0; i < V; i++)
-        if (e == lane + 32 * i) key[i] = -INFINITY;
+      if (key[i] > -INFINITY) v = (a.sigmoid ? sigmoid_key(key[i]) : softmax_part<float>(key[i], largest) * score_max) + bias[i];
+      if (v > -INFINITY) top = fmaxf(top, fabsf(v));
+      if (e < a.E) fk[e] = v;
     }
-    if (!sure) id = choose_f64<L>(a, t, lane, largest, sk);
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    __syncwarp();
+    // Two sums of two keys, each with its own rounding, and theirs.
+    sure = keep_groups<float>(fk, a, lane, true, 4 * err + 4.7683716e-7f * top);
+    // Without a bias the order within the groups that stay is the logits' own.
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const float v = lane + 32 * i < a.E ? fk[lane + 32 * i] : -INFINITY;
+      key[i] = v == -INFINITY ? -INFINITY : a.bias ? v : key[i];
+    }
+    __syncwarp();
+  } else if (a.bias) {
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      key[i] = key[i] > -INFINITY ? (a.sigmoid ? sigmoid_key(key[i]) : softmax_part<float>(key[i], largest) * score_max) + bias[i] : -INFINITY;
+  }
+  // The need-th largest of the lanes' largest keys: need keys at least are not under it.
+  const uint32_t need = a.bias ? a.k + 1 : a.k;  // with a bias the first key left out is looked at too
+  float best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; i++) best = fmaxf(best, key[i]);  // NaN loses
+  uint32_t rank = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < 32; j++) {
+    const float o = __shfl_sync(0xffffffffu, best, j);
+    rank += o > best || (o == best && j < lane) ? 1u : 0u;
+  }
+  const uint32_t at = __ballot_sync(0xffffffffu, rank == need - 1);
+  const float least = __shfl_sync(0xffffffffu, best, __ffs(at) - 1);
+  // The keys from there on, a lane each.
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < V; i++) mine += key[i] >= least && key[i] > -INFINITY ? 1u : 0u;
+  uint32_t upto = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= (uint32_t)off) upto += o;
+  }
+  const uint32_t n = __shfl_sync(0xffffffffu, upto, 31);
+  uint32_t id = kNone;
+  if (n > 32) sure = false;
+  if (sure && n > 0) {
+    float2 *found = (float2 *)sk;  // (key, expert)
+    uint32_t put = upto - mine;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (key[i] >= least && key[i] > -INFINITY) found[put++] = make_float2(key[i], __uint_as_float(lane + 32 * i));
+    __syncwarp();
+    const float2 own = found[min(lane, n - 1)];
+    rank = 0;
+    for (uint32_t j = 0; j < n; j++) {
+      const float2 o = found[j];
+      rank += o.x > own.x || (o.x == own.x && __float_as_uint(o.y) < __float_as_uint(own.y)) ? 1u : 0u;
+    }
+    __syncwarp();
+    if (lane < n) found[rank] = own;
+    __syncwarp();
+    const float2 here = found[min(lane, n - 1)], next = found[min(lane + 1, n - 1)];
+    if (lane < a.k && lane < n) id = __float_as_uint(here.y);
+    __syncwarp();
+    // With a bias no two neighbours may lie within what their scores and their sums' roundings may be off by (rounding keeps an order, so
+    // neighbours are all that has to be looked at). Without one the keys are the logits, as they are.
+    if (a.bias) {
+      const bool open = lane < a.k && lane + 1 < n && !(here.x - next.x > 2 * err + 2.3841858e-7f * fmaxf(fabsf(here.x), fabsf(next.x)));
+      sure = !__any_sync(0xffffffffu, open);
+    }
+  }
+  if (!sure) {
+    float l = -INFINITY;
+    for (uint32_t e = lane; e < a.E; e += 32) l = fmaxf(l, logit_of<L>(a, t, e));
+    id = choose_f64<L>(a, t, lane, unordered(__reduce_max_sync(0xffffffffu, ordered(l))), sk);
   }
   // The weights: e^(l - c) and its like for the chosen, c the largest of them, so that a row's never all vanish.
   float s = 0.0f;
@@ -295,138 +355,136 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
   return id;
 }
 
-// A chunk of rows by a CTA of kRouteWarps warps; with lists, how many of its assignments each expert got.
+// A chunk of rows by a CTA. With lists, each expert's count of the chunk's rows, and every assignment's place among its expert's rows there.
 template <class L, int V>
 __global__ void __launch_bounds__(32 * kRouteWarps) k_route_rows(const RouteArgs a) {
   __shared__ double sk[kRouteWarps][32 * V];
-  __shared__ uint32_t hist[kRouteMaxExperts];
+  __shared__ uint32_t rows_of[32 * V];  // a bit a row
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (a.work) {
-    for (uint32_t i = threadIdx.x; i < a.E; i += blockDim.x) hist[i] = 0;
+    for (uint32_t i = threadIdx.x; i < a.E; i += 32 * kRouteWarps) rows_of[i] = 0;
     __syncthreads();
   }
+  float bias[V];
+  load_bias(a, lane, bias);
   const uint32_t t0 = blockIdx.x * kRouteChunk, t1 = min(a.T, t0 + kRouteChunk);
   for (uint32_t t = t0 + warp; t < t1; t += kRouteWarps) {
-    const uint32_t id = route_row<L, V>(a, t, lane, sk[warp]);
-    if (a.work && id != kNone) atomicAdd(&hist[id], 1u);
+    const uint32_t id = route_row<L, V>(a, t, lane, bias, sk[warp]);
+    if (a.work && id != kNone) atomicOr(&rows_of[id], 1u << (t - t0));
   }
-  if (a.work) {
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < a.E; i += blockDim.x) a.work[(uint64_t)blockIdx.x * a.E + i] = hist[i];
+  if (!a.work) return;
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < a.E; i += 32 * kRouteWarps) a.work[(uint64_t)blockIdx.x * a.E + i] = __popc(rows_of[i]);
+  const uint64_t a0 = (uint64_t)t0 * a.k;
+  for (uint32_t i = threadIdx.x; i < (t1 - t0) * a.k; i += 32 * kRouteWarps) {
+    const uint32_t e = (uint32_t)a.ids[a0 + i];  // this CTA's own writes, before the barrier
+    a.inv[a0 + i] = e < a.E ? (int32_t)__popc(rows_of[e] & ((1u << i / a.k) - 1)) : -1;
   }
 }
 
 // The chunks' counts become each expert's rows before the chunk; the totals come after the last chunk's. A CTA takes 32 experts, a
-// warp a 32nd of the chunks.
+// warp a 32nd of the chunks, sixteen counts on their way at once.
 __global__ void __launch_bounds__(1024) k_route_scan(uint32_t *work, uint32_t chunks, uint32_t E) {
   __shared__ uint32_t part[32][33];
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, e = blockIdx.x * 32 + lane;
-  const uint32_t per = (chunks + 31) / 32, c0 = min(chunks, warp * per), c1 = min(chunks, c0 + per);
+  const uint32_t per = (chunks + 31) / 32, c0 = min(chunks, warp * per), c1 = e < E ? min(chunks, c0 + per) : c0;
+  uint32_t *at = work + e, v[16];
   uint32_t run = 0;
-  if (e < E)
-    for (uint32_t c = c0; c < c1; c++) run += work[(uint64_t)c * E + e];
+  for (uint32_t c = c0; c < c1; c += 16) {
+#pragma unroll
+    for (uint32_t j = 0; j < 16; j++) v[j] = c + j < c1 ? at[(uint64_t)(c + j) * E] : 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 16; j++) run += v[j];
+  }
   part[warp][lane] = run;
   __syncthreads();
-  uint32_t before = 0;
-  for (uint32_t i = 0; i < warp; i++) before += part[i][lane];
-  if (e >= E) return;
-  run = before;
-  for (uint32_t c = c0; c < c1; c++) {
-    const uint32_t n = work[(uint64_t)c * E + e];
-    work[(uint64_t)c * E + e] = run;
-    run += n;
+  run = 0;
+  for (uint32_t i = 0; i < warp; i++) run += part[i][lane];
+  for (uint32_t c = c0; c < c1; c += 16) {
+#pragma unroll
+    for (uint32_t j = 0; j < 16; j++) v[j] = c + j < c1 ? at[(uint64_t)(c + j) * E] : 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 16; j++) {
+      if (c + j < c1) at[(uint64_t)(c + j) * E] = run;
+      run += v[j];
+    }
   }
-  if (warp == 31) work[(uint64_t)chunks * E + e] = run;
+  if (warp == 31 && e < E) at[(uint64_t)chunks * E] = run;
 }
 
-// Exclusive sums of E <= 512 counts (thread e's in n) over a block of 512 threads or more; s: 16 words.
-__device__ __forceinline__ uint32_t exclusive_sum(uint32_t n, uint32_t *s) {
+// Exclusive sums of E <= 512 counts, thread i's of experts 2 i and 2 i + 1, by a block of W >= 8 warps; s: 8 words.
+__device__ __forceinline__ uint32_t exclusive_sum(uint32_t pair, uint32_t *s) {
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  uint32_t v = n;
+  uint32_t v = pair;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const uint32_t o = __shfl_up_sync(0xffffffffu, v, off);
     if (lane >= (uint32_t)off) v += o;
   }
-  if (lane == 31 && warp < 16) s[warp] = v;
+  if (lane == 31 && warp < 8) s[warp] = v;
   __syncthreads();
   uint32_t before = 0;
-  for (uint32_t i = 0; i < min(warp, 16u); i++) before += s[i];
-  return before + v - n;
+  for (uint32_t i = 0; i < min(warp, 8u); i++) before += s[i];
+  return before + v - pair;
 }
 
-// Each assignment's row: its expert's first, the expert's rows of earlier chunks, and those before it in its own chunk. A thread an
-// assignment (512 at most); CTA 0 leaves the offsets.
-__global__ void __launch_bounds__(512) k_route_fill(const RouteArgs a, uint32_t chunks) {
-  __shared__ uint32_t s_scan[16];
-  __shared__ uint32_t s_first[kRouteMaxExperts];
-  __shared__ uint16_t s_cnt[16][kRouteMaxExperts];
+// Each assignment's row: its expert's first, the expert's rows of earlier chunks, and its place in its own chunk, which inv holds.
+// CTA 0 leaves the offsets.
+__global__ void __launch_bounds__(256) k_route_places(const RouteArgs a, uint32_t chunks) {
+  __shared__ uint32_t s_scan[8], s_first[kRouteMaxExperts];
   dependents_may_launch(), wait_for_predecessors();
-  const uint32_t i = threadIdx.x, warp = i / 32, lane = i % 32;
-  const uint32_t n = i < a.E ? a.work[(uint64_t)chunks * a.E + i] : 0;
-  const uint32_t first = exclusive_sum(n, s_scan);
+  const uint32_t e = 2 * threadIdx.x;
+  const uint32_t *total = a.work + (uint64_t)chunks * a.E;
+  const uint32_t n0 = e < a.E ? total[e] : 0, n1 = e + 1 < a.E ? total[e + 1] : 0, first = exclusive_sum(n0 + n1, s_scan);
+  s_first[e] = first, s_first[e + 1] = first + n0;
   if (blockIdx.x == 0) {
-    if (i < a.E) a.offsets[i] = (int32_t)first;
-    if (i == a.E - 1) a.offsets[a.E] = (int32_t)(first + n);
-  }
-  for (uint32_t j = i; j < 16 * kRouteMaxExperts / 2; j += 512) ((uint32_t *)s_cnt)[j] = 0;
-  if (i < a.E) s_first[i] = first + a.work[(uint64_t)blockIdx.x * a.E + i];
-  const uint64_t a0 = (uint64_t)blockIdx.x * kRouteChunk * a.k;
-  const uint32_t m = (min(a.T, (blockIdx.x + 1) * kRouteChunk) - blockIdx.x * kRouteChunk) * a.k;
-  const uint32_t e = i < m ? (uint32_t)a.ids[a0 + i] : kNone;
-  const bool valid = e < a.E;
-  const uint32_t same = __match_any_sync(0xffffffffu, valid ? e : kRouteMaxExperts + lane), before = __popc(same & ((1u << lane) - 1));
-  __syncthreads();
-  if (valid && before == 0) s_cnt[warp][e] = (uint16_t)__popc(same);
-  __syncthreads();
-  if (i < a.E) {
-    uint32_t run = 0;
-    for (uint32_t w = 0; w < 16; w++) {
-      const uint32_t c = s_cnt[w][i];
-      s_cnt[w][i] = (uint16_t)run;
-      run += c;
-    }
+    if (e < a.E) a.offsets[e] = (int32_t)first;
+    if (e + 1 < a.E) a.offsets[e + 1] = (int32_t)(first + n0);
+    if (e == a.E - 1 || e + 1 == a.E - 1) a.offsets[a.E] = (int32_t)(first + n0 + n1);
   }
   __syncthreads();
-  if (i < m) a.inv[a0 + i] = valid ? (int32_t)(s_first[e] + s_cnt[warp][e] + before) : -1;
+  const uint64_t A = (uint64_t)a.T * a.k, a0 = (uint64_t)blockIdx.x * kRoutePlaces;
+  const uint32_t per = kRouteChunk * a.k;  // assignments of a chunk
+#pragma unroll 4
+  for (uint32_t j = 0; j < kRoutePlaces / 256; j++) {
+    const uint64_t i = a0 + j * 256 + threadIdx.x;
+    if (i >= A) break;
+    const uint32_t id = (uint32_t)a.ids[i];
+    if (id < a.E) a.inv[i] += (int32_t)(s_first[id] + a.work[(i / per) * a.E + id]);
+  }
 }
 
-// A short step by one CTA of 32 warps: rows, counts, offsets and places in one launch. Dynamic shared memory: 32 V doubles a warp, or
-// the warps' counts.
-template <class L, int V>
-__global__ void __launch_bounds__(1024) k_route_short(const RouteArgs a) {
+// A short step by one CTA of W warps: rows, counts, offsets and places in one launch. Dynamic shared memory: 32 V doubles a warp.
+template <class L, int V, int W>
+__global__ void __launch_bounds__(32 * W) k_route_short(const RouteArgs a) {
   extern __shared__ double s_dyn[];
-  __shared__ uint32_t s_ids[kRouteOneCta * kRouteMaxUsed], s_scan[16], s_first[kRouteMaxExperts];
+  __shared__ uint32_t s_ids[kRouteOneCta * kRouteMaxUsed], s_scan[8], s_first[kRouteMaxExperts], rows_of[2][kRouteMaxExperts];  // a bit a row, 64 in all
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t i = threadIdx.x, warp = i / 32, lane = i % 32;
-  for (uint32_t t = warp; t < a.T; t += 32) {
-    const uint32_t id = route_row<L, V>(a, t, lane, s_dyn + warp * 32 * V);
+  for (uint32_t j = i; j < kRouteMaxExperts; j += 32 * W) rows_of[0][j] = rows_of[1][j] = 0;
+  float bias[V];
+  load_bias(a, lane, bias);
+  __syncthreads();
+  for (uint32_t t = warp; t < a.T; t += W) {
+    const uint32_t id = route_row<L, V>(a, t, lane, bias, s_dyn + warp * 32 * V);
     if (lane < a.k) s_ids[t * a.k + lane] = id;
+    if (id != kNone) atomicOr(&rows_of[t / 32][id], 1u << (t % 32));
   }
   if (!a.offsets) return;
   __syncthreads();
-  uint16_t *s_cnt = (uint16_t *)s_dyn;  // [32][E]
-  for (uint32_t j = i; j < 32 * a.E; j += 1024) s_cnt[j] = 0;
-  const uint32_t m = a.T * a.k, e = i < m ? s_ids[i] : kNone;
-  const bool valid = e < a.E;
-  const uint32_t same = __match_any_sync(0xffffffffu, valid ? e : kRouteMaxExperts + lane), before = __popc(same & ((1u << lane) - 1));
+  const uint32_t e = 2 * i;
+  auto count = [&](uint32_t x) { return x < a.E ? (uint32_t)(__popc(rows_of[0][x]) + __popc(rows_of[1][x])) : 0u; };
+  const uint32_t n0 = count(e), n1 = count(e + 1), first = exclusive_sum(n0 + n1, s_scan);
+  if (e < a.E) a.offsets[e] = (int32_t)first, s_first[e] = first;
+  if (e + 1 < a.E) a.offsets[e + 1] = (int32_t)(first + n0), s_first[e + 1] = first + n0;
+  if (e == a.E - 1 || e + 1 == a.E - 1) a.offsets[a.E] = (int32_t)(first + n0 + n1);
   __syncthreads();
-  if (valid && before == 0) s_cnt[warp * a.E + e] = (uint16_t)__popc(same);
-  __syncthreads();
-  uint32_t run = 0;
-  if (i < a.E)
-    for (uint32_t w = 0; w < 32; w++) {
-      const uint32_t c = s_cnt[w * a.E + i];
-      s_cnt[w * a.E + i] = (uint16_t)run;
-      run += c;
-    }
-  const uint32_t first = exclusive_sum(run, s_scan);
-  if (i < a.E) a.offsets[i] = (int32_t)first, s_first[i] = first;
-  if (i == a.E - 1) a.offsets[a.E] = (int32_t)(first + run);
-  __syncthreads();
-  if (i < m) a.inv[i] = valid ? (int32_t)(s_first[e] + s_cnt[warp * a.E + e] + before) : -1;
+  for (uint32_t j = i; j < a.T * a.k; j += 32 * W) {
+    const uint32_t id = s_ids[j], t = j / a.k, below = (1u << (t % 32)) - 1;
+    a.inv[j] = id < a.E ? (int32_t)(s_first[id] + (t < 32 ? __popc(rows_of[0][id] & below) : __popc(rows_of[0][id]) + __popc(rows_of[1][id] & below))) : -1;
+  }
 }
 
 __global__ void __launch_bounds__(512) k_route_empty(int32_t *offsets, uint32_t n) {
@@ -434,20 +492,23 @@ __global__ void __launch_bounds__(512) k_route_empty(int32_t *offsets, uint32_t 
   for (uint32_t i = threadIdx.x; i < n; i += 512) offsets[i] = 0;
 }
 
+template <class L, int V, int W>
+void launch_short(const RouteArgs &a, int device, cudaStream_t st) {
+  constexpr size_t smem = W * 32 * V * sizeof(double);
+  static std::atomic<uint32_t> done{0};
+  CUDA_OK(ensure_dynamic_smem(k_route_short<L, V, W>, smem, done, device));
+  CUDA_OK(launch_kernel(true, k_route_short<L, V, W>, dim3(1), dim3(32 * W), smem, st, a));
+}
+
 template <class L, int V>
 void launch_rows(const RouteArgs &a, int device, cudaStream_t st) {
-  if (a.T <= kRouteOneCta) {
-    constexpr size_t smem = 32 * 32 * V * sizeof(double);  // 32 warps' keys; the counts, 64 V bytes a warp, lie in it too
-    static std::atomic<uint32_t> done{0};
-    CUDA_OK(ensure_dynamic_smem(k_route_short<L, V>, smem, done, device));
-    CUDA_OK(launch_kernel(true, k_route_short<L, V>, dim3(1), dim3(1024), smem, st, a));
-    return;
-  }
+  if (a.T <= kRouteFewRows) return launch_short<L, V, kRouteWarps>(a, device, st);
+  if (a.T <= kRouteOneCta) return launch_short<L, V, 32>(a, device, st);
   const uint32_t chunks = (a.T + kRouteChunk - 1) / kRouteChunk;
   CUDA_OK(launch_kernel(true, k_route_rows<L, V>, dim3(chunks), dim3(32 * kRouteWarps), 0, st, a));
   if (!a.offsets) return;
   CUDA_OK(launch_kernel(true, k_route_scan, dim3((a.E + 31) / 32), dim3(1024), 0, st, a.work, chunks, a.E));
-  CUDA_OK(launch_kernel(true, k_route_fill, dim3(chunks), dim3(512), 0, st, a, chunks));
+  CUDA_OK(launch_kernel(true, k_route_places, dim3((uint32_t)(((uint64_t)a.T * a.k + kRoutePlaces - 1) / kRoutePlaces)), dim3(256), 0, st, a, chunks));
 }
 
 template <class L>
