@@ -105,6 +105,7 @@ struct Mx4Form {
   static constexpr uint32_t kTileExperts = kTables + 2 * (kMaxExperts + 1) * 4;
   static constexpr uint32_t kBytes = kTileExperts + 2 * kTileTable + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
+  static_assert(2 * kThreads > kMaxExperts + 1, "two experts a thread");
   // Tensor memory: two accumulators, then two sets of columns for scales, of kScaleStages stages where they have the room, else of one.
   static constexpr uint32_t kStageCols = 2 * 4 * (1 + kRowPieces);
   static constexpr uint32_t kUnitStages = 2 * NT + 2 * kScaleStages * kStageCols <= 512 ? kScaleStages : 1;
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   volatile uint32_t *abort = tmem_slot + 1;
   uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *first_tile = first_row + kMaxExperts + 1;  // [E + 1] each
   uint16_t *tile_expert = (uint16_t *)(smem + SM::kTileExperts);
+  uint32_t *warp_part = (uint32_t *)(smem + SM::kScales);  // before the scales come
   uint32_t *error = &g_gave_up;
 
   if (tid == 0) {
@@ -163,39 +165,44 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
       tmem_alloc(smem_u32(tmem_slot), SM::kCols);
   }
   dependents_may_launch(), wait_for_predecessors();
-  // The experts' first rows and tiles by one warp, 16 experts a lane. Offsets are held to 0 .. R, and to rise: each to the largest before it.
-  if (warp == kEpilogueWarp) {
-    const uint32_t per = (a.E + 32) / 32, e0 = min(a.E + 1, lane * per), e1 = min(a.E + 1, e0 + per);
-    uint32_t top = 0;
-    for (uint32_t e = e0; e < e1; e++) {
-      top = max(top, a.offsets ? min((uint32_t)max(a.offsets[e], 0), a.R) : e ? a.R : 0u);
-      first_row[e] = top;
-    }
+  // The experts' first rows and first tiles, E + 1 <= 513 entries, two a thread. Offsets are held to 0 .. R, and to rise: each to the largest
+  // before it.
+  {
+    const uint32_t e = 2 * tid;
+    auto row_of = [&](uint32_t x) { return x > a.E ? 0u : a.offsets ? min((uint32_t)max(a.offsets[x], 0), a.R) : x ? a.R : 0u; };
+    uint32_t r0 = row_of(e), r1 = row_of(e + 1);
+    r1 = max(r0, r1);
+    uint32_t top = r1;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const uint32_t o = __shfl_up_sync(0xffffffffu, top, off);
       if (lane >= (uint32_t)off) top = max(top, o);
     }
-    top = __shfl_up_sync(0xffffffffu, top, 1);  // the largest of the lanes before
-    if (lane > 0)
-      for (uint32_t e = e0; e < e1; e++) first_row[e] = max(first_row[e], top);
-    __syncwarp();
-    auto tiles_of = [&](uint32_t e) { return e < a.E ? (first_row[e + 1] - first_row[e] + NT - 1) / NT : 0u; };
-    uint32_t sum = 0;
-    for (uint32_t e = e0; e < e1; e++) sum += tiles_of(e);
-    uint32_t before = sum;
+    if (lane == 31) warp_part[warp] = top;
+    top = __shfl_up_sync(0xffffffffu, top, 1);
+    if (lane == 0) top = 0;
+    __syncthreads();
+    for (uint32_t w = 0; w < min(warp, 9u); w++) top = max(top, warp_part[w]);
+    r0 = max(r0, top), r1 = max(r1, top);
+    if (e <= a.E) first_row[e] = r0;
+    if (e < a.E) first_row[e + 1] = r1;
+    __syncthreads();
+    const uint32_t r2 = e + 2 <= a.E ? first_row[e + 2] : r1;
+    const uint32_t t0 = e < a.E ? (r1 - r0 + NT - 1) / NT : 0, t1 = e + 1 < a.E ? (r2 - r1 + NT - 1) / NT : 0;
+    uint32_t sum = t0 + t1;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, before, off);
-      if (lane >= (uint32_t)off) before += o;
+      const uint32_t o = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= (uint32_t)off) sum += o;
     }
-    before -= sum;
-    for (uint32_t e = e0; e < e1; e++) {
-      first_tile[e] = before;
-      before += tiles_of(e);
-    }
+    if (lane == 31) warp_part[warp] = sum;
+    __syncthreads();
+    sum -= t0 + t1;
+    for (uint32_t w = 0; w < min(warp, 9u); w++) sum += warp_part[w];
+    if (e <= a.E) first_tile[e] = sum;
+    if (e < a.E) first_tile[e + 1] = sum + t0;
+    __syncthreads();
   }
-  __syncthreads();
   const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK, ntiles = first_tile[a.E];
   auto expert_at = [&](uint32_t t) {  // the last expert whose first tile is at most t
     uint32_t lo = 0, hi = a.E;
