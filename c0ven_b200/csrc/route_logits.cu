@@ -2,11 +2,11 @@
 // experts, the top n_used, and the lists of expert order (moe_route_logits_device).
 //
 // A warp takes a row; lane l holds experts l, l + 32, .... Keys (score + bias) are first worked out in f32 with the fast exponential and
-// reciprocal. The n_used-th largest of the lanes' own largest keys bounds the n_used-th largest key from below: the few keys not under it
-// (some 13 for 10 of 512) are gathered, one a lane, and each finds its rank by looking at the others. That decides the row when every two
+// reciprocal. A bound that n_used of the lanes' own largest keys reach, found by halving between the least and the largest of them, is one that
+// n_used keys reach: the few keys not under it (some 18 for 10 of 512) are gathered, one a lane, and each finds its rank by looking at the others. That decides the row when every two
 // neighbours among the first n_used + 1 are further apart than the f32 keys' error (key_error): the order is then that of the exact
-// keys. Else (a row in a few hundred for a bias and 512 experts), and where ties leave more than 32 keys, the warp takes the row again with
-// keys in f64. Without bias and groups the scores' order is the logits' own, which are exact. The weights come from the chosen
+// keys. Else (a row in some 600 for a bias and 512 experts) the candidates' own keys are worked out in f64, or, where keys that are no
+// candidates may come near them, where groups lie that near or ties leave more than 32 keys, the whole row's. Without bias and groups the scores' order is the logits' own, which are exact. The weights come from the chosen
 // logits alone, by the accurate exponential, relative to the largest of them, so that they neither overflow nor vanish together.
 //
 // The lists: rows are counted by chunks of 32, an expert's rows of a chunk a bit each of a word in shared memory, so that a row's place
@@ -35,7 +35,7 @@ constexpr uint32_t kRouteChunk = 32;       // rows whose experts are counted tog
 constexpr uint32_t kRouteWarps = 8;        // of a CTA that takes a chunk, or a step of up to kRouteFewRows rows
 constexpr uint32_t kRouteFewRows = 16;
 constexpr uint32_t kRouteOneCta = 64;      // rows that one CTA of 32 warps routes and lists by itself
-constexpr uint32_t kRoutePlaces = 2048;    // assignments a CTA of the last pass takes
+constexpr uint32_t kRoutePlaces = 512;     // assignments a CTA of the last pass takes
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
 struct RouteArgs {
@@ -209,23 +209,32 @@ __device__ __noinline__ uint32_t choose_f64(const RouteArgs &a, uint64_t t, uint
   return id;
 }
 
+// Whether the lane's i-th expert exists: the launch's V is the least that holds E, so the first half's always do.
+template <int V>
+__device__ __forceinline__ bool exists(const RouteArgs &a, uint32_t lane, int i) {
+  return (V > 1 && i < V / 2) || lane + 32 * i < a.E;
+}
 // The bias of the lane's experts, as every row of the warp takes it: NaN is out like -infinity.
 template <int V>
 __device__ __forceinline__ void load_bias(const RouteArgs &a, uint32_t lane, float (&bias)[V]) {
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    bias[i] = a.bias && lane + 32 * i < a.E ? a.bias[lane + 32 * i] : 0.0f;
+    bias[i] = a.bias && exists<V>(a, lane, i) ? a.bias[lane + 32 * i] : 0.0f;
     if (!(bias[i] > -INFINITY)) bias[i] = -INFINITY;
   }
 }
 
-// One row, by a warp, with 32 V doubles of shared memory of its own. Lane j < k returns the j-th expert (kNone: none) after writing ids and w.
+// Doubles of shared memory a warp has for a row: a key an expert, and room for 32 candidates and one place behind them.
+template <int V>
+constexpr uint32_t kRouteScratch = V == 1 ? 34 : 32 * V;
+
+// One row, by a warp, with kRouteScratch<V> doubles of shared memory of its own. Lane j < k returns the j-th expert (kNone: none) after writing ids and w.
 template <class L, int V>
 __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, uint32_t lane, const float (&bias)[V], double *sk) {
   float key[V];  // the logits, then the keys
-  const L *row = (const L *)a.logits + t * a.stride;
+  const L *row = (const L *)a.logits + t * a.stride + lane;
 #pragma unroll
-  for (int i = 0; i < V; i++) key[i] = lane + 32 * i < a.E ? (float)row[lane + 32 * i] : -INFINITY;
+  for (int i = 0; i < V; i++) key[i] = exists<V>(a, lane, i) ? (float)row[32 * i] : -INFINITY;
   const bool scored = a.bias || a.G > 1;
   float largest = -INFINITY, score_max = 1.0f;
   if (!a.sigmoid && (scored || !a.renorm)) {
@@ -270,23 +279,30 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
     for (int i = 0; i < V; i++)
       key[i] = key[i] > -INFINITY ? (a.sigmoid ? sigmoid_key(key[i]) : softmax_part<float>(key[i], largest) * score_max) + bias[i] : -INFINITY;
   }
-  // The need-th largest of the lanes' largest keys: need keys at least are not under it.
+  // least: need keys at least are not under it. It begins as the least of the lanes' largest keys, where need of them are finite, and rises to
+  // the middle between it and the largest as long as need of them reach that; ten steps at most, fewer once few more than need do.
   const uint32_t need = a.bias ? a.k + 1 : a.k;  // with a bias the first key left out is looked at too
   float best = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; i++) best = fmaxf(best, key[i]);  // NaN loses
-  uint32_t rank = 0;
-#pragma unroll
-  for (uint32_t j = 0; j < 32; j++) {
-    const float o = __shfl_sync(0xffffffffu, best, j);
-    rank += o > best || (o == best && j < lane) ? 1u : 0u;
+  constexpr float kLowest = -3.402823466e38f;
+  float least = kLowest, most = unordered(__reduce_max_sync(0xffffffffu, ordered(best)));
+  uint32_t reach = __popc(__ballot_sync(0xffffffffu, best >= kLowest));
+  if (reach > need) {
+    least = unordered(__reduce_min_sync(0xffffffffu, best >= kLowest ? ordered(best) : 0xFFFFFFFFu));
+    for (int step = 0; step < 10 && reach > need + 2; step++) {
+      const float mid = 0.5f * least + 0.5f * most;
+      const uint32_t c = __popc(__ballot_sync(0xffffffffu, best >= mid));
+      if (c >= need)
+        least = mid, reach = c;
+      else
+        most = mid;
+    }
   }
-  const uint32_t at = __ballot_sync(0xffffffffu, rank == need - 1);
-  const float least = __shfl_sync(0xffffffffu, best, __ffs(at) - 1);
   // The keys from there on, a lane each.
   uint32_t mine = 0;
 #pragma unroll
-  for (int i = 0; i < V; i++) mine += key[i] >= least && key[i] > -INFINITY ? 1u : 0u;
+  for (int i = 0; i < V; i++) mine += key[i] >= least ? 1u : 0u;
   uint32_t upto = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -297,29 +313,59 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
   uint32_t id = kNone;
   if (n > 32) sure = false;
   if (sure && n > 0) {
-    float2 *found = (float2 *)sk;  // (key, expert)
+    // (key, expert) of each, all keys written without a branch, those that are none into a place behind; then as integers that order as they do.
+    float2 *found = (float2 *)sk;
     uint32_t put = upto - mine;
 #pragma unroll
-    for (int i = 0; i < V; i++)
-      if (key[i] >= least && key[i] > -INFINITY) found[put++] = make_float2(key[i], __uint_as_float(lane + 32 * i));
-    __syncwarp();
-    const float2 own = found[min(lane, n - 1)];
-    rank = 0;
-    for (uint32_t j = 0; j < n; j++) {
-      const float2 o = found[j];
-      rank += o.x > own.x || (o.x == own.x && __float_as_uint(o.y) < __float_as_uint(own.y)) ? 1u : 0u;
+    for (int i = 0; i < V; i++) {
+      const bool in = key[i] >= least;
+      found[in ? put : 32u] = make_float2(key[i], __uint_as_float(lane + 32 * i));
+      put += in ? 1u : 0u;
     }
     __syncwarp();
-    if (lane < n) found[rank] = own;
+    const float2 got = found[lane];
+    uint64_t own = lane < n ? (uint64_t)ordered(got.x) << 32 | ~__float_as_uint(got.y) : 0;
+    uint64_t *order = (uint64_t *)sk;
     __syncwarp();
-    const float2 here = found[min(lane, n - 1)], next = found[min(lane + 1, n - 1)];
-    if (lane < a.k && lane < n) id = __float_as_uint(here.y);
+    order[lane] = own;
     __syncwarp();
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < n; j += 4) {
+      const ulonglong2 o = *(const ulonglong2 *)(order + j), q = *(const ulonglong2 *)(order + j + 2);
+      rank += (o.x > own ? 1u : 0u) + (o.y > own ? 1u : 0u) + (q.x > own ? 1u : 0u) + (q.y > own ? 1u : 0u);
+    }
+    __syncwarp();
+    if (lane < n) order[rank] = own;
+    __syncwarp();
+    own = order[lane];
+    const uint64_t after = order[min(lane + 1, 31u)];
+    __syncwarp();
+    if (lane < a.k && lane < n) id = ~(uint32_t)own;
     // With a bias no two neighbours may lie within what their scores and their sums' roundings may be off by (rounding keeps an order, so
     // neighbours are all that has to be looked at). Without one the keys are the logits, as they are.
     if (a.bias) {
-      const bool open = lane < a.k && lane + 1 < n && !(here.x - next.x > 2 * err + 2.3841858e-7f * fmaxf(fabsf(here.x), fabsf(next.x)));
+      const float here = unordered((uint32_t)(own >> 32)), next = unordered((uint32_t)(after >> 32));
+      const float off = 2 * err + 2.3841858e-7f * fmaxf(fabsf(here), fabsf(next));
+      const bool open = lane < a.k && lane + 1 < n && !(here - next > off);
       sure = !__any_sync(0xffffffffu, open);
+      // Sigmoids of the candidates alone in f64, a lane each, where no other key can come near the last one taken.
+      const float kth = __shfl_sync(0xffffffffu, here, a.k - 1);
+      if (!sure && a.sigmoid && n >= need && kth - least > 2 * err + 2.3841858e-7f * fmaxf(fabsf(kth), fabsf(least))) {
+        const uint32_t e = lane < n ? ~(uint32_t)own : kNone;
+        const double v = lane < n ? sigmoid_key((double)logit_of<L>(a, t, e)) + a.bias[e] : -INFINITY;
+        rank = 0;
+        for (uint32_t j = 0; j < n; j++) {
+          const double o = __shfl_sync(0xffffffffu, v, j);
+          const uint32_t oe = __shfl_sync(0xffffffffu, e, j);
+          rank += o > v || (o == v && oe < e) ? 1u : 0u;
+        }
+        uint32_t *place = (uint32_t *)sk;
+        if (lane < n) place[rank] = e;
+        __syncwarp();
+        if (lane < a.k) id = place[lane];
+        __syncwarp();
+        sure = true;
+      }
     }
   }
   if (!sure) {
@@ -336,17 +382,17 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
       if (!a.sigmoid)
         s = exp_below(lj, c);
       else if (c > 0.0f)
-        s = lj > 0.0f ? 1.0f / (1.0f + expf(-lj)) : expf(lj) / (1.0f + expf(lj));
+        s = __fdividef(1.0f, 1.0f + expf(-lj));
       else
-        s = exp_below(lj, c) / (1.0f + expf(lj));
+        s = __fdividef(exp_below(lj, c), 1.0f + expf(lj));
     }
     float sum = s;
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (id != kNone) s = s / sum;  // the largest's own e^0 is in the sum
+    if (id != kNone) s = __fdividef(s, sum);  // the largest's own e^0 is in the sum
   } else if (id != kNone) {
     const float ex = a.sigmoid ? expf(-fabsf(lj)) : exp_below(lj, largest);
-    s = !a.sigmoid ? ex * score_max : lj < 0.0f ? ex / (1.0f + ex) : 1.0f / (1.0f + ex);
+    s = !a.sigmoid ? ex * score_max : __fdividef(lj < 0.0f ? ex : 1.0f, 1.0f + ex);
   }
   if (lane < a.k) {
     a.ids[t * a.k + lane] = (int32_t)id;
@@ -357,8 +403,8 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
 
 // A chunk of rows by a CTA. With lists, each expert's count of the chunk's rows, and every assignment's place among its expert's rows there.
 template <class L, int V>
-__global__ void __launch_bounds__(32 * kRouteWarps) k_route_rows(const RouteArgs a) {
-  __shared__ double sk[kRouteWarps][32 * V];
+__global__ void __launch_bounds__(32 * kRouteWarps, 4) k_route_rows(const RouteArgs a) {
+  __shared__ __align__(16) double sk[kRouteWarps][kRouteScratch<V>];
   __shared__ uint32_t rows_of[32 * V];  // a bit a row
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -383,35 +429,45 @@ __global__ void __launch_bounds__(32 * kRouteWarps) k_route_rows(const RouteArgs
   }
 }
 
-// The chunks' counts become each expert's rows before the chunk; the totals come after the last chunk's. A CTA takes 32 experts, a
-// warp a 32nd of the chunks, sixteen counts on their way at once.
+// The chunks' counts become each expert's rows before the chunk; the totals come after the last chunk's. A CTA takes 8 experts (a sector of a
+// chunk's counts), eight threads a 128th of the chunks, eight counts each on their way at once.
 __global__ void __launch_bounds__(1024) k_route_scan(uint32_t *work, uint32_t chunks, uint32_t E) {
-  __shared__ uint32_t part[32][33];
+  __shared__ uint32_t part[32][8];
   dependents_may_launch(), wait_for_predecessors();
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, e = blockIdx.x * 32 + lane;
-  const uint32_t per = (chunks + 31) / 32, c0 = min(chunks, warp * per), c1 = e < E ? min(chunks, c0 + per) : c0;
-  uint32_t *at = work + e, v[16];
-  uint32_t run = 0;
-  for (uint32_t c = c0; c < c1; c += 16) {
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, e = blockIdx.x * 8 + lane % 8;
+  const uint32_t per = (chunks + 127) / 128, c0 = min(chunks, (warp * 4 + lane / 8) * per), c1 = e < E ? min(chunks, c0 + per) : c0;
+  uint32_t *at = work + e, v[8];
+  auto load = [&](uint32_t c) {
 #pragma unroll
-    for (uint32_t j = 0; j < 16; j++) v[j] = c + j < c1 ? at[(uint64_t)(c + j) * E] : 0;
+    for (uint32_t j = 0; j < 8; j++) v[j] = c + j < c1 ? at[(uint64_t)(c + j) * E] : 0;
+  };
+  uint32_t sum = 0;
+  for (uint32_t c = c0; c < c1; c += 8) {
+    load(c);
 #pragma unroll
-    for (uint32_t j = 0; j < 16; j++) run += v[j];
+    for (uint32_t j = 0; j < 8; j++) sum += v[j];
   }
-  part[warp][lane] = run;
+  // Before this thread's chunks: those of the warp's threads 8, 16, 24 lanes down, and of the warps before.
+  uint32_t run = 0, all = sum;
+  __syncwarp();
+#pragma unroll
+  for (uint32_t d = 8; d < 32; d += 8) {
+    const uint32_t o = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) run += o;
+  }
+  all += run;
+  if (lane >= 24) part[warp][lane - 24] = all;
   __syncthreads();
-  run = 0;
-  for (uint32_t i = 0; i < warp; i++) run += part[i][lane];
-  for (uint32_t c = c0; c < c1; c += 16) {
+  for (uint32_t i = 0; i < warp; i++) run += part[i][lane % 8];
+  for (uint32_t c = c0; c < c1; c += 8) {
+    if (per > 8) load(c);  // else they are here still
 #pragma unroll
-    for (uint32_t j = 0; j < 16; j++) v[j] = c + j < c1 ? at[(uint64_t)(c + j) * E] : 0;
-#pragma unroll
-    for (uint32_t j = 0; j < 16; j++) {
+    for (uint32_t j = 0; j < 8; j++) {
       if (c + j < c1) at[(uint64_t)(c + j) * E] = run;
       run += v[j];
     }
   }
-  if (warp == 31 && e < E) at[(uint64_t)chunks * E] = run;
+  if (threadIdx.x >= 1016 && e < E) at[(uint64_t)chunks * E] = run;
 }
 
 // Exclusive sums of E <= 512 counts, thread i's of experts 2 i and 2 i + 1, by a block of W >= 8 warps; s: 8 words.
@@ -447,7 +503,7 @@ __global__ void __launch_bounds__(256) k_route_places(const RouteArgs a, uint32_
   __syncthreads();
   const uint64_t A = (uint64_t)a.T * a.k, a0 = (uint64_t)blockIdx.x * kRoutePlaces;
   const uint32_t per = kRouteChunk * a.k;  // assignments of a chunk
-#pragma unroll 4
+#pragma unroll
   for (uint32_t j = 0; j < kRoutePlaces / 256; j++) {
     const uint64_t i = a0 + j * 256 + threadIdx.x;
     if (i >= A) break;
@@ -456,10 +512,10 @@ __global__ void __launch_bounds__(256) k_route_places(const RouteArgs a, uint32_
   }
 }
 
-// A short step by one CTA of W warps: rows, counts, offsets and places in one launch. Dynamic shared memory: 32 V doubles a warp.
+// A short step by one CTA of W warps: rows, counts, offsets and places in one launch. Dynamic shared memory: kRouteScratch<V> doubles a warp.
 template <class L, int V, int W>
 __global__ void __launch_bounds__(32 * W) k_route_short(const RouteArgs a) {
-  extern __shared__ double s_dyn[];
+  extern __shared__ __align__(16) double s_dyn[];
   __shared__ uint32_t s_ids[kRouteOneCta * kRouteMaxUsed], s_scan[8], s_first[kRouteMaxExperts], rows_of[2][kRouteMaxExperts];  // a bit a row, 64 in all
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t i = threadIdx.x, warp = i / 32, lane = i % 32;
@@ -468,7 +524,7 @@ __global__ void __launch_bounds__(32 * W) k_route_short(const RouteArgs a) {
   load_bias(a, lane, bias);
   __syncthreads();
   for (uint32_t t = warp; t < a.T; t += W) {
-    const uint32_t id = route_row<L, V>(a, t, lane, bias, s_dyn + warp * 32 * V);
+    const uint32_t id = route_row<L, V>(a, t, lane, bias, s_dyn + warp * kRouteScratch<V>);
     if (lane < a.k) s_ids[t * a.k + lane] = id;
     if (id != kNone) atomicOr(&rows_of[t / 32][id], 1u << (t % 32));
   }
@@ -494,7 +550,7 @@ __global__ void __launch_bounds__(512) k_route_empty(int32_t *offsets, uint32_t 
 
 template <class L, int V, int W>
 void launch_short(const RouteArgs &a, int device, cudaStream_t st) {
-  constexpr size_t smem = W * 32 * V * sizeof(double);
+  constexpr size_t smem = W * kRouteScratch<V> * sizeof(double);
   static std::atomic<uint32_t> done{0};
   CUDA_OK(ensure_dynamic_smem(k_route_short<L, V, W>, smem, done, device));
   CUDA_OK(launch_kernel(true, k_route_short<L, V, W>, dim3(1), dim3(32 * W), smem, st, a));
@@ -507,7 +563,7 @@ void launch_rows(const RouteArgs &a, int device, cudaStream_t st) {
   const uint32_t chunks = (a.T + kRouteChunk - 1) / kRouteChunk;
   CUDA_OK(launch_kernel(true, k_route_rows<L, V>, dim3(chunks), dim3(32 * kRouteWarps), 0, st, a));
   if (!a.offsets) return;
-  CUDA_OK(launch_kernel(true, k_route_scan, dim3((a.E + 31) / 32), dim3(1024), 0, st, a.work, chunks, a.E));
+  CUDA_OK(launch_kernel(true, k_route_scan, dim3((a.E + 7) / 8), dim3(1024), 0, st, a.work, chunks, a.E));
   CUDA_OK(launch_kernel(true, k_route_places, dim3((uint32_t)(((uint64_t)a.T * a.k + kRoutePlaces - 1) / kRoutePlaces)), dim3(256), 0, st, a, chunks));
 }
 
