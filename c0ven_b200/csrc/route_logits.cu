@@ -253,15 +253,24 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
   }
   const float err = key_error(a.sigmoid, score_max);
   bool sure = true;
+  // key[i] becomes the expert's key, -infinity if it is out: what is added for that has no branch.
+  auto to_keys = [&](float (&v)[V]) {
+    if (a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] = sigmoid_key(key[i]) + bias[i] + (key[i] > -INFINITY ? 0.0f : -INFINITY);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] = softmax_part<float>(key[i], largest) * score_max + bias[i] + (key[i] > -INFINITY ? 0.0f : -INFINITY);
+    }
+  };
   if (a.G > 1) {
-    float *fk = (float *)sk, top = 0.0f;
+    float *fk = (float *)sk, v[V], top = 0.0f;
+    to_keys(v);
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const uint32_t e = lane + 32 * i;
-      float v = -INFINITY;
-      if (key[i] > -INFINITY) v = (a.sigmoid ? sigmoid_key(key[i]) : softmax_part<float>(key[i], largest) * score_max) + bias[i];
-      if (v > -INFINITY) top = fmaxf(top, fabsf(v));
-      if (e < a.E) fk[e] = v;
+      const bool out = !(v[i] > -INFINITY);
+      if (exists<V>(a, lane, i)) fk[lane + 32 * i] = out ? -INFINITY : v[i];
+      top = fmaxf(top, out ? 0.0f : fabsf(v[i]));
     }
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
     __syncwarp();
@@ -270,14 +279,12 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
     // Without a bias the order within the groups that stay is the logits' own.
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const float v = lane + 32 * i < a.E ? fk[lane + 32 * i] : -INFINITY;
-      key[i] = v == -INFINITY ? -INFINITY : a.bias ? v : key[i];
+      const float w = exists<V>(a, lane, i) ? fk[lane + 32 * i] : -INFINITY;
+      key[i] = w == -INFINITY ? -INFINITY : a.bias ? w : key[i];
     }
     __syncwarp();
   } else if (a.bias) {
-#pragma unroll
-    for (int i = 0; i < V; i++)
-      key[i] = key[i] > -INFINITY ? (a.sigmoid ? sigmoid_key(key[i]) : softmax_part<float>(key[i], largest) * score_max) + bias[i] : -INFINITY;
+    to_keys(key);
   }
   // least: need keys at least are not under it. It begins as the least of the lanes' largest keys, where need of them are finite, and rises to
   // the middle between it and the largest as long as need of them reach that; ten steps at most, fewer once few more than need do.
