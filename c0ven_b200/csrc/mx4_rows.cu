@@ -12,49 +12,81 @@ namespace {
 
 constexpr uint32_t kRowsMaxUsed = 16;
 
-// A thread takes 8 values, four threads a block of 32, a CTA 2,048 values of one row (grid.x the row, grid.y the piece). The block's
-// largest magnitude is an integer maximum over the four threads: magnitudes order as their bits do.
-template <class X>
-__global__ void __launch_bounds__(256) k_mx4_quantize(const X *x, uint64_t stride, uint32_t K, const int32_t *inv, uint32_t n_used, uint32_t R,
+// How rows are dealt to a CTA of 256 threads: 2^log2 neighbouring threads a row, eight values each (grid.y where a row has more), and U rows a
+// thread, whose loads are on their way together. Four rows a thread where that leaves every SM some four CTAs: 32,768 rows of 2,048 bf16
+// values to MX rows and back take 63 us so and 79 with one, bound by the loads' round trip and the CTAs' coming and going; 13 rows of 2,560 to
+// eight places each and back 7.2 and 3.5 us, bound by the one round trip after another.
+constexpr uint32_t kManyOctets = 4 * 148 * 4 * 256;
+template <uint32_t U>
+struct RowsMap {
+  static constexpr uint32_t kRows = U;
+  uint32_t T, log2;
+  __device__ uint32_t octet() const { return (blockIdx.y << log2) + (threadIdx.x & ((1u << log2) - 1)); }
+  __device__ uint64_t row(uint32_t u) const { return ((uint64_t)blockIdx.x * U + u) * (256u >> log2) + (threadIdx.x >> log2); }
+};
+
+// Four threads hold a block of 32. The block's largest magnitude is an integer maximum over them: magnitudes order as their bits do.
+template <class X, uint32_t U>
+__global__ void __launch_bounds__(256) k_mx4_quantize(const X *x, uint64_t stride, const RowsMap<U> map, uint32_t K, const int32_t *inv, uint32_t n_used, uint32_t R,
                                                       uint8_t *codes, uint8_t *scales) {
   dependents_may_launch(), wait_for_predecessors();
-  const uint64_t t = blockIdx.x;
-  const uint32_t k = (blockIdx.y * 256 + threadIdx.x) * 8;
+  const uint32_t k = 8 * map.octet(), srow = mx_scale_row_bytes(K), b = k / kMxBlock;
   const bool in = k < K;  // K is a multiple of 32: a block's four threads alike
-  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (in) load8(x + t * stride + k, v);
-  uint32_t m = 0;
+  float v[U][8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const uint32_t scale = mx_scale_of(m);
-  const float f = mx_inverse(scale);
+  for (uint32_t u = 0; u < U; u++) {
+    const uint64_t t = map.row(u);
+    if (in && t < map.T)
+      load8(x + t * stride + k, v[u]);
+    else
+      for (int i = 0; i < 8; i++) v[u][i] = 0.0f;
+  }
 #pragma unroll
-  for (int i = 0; i < 8; i++) v[i] *= f;
-  const uint32_t c = scale == 255 ? 0u : mx_codes8(v);
-  const uint32_t srow = mx_scale_row_bytes(K), b = k / kMxBlock;
-  const uint32_t n = inv ? n_used : 1;
-  for (uint32_t j = 0; j < n; j++) {
-    const uint64_t r = inv ? (uint64_t)(uint32_t)inv[t * n_used + j] : t;
-    if (r >= R) continue;
-    if (in) *(uint32_t *)(codes + r * (K / 2) + k / 2) = c;
-    if (threadIdx.x % 4 == 0 && b < srow) scales[r * srow + b] = in ? (uint8_t)scale : 0;
+  for (uint32_t u = 0; u < U; u++) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[u][i]) & 0x7FFFFFFFu);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint32_t scale = mx_scale_of(m);
+    const float f = mx_inverse(scale);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[u][i] *= f;
+    const uint32_t c = scale == 255 ? 0u : mx_codes8(v[u]);
+    const uint64_t t = map.row(u);
+    if (t >= map.T) break;
+    for (uint32_t j = 0; j < (inv ? n_used : 1); j++) {
+      const uint64_t r = inv ? (uint64_t)(uint32_t)inv[t * n_used + j] : t;
+      if (r >= R) continue;
+      if (in) *(uint32_t *)(codes + r * (K / 2) + k / 2) = c;
+      if (threadIdx.x % 4 == 0 && b < srow) scales[r * srow + b] = in ? (uint8_t)scale : 0;
+    }
   }
 }
 
-template <class Y>
-__global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, uint32_t K, Y *out) {
+template <class Y, uint32_t U>
+__global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, const RowsMap<U> map, uint32_t K, Y *out) {
   dependents_may_launch(), wait_for_predecessors();
-  const uint64_t r = blockIdx.x;
-  const uint32_t k = (blockIdx.y * 256 + threadIdx.x) * 8;
+  const uint32_t k = 8 * map.octet(), srow = mx_scale_row_bytes(K);
   if (k >= K) return;
-  float v[8];
-  mx_values8(*(const uint32_t *)(codes + r * (K / 2) + k / 2), v);
-  const float f = mx_scale(scales[r * mx_scale_row_bytes(K) + k / kMxBlock]);
+  uint32_t c[U], s[U];
 #pragma unroll
-  for (int i = 0; i < 8; i++) v[i] *= f;
-  store8(out + r * K + k, v);
+  for (uint32_t u = 0; u < U; u++) {
+    const uint64_t r = map.row(u);
+    c[u] = s[u] = 0;
+    if (r < map.T) c[u] = *(const uint32_t *)(codes + r * (K / 2) + k / 2), s[u] = scales[r * srow + k / kMxBlock];
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) {
+    const uint64_t r = map.row(u);
+    if (r >= map.T) break;
+    float v[8];
+    mx_values8(c[u], v);
+    const float f = mx_scale(s[u]);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= f;
+    store8(out + r * K + k, v);
+  }
 }
 
 // A thread a block of the file: its bytes hold value j and value j + 16, the rows' hold neighbours.
@@ -110,6 +142,36 @@ __global__ void __launch_bounds__(256) k_combine_rows(const Y *y, uint32_t R, co
 // Grids of (rows, pieces of a row): rows up to 2^31 - 1.
 dim3 rows_grid(uint32_t rows, uint32_t per_row) { return dim3(rows, (per_row + 255) / 256); }
 
+// Calls f with the map for rows of so many groups of eight values, and its grid.
+template <class F>
+void with_rows_map(uint32_t T, uint32_t octets, F &&f) {
+  uint32_t log2 = 2;
+  while (log2 < 8 && (1u << log2) < octets) log2++;
+  auto go = [&](auto map, uint32_t u) {
+    const uint32_t rows = u * (256u >> log2);
+    f(map, dim3((T + rows - 1) / rows, (octets + (1u << log2) - 1) >> log2));
+  };
+  if ((uint64_t)T * octets >= kManyOctets)
+    go(RowsMap<4>{T, log2}, 4);
+  else
+    go(RowsMap<1>{T, log2}, 1);
+}
+
+// Launches for rows of one type.
+template <class X>
+void quantize(const void *x, uint64_t stride, uint32_t T, uint32_t K, const int32_t *inv, uint32_t n_used, uint32_t R, void *codes, void *scales, cudaStream_t st) {
+  with_rows_map(T, mx_scale_row_bytes(K) * 4, [&](auto map, dim3 grid) {  // the scales' filling has its threads too
+    CUDA_OK(launch_kernel(true, k_mx4_quantize<X, decltype(map)::kRows>, grid, dim3(256), 0, st, (const X *)x, stride, map, K, inv, n_used, R,
+                          (uint8_t *)codes, (uint8_t *)scales));
+  });
+}
+template <class Y>
+void dequantize(const void *codes, const void *scales, uint32_t R, uint32_t K, void *out, cudaStream_t st) {
+  with_rows_map(R, K / 8, [&](auto map, dim3 grid) {
+    CUDA_OK(launch_kernel(true, k_mx4_dequantize<Y, decltype(map)::kRows>, grid, dim3(256), 0, st, (const uint8_t *)codes, (const uint8_t *)scales, map, K, (Y *)out));
+  });
+}
+
 void need_mx_row(uint32_t K) { need(K >= kMxBlock && K % kMxBlock == 0 && K <= kMxMaxValues, "a row's values must be a multiple of 32, 32 .. 65536"); }
 
 }  // namespace
@@ -132,17 +194,8 @@ MOE_API moe_status moe_mx4_quantize_rows_device(const void *x_dev, uint32_t type
     need(T < 1u << 31 && R < 1u << 31, "T and R must be below 2^31");
     if (T == 0 || R == 0) return;
     need_device({{x_dev, "x", 16}, {inv_dev, "inv", 4, true}, {codes_dev, "codes", 16}, {scales_dev, "scales", 4}});
-    const uint64_t s = stride ? stride : K;
-    uint8_t *codes = (uint8_t *)codes_dev, *scales = (uint8_t *)scales_dev;
-    // A piece more than the codes need where the scales' filling lies past the last thread.
-    const dim3 grid = rows_grid(T, mx_scale_row_bytes(K) * 4), block(256);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (type == MOE_TYPE_F32)
-      CUDA_OK(launch_kernel(true, k_mx4_quantize<float>, grid, block, 0, st, (const float *)x_dev, s, K, inv_dev, n_used, R, codes, scales));
-    else if (type == MOE_TYPE_F16)
-      CUDA_OK(launch_kernel(true, k_mx4_quantize<__half>, grid, block, 0, st, (const __half *)x_dev, s, K, inv_dev, n_used, R, codes, scales));
-    else
-      CUDA_OK(launch_kernel(true, k_mx4_quantize<__nv_bfloat16>, grid, block, 0, st, (const __nv_bfloat16 *)x_dev, s, K, inv_dev, n_used, R, codes, scales));
+    const auto call = type == MOE_TYPE_F32 ? quantize<float> : type == MOE_TYPE_F16 ? quantize<__half> : quantize<__nv_bfloat16>;
+    call(x_dev, stride ? stride : K, T, K, inv_dev, n_used, R, codes_dev, scales_dev, (cudaStream_t)stream);
   });
 }
 
@@ -154,15 +207,8 @@ MOE_API moe_status moe_mx4_dequantize_rows_device(const void *codes_dev, const v
     need(R < 1u << 31, "R must be below 2^31");
     if (R == 0) return;
     need_device({{codes_dev, "codes", 16}, {scales_dev, "scales", 4}, {out_dev, "out", 16}});
-    const uint8_t *codes = (const uint8_t *)codes_dev, *scales = (const uint8_t *)scales_dev;
-    const dim3 grid = rows_grid(R, K / 8), block(256);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (type == MOE_TYPE_F32)
-      CUDA_OK(launch_kernel(true, k_mx4_dequantize<float>, grid, block, 0, st, codes, scales, K, (float *)out_dev));
-    else if (type == MOE_TYPE_F16)
-      CUDA_OK(launch_kernel(true, k_mx4_dequantize<__half>, grid, block, 0, st, codes, scales, K, (__half *)out_dev));
-    else
-      CUDA_OK(launch_kernel(true, k_mx4_dequantize<__nv_bfloat16>, grid, block, 0, st, codes, scales, K, (__nv_bfloat16 *)out_dev));
+    const auto call = type == MOE_TYPE_F32 ? dequantize<float> : type == MOE_TYPE_F16 ? dequantize<__half> : dequantize<__nv_bfloat16>;
+    call(codes_dev, scales_dev, R, K, out_dev, (cudaStream_t)stream);
   });
 }
 

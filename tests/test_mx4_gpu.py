@@ -41,7 +41,7 @@ def rows_of(rng, T, K):
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("T, K", [(1, 32), (3, 96), (5, 2048), (2, 2080), (33, 2880), (1, 65536), (700, 160)])
+@pytest.mark.parametrize("T, K", [(1, 32), (3, 96), (5, 2048), (2, 2080), (33, 2880), (1, 65536), (700, 160), (2501, 2080), (19001, 288)])
 def test_quantize_rows_bit_for_bit(type, T, K):
     import torch
 
@@ -113,6 +113,74 @@ def test_quantize_scatters_strided_rows(type):
             if 0 <= r < rows:
                 want_c[r], want_s[r] = c[t], s[t]
     assert np.array_equal(codes.cpu().numpy(), want_c) and np.array_equal(scales.cpu().numpy(), want_s)
+
+
+def test_quantize_scatters_many_rows():
+    import torch
+
+    rng = np.random.default_rng(4)
+    T, K, n = 5003, 1056, 3
+    x = dev(rng.standard_normal((T, K)).astype(np.float32), "f16")
+    inv = rng.permutation(T * n).reshape(T, n).astype(np.int32)
+    codes, scales = mx_buffers(T * n, K)
+    di = dev(inv)
+    ops.mx4_quantize_rows_device(x.data_ptr(), ops.F16, T, K, codes.data_ptr(), scales.data_ptr(), T * n, inv_ptr=di.data_ptr(), n_used=n)
+    torch.cuda.synchronize()
+    c, s = R.pack(*R.quantize(x.double().cpu().numpy()))
+    for j in range(n):
+        assert np.array_equal(codes.cpu().numpy()[inv[:, j]], c) and np.array_equal(scales.cpu().numpy()[inv[:, j]], s)
+
+
+def test_offsets_past_32_bits():
+    """Rows, matrices and results whose places do not fit 32 bits: the last ones are right."""
+    import torch
+
+    rng = np.random.default_rng(5)
+    T, K = 66000, 65536  # 8.6 GB of bf16, 2.2 GB of codes
+    x = torch.zeros((T, K), dtype=torch.bfloat16, device="cuda")
+    tail = dev(rng.standard_normal((3, K)).astype(np.float32), "bf16")
+    x[-3:] = tail
+    codes, scales = mx_buffers(T, K)
+    ops.mx4_quantize_rows_device(x.data_ptr(), ops.BF16, T, K, codes.data_ptr(), scales.data_ptr(), T)
+    c, s = R.quantize(tail.double().cpu().numpy())
+    want = R.pack(c, s)
+    assert np.array_equal(codes[-3:].cpu().numpy(), want[0]) and np.array_equal(scales[-3:].cpu().numpy(), want[1]) and (codes[:-3] == 0).all()
+    x.fill_(7)
+    ops.mx4_dequantize_rows_device(codes.data_ptr(), scales.data_ptr(), T, K, x.data_ptr(), ops.BF16)
+    assert np.array_equal(x[-3:].double().cpu().numpy(), R.values(c, s)) and (x[:-3] == 0).all()
+    # The same 4.3 thousand million values as results of 64 columns, two of which are summed.
+    del codes, scales
+    rows = T * K // 64
+    inv, w = dev(np.array([[rows - 1, rows - 2]], np.int32)), torch.ones((1, 2), device="cuda")
+    out = torch.empty((1, 64), device="cuda")
+    ops.combine_rows_device(x.data_ptr(), ops.BF16, rows, inv.data_ptr(), w.data_ptr(), 1, 2, 64, out.data_ptr())
+    assert torch.equal(out[0], (x.view(-1, 64)[-1].float() + x.view(-1, 64)[-2].float()))
+    del x
+    # Matrices of more than 2^32 bytes of codes, rows for the last alone.
+    E, N, K = 512, 4128, 4128
+    wc = torch.zeros((E, N, K // 2), dtype=torch.uint8, device="cuda")
+    ws = torch.full((E, N, R.scale_row_bytes(K)), 127, dtype=torch.uint8, device="cuda")
+    c1, s1, w1, xc, xs, xv = product_case(rng, 1, N, K, None, 40)
+    wc[-1], ws[-1] = c1[0], s1[0]
+    offsets = dev(np.array([0] * E + [40], np.int32))
+    y = torch.empty((40, N), dtype=torch.float16, device="cuda")
+    ops.mx4_product_device(ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), 40, offsets.data_ptr(), y.data_ptr(), ops.F16)
+    ops.status()
+    want = xv @ w1[0].T
+    assert np.linalg.norm(y.double().cpu().numpy() - want) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(want)
+    del wc, ws, y
+    # Results past 2^32 bytes, and past 2^32 values.
+    rows, N, K = 1 << 20, 4128, 32
+    (c1, s1), w1 = R.random_mx(rng, (1, N, K))
+    xc, xs = torch.zeros((rows, K // 2), dtype=torch.uint8, device="cuda"), torch.full((rows, 4), 127, dtype=torch.uint8, device="cuda")
+    (c2, s2), xv = R.random_mx(rng, (5, K), 125, 129)
+    xc[-5:], xs[-5:] = dev(c2), dev(s2)
+    y = torch.full((rows, N), 7.0, dtype=torch.float16, device="cuda")
+    dc, ds = dev(c1), dev(s1)
+    ops.mx4_product_device(ops.Mx4Weights(1, N, K, dc.data_ptr(), ds.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, None, y.data_ptr(), ops.F16)
+    ops.status()
+    want = xv @ w1[0].T
+    assert np.linalg.norm(y[-5:].double().cpu().numpy() - want) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(want) and (y[:-5] == 0).all()
 
 
 def test_rows_of_a_files_blocks():
