@@ -62,6 +62,21 @@ __device__ __forceinline__ uint32_t transpose_codes(uint32_t v, uint32_t lane) {
   return lane & 1 ? (v & 0xF0F0F0F0u) | (c >> 4 & 0x0F0F0F0Fu) : (v & 0x0F0F0F0Fu) | (c << 4 & 0xF0F0F0F0u);
 }
 
+// silu(min(g, limit)) * u held to +-limit, in the fast forms: two significant bits of it stay. NaN passes through.
+__device__ __forceinline__ float swiglu_mx(float g, float u, float limit) {
+  float e, r;
+  asm("min.NaN.f32 %0, %0, %2;\n\tmin.NaN.f32 %1, %1, %2;\n\tmax.NaN.f32 %1, %1, %3;" : "+f"(g), "+f"(u) : "f"(limit), "f"(-limit));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+// The warp's largest magnitude; NaN if there is one.
+__device__ __forceinline__ float largest_magnitude(float v) {
+  float m;
+  asm("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
 __device__ uint32_t g_gave_up;  // a wait ran out since moe_ops_status last asked
 
 struct Mx4Args {
@@ -284,12 +299,11 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
       }
     }
   } else if (warp >= kScaleWarp && warp < kScaleWarp + SL) {
-    // A slot of scales by a warp: eight words of rows i, i + 32, i + 64 and i + 96 an instruction, so that a row's 32 bytes are one request and the
-    // 32 words, at 16 i + 4 (row / 32) of pieces 528 bytes apart, fall on 32 banks. (Of four neighbouring rows into pieces 512 bytes apart,
-    // eight words to a bank, this took a third of shared memory's cycles.)
+    // A slot of scales by a warp, a word a lane: eight words of rows i, i + 32, i + 64 and i + 96 an instruction, so that a row's 32 bytes are one
+    // request; the words, at 16 i + 4 (row / 32) of pieces 528 bytes apart, fall on 32 banks. (Loads into registers, 16 on their way at once, took
+    // half as long again for a whole step: what counts is that a slot's copies are all on their way.)
     const uint32_t mine = warp - kScaleWarp, srow = mx_scale_row_bytes(K), nb = K / kMxBlock, slots = (KT + kScaleStages - 1) / kScaleStages;
-    const uint32_t word = lane % 8, slot = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes);
-    const uint32_t quarter = lane / 8, at = slot + word * kPiece + 4 * quarter, x_at = at + 8 * kPiece;
+    const uint32_t word = lane % 8, quarter = lane / 8, at = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes) + word * kPiece + 4 * quarter;
     uint32_t turn = 0, phase = 1;  // whose turn the next slot is
     for (Item i = first; i.t < ntiles && ok; step(i)) {
       const Tile t = tile_at(i);
@@ -298,30 +312,27 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
         ok = mbar_wait_warp(bar(kScEmpty + mine), phase, abort, error);
         if (!ok) break;
         phase ^= 1;
+        // The scales from byte b0 of a row on, n of the word's four.
         const uint32_t b0 = j * (kScaleStages * kStageK / kMxBlock) + 4 * word, n = b0 < nb ? min(4u, nb - b0) : 0u;
-        {
-          // This lane's 32 rows of the matrix follow one another.
-          const uint32_t r = 32 * quarter, row = GU ? (r < 64 ? t.row0 + r : F + t.row0 + r - 64) : t.row0 + r;
-          const uint8_t *src = a.ws + ((uint64_t)t.expert * a.N + row) * srow + b0;
+        // Up to 32 rows from src on, have of them, to the lane's places from `to` on; zeros behind them.
+        auto bring = [&](uint32_t to, const uint8_t *src, uint32_t have) {
 #pragma unroll 8
           for (uint32_t k = 0; k < 32; k++, src += srow) {
-            const uint32_t have = row + k < a.N ? n : 0;
-            copy_word(at + 16 * k, have ? src : a.ws, have);
+            const uint32_t m = k < have ? n : 0;
+            copy_word(to + 16 * k, m ? src : a.ws, m);
           }
+        };
+        {
+          const uint32_t r = 32 * quarter, row = GU ? (r < 64 ? t.row0 + r : F + t.row0 + r - 64) : t.row0 + r;
+          bring(at, a.ws + ((uint64_t)t.expert * a.N + row) * srow + b0, row < a.N ? min(32u, a.N - row) : 0);
         }
         if constexpr (NT <= 32) {
           // Up to 32 rows, which lie in the first column of a piece: four neighbours an instruction.
-          for (uint32_t r = quarter; r < t.count; r += 4) copy_word(x_at - 4 * quarter + 16 * r, a.xs + (n ? (uint64_t)(t.start + r) * srow + b0 : 0), n);
+          for (uint32_t r = quarter; r < t.count; r += 4) copy_word(at + 8 * kPiece - 4 * quarter + 16 * r, a.xs + (n ? (uint64_t)(t.start + r) * srow + b0 : 0), n);
         } else {
-#pragma unroll
-          for (uint32_t p = 0; p < SM::kRowPieces; p++) {
-            const uint32_t r0 = 128 * p + 32 * quarter, left = t.count > 128 * p ? min(32u, t.count - 128 * p) : 0;
-            const uint8_t *src = a.xs + (uint64_t)(t.start + r0) * srow + b0;
-#pragma unroll 8
-            for (uint32_t k = 0; k < left; k++, src += srow) {
-              const uint32_t have = r0 + k < t.count ? n : 0;
-              copy_word(x_at + p * 8 * kPiece + 16 * k, have ? src : a.xs, have);
-            }
+          for (uint32_t p = 0; p < SM::kRowPieces && 128 * p < t.count; p++) {
+            const uint32_t r = 128 * p + 32 * quarter;
+            bring(at + 8 * (1 + p) * kPiece, a.xs + (uint64_t)(t.start + r) * srow + b0, r < t.count ? min(32u, t.count - r) : 0);
           }
         }
         copy_words_wait();
@@ -418,6 +429,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     // Warp w reads tensor memory's lanes 32 (w % 4) ...; the groups take chunks of 16 rows in turn.
     const uint32_t q = warp % 4, group = (warp - kEpilogueWarp) / 4;
     uint32_t b = 0, phase = 0;
+    [[maybe_unused]] const float limit = a.limit > 0.0f ? a.limit : INFINITY;
     for (Item i = first; i.t < ntiles && ok; step(i)) {
       const Tile t = tile_at(i);
       const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT;
@@ -458,37 +470,45 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
         // when one is written again both warps have passed the barrier that came after its reading.
         const uint32_t up = q / 2, at = t.row0 + 32 * (q % 2), hrow = mx_scale_row_bytes(F);
         float *mine = (float *)(smem + SM::kStaging) + (4 * group + q) * 512 + lane, *theirs = (float *)(smem + SM::kStaging) + (4 * group + (q ^ 2)) * 512 + lane;
-        const uint32_t own = 8 * up;  // the first of the rows this warp keeps
-        uint32_t v[16], turn = 0;
-        if (c0 < t.count) tmem_ld16(from + c0, v);
-        for (uint32_t c = c0; c < t.count; c += dc, turn ^= 256) {
-          tmem_ld_wait16(v);
-          float keep[8];
-#pragma unroll
-          for (uint32_t j = 0; j < 8; j++) {
-            keep[j] = __uint_as_float(up ? v[8 + j] : v[j]);
-            mine[turn + 32 * j] = __uint_as_float(up ? v[j] : v[8 + j]);
-          }
-          if (c + dc < t.count) tmem_ld16(from + c + dc, v);
-          two_warps_sync(2 * group + q % 2);
-          uint32_t scale_of = 0;  // lane j's: of the warp's row j
+        const uint32_t keep_at = from + 8 * up, give_at = from + 8 - 8 * up;
+        uint32_t r = c0 + 8 * up + lane % 8;  // the row whose codes this lane gets
+        uint8_t *hc = a.hc + (uint64_t)(t.start + r) * (F / 2) + at / 2 + 4 * (lane / 8), *hs = a.hs + (uint64_t)(t.start + r) * hrow + at / kMxBlock;
+        uint32_t keep[8], give[8], turn = 0;
+        if (c0 < t.count) tmem_ld8(keep_at + c0, keep), tmem_ld8(give_at + c0, give);
+        for (uint32_t c = c0; c < t.count; c += dc, r += dc, hc += (uint64_t)dc * (F / 2), hs += (uint64_t)dc * hrow, turn ^= 256) {
+          tmem_ld_wait8(keep), tmem_ld_wait8(give);
           float h[8];
 #pragma unroll
+          for (uint32_t j = 0; j < 8; j++) mine[turn + 32 * j] = __uint_as_float(give[j]), h[j] = __uint_as_float(keep[j]);
+          if (c + dc < t.count) tmem_ld8(keep_at + c + dc, keep), tmem_ld8(give_at + c + dc, give);
+          two_warps_sync(2 * group + q % 2);
+          if (up) {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) h[j] = swiglu_mx(theirs[turn + 32 * j], h[j], limit);
+          } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) h[j] = swiglu_mx(h[j], theirs[turn + 32 * j], limit);
+          }
+          // The rows' scales: f is the exponent of the largest magnitude, at least 2; 2^(127 - (f - 2)) is what the values are multiplied by. A row with
+          // an infinity or NaN (f 255) gets codes 0.
+          uint32_t f_of = 0;  // lane j's, and lanes 8 + j, ..: of the warp's row j
+#pragma unroll
           for (uint32_t j = 0; j < 8; j++) {
-            const float got = theirs[turn + 32 * j];
-            h[j] = up ? swiglu_fast(got, keep[j], a.limit) : swiglu_fast(keep[j], got, a.limit);  // two significant bits of it stay
-            const uint32_t scale = mx_scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(h[j]) & 0x7FFFFFFFu));
-            h[j] = scale == 255 ? 0.0f : h[j] * mx_inverse(scale);
-            if (lane == j) scale_of = scale;
+            const uint32_t f = max(__float_as_uint(largest_magnitude(h[j])) & 0x7F800000u, 2u << 23);
+            h[j] *= __uint_as_float(0x80000000u - f);
+            if (lane % 8 == j) f_of = f;
           }
           // The warp's eight rows by eight features: lane j of each eight gets row j's codes of those features.
-          const uint32_t codes = transpose_codes(mx_codes8(h), lane), r = c + own + lane % 8;
-          if (r < t.count && at < F) *(uint32_t *)(a.hc + (uint64_t)(t.start + r) * (F / 2) + at / 2 + 4 * (lane / 8)) = codes;
-          if (lane < 8 && r < t.count && at < F) {
-            uint8_t *hs = a.hs + (uint64_t)(t.start + r) * hrow;
-            hs[at / kMxBlock] = (uint8_t)scale_of;
-            if (at + kMxBlock == F)
-              for (uint32_t z = F / kMxBlock; z < hrow; z++) hs[z] = 0;
+          uint32_t codes = transpose_codes(mx_codes8(h), lane);
+          const bool bad = f_of == 0x7F800000u;
+          if (bad) codes = 0;
+          if (r < t.count && at < F) {
+            *(uint32_t *)hc = codes;
+            if (lane < 8) {
+              *hs = bad ? 255 : (uint8_t)((f_of >> 23) - 2);
+              if (at + kMxBlock == F)
+                for (uint32_t z = 1; z < hrow - (F / kMxBlock - 1); z++) hs[z] = 0;
+            }
           }
         }
       }
@@ -545,10 +565,14 @@ void launch_product(const Mx4Args &args, const void *wc, const void *xc, cudaStr
   CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, maps));
 }
 
-// Tiles of 224 rows by pairs of CTAs, or of 32 by single ones.
+// Tiles of 224 rows by pairs of CTAs where experts have more than 32 rows on average and there are 32 items for pairs at least; else of 32 by single
+// CTAs. gate_up and down by pairs and by single CTAs, us: 512 experts of 2,048 x 512, 10 rows 9 + 7 and 8 + 6, 1,000 rows 80 + 48 and 80 + 45,
+// 10,000 rows 98 + 60 and 97 + 54, 16,000 rows 100 + 67 and 107 + 72, 32,000 rows 105 + 75 and 185 + 129; one of 2,080 x 1,440, 200 rows (12 items for
+// pairs) 15 + 11 and 11 + 6, 777 rows (48) 15 + 11 and 17 + 10; one of 8,192 x 4,096, 128 rows (32) 19 + 12 and 24 + 14.
 template <class Out>
 void launch(const Mx4Args &a, const void *wc, const void *xc, cudaStream_t st) {
-  if (a.R > 32ull * a.E)
+  const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 224 + 1;
+  if (a.R > 32ull * a.E && pieces * tiles >= 32)
     launch_product<Out, 2, 224>(a, wc, xc, st);
   else
     launch_product<Out, 1, 32>(a, wc, xc, st);
