@@ -89,9 +89,9 @@ struct Mx4Args {
   uint8_t *hc, *hs;
 };
 
-// Maps over the codes of the matrices and, in boxes of 16, 32, 64 and 112 rows, of the rows.
+// Maps over the codes of the matrices and, in boxes of 16, 32, 64 and 104 rows, of the rows.
 constexpr uint32_t kBoxes = 4;
-__host__ __device__ constexpr uint32_t box_rows(uint32_t i) { return i == 3 ? 112u : 16u << i; }
+__host__ __device__ constexpr uint32_t box_rows(uint32_t i) { return i == 3 ? 104u : 16u << i; }
 struct Mx4Maps {
   CUtensorMap w, x[kBoxes];
 };
@@ -116,24 +116,28 @@ struct Mx4Form {
   static constexpr uint32_t kSlotBytes = 8 * (1 + kRowPieces) * kPiece;
   static constexpr uint32_t kStaging = kScales + kScaleSlots * kSlotBytes;
   static constexpr uint32_t kBarriers = kStaging + (GU ? 4 * kGroups * 2048 : 0);
-  static constexpr uint32_t kTables = kBarriers + 256;
+  static constexpr uint32_t kTables = kBarriers + 320;
   static constexpr uint32_t kTileExperts = kTables + 2 * (kMaxExperts + 1) * 4;
   static constexpr uint32_t kBytes = kTileExperts + 2 * kTileTable + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
   static_assert(2 * kThreads > kMaxExperts + 1, "two experts a thread");
-  // Tensor memory: two accumulators, then two sets of columns for scales, of kScaleStages stages where they have the room, else of one.
+  // Tensor memory: two accumulators, then sets of columns for scales, of kScaleStages stages where they have the room, else of one. From the MMAs of
+  // a unit of stages to those that find its columns filled again takes three hand-overs between warps, longer than the MMAs of a stage: with two
+  // sets of one stage, beside accumulators of 224 columns, every stage waited 0.14 us.
   static constexpr uint32_t kStageCols = 2 * 4 * (1 + kRowPieces);
-  static constexpr uint32_t kUnitStages = 2 * NT + 2 * kScaleStages * kStageCols <= 512 ? kScaleStages : 1;
+  static constexpr uint32_t kUnitStages = 2 * NT + 3 * kScaleStages * kStageCols <= 512 ? kScaleStages : 1;
+  static constexpr uint32_t kSets = kUnitStages == 1 ? 4 : 3;
   static constexpr uint32_t kUnitCols = kUnitStages * kStageCols;
-  static constexpr uint32_t kUsedCols = 2 * NT + 2 * kUnitCols;
+  static constexpr uint32_t kUsedCols = 2 * NT + kSets * kUnitCols;
   static constexpr uint32_t kCols = kUsedCols <= 256 ? 256 : 512;
   static_assert(kUsedCols <= kCols, "tensor memory");
+  static_assert(kSets < kStages, "the stage whose MMAs a set waits for has not been filled again");
 };
 
 enum : uint32_t { kCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kScaleCopyWarp = 5, kEpilogueWarp = 6 };
 
 // Rows a tile of an expert's n rows has: the tiles of a few share them evenly (which 16 rows a tile can be off by leaves no tile empty up to
-// eight tiles of 224).
+// eight tiles of 208).
 template <uint32_t NT>
 __device__ __forceinline__ uint32_t tile_rows(uint32_t n) {
   const uint32_t tiles = (n + NT - 1) / NT;
@@ -154,8 +158,8 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   // Barriers: stages full, empty; scales full, empty; accumulators full, empty; sets of scales in tensor memory full, empty. Of a pair the first CTA's "full" of stages and scales and "empty"
   // of accumulators take both CTAs' arrivals.
   constexpr uint32_t kEmpty = S, kScFull = 2 * S, kScEmpty = kScFull + SL, kAccFull = kScEmpty + SL, kAccEmpty = kAccFull + 2, kSetFull = kAccEmpty + 2,
-                     kSetEmpty = kSetFull + 2, kBars = kSetEmpty + 2;
-  static_assert(8 * kBars + 8 <= 256, "the barriers' room");
+                     kSetEmpty = kSetFull + SM::kSets, kBars = kSetEmpty + SM::kSets;
+  static_assert(8 * kBars + 8 <= 320, "the barriers' room");
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](uint32_t i) { return bar0 + 8 * i; };
   uint32_t *tmem_slot = (uint32_t *)(bars + kBars);
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     for (uint32_t s = 0; s < S; s++) mbar_init(bar(s), CTAS), mbar_init(bar(kEmpty + s), 1);
     for (uint32_t s = 0; s < SL; s++) mbar_init(bar(kScFull + s), CTAS), mbar_init(bar(kScEmpty + s), 1);
     for (uint32_t b = 0; b < 2; b++) mbar_init(bar(kAccFull + b), 1), mbar_init(bar(kAccEmpty + b), CTAS * 4 * SM::kGroups);
-    for (uint32_t b = 0; b < 2; b++) mbar_init(bar(kSetFull + b), 1), mbar_init(bar(kSetEmpty + b), 1);
+    for (uint32_t b = 0; b < SM::kSets; b++) mbar_init(bar(kSetFull + b), 1), mbar_init(bar(kSetEmpty + b), 1);
     *abort = 0;
     fence_barrier_init();
   }
@@ -347,15 +351,15 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     if (rank == 0) {
       constexpr uint32_t U = SM::kUnitStages;
       const uint32_t leader = elect_leader();
-      // The MMAs of two units ago, which read the set's columns, are done: a unit of one stage has that stage's "empty" say so.
-      uint32_t slot = 0, slot_phase = 0, set = 0, done = U == 1 ? S - 2 : 0, done_phase = 1;
+      // The MMAs of kSets units ago, which read the set's columns, are done: a unit of one stage has that stage's "empty" say so.
+      uint32_t slot = 0, slot_phase = 0, set = 0, done = U == 1 ? S - SM::kSets : 0, done_phase = 1;
       for (Item i = first; i.t < ntiles && ok; step(i)) {
         for (uint32_t it = 0; it < KT && ok; it += U) {
           const uint32_t sub = it % kScaleStages;
           if (sub == 0) ok = mbar_wait_warp(bar(kScFull + slot), slot_phase, abort, error);
           if (ok) ok = mbar_wait_warp(bar((U == 1 ? kEmpty : kSetEmpty) + done), done_phase, abort, error);
           if (!ok) break;
-          if (++done == (U == 1 ? S : 2)) done = 0, done_phase ^= 1;
+          if (++done == (U == 1 ? S : SM::kSets)) done = 0, done_phase ^= 1;
           tc_fence_after();
           const uint32_t to = tmem_base + 2 * NT + set * SM::kUnitCols, to_rows = to + 8 * U, from = smem_u32(smem + SM::kScales + slot * SM::kSlotBytes);
           const uint32_t words = min(2 * U, (K - it * kStageK + 127) / 128);
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
               mma_commit(leader, bar(kScEmpty + slot));
             if (++slot == SL) slot = 0, slot_phase ^= 1;
           }
-          set ^= 1;
+          if (++set == SM::kSets) set = 0;
         }
       }
     }
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
           if (++s == S) s = 0, phase ^= 1;
           if (in_unit == U - 1 || it == KT - 1) {
             if constexpr (U > 1) commit(kSetEmpty + set, 1);
-            set_phase ^= set, set ^= 1;
+            if (++set == SM::kSets) set = 0, set_phase ^= 1;
           }
         }
         if (!ok) break;
@@ -565,15 +569,15 @@ void launch_product(const Mx4Args &args, const void *wc, const void *xc, cudaStr
   CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, maps));
 }
 
-// Tiles of 224 rows by pairs of CTAs where experts have more than 32 rows on average and there are 32 items for pairs at least; else of 32 by single
+// Tiles of 208 rows by pairs of CTAs where experts have more than 32 rows on average and there are 32 items for pairs at least; else of 32 by single
 // CTAs. gate_up and down by pairs and by single CTAs, us: 512 experts of 2,048 x 512, 10 rows 9 + 7 and 8 + 6, 1,000 rows 80 + 48 and 80 + 45,
 // 10,000 rows 98 + 60 and 97 + 54, 16,000 rows 100 + 67 and 107 + 72, 32,000 rows 105 + 75 and 185 + 129; one of 2,080 x 1,440, 200 rows (12 items for
 // pairs) 15 + 11 and 11 + 6, 777 rows (48) 15 + 11 and 17 + 10; one of 8,192 x 4,096, 128 rows (32) 19 + 12 and 24 + 14.
 template <class Out>
 void launch(const Mx4Args &a, const void *wc, const void *xc, cudaStream_t st) {
-  const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 224 + 1;
+  const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 208 + 1;
   if (a.R > 32ull * a.E && pieces * tiles >= 32)
-    launch_product<Out, 2, 224>(a, wc, xc, st);
+    launch_product<Out, 2, 208>(a, wc, xc, st);
   else
     launch_product<Out, 1, 32>(a, wc, xc, st);
 }
