@@ -52,20 +52,27 @@ __device__ __forceinline__ bool two_warps_all(uint32_t id, bool ok) {
   return r != 0;
 }
 
-// Eight lanes hold eight 4-bit codes each, code j of lane i becomes code i of lane j: three exchanges of the half a lane does not keep.
-__device__ __forceinline__ uint32_t transpose_codes(uint32_t v, uint32_t lane) {
-  const uint32_t a = __shfl_xor_sync(0xffffffffu, v, 4);
-  v = lane & 4 ? (v & 0xFFFF0000u) | a >> 16 : (v & 0x0000FFFFu) | a << 16;
-  const uint32_t b = __shfl_xor_sync(0xffffffffu, v, 2);
-  v = lane & 2 ? (v & 0xFF00FF00u) | (b >> 8 & 0x00FF00FFu) : (v & 0x00FF00FFu) | (b << 8 & 0xFF00FF00u);
-  const uint32_t c = __shfl_xor_sync(0xffffffffu, v, 1);
-  return lane & 1 ? (v & 0xF0F0F0F0u) | (c >> 4 & 0x0F0F0F0Fu) : (v & 0x0F0F0F0Fu) | (c << 4 & 0xF0F0F0F0u);
-}
+// Eight lanes hold eight 4-bit codes each, code j of lane i becomes code i of lane j: three exchanges of the half a lane does not keep, by halves,
+// by bytes and by codes.
+struct CodeTranspose {
+  uint32_t halves, bytes, shift, keep;
+  __device__ explicit CodeTranspose(uint32_t lane)
+      : halves(lane & 4 ? 0x3276u : 0x5410u), bytes(lane & 2 ? 0x3715u : 0x6240u), shift(lane & 1 ? 28 : 4), keep(lane & 1 ? 0xF0F0F0F0u : 0x0F0F0F0Fu) {}
+  __device__ uint32_t operator()(uint32_t v) const {
+    v = __byte_perm(v, __shfl_xor_sync(0xffffffffu, v, 4), halves);
+    v = __byte_perm(v, __shfl_xor_sync(0xffffffffu, v, 2), bytes);
+    const uint32_t c = __shfl_xor_sync(0xffffffffu, v, 1);
+    return (v & keep) | (__funnelshift_l(c, c, shift) & ~keep);
+  }
+};
 
-// silu(min(g, limit)) * u held to +-limit, in the fast forms: two significant bits of it stay. NaN passes through.
-__device__ __forceinline__ float swiglu_mx(float g, float u, float limit) {
-  float e, r;
+// min(g, limit) and u held to +-limit. NaN passes through.
+__device__ __forceinline__ void hold(float &g, float &u, float limit) {
   asm("min.NaN.f32 %0, %0, %2;\n\tmin.NaN.f32 %1, %1, %2;\n\tmax.NaN.f32 %1, %1, %3;" : "+f"(g), "+f"(u) : "f"(limit), "f"(-limit));
+}
+// silu(g) * u in the approximate forms: two significant bits of it stay.
+__device__ __forceinline__ float swiglu_mx(float g, float u) {
+  float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return g * r * u;
@@ -104,7 +111,7 @@ struct GateUp {};
 template <class Out, uint32_t CTAS, uint32_t NT>
 struct Mx4Form {
   static constexpr bool GU = std::is_same<Out, GateUp>::value;
-  static constexpr uint32_t kGroups = CTAS;  // of four epilogue warps
+  static constexpr uint32_t kGroups = CTAS == 1 ? 1 : GU ? 4 : 2;  // of four epilogue warps
   static constexpr uint32_t kThreads = 32 * (6 + 4 * kGroups);
   static constexpr uint32_t kStages = CTAS == 2 ? 5 : 8;
   static constexpr uint32_t kStageBytes = (kRowsM + NT / CTAS) * 128;
@@ -433,7 +440,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     // Warp w reads tensor memory's lanes 32 (w % 4) ...; the groups take chunks of 16 rows in turn.
     const uint32_t q = warp % 4, group = (warp - kEpilogueWarp) / 4;
     uint32_t b = 0, phase = 0;
-    [[maybe_unused]] const float limit = a.limit > 0.0f ? a.limit : INFINITY;
+    [[maybe_unused]] const CodeTranspose transpose(lane);
     for (Item i = first; i.t < ntiles && ok; step(i)) {
       const Tile t = tile_at(i);
       const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT;
@@ -486,30 +493,39 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
           for (uint32_t j = 0; j < 8; j++) mine[turn + 32 * j] = __uint_as_float(give[j]), h[j] = __uint_as_float(keep[j]);
           if (c + dc < t.count) tmem_ld8(keep_at + c + dc, keep), tmem_ld8(give_at + c + dc, give);
           two_warps_sync(2 * group + q % 2);
-          if (up) {
+          float got[8];
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++) h[j] = swiglu_mx(theirs[turn + 32 * j], h[j], limit);
-          } else {
+          for (uint32_t j = 0; j < 8; j++) got[j] = theirs[turn + 32 * j];
+          auto make_h = [&](float (&g)[8], float (&u)[8]) {
+            if (a.limit > 0.0f)
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++) h[j] = swiglu_mx(h[j], theirs[turn + 32 * j], limit);
-          }
-          // The rows' scales: f is the exponent of the largest magnitude, at least 2; 2^(127 - (f - 2)) is what the values are multiplied by. A row with
-          // an infinity or NaN (f 255) gets codes 0.
-          uint32_t f_of = 0;  // lane j's, and lanes 8 + j, ..: of the warp's row j
+              for (uint32_t j = 0; j < 8; j++) hold(g[j], u[j], a.limit);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) h[j] = swiglu_mx(g[j], u[j]);
+          };
+          if (up)
+            make_h(got, h);
+          else
+            make_h(h, got);
+          // The rows' scales: f is the exponent of the largest magnitude, at least 2; 2^(127 - (f - 2)) is what the values are multiplied by. A lane works
+          // one out, of row lane % 8, and the rows' eight lanes hand theirs round. A row with an infinity or NaN (f 255) gets codes 0.
+          float top = 0.0f;
 #pragma unroll
           for (uint32_t j = 0; j < 8; j++) {
-            const uint32_t f = max(__float_as_uint(largest_magnitude(h[j])) & 0x7F800000u, 2u << 23);
-            h[j] *= __uint_as_float(0x80000000u - f);
-            if (lane % 8 == j) f_of = f;
+            const float m = largest_magnitude(h[j]);
+            if (lane % 8 == j) top = m;
           }
+          const uint32_t f = max(__float_as_uint(top) & 0x7F800000u, 2u << 23);
+#pragma unroll
+          for (uint32_t j = 0; j < 8; j++) h[j] *= __uint_as_float(0x80000000u - __shfl_sync(0xffffffffu, f, j));
           // The warp's eight rows by eight features: lane j of each eight gets row j's codes of those features.
-          uint32_t codes = transpose_codes(mx_codes8(h), lane);
-          const bool bad = f_of == 0x7F800000u;
+          uint32_t codes = transpose(mx_codes8(h));
+          const bool bad = f == 0x7F800000u;
           if (bad) codes = 0;
           if (r < t.count && at < F) {
             *(uint32_t *)hc = codes;
             if (lane < 8) {
-              *hs = bad ? 255 : (uint8_t)((f_of >> 23) - 2);
+              *hs = bad ? 255 : (uint8_t)((f >> 23) - 2);
               if (at + kMxBlock == F)
                 for (uint32_t z = 1; z < hrow - (F / kMxBlock - 1); z++) hs[z] = 0;
             }
