@@ -113,7 +113,7 @@ struct Mx4Form {
   static constexpr bool GU = std::is_same<Out, GateUp>::value;
   static constexpr uint32_t kGroups = CTAS == 1 ? 1 : GU ? 4 : 2;  // of four epilogue warps
   static constexpr uint32_t kThreads = 32 * (6 + 4 * kGroups);
-  static constexpr uint32_t kStages = CTAS == 2 ? 5 : 8;
+  static constexpr uint32_t kStages = CTAS == 2 ? 5 : 6;
   static constexpr uint32_t kStageBytes = (kRowsM + NT / CTAS) * 128;
   static constexpr uint32_t kScaleSlots = 3;  // and as many warps to fill them
   // A word of 128 rows' scales is a piece of 512 bytes and four columns of tensor memory, even where there are fewer rows: an instruction's scales
@@ -142,14 +142,6 @@ struct Mx4Form {
 };
 
 enum : uint32_t { kCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kScaleCopyWarp = 5, kEpilogueWarp = 6 };
-
-// Rows a tile of an expert's n rows has: the tiles of a few share them evenly (which 16 rows a tile can be off by leaves no tile empty up to
-// eight tiles of 208).
-template <uint32_t NT>
-__device__ __forceinline__ uint32_t tile_rows(uint32_t n) {
-  const uint32_t tiles = (n + NT - 1) / NT;
-  return NT >= 128 && tiles > 1 && tiles <= 8 ? ((n + tiles - 1) / tiles + 15) & ~15u : NT;
-}
 
 template <class Out, uint32_t CTAS, uint32_t NT>
 __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_product(const __grid_constant__ Mx4Args a, const __grid_constant__ Mx4Maps maps) {
@@ -273,8 +265,8 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   };
   auto tile_at = [&](const Item &i) {
     const uint32_t e = i.t < kTileTable ? tile_expert[i.t] : expert_at(i.t);
-    const uint32_t r0 = first_row[e], r1 = first_row[e + 1], per = tile_rows<NT>(r1 - r0), start = r0 + (i.t - first_tile[e]) * per;
-    return Tile{e, start, min(per, r1 - start), (i.m * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
+    const uint32_t start = first_row[e] + (i.t - first_tile[e]) * NT;
+    return Tile{e, start, min(NT, first_row[e + 1] - start), (i.m * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
   };
 
   if (warp == kCopyWarp) {
