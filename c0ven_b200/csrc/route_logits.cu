@@ -224,9 +224,9 @@ __device__ __forceinline__ void load_bias(const RouteArgs &a, uint32_t lane, flo
   }
 }
 
-// Doubles of shared memory a warp has for a row: a key an expert, and room for 32 candidates and one place behind them.
+// Doubles of shared memory a warp has for a row: a key an expert, or 32 candidates.
 template <int V>
-constexpr uint32_t kRouteScratch = V == 1 ? 34 : 32 * V;
+constexpr uint32_t kRouteScratch = 32 * V;
 
 // One row, by a warp, with kRouteScratch<V> doubles of shared memory of its own. Lane j < k returns the j-th expert (kNone: none) after writing ids and w.
 template <class L, int V>
@@ -320,17 +320,14 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
   uint32_t id = kNone;
   if (n > 32) sure = false;
   if (sure && n > 0) {
-    // (key, expert) of each, all keys written without a branch, those that are none into a place behind; then as integers that order as they do.
+    // (key, expert) of each, then as integers that order as they do.
     float2 *found = (float2 *)sk;
     uint32_t put = upto - mine;
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      const bool in = key[i] >= least;
-      found[in ? put : 32u] = make_float2(key[i], __uint_as_float(lane + 32 * i));
-      put += in ? 1u : 0u;
-    }
+    for (int i = 0; i < V; i++)
+      if (key[i] >= least) found[put++] = make_float2(key[i], __uint_as_float(lane + 32 * i));
     __syncwarp();
-    const float2 got = found[lane];
+    const float2 got = found[lane];  // behind the n-th: whatever is there
     uint64_t own = lane < n ? (uint64_t)ordered(got.x) << 32 | ~__float_as_uint(got.y) : 0;
     uint64_t *order = (uint64_t *)sk;
     __syncwarp();
