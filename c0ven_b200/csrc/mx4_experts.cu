@@ -176,13 +176,15 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     *abort = 0;
     fence_barrier_init();
   }
+  // Tensor memory is taken when the kernels before are done, and the next may come when it is: a kernel that held it while it waits for another on the
+  // same SM, which asks for it later, would wait for ever.
+  wait_for_predecessors();
   if (warp == kMmaWarp) {
     if constexpr (CTAS == 2)
       tmem_alloc_pair(smem_u32(tmem_slot), SM::kCols);
     else
       tmem_alloc(smem_u32(tmem_slot), SM::kCols);
   }
-  dependents_may_launch(), wait_for_predecessors();
   // The experts' first rows and first tiles, E + 1 <= 513 entries, two a thread. Offsets are held to 0 .. R, and to rise: each to the largest
   // before it.
   {
@@ -205,6 +207,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     if (e <= a.E) first_row[e] = r0;
     if (e < a.E) first_row[e + 1] = r1;
     __syncthreads();
+    dependents_may_launch();
     const uint32_t r2 = e + 2 <= a.E ? first_row[e + 2] : r1;
     const uint32_t t0 = e < a.E ? (r1 - r0 + NT - 1) / NT : 0, t1 = e + 1 < a.E ? (r2 - r1 + NT - 1) / NT : 0;
     uint32_t sum = t0 + t1;
