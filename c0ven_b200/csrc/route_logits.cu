@@ -10,8 +10,9 @@
 // logits alone, by the accurate exponential, relative to the largest of them, so that they neither overflow nor vanish together.
 //
 // The lists: rows are counted by chunks of 32, an expert's rows of a chunk a bit each of a word in shared memory, so that a row's place
-// among them is a population count. A scan over the chunks' counts and a pass over the assignments follow; short steps are one CTA's.
+// among them is a population count. A scan over the chunks' counts and a pass over the assignments follow; short steps are one cluster's.
 //
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -32,9 +33,8 @@ namespace {
 
 constexpr uint32_t kRouteMaxExperts = 512, kRouteMaxUsed = 16, kRouteMaxGroups = 32;
 constexpr uint32_t kRouteChunk = 32;       // rows whose experts are counted together
-constexpr uint32_t kRouteWarps = 8;        // of a CTA that takes a chunk, or a step of up to kRouteFewRows rows
-constexpr uint32_t kRouteFewRows = 16;
-constexpr uint32_t kRouteOneCta = 64;      // rows that one CTA of 32 warps routes and lists by itself
+constexpr uint32_t kRouteWarps = 8;        // of a CTA
+constexpr uint32_t kRouteShort = 64;       // rows that one cluster of eight CTAs routes and lists by itself, a warp a row
 constexpr uint32_t kRoutePlaces = 512;     // assignments a CTA of the last pass takes
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(1024) k_route_scan(uint32_t *work, uint32_t ch
   if (threadIdx.x >= 1016 && e < E) at[(uint64_t)chunks * E] = run;
 }
 
-// Exclusive sums of E <= 512 counts, thread i's of experts 2 i and 2 i + 1, by a block of W >= 8 warps; s: 8 words.
+// Exclusive sums of E <= 512 counts, thread i's of experts 2 i and 2 i + 1, by a block of 8 warps; s: 8 words.
 __device__ __forceinline__ uint32_t exclusive_sum(uint32_t pair, uint32_t *s) {
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   uint32_t v = pair;
@@ -483,10 +483,10 @@ __device__ __forceinline__ uint32_t exclusive_sum(uint32_t pair, uint32_t *s) {
     const uint32_t o = __shfl_up_sync(0xffffffffu, v, off);
     if (lane >= (uint32_t)off) v += o;
   }
-  if (lane == 31 && warp < 8) s[warp] = v;
+  if (lane == 31) s[warp] = v;
   __syncthreads();
   uint32_t before = 0;
-  for (uint32_t i = 0; i < min(warp, 8u); i++) before += s[i];
+  for (uint32_t i = 0; i < warp; i++) before += s[i];
   return before + v - pair;
 }
 
@@ -516,35 +516,51 @@ __global__ void __launch_bounds__(256) k_route_places(const RouteArgs a, uint32_
   }
 }
 
-// A short step by one CTA of W warps: rows, counts, offsets and places in one launch. Dynamic shared memory: kRouteScratch<V> doubles a warp.
-template <class L, int V, int W>
-__global__ void __launch_bounds__(32 * W) k_route_short(const RouteArgs a) {
-  extern __shared__ __align__(16) double s_dyn[];
-  __shared__ uint32_t s_ids[kRouteOneCta * kRouteMaxUsed], s_scan[8], s_first[kRouteMaxExperts], rows_of[2][kRouteMaxExperts];  // a bit a row, 64 in all
+// A short step in one launch, a warp a row: a cluster of up to eight CTAs, each with eight rows, which read one another's counts. (One CTA of 32 warps
+// took 11 us for 37 rows in groups, bound by its SM's issue slots; this takes 6.)
+template <class L, int V>
+__global__ void __launch_bounds__(32 * kRouteWarps) k_route_short(const RouteArgs a) {
+  __shared__ __align__(16) double sk[kRouteWarps][kRouteScratch<V>];
+  __shared__ uint32_t s_scan[8], s_first[kRouteMaxExperts];
+  __shared__ __align__(8) uint32_t rows_of[kRouteMaxExperts];  // a bit a row of this CTA
+  __shared__ uint64_t all_rows_of[kRouteMaxExperts];           // a bit a row
   dependents_may_launch(), wait_for_predecessors();
-  const uint32_t i = threadIdx.x, warp = i / 32, lane = i % 32;
-  for (uint32_t j = i; j < kRouteMaxExperts; j += 32 * W) rows_of[0][j] = rows_of[1][j] = 0;
-  float bias[V];
-  load_bias(a, lane, bias);
+  const uint32_t i = threadIdx.x, warp = i / 32, lane = i % 32, t = blockIdx.x * kRouteWarps + warp;
+  rows_of[2 * i] = rows_of[2 * i + 1] = 0;
   __syncthreads();
-  for (uint32_t t = warp; t < a.T; t += W) {
-    const uint32_t id = route_row<L, V>(a, t, lane, bias, s_dyn + warp * kRouteScratch<V>);
-    if (lane < a.k) s_ids[t * a.k + lane] = id;
-    if (id != kNone) atomicOr(&rows_of[t / 32][id], 1u << (t % 32));
+  uint32_t id = kNone;
+  if (t < a.T) {
+    float bias[V];
+    load_bias(a, lane, bias);
+    id = route_row<L, V>(a, t, lane, bias, sk[warp]);
+    if (a.offsets && id != kNone) atomicOr(&rows_of[id], 1u << warp);
   }
   if (!a.offsets) return;
-  __syncthreads();
   const uint32_t e = 2 * i;
-  auto count = [&](uint32_t x) { return x < a.E ? (uint32_t)(__popc(rows_of[0][x]) + __popc(rows_of[1][x])) : 0u; };
-  const uint32_t n0 = count(e), n1 = count(e + 1), first = exclusive_sum(n0 + n1, s_scan);
-  if (e < a.E) a.offsets[e] = (int32_t)first, s_first[e] = first;
-  if (e + 1 < a.E) a.offsets[e + 1] = (int32_t)(first + n0), s_first[e + 1] = first + n0;
-  if (e == a.E - 1 || e + 1 == a.E - 1) a.offsets[a.E] = (int32_t)(first + n0 + n1);
-  __syncthreads();
-  for (uint32_t j = i; j < a.T * a.k; j += 32 * W) {
-    const uint32_t id = s_ids[j], t = j / a.k, below = (1u << (t % 32)) - 1;
-    a.inv[j] = id < a.E ? (int32_t)(s_first[id] + (t < 32 ? __popc(rows_of[0][id] & below) : __popc(rows_of[0][id]) + __popc(rows_of[1][id] & below))) : -1;
+  uint64_t r0 = 0, r1 = 0;
+  if (gridDim.x == 1) {  // a CTA alone is launched as no cluster
+    __syncthreads();
+    r0 = rows_of[e], r1 = rows_of[e + 1];
+  } else {
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    for (uint32_t c = 0; c < gridDim.x; c++) {
+      const uint2 r = *(const uint2 *)(cluster.map_shared_rank(rows_of, c) + e);
+      r0 |= (uint64_t)r.x << kRouteWarps * c, r1 |= (uint64_t)r.y << kRouteWarps * c;
+    }
+    cluster.sync();  // no CTA leaves while another reads its counts
   }
+  all_rows_of[e] = r0, all_rows_of[e + 1] = r1;
+  const uint32_t n0 = __popcll(r0), n1 = __popcll(r1), first = exclusive_sum(n0 + n1, s_scan);
+  s_first[e] = first, s_first[e + 1] = first + n0;
+  if (blockIdx.x == 0) {
+    if (e < a.E) a.offsets[e] = (int32_t)first;
+    if (e + 1 < a.E) a.offsets[e + 1] = (int32_t)(first + n0);
+    if (e == a.E - 1 || e + 1 == a.E - 1) a.offsets[a.E] = (int32_t)(first + n0 + n1);
+  }
+  __syncthreads();
+  if (t < a.T && lane < a.k)
+    a.inv[(uint64_t)t * a.k + lane] = id < a.E ? (int32_t)(s_first[id] + __popcll(all_rows_of[id] & ((1ull << t) - 1))) : -1;
 }
 
 __global__ void __launch_bounds__(512) k_route_empty(int32_t *offsets, uint32_t n) {
@@ -552,18 +568,17 @@ __global__ void __launch_bounds__(512) k_route_empty(int32_t *offsets, uint32_t 
   for (uint32_t i = threadIdx.x; i < n; i += 512) offsets[i] = 0;
 }
 
-template <class L, int V, int W>
-void launch_short(const RouteArgs &a, int device, cudaStream_t st) {
-  constexpr size_t smem = W * kRouteScratch<V> * sizeof(double);
-  static std::atomic<uint32_t> done{0};
-  CUDA_OK(ensure_dynamic_smem(k_route_short<L, V, W>, smem, done, device));
-  CUDA_OK(launch_kernel(true, k_route_short<L, V, W>, dim3(1), dim3(32 * W), smem, st, a));
-}
-
 template <class L, int V>
-void launch_rows(const RouteArgs &a, int device, cudaStream_t st) {
-  if (a.T <= kRouteFewRows) return launch_short<L, V, kRouteWarps>(a, device, st);
-  if (a.T <= kRouteOneCta) return launch_short<L, V, 32>(a, device, st);
+void launch_rows(const RouteArgs &a, cudaStream_t st) {
+  if (a.T <= kRouteShort) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension, at[1].val.clusterDim = {(a.T + kRouteWarps - 1) / kRouteWarps, 1, 1};
+    cfg.gridDim = dim3(at[1].val.clusterDim.x), cfg.blockDim = dim3(32 * kRouteWarps), cfg.stream = st, cfg.attrs = at, cfg.numAttrs = cfg.gridDim.x > 1 ? 2 : 1;
+    CUDA_OK(cudaLaunchKernelEx(&cfg, k_route_short<L, V>, a));
+    return;
+  }
   const uint32_t chunks = (a.T + kRouteChunk - 1) / kRouteChunk;
   CUDA_OK(launch_kernel(true, k_route_rows<L, V>, dim3(chunks), dim3(32 * kRouteWarps), 0, st, a));
   if (!a.offsets) return;
@@ -572,17 +587,17 @@ void launch_rows(const RouteArgs &a, int device, cudaStream_t st) {
 }
 
 template <class L>
-void launch_route(const RouteArgs &a, int device, cudaStream_t st) {
+void launch_route(const RouteArgs &a, cudaStream_t st) {
   if (a.E <= 32)
-    launch_rows<L, 1>(a, device, st);
+    launch_rows<L, 1>(a, st);
   else if (a.E <= 64)
-    launch_rows<L, 2>(a, device, st);
+    launch_rows<L, 2>(a, st);
   else if (a.E <= 128)
-    launch_rows<L, 4>(a, device, st);
+    launch_rows<L, 4>(a, st);
   else if (a.E <= 256)
-    launch_rows<L, 8>(a, device, st);
+    launch_rows<L, 8>(a, st);
   else
-    launch_rows<L, 16>(a, device, st);
+    launch_rows<L, 16>(a, st);
 }
 
 }  // namespace
@@ -621,21 +636,19 @@ MOE_API moe_status moe_route_logits_device(const moe_route_config *config, const
       if (offsets_dev) CUDA_OK(launch_kernel(true, k_route_empty, dim3(1), dim3(512), 0, st, offsets_dev, c.n_experts + 1));
       return;
     }
-    const bool lists = offsets_dev && T > kRouteOneCta;
+    const bool lists = offsets_dev && T > kRouteShort;
     need(!lists || work_bytes >= moe_route_work_bytes(T, c.n_experts), "work must hold moe_route_work_bytes bytes");
     need_device({{logits_dev, "logits", size}, {bias_dev, "bias", 4, true}, {ids_dev, "ids", 4}, {w_dev, "w", 4}, {offsets_dev, "offsets", 4, true},
                  {inv_dev, "inv", 4, true}, {lists ? work_dev : nullptr, "work", 4, !lists}});
     RouteArgs a{logits_dev, stride ? stride : c.n_experts, bias_dev, T, c.n_experts, c.n_used, G, c.n_groups_used, c.n_experts / G,
                 c.score == MOE_SCORE_SIGMOID, c.no_renorm == 0, c.scale == 0.0f ? 1.0f : c.scale, ids_dev, w_dev, offsets_dev, inv_dev,
                 lists ? (uint32_t *)work_dev : nullptr};
-    int device = 0;
-    CUDA_OK(cudaGetDevice(&device));
     if (c.logits_type == MOE_TYPE_F32)
-      launch_route<float>(a, device, st);
+      launch_route<float>(a, st);
     else if (c.logits_type == MOE_TYPE_F16)
-      launch_route<__half>(a, device, st);
+      launch_route<__half>(a, st);
     else
-      launch_route<__nv_bfloat16>(a, device, st);
+      launch_route<__nv_bfloat16>(a, st);
   });
 }
 
