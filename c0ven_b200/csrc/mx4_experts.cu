@@ -645,11 +645,14 @@ MOE_API moe_status moe_mx4_gate_up_device(const moe_mx4_weights *w, const void *
 
 MOE_API moe_status moe_ops_status(uint32_t timeout_ms, void *stream) {
   return ops_call([&] {
-    Stream::wait_on((cudaStream_t)stream, timeout_ms);
+    cudaStream_t st = (cudaStream_t)stream;
+    Stream::wait_on(st, timeout_ms);
     uint32_t gave_up = 0, none = 0;
-    CUDA_OK(cudaMemcpyFromSymbol(&gave_up, g_gave_up, sizeof gave_up));
+    CUDA_OK(cudaMemcpyFromSymbolAsync(&gave_up, g_gave_up, sizeof gave_up, 0, cudaMemcpyDeviceToHost, st));
+    Stream::wait_on(st, timeout_ms);
     if (!gave_up) return;
-    CUDA_OK(cudaMemcpyToSymbol(g_gave_up, &none, sizeof none));
+    CUDA_OK(cudaMemcpyToSymbolAsync(g_gave_up, &none, sizeof none, 0, cudaMemcpyHostToDevice, st));
+    Stream::wait_on(st, timeout_ms);
     throw Timeout("a product gave up waiting for its copies or its products: its results are not to be used");
   });
 }

@@ -361,7 +361,8 @@ MOE_API moe_status moe_route_logits_device(const moe_route_config *config, const
 /* Rows of K values (type MOE_TYPE_F32, F16 or BF16; stride values apart, 0: K; rows 16-byte aligned) to MX rows. A block's
  * scale is 2^(floor(log2 of its largest magnitude) - 2), at least 2^-127; codes are the nearest values, ties to even, beyond 6
  * to 6. A block with an infinity or NaN gets scale 255 and codes 0. inv_dev null: row t to row t of R = T rows. Else [T][n_used], and
- * row t goes to each row inv_dev[t][k] of the R (one outside 0 .. R - 1 is skipped); a row no entry names is left as it was.
+ * row t goes to each row inv_dev[t][k] of the R (one outside 0 .. R - 1 is skipped); a row no entry names is left as it was,
+ * a row that two name may get a mixture of them.
  * dequantize: what R MX rows stand for, rounded to type where that has fewer bits or less range; [R][K], 16-byte aligned.
  * from_blocks: rows of a GGUF tensor of ggml type 39 (17-byte blocks: the scale, then 16 bytes whose low halves are values 0 .. 15
  * and high halves 16 .. 31) to MX rows, which is how the experts' matrices of a file get into the form below. */
@@ -401,7 +402,7 @@ MOE_API moe_status moe_mx4_gate_up_device(const moe_mx4_weights *w, const void *
 MOE_API moe_status moe_combine_rows_device(const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev, const float *w_dev, uint32_t T,
                                            uint32_t n_used, uint32_t n_embd, const float *residual_dev, float *out_dev, void *stream);
 /* Waits for stream, timeout_ms at most (0: 60 s). MOE_TIMEOUT when that ran out, or when a product on the current device has given up one of its
- * own waits (each bounded, some seconds) since this was last asked: its results are then not to be used. */
+ * own waits (each bounded, about a second) since this was last asked: its results are then not to be used. Not while stream is captured. */
 MOE_API moe_status moe_ops_status(uint32_t timeout_ms, void *stream);
 MOE_API const char *moe_ops_error(void);
 

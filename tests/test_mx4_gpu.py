@@ -227,7 +227,10 @@ def sum_bound(magnitude, K):
 
 SHAPES = [(1, 32, 32, [5]), (1, 64, 96, [1]), (1, 160, 256, [300]), (3, 128, 64, [0, 7, 130]), (8, 96, 544, [1, 0, 2, 64, 65, 0, 17, 1]),
           (5, 288, 2880, [16, 15, 0, 33, 1]), (2, 2080, 160, [129, 257]), (70, 64, 128, [1] * 70), (4, 32, 4096, [0, 0, 0, 3]), (512, 32, 32, [0, 1] * 256),
-          (2, 256, 2880, [225, 33]), (1, 288, 1312, [1793]), (7, 544, 4128, [0, 448, 449, 1, 100, 17, 224])]
+          (2, 256, 2880, [225, 33]), (1, 288, 1312, [1793]), (7, 544, 4128, [0, 448, 449, 1, 100, 17, 224]), (1, 32, 65536, [3]), (1, 65536, 32, [2]),
+          # Enough rows an expert and items for pairs of CTAs.
+          (1, 2080, 160, [900]), (3, 1056, 1312, [209, 0, 1100]), (7, 544, 2880, [0, 448, 449, 1, 100, 17, 1700]), (2, 8224, 96, [33, 64]), (2, 4128, 4064, [417, 16]),
+          (1, 65536, 64, [40])]
 
 
 @pytest.mark.parametrize("y_type", ["f16", "bf16"])
@@ -302,7 +305,8 @@ def test_nan_scales_reach_their_rows_alone():
 
 @pytest.mark.parametrize("limit", [0.0, 2.0])
 @pytest.mark.parametrize("E, F, K, counts", [(1, 32, 32, [5]), (3, 64, 96, [0, 7, 130]), (6, 96, 2880, [1, 0, 33, 64, 2, 0]), (2, 224, 256, [129, 257]), (1, 640, 544, [300]),
-                                           (3, 288, 1312, [225, 0, 500]), (2, 160, 2880, [100, 40])])
+                                           (3, 288, 1312, [225, 0, 500]), (2, 160, 2880, [100, 40]),
+                                           (1, 1056, 160, [900]), (3, 672, 1312, [209, 0, 1100]), (7, 288, 2880, [0, 448, 449, 1, 100, 17, 1700]), (2, 4128, 96, [33, 64])])
 def test_gate_up(E, F, K, counts, limit):
     import torch
 
@@ -378,6 +382,51 @@ def test_products_on_a_stream_and_in_a_graph():
     want = by_expert(x2, w, [0, 0, 64, 64, 65, 66, 99], rows)
     assert (z[99] == 7).all()
     assert np.linalg.norm(z[:99].double().cpu().numpy() - want[:99]) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(want)
+
+
+def test_products_side_by_side():
+    """Two products and a routing on three streams at once, many times over: each has its own results."""
+    import torch
+
+    rng = np.random.default_rng(14)
+    jobs = []
+    for E, N, K, rows in ((6, 2080, 544, 900), (40, 128, 2080, 90)):
+        offsets = np.sort(rng.integers(0, rows + 1, E + 1)).astype(np.int32)
+        offsets[0], offsets[-1] = 0, rows
+        wc, ws, w, xc, xs, x = product_case(rng, E, N, K, None, rows)
+        jobs.append((torch.cuda.Stream(), ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr()), xc, xs, rows, dev(offsets), torch.zeros((rows, N), dtype=torch.float16, device="cuda"),
+                     by_expert(x, w, offsets, rows), (wc, ws)))
+    logits = dev(rng.standard_normal((500, 64)).astype(np.float32))
+    ids, rw, st = torch.zeros((500, 4), dtype=torch.int32, device="cuda"), torch.zeros((500, 4), device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, w, xc, xs, rows, od, y, _, _ in jobs:
+            ops.mx4_product_device(w, xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), y.data_ptr(), ops.F16, stream=s.cuda_stream)
+        ops.route_logits_device(logits.data_ptr(), ops.F32, 500, 64, 4, ids.data_ptr(), rw.data_ptr(), stream=st.cuda_stream)
+    for s, *_ in jobs:
+        ops.status(s.cuda_stream)
+    torch.cuda.synchronize()
+    for *_, y, want, _ in jobs:
+        assert np.linalg.norm(y.double().cpu().numpy() - want) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(want)
+    assert np.array_equal(ids.cpu().numpy(), R.route(logits.double().cpu().numpy(), 4)[0])
+
+
+def test_same_bits_every_time():
+    import torch
+
+    rng = np.random.default_rng(15)
+    E, N, K, rows = 4, 1088, 1312, 1300
+    offsets = dev(np.array([0, 300, 301, 900, 1300], np.int32))
+    wc, ws, _, xc, xs, _ = product_case(rng, E, N, K, None, rows)
+    weights = ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr())
+    y, first = torch.empty((rows, N), dtype=torch.bfloat16, device="cuda"), None
+    (hc, hs), h_first = mx_buffers(rows, N // 2), None
+    for _ in range(10):
+        y.fill_(9)
+        ops.mx4_product_device(weights, xc.data_ptr(), xs.data_ptr(), rows, offsets.data_ptr(), y.data_ptr(), ops.BF16)
+        ops.mx4_gate_up_device(weights, xc.data_ptr(), xs.data_ptr(), rows, offsets.data_ptr(), hc.data_ptr(), hs.data_ptr())
+        first, h_first = first if first is not None else y.clone(), h_first if h_first is not None else (hc.clone(), hs.clone())
+        assert torch.equal(y, first) and torch.equal(hc, h_first[0]) and torch.equal(hs, h_first[1])
 
 
 @pytest.mark.parametrize("y_type", ["f32", "f16", "bf16"])
