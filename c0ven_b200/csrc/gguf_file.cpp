@@ -58,6 +58,7 @@ uint32_t scalar_size(uint32_t type) {
 uint64_t gguf_type_bytes(uint32_t type, uint64_t elements) {
   if (type == GGML_F32) return elements * 4;
   if (type == GGML_F16 || type == GGML_BF16) return elements * 2;
+  if (type == GGML_MXFP4) return elements % 32 ? 0 : elements / 32 * 17;  // for moe_mx4_from_blocks_device; no layer takes it
   if (!type_known(type) || elements % block_values(type)) return 0;
   return elements / block_values(type) * block_bytes(type);
 }

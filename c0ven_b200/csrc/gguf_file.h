@@ -12,7 +12,7 @@
 namespace moe {
 
 // ggml's numbers for the unquantised types a router or a norm may be stored in (shared/quant.h:10-33).
-enum : uint32_t { GGML_F32 = 0, GGML_F16 = 1, GGML_BF16 = 30 };
+enum : uint32_t { GGML_F32 = 0, GGML_F16 = 1, GGML_BF16 = 30, GGML_MXFP4 = 39 };
 
 struct GgufTensorInfo {
   std::string name;

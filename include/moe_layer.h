@@ -188,7 +188,8 @@ MOE_API moe_status moe_layer_combine_device(moe_layer *l, const void *y_dev, uin
  *   moe_gguf_layers: "<general.architecture>.block_count", or 0 if the file does not say.
  *   moe_gguf_tensors: the table, up to cap rows into table (which may be null); returns how many tensors there are.
  *     name points into the handle and lives as long as it; shape is in ggml's order (shape[0] the contiguous axis);
- *     offset is from the file's start; bytes is 0 for a type this library does not read.
+ *     offset is from the file's start; bytes is 0 for a type this library does not read (ggml type 39 is read by
+ *     moe_mx4_from_blocks_device alone, not by a layer).
  *   moe_layer_create_from_gguf: layer N's blk.N.ffn_gate_inp.weight [n_embd][n_experts] (F32, F16 or BF16),
  *     ffn_gate_exps, ffn_up_exps [n_embd][n_ff][n_experts], ffn_down_exps [n_ff][n_embd][n_experts] and, when the file
  *     has them, ffn_gate_inp_shexp [n_embd] with ffn_{gate,up,down}_shexp. The sizes and types come from the tensors;

@@ -199,6 +199,19 @@ def test_rows_of_a_files_blocks():
         assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
 
 
+def test_blocks_stand_for_what_gguf_py_says():
+    import torch
+
+    gguf = pytest.importorskip("gguf")
+    blocks = np.random.default_rng(6).integers(0, 256, (50, 9 * 17), dtype=np.uint8)
+    blocks[:, ::17] = np.random.default_rng(7).integers(1, 250, (50, 9))
+    codes, scales = mx_buffers(50, 288)
+    out, bd = torch.empty((50, 288), device="cuda"), dev(blocks)
+    ops.mx4_from_blocks_device(bd.data_ptr(), 50, 288, codes.data_ptr(), scales.data_ptr())
+    ops.mx4_dequantize_rows_device(codes.data_ptr(), scales.data_ptr(), 50, 288, out.data_ptr(), ops.F32)
+    assert np.array_equal(out.cpu().numpy(), gguf.quants.dequantize(blocks, gguf.GGMLQuantizationType.MXFP4))
+
+
 def product_case(rng, E, N, K, offsets, rows):
     """Weights and rows with their values: w (codes, scales) [E][N], x [rows]."""
     (wc, ws), w = R.random_mx(rng, (E, N, K))

@@ -139,3 +139,28 @@ def test_the_plain_forms_agree_with_the_cases_plain_forms():
 def test_scale_rows_fill_words():
     assert [ops.mx4_scale_row_bytes(k) for k in (32, 128, 160, 2880, 4096)] == [4, 4, 8, 92, 128]
     assert C.sizeof(_lib.Mx4Weights) == 32 and C.sizeof(_lib.RouteConfig) == 32
+
+
+def test_a_files_mx_tensors_are_listed_and_no_layers(tmp_path):
+    """ggml type 39: the table says where the blocks lie, as gguf-py does; a layer of them is refused with the reason."""
+    gguf = pytest.importorskip("gguf")
+    from c0ven_b200 import synth
+    from c0ven_b200.layer import GgufFile, MoELayer
+
+    layer = synth.make_layer(n_embd=256, n_ff=256, n_experts=32, n_used=4, gate_type=synth.Q8_0, seed=9)
+    blocks = np.random.default_rng(9).integers(0, 255, (32, 256, 256 // 32 * 17), dtype=np.uint8)
+    mx = dict(layer, gate_type=39, gate_exps=blocks, up_exps=blocks)
+    synth.write_gguf(tmp_path / "mx.gguf", [mx])
+    f = GgufFile(tmp_path / "mx.gguf")
+    theirs = {t.name: t for t in gguf.GGUFReader(str(tmp_path / "mx.gguf")).tensors}
+    ty, shape, offset, nbytes = f.tensors()["blk.0.ffn_gate_exps.weight"]
+    t = theirs["blk.0.ffn_gate_exps.weight"]
+    assert (ty, shape, offset, nbytes) == (39, (256, 256, 32), t.data_offset, t.n_bytes) and nbytes == blocks.size
+    assert open(tmp_path / "mx.gguf", "rb").read()[offset:offset + nbytes] == blocks.tobytes()
+    with pytest.raises(MoEError) as e:
+        MoELayer.from_gguf(f, 0)
+    assert "type 39" in str(e.value) and "does not decode" in str(e.value)
+    with pytest.raises(MoEError) as e:
+        MoELayer(mx)
+    assert e.value.status == _lib.MOE_BAD_ARGUMENT
+    f.close()
