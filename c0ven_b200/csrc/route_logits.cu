@@ -320,42 +320,40 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
   uint32_t id = kNone;
   if (n > 32) sure = false;
   if (sure && n > 0) {
-    // (key, expert) of each, then as integers that order as they do.
-    float2 *found = (float2 *)sk;
+    float *found = (float *)sk;                // the keys, and behind them
+    uint32_t *expert = (uint32_t *)sk + 32;    // their experts
     uint32_t put = upto - mine;
 #pragma unroll
     for (int i = 0; i < V; i++)
-      if (key[i] >= least) found[put++] = make_float2(key[i], __uint_as_float(lane + 32 * i));
+      if (key[i] >= least) found[put] = key[i], expert[put++] = lane + 32 * i;
+    if (lane >= n) found[lane] = -INFINITY;
     __syncwarp();
-    const float2 got = found[lane];  // behind the n-th: whatever is there
-    uint64_t own = lane < n ? (uint64_t)ordered(got.x) << 32 | ~__float_as_uint(got.y) : 0;
-    uint64_t *order = (uint64_t *)sk;
-    __syncwarp();
-    order[lane] = own;
-    __syncwarp();
+    const float own = found[lane];
+    const uint32_t own_e = expert[lane];
     uint32_t rank = 0;
     for (uint32_t j = 0; j < n; j += 4) {
-      const ulonglong2 o = *(const ulonglong2 *)(order + j), q = *(const ulonglong2 *)(order + j + 2);
-      rank += (o.x > own ? 1u : 0u) + (o.y > own ? 1u : 0u) + (q.x > own ? 1u : 0u) + (q.y > own ? 1u : 0u);
+      const float4 o = *(const float4 *)(found + j);
+      rank += (o.x > own ? 1u : 0u) + (o.y > own ? 1u : 0u) + (o.z > own ? 1u : 0u) + (o.w > own ? 1u : 0u);
     }
+    // Without ties the ranks are 0 .. n - 1. With them, a lane's equals of lower experts come before it too.
+    if (__reduce_add_sync(0xffffffffu, lane < n ? rank : 0u) != n * (n - 1) / 2)
+      for (uint32_t j = 0; j < n; j++) rank += found[j] == own && expert[j] < own_e ? 1u : 0u;
     __syncwarp();
-    if (lane < n) order[rank] = own;
+    if (lane < n) found[rank] = own, expert[rank] = own_e;
     __syncwarp();
-    own = order[lane];
-    const uint64_t after = order[min(lane + 1, 31u)];
+    const float here = found[lane], next = found[min(lane + 1, 31u)];
+    const uint32_t e = expert[lane];
     __syncwarp();
-    if (lane < a.k && lane < n) id = ~(uint32_t)own;
+    if (lane < a.k && lane < n) id = e;
     // With a bias no two neighbours may lie within what their scores and their sums' roundings may be off by (rounding keeps an order, so
     // neighbours are all that has to be looked at). Without one the keys are the logits, as they are.
     if (a.bias) {
-      const float here = unordered((uint32_t)(own >> 32)), next = unordered((uint32_t)(after >> 32));
       const float off = 2 * err + 2.3841858e-7f * fmaxf(fabsf(here), fabsf(next));
       const bool open = lane < a.k && lane + 1 < n && !(here - next > off);
       sure = !__any_sync(0xffffffffu, open);
       // Sigmoids of the candidates alone in f64, a lane each, where no other key can come near the last one taken.
       const float kth = __shfl_sync(0xffffffffu, here, a.k - 1);
       if (!sure && a.sigmoid && n >= need && kth - least > 2 * err + 2.3841858e-7f * fmaxf(fabsf(kth), fabsf(least))) {
-        const uint32_t e = lane < n ? ~(uint32_t)own : kNone;
         const double v = lane < n ? sigmoid_key((double)logit_of<L>(a, t, e)) + a.bias[e] : -INFINITY;
         rank = 0;
         for (uint32_t j = 0; j < n; j++) {
