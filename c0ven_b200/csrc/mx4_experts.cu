@@ -322,6 +322,11 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
         const uint32_t b0 = j * (kScaleStages * kStageK / kMxBlock) + 4 * word, n = b0 < nb ? min(4u, nb - b0) : 0u;
         // Up to 32 rows from src on, have of them, to the lane's places from `to` on; zeros behind them.
         auto bring = [&](uint32_t to, const uint8_t *src, uint32_t have) {
+          if (__all_sync(0xffffffffu, have == 32 && n == 4)) {
+#pragma unroll 8
+            for (uint32_t k = 0; k < 32; k++, src += srow) copy_word(to + 16 * k, src);
+            return;
+          }
 #pragma unroll 8
           for (uint32_t k = 0; k < 32; k++, src += srow) {
             const uint32_t m = k < have ? n : 0;

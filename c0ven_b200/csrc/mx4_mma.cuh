@@ -79,6 +79,9 @@ __device__ __forceinline__ void tma_load_codes(uint32_t dst_smem, const CUtensor
 __device__ __forceinline__ void copy_word(uint32_t dst, const void *src, uint32_t n) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void copy_word(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy_words_wait() {
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
 }
