@@ -3,15 +3,18 @@
 //
 // A warp takes a row; lane l holds experts l, l + 32, .... Keys (score + bias) are first worked out in f32 with the fast exponential and
 // reciprocal. A bound that n_used of the lanes' own largest keys reach, found by halving between the least and the largest of them, is one that
-// n_used keys reach: the few keys not under it (some 18 for 10 of 512) are gathered, one a lane, and each finds its rank by looking at the others. That decides the row when every two
-// neighbours among the first n_used + 1 are further apart than the f32 keys' error (key_error): the order is then that of the exact
-// keys. Else (a row in some 600 for a bias and 512 experts) the candidates' own keys are worked out in f64, or, where keys that are no
-// candidates may come near them, where groups lie that near or ties leave more than 32 keys, the whole row's. Without bias and groups the scores' order is the logits' own, which are exact. The weights come from the chosen
-// logits alone, by the accurate exponential, relative to the largest of them, so that they neither overflow nor vanish together.
+// n_used keys reach: the few keys not under it are gathered, one a lane, and each finds its rank by looking at the others. That decides the
+// row when every two neighbours among the first n_used + 1 are further apart than the f32 keys' error (key_error): the order is then that of the
+// exact keys. Else (a row in some 600 for a bias and 512 experts) the candidates' own keys are worked out in f64, or, where keys that are no
+// candidates may come near them, where groups lie that near or ties leave more than 32 keys, the whole row's. Without bias and groups the
+// scores' order is the logits' own, which are exact. The weights come from the chosen logits alone, by the accurate exponential, relative to the
+// largest of them, so that they neither overflow nor vanish together.
+//
+// What bounds it: instructions. 32,768 rows of 512 with a bias take 45 us, lists included, 11 of them the bytes at HBM's rate; a row takes 900 warp
+// instructions, at 71 % of the issue slots. A warp-wide maximum for each of the first n_used + 1 took 270 us.
 //
 // The lists: rows are counted by chunks of 32, an expert's rows of a chunk a bit each of a word in shared memory, so that a row's place
 // among them is a population count. A scan over the chunks' counts and a pass over the assignments follow; short steps are one cluster's.
-//
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -118,7 +121,8 @@ __device__ __forceinline__ void warp_best(double &v, uint32_t &e) {
 // reciprocal within 2^-23; the exponent x log2(e) is rounded twice, by 2^-23 |x| in all, and l - largest once more. A sigmoid s = 1 / (1 + e)
 // moves by s (1 - s) times e's relative error, (1 + |l|) 2^-22 at most, and s (1 - s) (1 + |l|) < 0.5: 2^-20 covers it, the reciprocal and the sum. A softmax
 // score e^-d / sum is within (4 + d) 2^-22 of itself, so within 2^-20 of the largest score; and its sum, the mean of (4 + d) over 512
-// experts by their e^-d being 8 at most, within 2^-19: 2^-18 of the largest score covers both.
+// experts by their e^-d being 8 at most, within 2^-19, and 20 roundings of its own, 2^-19 again at most. The sum's error is all scores' alike, and so
+// counts once in the difference of two: 2 x 2^-20 + 2 x 2^-19, and 2^-18 of the largest score a key covers twice that.
 __device__ __forceinline__ float key_error(bool sigmoid, float largest_score) { return sigmoid ? 9.5367432e-7f : 3.8146973e-6f * largest_score; }
 
 // Groups, on the warp's E keys in shared memory: each ranked by the sum of its two best; the keys of all but the best a.used become
@@ -172,24 +176,28 @@ __device__ __forceinline__ bool keep_groups(T *sk, const RouteArgs &a, uint32_t 
   return sure;
 }
 
-// The row in f64, where f32 leaves it open: keys in shared memory, few registers, as it is rare. Lane j < k returns the j-th expert.
+// The row where f32 leaves it open: keys in shared memory, few registers, as it is rare. In f64; without a bias the order, or that within the groups
+// that stay, is the logits' own, which scores that vanish or come to 1 would lose. Lane j < k returns the j-th expert.
 template <class L>
 __device__ __noinline__ uint32_t choose_f64(const RouteArgs &a, uint64_t t, uint32_t lane, float largest, double *sk) {
+  const bool scored = a.bias || a.G > 1;
   double sum = 0;
   for (uint32_t e = lane; e < a.E; e += 32) {
     const float l = logit_of<L>(a, t, e);
-    sk[e] = l == -INFINITY ? -INFINITY : a.sigmoid ? sigmoid_key((double)l) : softmax_part<double>(l, largest);
+    sk[e] = l == -INFINITY || !scored ? l : a.sigmoid ? sigmoid_key((double)l) : softmax_part<double>(l, largest);
     if (l > -INFINITY) sum += sk[e];
   }
-  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  for (uint32_t e = lane; e < a.E; e += 32) {
-    if (!a.sigmoid) sk[e] /= sum;  // -infinity stays
-    if (a.bias && sk[e] > -INFINITY) sk[e] += a.bias[e];
+  if (scored) {
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    for (uint32_t e = lane; e < a.E; e += 32) {
+      if (!a.sigmoid) sk[e] /= sum;  // -infinity stays
+      if (a.bias && sk[e] > -INFINITY) sk[e] += a.bias[e];
+    }
   }
   __syncwarp();
   if (a.G > 1) {
     keep_groups<double>(sk, a, lane, false, 0.0f);
-    if (!a.bias)  // within the groups that stay the order is the logits' own
+    if (!a.bias)
       for (uint32_t e = lane; e < a.E; e += 32)
         if (sk[e] > -INFINITY) sk[e] = logit_of<L>(a, t, e);
     __syncwarp();

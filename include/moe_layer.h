@@ -322,7 +322,8 @@ MOE_API const char *moe_route_rows_static_error(void);
  * device (a host pointer or another device's is refused), and every call queues on stream (a cudaStream_t; null: the
  * default stream) without waiting, so a call can be captured into a graph. The first call of each on a device sets
  * kernel attributes; that may happen during a capture too. Calls with different buffers may overlap. T or R of 0 is a
- * call with nothing to do (offsets become 0). moe_ops_error: the calling thread's last message from any of them.
+ * call with nothing to do (offsets become 0). A call's outputs share no bytes with its inputs or with one another, but for
+ * moe_combine_rows_device's residual. moe_ops_error: the calling thread's last message from any of them.
  *
  * MX rows: values in blocks of 32 along the row, a value an e2m1 code (sign, 0 0.5 1 1.5 2 3 4 6), a block one e8m0 scale
  * byte (2^(byte - 127); 255: the block is NaN). codes [rows][K / 2]: value 2i in the low half of byte i, 2i + 1 in the high
@@ -347,13 +348,14 @@ typedef struct {
  * the softmax of its logits or their sigmoids; an expert's key is s + bias_dev[expert] (null: the score). With groups, the
  * n_groups_used groups whose two best keys have the largest sums stay (of one expert: its key). ids_dev [T][n_used] are the
  * largest keys' experts, best first; w_dev [T][n_used] their scores (without the bias), renormalised, times scale. Ties go to
- * the lower expert, or group. Which experts are chosen is decided as in 64-bit arithmetic on the given logits and bias.
+ * the lower expert, or group. Which experts are chosen is decided as in 64-bit arithmetic on the given logits and bias; without a
+ * bias the logits' own order stands for the scores'.
  * An expert whose logit or bias is -infinity or NaN is out: it takes no part in softmax and is never chosen; a row with too few
  * others has id -1 and weight 0 in its last places.
  * offsets_dev (null: no lists; then inv_dev is null too): [n_experts + 1], expert e's rows in expert order are offsets[e] ..
  * offsets[e + 1]; inv_dev [T][n_used], each assignment's row there, assignments in ascending order within an expert, -1 for
- * id -1. Rows of more than one launch need work_dev: moe_route_work_bytes(T, n_experts) bytes, 4-byte aligned, whose contents do
- * not matter and are not kept. T at most 2^24. */
+ * id -1. The lists of more than 64 rows need work_dev: moe_route_work_bytes(T, n_experts) bytes, 4-byte aligned, whose contents
+ * do not matter and are not kept. T at most 2^24. */
 MOE_API uint64_t moe_route_work_bytes(uint32_t T, uint32_t n_experts);
 MOE_API moe_status moe_route_logits_device(const moe_route_config *config, const void *logits_dev, uint64_t stride, const float *bias_dev,
                                            uint32_t T, int32_t *ids_dev, float *w_dev, int32_t *offsets_dev, int32_t *inv_dev,

@@ -80,6 +80,23 @@ def test_ties_go_to_the_lower_expert_and_zeros_have_no_sign():
         check(np.zeros((3, 128)), 9, **kw)
 
 
+def test_order_of_scores_that_vanish_or_come_to_one():
+    """Without a bias the logits' order decides, where 64-bit scores are equal and ties leave many keys too."""
+    E = 512
+    for some in (31, 64, 200, 512):
+        for k in (1, 8, 16):
+            low = np.full((70, some), -2000.0)
+            low[:, 0] = 0
+            low[:, some - 6:some - 1] = -1000
+            check(low, min(k, some), score="softmax")
+            high = np.full((70, some), 50.0)
+            high[:, some - 6:some - 1] = 60
+            check(high, min(k, some), score="sigmoid")
+    groups = np.full((70, E), 50.0)
+    groups[:, 100:104] = 60
+    check(groups, 10, score="sigmoid", n_groups=8, n_groups_used=3)
+
+
 def test_keys_that_f32_cannot_tell_apart():
     """Scores next to one another, saturated ones and large biases: the order is the exact keys'."""
     rng = np.random.default_rng(6)
