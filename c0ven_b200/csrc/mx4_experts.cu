@@ -6,6 +6,10 @@
 // short instruction and what an item costs is bringing the matrix. Persistent units (a CTA, or a pair of CTAs on two SMs that share the rows:
 // tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
 //
+// What bounds it: few rows an expert (1,000 over 512 experts of 2,048 x 512) HBM, 76 us of gate_up at 6.4 TB/s and 44 of the product at 5.6; many
+// (65,536 over 128 of 2,560 x 768) no one unit, 156 and 111 us, 2.4 PFLOP/s (5 on a dense 8,192 x 8,192 x 8,192): the warps' chain of hand-overs
+// from copies to MMAs, and the issue slots that epilogue and waits take from it; one row, 8 and 6 us, the latency of that chain.
+//
 // Roles of a CTA's warps: one thread brings codes by bulk-tensor copies, 256 values of the contraction a stage; three warps bring the scales,
 // four stages (1,024 values: a sector of a row's scales) at a time in turn, word by word into the layout that the tensor core's copy reads
 // (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance); one lane (of a pair's first CTA) issues the copies of
@@ -306,8 +310,8 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     }
   } else if (warp >= kScaleWarp && warp < kScaleWarp + SL) {
     // A slot of scales by a warp, a word a lane: eight words of rows i, i + 32, i + 64 and i + 96 an instruction, so that a row's 32 bytes are one
-    // request; the words, at 16 i + 4 (row / 32) of pieces 528 bytes apart, fall on 32 banks. (Loads into registers, 16 on their way at once, took
-    // half as long again for a whole step: what counts is that a slot's copies are all on their way.)
+    // request; the words, at 16 i + 4 (row / 32) of pieces 528 bytes apart, fall on 32 banks. (With loads into registers, 16 on their way at once, gate_up
+    // of 65,536 rows took 386 us where this took 182: what counts is that a slot's copies are all on their way.)
     const uint32_t mine = warp - kScaleWarp, srow = mx_scale_row_bytes(K), nb = K / kMxBlock, slots = (KT + kScaleStages - 1) / kScaleStages;
     const uint32_t word = lane % 8, quarter = lane / 8, at = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes) + word * kPiece + 4 * quarter;
     uint32_t turn = 0, phase = 1;  // whose turn the next slot is
