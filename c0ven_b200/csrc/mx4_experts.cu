@@ -131,13 +131,17 @@ struct Mx4Form {
   static constexpr uint32_t kTileExperts = kTables + 2 * (kMaxExperts + 1) * 4;
   static constexpr uint32_t kBytes = kTileExperts + 2 * kTileTable + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
-  static_assert(2 * kThreads > kMaxExperts + 1, "two experts a thread");
+  static_assert(2 * kThreads > kMaxExperts, "two experts a thread");
+  static_assert(kThreads <= 32 * 32, "a lane a warp");
   // Tensor memory: two accumulators, then sets of columns for scales, of kScaleStages stages where they have the room, else of one. From the MMAs of
   // a unit of stages to those that find its columns filled again takes three hand-overs between warps, longer than the MMAs of a stage: with two
   // sets of one stage, beside accumulators of 224 columns, every stage waited 0.14 us.
   static constexpr uint32_t kStageCols = 2 * 4 * (1 + kRowPieces);
   static constexpr uint32_t kUnitStages = 2 * NT + 3 * kScaleStages * kStageCols <= 512 ? kScaleStages : 1;
   static constexpr uint32_t kSets = kUnitStages == 1 ? 4 : 3;
+  // A stage is full when the CTAs' codes are there and, where units are single stages, its scales in tensor memory: one wait of the MMAs' warp less
+  // (3 % of a dense gate_up of 8,192 x 8,192 x 8,192).
+  static constexpr uint32_t kStageArrivals = CTAS + (kUnitStages == 1 ? 1 : 0);
   static constexpr uint32_t kUnitCols = kUnitStages * kStageCols;
   static constexpr uint32_t kUsedCols = 2 * NT + kSets * kUnitCols;
   static constexpr uint32_t kCols = kUsedCols <= 256 ? 256 : 512;
@@ -158,7 +162,8 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0, unit = blockIdx.x / CTAS, nunits = gridDim.x / CTAS;
   uint64_t *bars = (uint64_t *)(smem + SM::kBarriers);
-  // Barriers: stages full, empty; scales full, empty; accumulators full, empty; sets of scales in tensor memory full, empty. Of a pair the first CTA's "full" of stages and scales and "empty"
+  // Barriers: stages full, empty; scales full, empty; accumulators full, empty; sets of scales in tensor memory full, empty
+  // (where a unit is a stage, the stage's own say that). Of a pair the first CTA's "full" of stages and scales and "empty"
   // of accumulators take both CTAs' arrivals.
   constexpr uint32_t kEmpty = S, kScFull = 2 * S, kScEmpty = kScFull + SL, kAccFull = kScEmpty + SL, kAccEmpty = kAccFull + 2, kSetFull = kAccEmpty + 2,
                      kSetEmpty = kSetFull + SM::kSets, kBars = kSetEmpty + SM::kSets;
@@ -173,7 +178,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   uint32_t *error = &g_gave_up;
 
   if (tid == 0) {
-    for (uint32_t s = 0; s < S; s++) mbar_init(bar(s), CTAS), mbar_init(bar(kEmpty + s), 1);
+    for (uint32_t s = 0; s < S; s++) mbar_init(bar(s), SM::kStageArrivals), mbar_init(bar(kEmpty + s), 1);
     for (uint32_t s = 0; s < SL; s++) mbar_init(bar(kScFull + s), CTAS), mbar_init(bar(kScEmpty + s), 1);
     for (uint32_t b = 0; b < 2; b++) mbar_init(bar(kAccFull + b), 1), mbar_init(bar(kAccEmpty + b), CTAS * 4 * SM::kGroups);
     for (uint32_t b = 0; b < SM::kSets; b++) mbar_init(bar(kSetFull + b), 1), mbar_init(bar(kSetEmpty + b), 1);
@@ -189,31 +194,18 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     else
       tmem_alloc(smem_u32(tmem_slot), SM::kCols);
   }
-  // The experts' first rows and first tiles, E + 1 <= 513 entries, two a thread. Offsets are held to 0 .. R, and to rise: each to the largest
-  // before it.
+  // The experts' first rows and first tiles, and the tiles' experts, two experts a thread. Offsets are held to 0 .. R, and to rise: each to the largest
+  // before it, which is looked for where one does not.
   {
     const uint32_t e = 2 * tid;
-    auto row_of = [&](uint32_t x) { return x > a.E ? 0u : a.offsets ? min((uint32_t)max(a.offsets[x], 0), a.R) : x ? a.R : 0u; };
-    uint32_t r0 = row_of(e), r1 = row_of(e + 1);
-    r1 = max(r0, r1);
-    uint32_t top = r1;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, top, off);
-      if (lane >= (uint32_t)off) top = max(top, o);
+    auto row_of = [&](uint32_t x) { return a.offsets ? min((uint32_t)max(a.offsets[x], 0), a.R) : x ? a.R : 0u; };
+    uint32_t r0 = e <= a.E ? row_of(e) : 0, r1 = e < a.E ? row_of(e + 1) : r0, r2 = e + 1 < a.E ? row_of(e + 2) : r1;
+    if (__syncthreads_or(r1 < r0 || r2 < r1)) {
+      for (uint32_t x = 0; x < min(e, a.E); x++) r0 = max(r0, row_of(x));
+      r1 = max(r0, r1), r2 = max(r1, r2);
     }
-    if (lane == 31) warp_part[warp] = top;
-    top = __shfl_up_sync(0xffffffffu, top, 1);
-    if (lane == 0) top = 0;
-    __syncthreads();
-    for (uint32_t w = 0; w < min(warp, 9u); w++) top = max(top, warp_part[w]);
-    r0 = max(r0, top), r1 = max(r1, top);
-    if (e <= a.E) first_row[e] = r0;
-    if (e < a.E) first_row[e + 1] = r1;
-    __syncthreads();
     dependents_may_launch();
-    const uint32_t r2 = e + 2 <= a.E ? first_row[e + 2] : r1;
-    const uint32_t t0 = e < a.E ? (r1 - r0 + NT - 1) / NT : 0, t1 = e + 1 < a.E ? (r2 - r1 + NT - 1) / NT : 0;
+    const uint32_t t0 = (r1 - r0 + NT - 1) / NT, t1 = (r2 - r1 + NT - 1) / NT;
     uint32_t sum = t0 + t1;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -222,12 +214,15 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     }
     if (lane == 31) warp_part[warp] = sum;
     __syncthreads();
-    sum -= t0 + t1;
-    for (uint32_t w = 0; w < min(warp, 9u); w++) sum += warp_part[w];
-    if (e <= a.E) first_tile[e] = sum;
-    if (e < a.E) first_tile[e + 1] = sum + t0;
-    __syncthreads();
+    sum += __reduce_add_sync(0xffffffffu, lane < warp ? warp_part[lane] : 0) - t0 - t1;
+    if (e <= a.E) first_row[e] = r0, first_tile[e] = sum;
+    if (e < a.E) first_row[e + 1] = r1, first_tile[e + 1] = sum + t0;
+    for (uint32_t t = sum; t < min(sum + t0 + t1, kTileTable); t++) tile_expert[t] = (uint16_t)(t < sum + t0 ? e : e + 1);
   }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers exist before anything arrives on them
+  tc_fence_after();
   const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK, ntiles = first_tile[a.E];
   auto expert_at = [&](uint32_t t) {  // the last expert whose first tile is at most t
     uint32_t lo = 0, hi = a.E;
@@ -240,11 +235,6 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     }
     return lo;
   };
-  for (uint32_t t = tid; t < min(ntiles, kTileTable); t += SM::kThreads) tile_expert[t] = (uint16_t)expert_at(t);
-  tc_fence_before();
-  __syncthreads();
-  if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers exist before anything arrives on them
-  tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t lead0 = CTAS == 2 ? map_to_cta(bar0, 0) : bar0;  // the first CTA's barriers as this CTA names them
   auto lead = [&](uint32_t i) { return lead0 + 8 * i; };
@@ -363,7 +353,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
       constexpr uint32_t U = SM::kUnitStages;
       const uint32_t leader = elect_leader();
       // The MMAs of kSets units ago, which read the set's columns, are done: a unit of one stage has that stage's "empty" say so.
-      uint32_t slot = 0, slot_phase = 0, set = 0, done = U == 1 ? S - SM::kSets : 0, done_phase = 1;
+      uint32_t stage = 0, slot = 0, slot_phase = 0, set = 0, done = U == 1 ? S - SM::kSets : 0, done_phase = 1;
       for (Item i = first; i.t < ntiles && ok; step(i)) {
         for (uint32_t it = 0; it < KT && ok; it += U) {
           const uint32_t sub = it % kScaleStages;
@@ -382,10 +372,12 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
             for (uint32_t p = 0; p < SM::kRowPieces; p++)
               copy_scales<CTAS>(leader, to_rows + 4 * (w * SM::kRowPieces + p), from + (8 * (1 + p) + 2 * sub + w) * kPiece);
           }
+          const uint32_t full = bar(U == 1 ? stage : kSetFull + set);
           if constexpr (CTAS == 2)
-            mma_commit_pair(leader, bar(kSetFull + set), 1);
+            mma_commit_pair(leader, full, 1);
           else
-            mma_commit(leader, bar(kSetFull + set));
+            mma_commit(leader, full);
+          if (++stage == S) stage = 0;
           if (sub + U == kScaleStages || it + U >= KT) {
             if constexpr (CTAS == 2)
               mma_commit_pair(leader, bar(kScEmpty + slot), 3);
@@ -415,7 +407,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
         ok = mbar_wait_warp(bar(kAccEmpty + b), acc_phase, abort, error);
         for (uint32_t it = 0; it < KT && ok; it++) {
           const uint32_t in_unit = it % U, ta = tmem_base + 2 * NT + set * SM::kUnitCols, tb = ta + 8 * U;
-          if (in_unit == 0) ok = mbar_wait_warp(bar(kSetFull + set), set_phase, abort, error);
+          if (U > 1 && in_unit == 0) ok = mbar_wait_warp(bar(kSetFull + set), set_phase, abort, error);
           if (ok) ok = mbar_wait_warp(bar(s), phase, abort, error);
           if (!ok) break;
           tc_fence_after();
