@@ -10,8 +10,8 @@
 // scores' order is the logits' own, which are exact. The weights come from the chosen logits alone, by the accurate exponential, relative to the
 // largest of them, so that they neither overflow nor vanish together.
 //
-// What bounds it: instructions. 32,768 rows of 512 with a bias take 45 us, lists included, 11 of them the bytes at HBM's rate; a row takes 900 warp
-// instructions, at 71 % of the issue slots. A warp-wide maximum for each of the first n_used + 1 took 270 us.
+// What bounds it: instructions. 32,768 rows of 512 with a bias take 42 us, lists included, 11 of them the bytes at HBM's rate; the rest is a row's
+// warp instructions. A warp-wide maximum for each of the first n_used + 1 took 270 us.
 //
 // The lists: rows are counted by chunks of 32, an expert's rows of a chunk a bit each of a word in shared memory, so that a row's place
 // among them is a population count. A scan over the chunks' counts and a pass over the assignments follow; short steps are one cluster's.
@@ -232,7 +232,7 @@ __device__ __forceinline__ void load_bias(const RouteArgs &a, uint32_t lane, flo
   }
 }
 
-// Doubles of shared memory a warp has for a row: a key an expert, or 32 candidates.
+// Doubles of shared memory a warp has for a row: a key an expert in f64; or, in 32 bits, 32 candidates' keys and experts and, behind them, all keys.
 template <int V>
 constexpr uint32_t kRouteScratch = 32 * V;
 
@@ -261,11 +261,18 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
   }
   const float err = key_error(a.sigmoid, score_max);
   bool sure = true;
-  // key[i] becomes the expert's key, -infinity if it is out: what is added for that has no branch.
+  // v[i] becomes the expert's key, -infinity or NaN if it is out. Rows without experts out, by a minimum over the logits, take no look at each.
   auto to_keys = [&](float (&v)[V]) {
     if (a.sigmoid) {
+      float low = INFINITY;
 #pragma unroll
-      for (int i = 0; i < V; i++) v[i] = sigmoid_key(key[i]) + bias[i] + (key[i] > -INFINITY ? 0.0f : -INFINITY);
+      for (int i = 0; i < V; i++) asm("min.NaN.f32 %0, %0, %1;" : "+f"(low) : "f"(key[i]));
+      if (__any_sync(0xffffffffu, !(low > -INFINITY))) {
+#pragma unroll
+        for (int i = 0; i < V; i++) key[i] = key[i] > -INFINITY ? key[i] : __uint_as_float(0x7FFFFFFFu);
+      }
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] = sigmoid_key(key[i]) + bias[i];
     } else {
 #pragma unroll
       for (int i = 0; i < V; i++) v[i] = softmax_part<float>(key[i], largest) * score_max + bias[i] + (key[i] > -INFINITY ? 0.0f : -INFINITY);
@@ -315,9 +322,10 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
     }
   }
   // The keys from there on, a lane each.
-  uint32_t mine = 0;
+  uint32_t bits = 0;  // bit i: the lane's i-th is one
 #pragma unroll
-  for (int i = 0; i < V; i++) mine += key[i] >= least ? 1u : 0u;
+  for (int i = 0; i < V; i++) bits |= key[i] >= least ? 1u << i : 0u;
+  const uint32_t mine = __popc(bits);
   uint32_t upto = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -331,9 +339,18 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
     float *found = (float *)sk;                // the keys, and behind them
     uint32_t *expert = (uint32_t *)sk + 32;    // their experts
     uint32_t put = upto - mine;
+    // Through shared memory a lane takes its few by their numbers, where registers would want a branch a key.
+    if constexpr (V == 1) {
+      if (bits) found[put] = key[0], expert[put] = lane;
+    } else {
+      float *all = (float *)sk + 64 + lane;
 #pragma unroll
-    for (int i = 0; i < V; i++)
-      if (key[i] >= least) found[put] = key[i], expert[put++] = lane + 32 * i;
+      for (int i = 0; i < V; i++) all[32 * i] = key[i];
+      for (uint32_t left = bits; left; left &= left - 1) {
+        const uint32_t i = 32 * (__ffs(left) - 1);
+        found[put] = all[i], expert[put++] = lane + i;
+      }
+    }
     if (lane >= n) found[lane] = -INFINITY;
     __syncwarp();
     const float own = found[lane];
