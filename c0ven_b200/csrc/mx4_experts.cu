@@ -6,9 +6,11 @@
 // short instruction and what an item costs is bringing the matrix. Persistent units (a CTA, or a pair of CTAs on two SMs that share the rows:
 // tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
 //
-// What bounds it: few rows an expert (1,000 over 512 experts of 2,048 x 512) HBM, 76 us of gate_up at 6.4 TB/s and 44 of the product at 5.6; many
-// (65,536 over 128 of 2,560 x 768) no one unit, 156 and 111 us, 2.4 PFLOP/s (5 on a dense 8,192 x 8,192 x 8,192): the warps' chain of hand-overs
-// from copies to MMAs, and the issue slots that epilogue and waits take from it; one row, 8 and 6 us, the latency of that chain.
+// What bounds it: few rows an expert (1,000 over 512 experts of 2,048 x 512) HBM, 75 us of gate_up at 6.5 TB/s and 44 of the product at 5.7; many
+// (65,536 over 128 of 2,560 x 768) no one unit, 155 and 109 us at 3.3 and 2.4 PFLOP/s (5.3 on a dense 8,192 x 8,192 x 8,192, of which shared memory's
+// rate alone allows some 7): without its epilogue gate_up took 123 of 148, without scales too 104, and the product 66 of 104 and 57; one row, 7 and
+// 6 us, latency: 1,300 cycles until the experts' first rows are here, 700 for the tables, 2,600 until the first scales are in tensor memory, 490 a stage
+// of MMAs, 1,500 from the last to the end.
 //
 // Roles of a CTA's warps: one thread brings codes by bulk-tensor copies, 256 values of the contraction a stage; three warps bring the scales,
 // four stages (1,024 values: a sector of a row's scales) at a time in turn, word by word into the layout that the tensor core's copy reads
@@ -581,14 +583,15 @@ void launch_product(const Mx4Args &args, const void *wc, const void *xc, cudaStr
   CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, maps));
 }
 
-// Tiles of 208 rows by pairs of CTAs where experts have more than 32 rows on average and there are 32 items for pairs at least; else of 32 by single
-// CTAs. gate_up and down by pairs and by single CTAs, us: 512 experts of 2,048 x 512, 10 rows 9 + 7 and 8 + 6, 1,000 rows 80 + 48 and 80 + 45,
-// 10,000 rows 98 + 60 and 97 + 54, 16,000 rows 100 + 67 and 107 + 72, 32,000 rows 105 + 75 and 185 + 129; one of 2,080 x 1,440, 200 rows (12 items for
-// pairs) 15 + 11 and 11 + 6, 777 rows (48) 15 + 11 and 17 + 10; one of 8,192 x 4,096, 128 rows (32) 19 + 12 and 24 + 14.
+// Tiles of 208 rows by pairs of CTAs where experts have more than 26 rows on average (many then have more than 32, two tiles of a single CTA) and there
+// are 32 items for pairs at least; else of 32 by single CTAs. gate_up and down by pairs and by single CTAs, us: 512 experts of 2,048 x 512, 10 rows
+// 8 + 7 and 7 + 6, 1,000 rows 79 + 47 and 76 + 44, 12,000 rows 96 + 57 and 93 + 54, 14,000 rows 96 + 57 and 94 + 59, 16,000 rows 96 + 58 and 104 + 71,
+// 32,000 rows 100 + 66 and 177 + 128; 128 of 2,560 x 768, 2,800 rows 49 + 28 and 47 + 26, skewed 49 + 28 and 49 + 28; one of 2,080 x 1,440, 200 rows
+// (12 items for pairs) 11 + 8 and 10 + 6, 777 rows (48) 12 + 9 and 16 + 10; one of 8,192 x 4,096, 128 rows (32) 16 + 10 and 23 + 13.
 template <class Out>
 void launch(const Mx4Args &a, const void *wc, const void *xc, cudaStream_t st) {
   const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 208 + 1;
-  if (a.R > 32ull * a.E && pieces * tiles >= 32)
+  if (a.R > 26ull * a.E && pieces * tiles >= 32)
     launch_product<Out, 2, 208>(a, wc, xc, st);
   else
     launch_product<Out, 1, 32>(a, wc, xc, st);
