@@ -91,6 +91,37 @@ def test_quantize_extremes():
     assert np.array_equal(out.cpu().numpy().astype(np.float64), R.values(code, byte), equal_nan=True)
 
 
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_quantize_extremes_of_16_bit_types(type):
+    """An infinity or NaN of either sign at every place of a block, the type's largest and its denormals, magnitudes that differ in their last bit."""
+    import torch
+
+    rng = np.random.default_rng(2)
+    bits = dev(rng.uniform(-2, 2, (32 * 4 + 8, 96)), type).view(torch.int16).cpu().numpy().view(np.uint16).copy()
+    inf = 0x7C00 if type == "f16" else 0x7F80
+    for place in range(32):
+        for j, b in enumerate((inf, inf | 0x8000, inf | 1, 0xFFFF)):
+            bits[4 * place + j, 32 + place] = b
+    rest = bits[128:]
+    rest[0] = inf - 1                                       # the largest finite value
+    rest[1] = rng.integers(0, 4, 96)                        # denormals, zeros among them
+    rest[2] = rng.integers(0, 4, 96) | 0x8000
+    rest[3] = 1
+    rest[4] = rng.integers(0, inf & ~(inf << 1), 96)        # all denormals
+    rest[5] = rng.integers(0, inf, 96) | rng.integers(0, 2, 96) * 0x8000
+    rest[6] = 0x8000
+    rest[7] = rng.integers(inf - 3, inf, 96)
+    x = torch.from_numpy(bits.view(np.int16)).view(dtype(type)).cuda()
+    T = x.shape[0]
+    code, byte = R.quantize(x.double().cpu().numpy())
+    want = R.pack(code, byte)
+    codes, scales = mx_buffers(T, 96)
+    ops.mx4_quantize_rows_device(x.data_ptr(), TYPES[type], T, 96, codes.data_ptr(), scales.data_ptr(), T)
+    torch.cuda.synchronize()
+    assert (byte[:128, 1] == 255).all() and (byte[:128, 0] != 255).all() and (byte[128:] != 255).all()
+    assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 def test_quantize_scatters_strided_rows(type):
     """Every row to the places its assignments have; places of none and rows past R are left as they were."""
