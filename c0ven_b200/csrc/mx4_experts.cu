@@ -302,10 +302,12 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     }
   } else if (warp >= kScaleWarp && warp < kScaleWarp + SL) {
     // A slot of scales by a warp, a word a lane: eight words of rows i, i + 32, i + 64 and i + 96 an instruction, so that a row's 32 bytes are one
-    // request; the words, at 16 i + 4 (row / 32) of pieces 528 bytes apart, fall on 32 banks. (With loads into registers, 16 on their way at once, gate_up
-    // of 65,536 rows took 386 us where this took 182: what counts is that a slot's copies are all on their way.)
+    // request; the words, at 16 i + 4 (row / 32) of pieces 528 bytes apart, fall on 32 banks. Where the rest of a row is four words or fewer, those of
+    // rows i + 4, ... too. (With loads into registers, 16 on their way at once, gate_up of 65,536 rows took 386 us where this took 182: what counts is
+    // that a slot's copies are all on their way.) Only the bytes behind a row's last in its word are made zeros, as codes are there: words behind it are
+    // not copied on, and rows behind the tile's or the matrix's go into results nobody reads.
     const uint32_t mine = warp - kScaleWarp, srow = mx_scale_row_bytes(K), nb = K / kMxBlock, slots = (KT + kScaleStages - 1) / kScaleStages;
-    const uint32_t word = lane % 8, quarter = lane / 8, at = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes) + word * kPiece + 4 * quarter;
+    const uint32_t at = smem_u32(smem + SM::kScales + mine * SM::kSlotBytes);
     uint32_t turn = 0, phase = 1;  // whose turn the next slot is
     for (Item i = first; i.t < ntiles && ok; step(i)) {
       const Tile t = tile_at(i);
@@ -314,32 +316,41 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
         ok = mbar_wait_warp(bar(kScEmpty + mine), phase, abort, error);
         if (!ok) break;
         phase ^= 1;
-        // The scales from byte b0 of a row on, n of the word's four.
-        const uint32_t b0 = j * (kScaleStages * kStageK / kMxBlock) + 4 * word, n = b0 < nb ? min(4u, nb - b0) : 0u;
-        // Up to 32 rows from src on, have of them, to the lane's places from `to` on; zeros behind them.
+        // The lane's word, and its first row of each 128. Its bytes of a row's scales: n from b0 on.
+        constexpr uint32_t kSlotBlocks = kScaleStages * kStageK / kMxBlock;
+        const bool few = nb - j * kSlotBlocks <= kSlotBlocks / 2;
+        const uint32_t word = lane % (few ? 4 : 8), quarter = few ? lane / 4 % 4 : lane / 8, r0 = few ? lane / 16 * 4 : 0, every = few ? 8 : 4;
+        const uint32_t b0 = j * kSlotBlocks + 4 * word, n = b0 < nb ? min(4u, nb - b0) : 0u;
+        const uint32_t to = at + word * kPiece + 4 * quarter + 16 * r0;
+        // Rows src + 0 .. 3, every + 0 .. 3, ... of 32, have of them, to the places from `to` on.
         auto bring = [&](uint32_t to, const uint8_t *src, uint32_t have) {
-          if (__all_sync(0xffffffffu, have == 32 && n == 4)) {
-#pragma unroll 8
-            for (uint32_t k = 0; k < 32; k++, src += srow) copy_word(to + 16 * k, src);
+          const uint64_t skip = (uint64_t)(every - 4) * srow;
+          if (__all_sync(0xffffffffu, have >= 32 - r0 && (n == 4 || n == 0))) {
+            if (n)
+#pragma unroll 2
+              for (uint32_t k = 0; k < 32; k += every, to += 16 * every, src += skip)
+#pragma unroll
+                for (uint32_t u = 0; u < 4; u++, src += srow) copy_word(to + 16 * u, src);
             return;
           }
-#pragma unroll 8
-          for (uint32_t k = 0; k < 32; k++, src += srow) {
-            const uint32_t m = k < have ? n : 0;
-            copy_word(to + 16 * k, m ? src : a.ws, m);
-          }
+          for (uint32_t k = 0; k < 32; k += every, to += 16 * every, src += skip)
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++, src += srow)
+              if (n && k + u < have) copy_word(to + 16 * u, src, n);
         };
         {
-          const uint32_t r = 32 * quarter, row = GU ? (r < 64 ? t.row0 + r : F + t.row0 + r - 64) : t.row0 + r;
-          bring(at, a.ws + ((uint64_t)t.expert * a.N + row) * srow + b0, row < a.N ? min(32u, a.N - row) : 0);
+          const uint32_t r = 32 * quarter + r0, row = GU ? (r < 64 ? t.row0 + r : F + t.row0 + r - 64) : t.row0 + r;
+          bring(to, a.ws + ((uint64_t)t.expert * a.N + row) * srow + b0, row < a.N ? a.N - row : 0);
         }
         if constexpr (NT <= 32) {
-          // Up to 32 rows, which lie in the first column of a piece: four neighbours an instruction.
-          for (uint32_t r = quarter; r < t.count; r += 4) copy_word(at + 8 * kPiece - 4 * quarter + 16 * r, a.xs + (n ? (uint64_t)(t.start + r) * srow + b0 : 0), n);
+          // Up to 32 rows, which lie in the first column of a piece: neighbours an instruction.
+          const uint32_t lanes = few ? 4 : 8;
+          if (n)
+            for (uint32_t r = lane / lanes; r < t.count; r += 32 / lanes) copy_word(at + (8 + word) * kPiece + 16 * r, a.xs + (uint64_t)(t.start + r) * srow + b0, n);
         } else {
           for (uint32_t p = 0; p < SM::kRowPieces && 128 * p < t.count; p++) {
-            const uint32_t r = 128 * p + 32 * quarter;
-            bring(at + 8 * (1 + p) * kPiece, a.xs + (uint64_t)(t.start + r) * srow + b0, r < t.count ? min(32u, t.count - r) : 0);
+            const uint32_t r = 128 * p + 32 * quarter + r0;
+            bring(to + 8 * (1 + p) * kPiece, a.xs + (uint64_t)(t.start + r) * srow + b0, r < t.count ? t.count - r : 0);
           }
         }
         copy_words_wait();
