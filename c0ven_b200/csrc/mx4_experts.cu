@@ -187,6 +187,8 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
     *abort = 0;
     fence_barrier_init();
   }
+  __syncwarp();
+  if constexpr (CTAS == 2) cluster_arrive();
   // Tensor memory is taken when the kernels before are done, and the next may come when it is: a kernel that held it while it waits for another on the
   // same SM, which asks for it later, would wait for ever.
   wait_for_predecessors();
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CTAS == 2) cluster_sync();  // the other CTA's barriers exist before anything arrives on them
+  if constexpr (CTAS == 2) cluster_wait();  // the other CTA's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK, ntiles = first_tile[a.E];
   auto expert_at = [&](uint32_t t) {  // the last expert whose first tile is at most t

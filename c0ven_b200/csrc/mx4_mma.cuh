@@ -14,6 +14,9 @@
 namespace moe {
 namespace tc {
 
+// cluster_sync in two halves: what a thread wrote before the first is seen by the pair's threads after the second.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // 32 rows of 16 bytes, no swizzle: 8 rows 128 bytes on.
 __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t addr) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
