@@ -127,7 +127,8 @@ __device__ __forceinline__ float key_error(bool sigmoid, float largest_score) { 
 
 // Groups, on the warp's E keys in shared memory: each ranked by the sum of its two best; the keys of all but the best a.used become
 // -infinity. Returns whether the choice is sure: always for f64; for f32 when the sums of the last group that stays and the first
-// that goes are further apart than off, what two of them may be off by.
+// that goes are further apart than off, what two of them may be off by, and no group is left out for a sum below f32's range (of keys that a bias
+// near the type's lowest value makes), which f64 has room for.
 template <class T>
 __device__ __forceinline__ bool keep_groups(T *sk, const RouteArgs &a, uint32_t lane, bool check, float off) {
   const T none = minus_inf<T>();
@@ -160,7 +161,10 @@ __device__ __forceinline__ bool keep_groups(T *sk, const RouteArgs &a, uint32_t 
     T v = mine;
     uint32_t best = mine > none ? g : kNone;
     warp_best(v, best);
-    if (best == kNone) break;
+    if (best == kNone) {
+      sure = !check || !__any_sync(0xffffffffu, two > none && !(one + two > none));
+      break;
+    }
     if (j == a.used) {
       sure = (float)(last - v) > off;
       break;

@@ -261,3 +261,25 @@ def test_the_layers_own_router_agrees():
     assert np.allclose(got[1], w, rtol=1e-5)
     gpu.close()
     assert C.sizeof(_lib.RouteConfig) == 32
+
+
+def test_groups_whose_keys_sums_pass_f32():
+    """Biases of the type's lowest value are no experts out: groups of them, whose sums f32 has no room for, stay as 64-bit sums order them."""
+    rng = np.random.default_rng(10)
+    E, G = 64, 8
+    lowest = np.finfo(np.float32).min
+    masked = np.full(E, lowest)
+    masked[40:48] = 0.1 * rng.standard_normal(8)              # group 5 alone is not masked: the next to stay is group 0
+    apart = masked.copy()
+    apart[24:32] = lowest / 1.5                               # the sums of group 3's keys pass the lowest value too, but less far
+    one = np.full(E, lowest)
+    one[np.arange(E) % 8 == 3] = 0.0                          # a key a group that is not masked: no sum passes
+    high = np.full(E, np.finfo(np.float32).max)
+    high[:8] /= 4                                             # sums past the largest value, and group 0's below it
+    for T in (3, 70):
+        l = rng.standard_normal((T, E))
+        for bias in (masked, apart, one, high):
+            for used, k in ((2, 12), (3, 16), (8, 16)):
+                for score in ("sigmoid", "softmax"):
+                    got = check(l, k, score=score, bias=bias.astype(np.float32), n_groups=G, n_groups_used=used)
+                    assert (got[0] >= 0).all()
