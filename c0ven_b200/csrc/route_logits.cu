@@ -7,8 +7,9 @@
 // row when every two neighbours among the first n_used + 1 are further apart than the f32 keys' error (key_error): the order is then that of the
 // exact keys. Else (a row in some 600 for a bias and 512 experts) the candidates' own keys are worked out in f64, or, where keys that are no
 // candidates may come near them, where groups lie that near or ties leave more than 32 keys, the whole row's. Without bias and groups the
-// scores' order is the logits' own, which are exact. The weights come from the chosen logits alone, by the accurate exponential, relative to the
-// largest of them, so that they neither overflow nor vanish together.
+// scores' order is the logits' own, which are exact. Renormalised weights come from the chosen logits alone, by the accurate exponential, relative to
+// the largest of them, so that they neither overflow nor vanish together; a softmax's that are not, from them and the row's sum of accurate
+// exponentials, in f64.
 //
 // What bounds it: instructions. 32,768 rows of 512 with a bias take 42 us, lists included, 11 of them the bytes at HBM's rate; the rest is a row's
 // warp instructions. A warp-wide maximum for each of the first n_used + 1 took 270 us.
@@ -257,10 +258,21 @@ __device__ __forceinline__ uint32_t route_row(const RouteArgs &a, uint64_t t, ui
     }
     largest = unordered(__reduce_max_sync(0xffffffffu, ordered(largest)));
     float sum = 0.0f;
+    if (a.renorm) {
 #pragma unroll
-    for (int i = 0; i < V; i++) sum += key[i] == -INFINITY ? 0.0f : softmax_part<float>(key[i], largest);
+      for (int i = 0; i < V; i++) sum += key[i] == -INFINITY ? 0.0f : softmax_part<float>(key[i], largest);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    } else {
+      // The weights are divided by this sum: accurate exponentials, whose errors alone are in it. (32,768 rows of 512 take 56 us so, 46 with the fast ones,
+      // whose weights were off by more than eight half steps of f32.)
+      double exact = 0.0;
+#pragma unroll
+      for (int i = 0; i < V; i++) exact += key[i] == -INFINITY ? 0.0f : exp_below(key[i], largest);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) exact += __shfl_xor_sync(0xffffffffu, exact, off);
+      sum = (float)exact;
+    }
     score_max = largest == -INFINITY ? 0.0f : 1.0f / sum;
   }
   const float err = key_error(a.sigmoid, score_max);

@@ -283,3 +283,22 @@ def test_groups_whose_keys_sums_pass_f32():
                 for score in ("sigmoid", "softmax"):
                     got = check(l, k, score=score, bias=bias.astype(np.float32), n_groups=G, n_groups_used=used)
                     assert (got[0] >= 0).all()
+
+
+def test_softmax_weights_over_the_whole_row():
+    """Weights without renormalisation are divided by all experts' exponentials: many logits that lie alike, some 2 to 8 below the largest, whose
+    errors would add up."""
+    import torch
+
+    rng = np.random.default_rng(11)
+    T, E = 4096, 512
+    top = rng.uniform(-4, 4, T).astype(np.float32)
+    l = np.repeat((top - rng.uniform(2, 8, T).astype(np.float32))[:, None], E, 1)
+    l[np.arange(T), rng.integers(0, E, T)] = top
+    ids, w, _, _ = run(torch.from_numpy(l).cuda(), T, E, 2, lists=False, renorm=False)
+    x = np.sort(l, 1)[:, ::-1].astype(np.float64)
+    p = np.exp(x - x[:, :1])
+    # Half steps of 2^-24: an exponential 4 (2 ulp) and 1 for what its argument's rounding left out; the sum is of 64 bits and rounded once, its reciprocal
+    # and the product once each. The exponentials' errors are in the sum and in the weight alike, so that they count once at most.
+    assert np.allclose(w, (p / p.sum(1, keepdims=True))[:, :2], rtol=8 * 2.0 ** -24, atol=0)
+    assert np.array_equal(ids[:, 0], l.argmax(1))
