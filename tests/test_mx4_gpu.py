@@ -584,3 +584,50 @@ def test_a_block_put_together(T):
         if seed is None:
             assert torch.equal(out, first)  # the same bits, captured or not
         assert np.linalg.norm(out.double().cpu().numpy() - want(logits, x)) <= 2e-3 * np.linalg.norm(want(logits, x))
+
+
+def check_h(hc, hs, h, err):
+    """Each code of h's MX rows is right for some value within err of h's, each scale for some largest one."""
+    rows, F = h.shape
+    code, byte = R.unpack(hc.cpu().numpy(), hs.cpu().numpy())
+    hb, eb = np.abs(h).reshape(rows, -1, 32), err.reshape(rows, -1, 32)
+    lo, hi = ((hb - eb).clip(0).max(2), (hb + eb).max(2))
+    blo, bhi = (np.where(m > 0, np.maximum(np.frexp(np.where(m > 0, m, 1))[1] - 3, -127) + 127, 0) for m in (lo, hi))
+    assert ((byte >= blo) & (byte <= bhi)).all()
+    s = np.repeat(np.exp2(byte.astype(np.float64) - 127), 32, axis=1)
+    nearest = lambda a: np.sign(a) * R.E2M1[np.searchsorted([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.abs(a))]  # noqa: E731
+    got = R.E2M1[code & 7] * np.where(code & 8, -1.0, 1.0)
+    assert ((got >= nearest((h - err) / s - 1e-9)) & (got <= nearest((h + err) / s + 1e-9))).all()
+
+
+def mx_of(v):
+    """MX rows of values that the form holds exactly: (codes, scales) on the device."""
+    code, byte = R.quantize(v)
+    assert np.array_equal(R.values(code, byte), v)
+    c, s = R.pack(code, byte)
+    return dev(c), dev(s)
+
+
+@pytest.mark.parametrize("copies", [1, 20])
+def test_gates_far_below_zero(copies):
+    """Where e^g is below f32's normal values and u so large that h is not: an MX scale can hold it. By single CTAs and, with many copies, by pairs."""
+    import torch
+
+    gates = -np.array([1, 48, 64, 96, 128, 192, 256, 384], np.float64)
+    ups = np.array([0.5, 2.0 ** 40, 2.0 ** 101, 2.0 ** 124])
+    g1, u1 = (a.reshape(-1).repeat(32) for a in np.meshgrid(gates, ups))
+    u1 = u1 * np.tile(np.array([1, -1.5, 2, 0.5]), u1.size // 4)                     # a block's gates alike, its other factors not
+    F, K, rows = g1.size * copies, 32, 40
+    w = np.zeros((1, 2 * F, K))
+    w[0, :F, 0], w[0, F:, 0] = np.tile(g1, copies), np.tile(u1, copies)              # a row's first value alone meets the matrix
+    x = np.zeros((rows, K))
+    x[:, 0] = np.tile([1, 0.5, 2, 1.5], rows // 4)
+    (wc, ws), (xc, xs) = mx_of(w.reshape(-1, K)), mx_of(x)
+    hc, hs = mx_buffers(rows, F)
+    ops.mx4_gate_up_device(ops.Mx4Weights(1, 2 * F, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, None, hc.data_ptr(), hs.data_ptr())
+    ops.status()
+    v = x @ w[0].T
+    h = R.swiglu(v[:, :F], v[:, F:], 0.0)
+    # g and u are exact. To g = -80 the exponential's argument is below 116 and rounds by 2^-18 of one, log2(e) is within 2^-25 of itself, and the four other
+    # roundings are 2^-22 at most: 2^-17 covers it, and with it four exponentials of 2 ulp each. Below f32's normal values a step is 2^-149.
+    check_h(hc, hs, h, 2.0 ** -17 * np.abs(h) + 2.0 ** -148)
