@@ -21,7 +21,7 @@ SYMBOLS = ("moe_layer_create", "moe_layer_destroy", "moe_layer_forward", "moe_la
            "moe_layer_read_config", "moe_layer_forward_residual_device", "moe_rmsnorm_rows_device", "moe_layer_dispatch_row_bytes", "moe_layer_dispatch_plan_device", "moe_layer_dispatch_rows_device",
            "moe_layer_experts_partial_device", "moe_layer_combine_partials_device", "moe_gguf_open", "moe_gguf_close", "moe_gguf_layers", "moe_gguf_tensors", "moe_layer_create_from_gguf",
            "moe_route_work_bytes", "moe_route_logits_device", "moe_mx4_scale_row_bytes", "moe_mx4_quantize_rows_device", "moe_mx4_dequantize_rows_device",
-           "moe_mx4_from_blocks_device", "moe_mx4_product_device", "moe_mx4_gate_up_device", "moe_combine_rows_device", "moe_ops_status", "moe_ops_error")
+           "moe_mx4_from_blocks_device", "moe_mx4_product_device", "moe_mx4_gate_up_device", "moe_combine_rows_device", "moe_ops_status", "moe_ops_note_give_up", "moe_ops_error")
 
 
 class Config(C.Structure):
@@ -149,6 +149,7 @@ def lib():
         L.moe_mx4_gate_up_device.argtypes = [C.POINTER(Mx4Weights), vp, vp, u32, vp, C.c_float, vp, vp, vp]
         L.moe_combine_rows_device.argtypes = [vp, u32, u32, vp, vp, u32, u32, u32, vp, vp, vp]
         L.moe_ops_status.argtypes = [u32, vp]
+        L.moe_ops_note_give_up.argtypes = [vp]
         L.moe_ops_error.restype = C.c_char_p
         L.moe_abi_layout.argtypes = [C.POINTER(AbiRow), u32]
         L.moe_abi_layout.restype = u32

@@ -17,14 +17,16 @@
 // (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance); one lane (of a pair's first CTA) issues the copies of
 // scales to tensor memory, and one the MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
 //
-// Every wait on an mbarrier is bounded: one that runs out raises the CTA's abort flag and the device's error word (moe_ops_status), the other
-// waits return at once, and the CTA frees its tensor memory before it exits.
+// Every wait on an mbarrier is bounded: one that runs out raises the CTA's abort flag, the other waits return at once, and the CTA frees its tensor
+// memory and counts itself among the device's CTAs that gave up (moe_ops_status) before it exits.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <map>
 #include <type_traits>
+#include <utility>
 
 #include "mx4.cuh"
 #include "mx4_mma.cuh"
@@ -99,7 +101,8 @@ __device__ __forceinline__ float largest_magnitude(float v) {
   return m;
 }
 
-__device__ uint32_t g_gave_up;  // a wait ran out since moe_ops_status last asked
+__device__ uint32_t g_gave_up;  // CTAs that gave up a wait, ever: whoever asks compares it with what they were told last
+__global__ void k_note_give_up() { atomicAdd(&g_gave_up, 1u); }
 
 struct Mx4Args {
   const uint8_t *ws, *xs;   // scales of the matrices and the rows
@@ -186,7 +189,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *first_tile = first_row + kMaxExperts + 1;  // [E + 1] each
   uint16_t *tile_expert = (uint16_t *)(smem + SM::kTileExperts);
   uint32_t *warp_part = (uint32_t *)(smem + SM::kScales);  // before the scales come
-  uint32_t *error = &g_gave_up;
+  uint32_t *error = (uint32_t *)abort;  // the waits' error word: the flag itself
 
   if (tid == 0) {
     for (uint32_t s = 0; s < S; s++) mbar_init(bar(s), SM::kStageArrivals), mbar_init(bar(kEmpty + s), 1);
@@ -568,6 +571,7 @@ __global__ void __launch_bounds__(Mx4Form<Out, CTAS, NT>::kThreads, 1) k_mx4_pro
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && *abort) atomicAdd(&g_gave_up, 1u);
   if constexpr (CTAS == 2) cluster_sync();  // neither CTA leaves while the other may still read its shared memory or write its tensor memory
   if (warp == kMmaWarp) {
     __syncwarp();
@@ -681,14 +685,23 @@ MOE_API moe_status moe_ops_status(uint32_t timeout_ms, void *stream) {
   return ops_call([&] {
     cudaStream_t st = (cudaStream_t)stream;
     Stream::wait_on(st, timeout_ms);
-    uint32_t gave_up = 0, none = 0;
+    int device = 0;
+    CUDA_OK(cudaGetDevice(&device));
+    uint32_t gave_up = 0;
     CUDA_OK(cudaMemcpyFromSymbolAsync(&gave_up, g_gave_up, sizeof gave_up, 0, cudaMemcpyDeviceToHost, st));
     Stream::wait_on(st, timeout_ms);
     if (!gave_up) return;
-    CUDA_OK(cudaMemcpyToSymbolAsync(g_gave_up, &none, sizeof none, 0, cudaMemcpyHostToDevice, st));
-    Stream::wait_on(st, timeout_ms);
-    throw Timeout("a product gave up waiting for its copies or its products: its results are not to be used");
+    // What this thread was told about the stream last. Nothing is cleared: others hear of the same products.
+    thread_local std::map<std::pair<int, cudaStream_t>, uint32_t> told;
+    uint32_t &last = told[{device, st}];
+    if (last == gave_up) return;
+    last = gave_up;
+    throw Timeout("a product gave up waiting for its copies or its products: the results of products since this thread last asked are not to be used");
   });
+}
+
+MOE_API moe_status moe_ops_note_give_up(void *stream) {
+  return ops_call([&] { CUDA_OK(launch_kernel(false, k_note_give_up, dim3(1), dim3(1), 0, (cudaStream_t)stream)); });
 }
 
 }  // extern "C"

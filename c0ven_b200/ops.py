@@ -87,5 +87,6 @@ def combine_rows_device(y_ptr: int, y_type: int, R: int, inv_ptr: int, w_ptr: in
 
 
 def status(stream: int | None = None, timeout_ms: int = 0):
-    """Waits for stream; raises MoEError where that runs out, or where a product gave up one of its own waits since this was last asked."""
+    """Waits for stream; raises MoEError where that runs out, or where a product on the device, on any stream, gave up one of its own waits since
+    the calling thread last asked about this stream: products' results since then are not to be used."""
     _check(_lib.lib().moe_ops_status(timeout_ms, stream))

@@ -23,7 +23,7 @@ extern "C" {
 #define MOE_API
 #endif
 
-#define MOE_API_VERSION 3
+#define MOE_API_VERSION 4
 
 /* engine_status's values (include/engine_api.h:28-34). */
 typedef enum {
@@ -404,9 +404,13 @@ MOE_API moe_status moe_mx4_gate_up_device(const moe_mx4_weights *w, const void *
  * n_used 1 .. 16. out_dev may be residual_dev. */
 MOE_API moe_status moe_combine_rows_device(const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev, const float *w_dev, uint32_t T,
                                            uint32_t n_used, uint32_t n_embd, const float *residual_dev, float *out_dev, void *stream);
-/* Waits for stream, timeout_ms at most (0: 60 s). MOE_TIMEOUT when that ran out, or when a product on the current device has given up one of its
- * own waits (each bounded, about a second) since this was last asked: its results are then not to be used. Not while stream is captured. */
+/* Waits for stream, timeout_ms at most (0: 60 s). MOE_TIMEOUT when that ran out, or when a product on the current device, on any stream, has given up one
+ * of its own waits (each bounded, about a second) since the calling thread last asked about this stream: products' results since then are not to be used.
+ * Every thread is told for every stream that it asks about, each once; a thread that has not asked about a stream before is told of all there
+ * ever were. Not while stream is captured.
+ * moe_ops_note_give_up: counts one, queued on stream, as a product that gave up would, for tests of a caller's handling. */
 MOE_API moe_status moe_ops_status(uint32_t timeout_ms, void *stream);
+MOE_API moe_status moe_ops_note_give_up(void *stream);
 MOE_API const char *moe_ops_error(void);
 
 /* The layout the GPU holds a slice of nblocks blocks in: one run per field of the block, quants first, as the

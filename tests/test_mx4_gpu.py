@@ -631,3 +631,45 @@ def test_gates_far_below_zero(copies):
     # g and u are exact. To g = -80 the exponential's argument is below 116 and rounds by 2^-18 of one, log2(e) is within 2^-25 of itself, and the four other
     # roundings are 2^-22 at most: 2^-17 covers it, and with it four exponentials of 2 ulp each. Below f32's normal values a step is 2^-149.
     check_h(hc, hs, h, 2.0 ** -17 * np.abs(h) + 2.0 ** -148)
+
+
+def test_a_give_up_is_told_to_everyone():
+    """A product that gave up is told to every thread for every stream that it asks about, once each, whoever asks first; the count is raised by hand,
+    since no sound product gives up."""
+    import threading
+
+    import torch
+
+    def asked(stream):
+        try:
+            ops.status(stream)
+        except MoEError as e:
+            assert e.status == _lib.MOE_TIMEOUT and "gave up" in str(e)
+            return True
+        return False
+
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    streams = (a.cuda_stream, b.cuda_stream, None)
+    [asked(s) for s in streams]                               # what earlier ones left
+    assert not any(asked(s) for s in streams)
+    for _ in range(2):
+        assert _lib.lib().moe_ops_note_give_up(b.cuda_stream) == _lib.MOE_OK
+        b.synchronize()
+        assert [asked(s) for s in streams] == [True] * 3      # a, whose work was sound, asks first: b is told all the same
+        assert not any(asked(s) for s in streams)
+        seen = []
+        t = threading.Thread(target=lambda: seen.extend(asked(b.cuda_stream) for _ in range(2)))
+        t.start()
+        t.join()
+        assert seen == [True, False]                          # a thread that has not asked before is told too
+    # Two at once are one answer; a product after them is sound.
+    for s in (a, b):
+        assert _lib.lib().moe_ops_note_give_up(s.cuda_stream) == _lib.MOE_OK
+    torch.cuda.synchronize()
+    rng = np.random.default_rng(20)
+    wc, ws, w, xc, xs, x = product_case(rng, 1, 64, 64, None, 5)
+    y = torch.empty((5, 64), dtype=torch.float16, device="cuda")
+    assert asked(a.cuda_stream)
+    ops.mx4_product_device(ops.Mx4Weights(1, 64, 64, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), 5, None, y.data_ptr(), ops.F16, stream=a.cuda_stream)
+    assert [asked(s) for s in streams] == [False, True, True]
+    assert np.linalg.norm(y.double().cpu().numpy() - x @ w[0].T) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(x @ w[0].T)
