@@ -64,20 +64,25 @@ __global__ void __launch_bounds__(256) k_mx4_quantize(const X *x, uint64_t strid
 #pragma unroll
     for (uint32_t i = 0; i < sizeof(X) / 2; i++) raw[u][i] = in && t < map.T ? ((const uint4 *)(x + t * stride + k))[i] : make_uint4(0, 0, 0, 0);
   }
+  // All of the warp's lanes exchange before any is done: narrow rows are several a warp, and the last of them ends some lanes' work before others'.
+  uint32_t top[U];
 #pragma unroll
   for (uint32_t u = 0; u < U; u++) {
     uint32_t m = largest_bits(raw[u], (const X *)nullptr);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const uint32_t scale = mx_scale_of(m);
+    top[u] = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) {
+    const uint64_t t = map.row(u);
+    if (t >= map.T) break;
+    const uint32_t scale = mx_scale_of(top[u]);
     const float f = mx_inverse(scale);
     float v[8];
     load8((const X *)raw[u], v);
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] *= f;
     const uint32_t c = scale == 255 ? 0u : mx_codes8(v);
-    const uint64_t t = map.row(u);
-    if (t >= map.T) break;
     for (uint32_t j = 0; j < (inv ? n_used : 1); j++) {
       const uint64_t r = inv ? (uint64_t)(uint32_t)inv[t * n_used + j] : t;
       if (r >= R) continue;

@@ -673,3 +673,22 @@ def test_a_give_up_is_told_to_everyone():
     ops.mx4_product_device(ops.Mx4Weights(1, 64, 64, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), 5, None, y.data_ptr(), ops.F16, stream=a.cuda_stream)
     assert [asked(s) for s in streams] == [False, True, True]
     assert np.linalg.norm(y.double().cpu().numpy() - x @ w[0].T) <= (2.0 ** -11 + 1e-5) * np.linalg.norm(x @ w[0].T)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("T, K", [(38001, 32), (38003, 96), (37999, 128), (38005, 160)])
+def test_quantize_many_narrow_rows(type, T, K):
+    """Rows of fewer threads than a warp, several a thread: some of a warp's rows are past the last."""
+    import torch
+
+    rng = np.random.default_rng(T)
+    x = dev(rows_of(rng, T, K).astype(np.float32), type)
+    want = R.pack(*R.quantize(x.double().cpu().numpy()))
+    codes, scales = mx_buffers(T + 1, K)
+    ops.mx4_quantize_rows_device(x.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), T)
+    torch.cuda.synchronize()
+    assert np.array_equal(codes[:T].cpu().numpy(), want[0]) and np.array_equal(scales[:T].cpu().numpy(), want[1])
+    assert (codes[T] == 0xEE).all() and (scales[T] == 0xEE).all()
+    out = torch.empty((T, K), device="cuda")
+    ops.mx4_dequantize_rows_device(codes.data_ptr(), scales.data_ptr(), T, K, out.data_ptr(), ops.F32)
+    assert np.array_equal(out.double().cpu().numpy(), R.values(*R.unpack(*want)))
