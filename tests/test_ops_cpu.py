@@ -164,3 +164,26 @@ def test_a_files_mx_tensors_are_listed_and_no_layers(tmp_path):
         MoELayer(mx)
     assert e.value.status == _lib.MOE_BAD_ARGUMENT
     f.close()
+
+
+@pytest.mark.parametrize("past", [1 << 32, -(1 << 32), 1 << 63])
+def test_numbers_past_32_bits_are_refused(past):
+    """None is cut down to its low bits, which alone would be a call that is allowed."""
+    route = dict(logits_ptr=P, type=ops.F32, T=0, n_experts=64, n_used=4, ids_ptr=P, w_ptr=P, score=0, n_groups=1, n_groups_used=1, stride=0)
+    rows = dict(x_ptr=P, type=ops.F32, T=0, K=64, codes_ptr=P, scales_ptr=P, R=0, stride=0, inv_ptr=P, n_used=1)
+    back = dict(codes_ptr=P, scales_ptr=P, R=0, K=64, out_ptr=P, type=ops.F32)
+    blocks = dict(blocks_ptr=P, R=0, K=64, codes_ptr=P, scales_ptr=P)
+    product = dict(weights=ops.Mx4Weights(1, 64, 64, P, P), codes_ptr=P, scales_ptr=P, R=0, offsets_ptr=P, y_ptr=P, y_type=ops.F16)
+    gate_up = dict(weights=ops.Mx4Weights(1, 64, 64, P, P), codes_ptr=P, scales_ptr=P, R=0, offsets_ptr=P, h_codes_ptr=P, h_scales_ptr=P)
+    combine = dict(y_ptr=P, y_type=ops.F16, R=0, inv_ptr=P, w_ptr=P, T=0, n_used=2, n_embd=64, out_ptr=P)
+    weights = dict(n_experts=1, n_out=64, n_in=64, codes_ptr=P, scales_ptr=P)
+    for call, a in ((ops.route_logits_device, route), (ops.mx4_quantize_rows_device, rows), (ops.mx4_dequantize_rows_device, back), (ops.mx4_from_blocks_device, blocks),
+                    (ops.mx4_product_device, product), (ops.mx4_gate_up_device, gate_up), (ops.combine_rows_device, combine), (ops.Mx4Weights, weights),
+                    (ops.route_work_bytes, dict(T=1, n_experts=64)), (ops.mx4_scale_row_bytes, dict(K=64))):
+        if call is not ops.route_logits_device:  # which asks for the device before it finds that there is nothing to do
+            call(**a)
+        for name, v in a.items():
+            if isinstance(v, int) and not name.endswith("_ptr"):
+                refused(lambda: call(**(a | {name: v + past})), "stride" if name == "stride" else "32 bits")
+    refused(lambda: ops.route_logits_device(**(route | dict(T=100, offsets_ptr=P, inv_ptr=P, work_ptr=P, work_bytes=-1))), "32 bits")
+    refused(lambda: ops.status(timeout_ms=past), "32 bits")
