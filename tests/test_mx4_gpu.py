@@ -633,6 +633,135 @@ def test_gates_far_below_zero(copies):
     check_h(hc, hs, h, 2.0 ** -17 * np.abs(h) + 2.0 ** -148)
 
 
+def test_h_of_infinities_and_nans():
+    """NaN scales, sums past f32 and NaN under a limit: a block of h with an infinity or NaN is NaN, the others are as ever."""
+    import torch
+
+    rng = np.random.default_rng(16)
+    for E, F, rows, first in ((2, 64, 50, 20), (1, 4128, 208, 0)):                   # single CTAs; pairs
+        K = 320
+        wc, ws, w, xc, xs, x = product_case(rng, E, 2 * F, K, None, rows)
+        xs[17, 3] = 255                                                              # a row
+        ws[-1, 40, 9] = 255                                                          # a gate of the last expert
+        ws[-1, F + 3, 0] = 255                                                       # an up row of it
+        offsets = dev(np.array([0, first, rows][-E - 1:], np.int32))
+        bad = np.zeros((rows, F), bool)
+        bad[17] = True
+        bad[first:, [3, 40]] = True
+        w[-1, [40, F + 3]] = 0
+        x[17] = 0
+        off = [0, first, rows][-E - 1:]
+        v, size = by_expert(x, w, off, rows), by_expert(x, w, off, rows, True)
+        for limit in (0.0, 2.0):
+            hc, hs = mx_buffers(rows, F)
+            ops.mx4_gate_up_device(ops.Mx4Weights(E, 2 * F, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), rows, offsets.data_ptr(),
+                                   hc.data_ptr(), hs.data_ptr(), swiglu_limit=limit)
+            ops.status()
+            code, byte = R.unpack(hc.cpu().numpy(), hs.cpu().numpy())
+            block = bad.reshape(rows, -1, 32).any(2)
+            assert np.array_equal(byte == 255, block) and (code[np.repeat(block, 32, axis=1)] == 0).all()
+            h = R.swiglu(v[:, :F], v[:, F:], limit)
+            got = R.values(code, byte)
+            keep = ~np.repeat(block, 32, axis=1)
+            # A value that is no border's differs by a step of its code at most: 2 of the scale, an eighth to a quarter of the largest.
+            top = np.repeat(np.abs(h).reshape(rows, -1, 32).max(2), 32, axis=1)
+            assert (np.abs(got - h)[keep] <= 0.26 * top[keep] + 1e-30).all()
+    # Sums past f32, one value of the contraction alone: (g, u) of infinities, with and without a limit.
+    inf = np.inf
+    pairs = [(2.0, inf), (inf, 2.0), (-2.0, inf), (inf, -inf), (-192.0, -inf), (-inf, 2.0), (inf, 0.0), (2.0, 3.0)]
+    F, K = 32 * len(pairs), 32
+    big = 1.5 * 2.0 ** 100
+    w, x = np.zeros((2 * F, K)), np.zeros((4, K))
+    fill = lambda a: np.array([np.sign(p) * big if np.isinf(p) else p / 2.0 ** 60 for p in a]).repeat(32)  # noqa: E731
+    w[:F, 0], w[F:, 0] = fill([p[0] for p in pairs]), fill([p[1] for p in pairs])
+    x[:, 0] = 2.0 ** 60
+    (wc, ws), (xc, xs) = mx_of(w), mx_of(x)
+    for limit in (0.0, 7.0):
+        hc, hs = mx_buffers(4, F)
+        ops.mx4_gate_up_device(ops.Mx4Weights(1, 2 * F, K, wc.data_ptr(), ws.data_ptr()), xc.data_ptr(), xs.data_ptr(), 4, None, hc.data_ptr(), hs.data_ptr(), swiglu_limit=limit)
+        ops.status()
+        _, byte = R.unpack(hc.cpu().numpy(), hs.cpu().numpy())
+        with np.errstate(invalid="ignore"):
+            g, u = (np.array(a) for a in zip(*pairs))
+            want = ~np.isfinite(R.swiglu(g, u, limit))
+        assert want.sum() == (7 if limit == 0 else 1) and np.array_equal(byte == 255, np.tile(want, (4, 1)))
+
+
+def run_both(E, N, K, offsets, rows, rng):
+    """Product and gate_up of the same rows and matrices (2 F = N): y, h's codes and scales, filled with 7 and 0xEE before."""
+    import torch
+
+    wc, ws, w, xc, xs, x = product_case(rng, E, N, K, None, rows)
+    y = torch.full((rows, N), 7.0, dtype=torch.float16, device="cuda")
+    hc, hs = mx_buffers(rows, N // 2)
+    od, weights = dev(np.asarray(offsets, np.int32)), ops.Mx4Weights(E, N, K, wc.data_ptr(), ws.data_ptr())
+    ops.mx4_product_device(weights, xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), y.data_ptr(), ops.F16)
+    ops.mx4_gate_up_device(weights, xc.data_ptr(), xs.data_ptr(), rows, od.data_ptr(), hc.data_ptr(), hs.data_ptr())
+    ops.status()
+    return y, hc, hs, w, x
+
+
+def check_both(y, hc, hs, w, x, sound):
+    """Every row with the expert that the sound offsets give it; rows of none as they were."""
+    rows, N, K = y.shape[0], w.shape[1], w.shape[2]
+    F, mine = N // 2, np.zeros(rows, bool)
+    for e in range(w.shape[0]):
+        mine[sound[e]:sound[e + 1]] = True
+    v, size = by_expert(x, w, sound, rows), by_expert(x, w, sound, rows, True)
+    got = y.double().cpu().numpy()
+    off = 2.0 ** -11 * np.abs(v) + sum_bound(size, K) * (1 + 2.0 ** -11) + 2.0 ** -25
+    assert (np.abs(got - v)[mine] <= off[mine]).all() and (got[~mine] == 7.0).all()
+    g, u, e = v[:, :F], v[:, F:], sum_bound(size, K)
+    h = R.swiglu(g, u, 0.0)
+    err = 1.1 * (np.abs(u) + e[:, F:]) * e[:, :F] + np.maximum(g + e[:, :F], 0.28) * e[:, F:] + 2.0 ** -20 * np.abs(h) + 1e-38  # as in test_gate_up
+    at = np.flatnonzero(mine)
+    hc, hs = hc.cpu(), hs.cpu()
+    check_h(hc[at], hs[at], h[at], err[at])
+    assert (hc.numpy()[~mine] == 0xEE).all() and (hs.numpy()[~mine] == 0xEE).all()
+
+
+@pytest.mark.parametrize("N, K, rows, offsets, sound", [
+    (64, 64, 40, [30, 20, 35, 10, 5], [30, 30, 35, 35, 35]),
+    (64, 64, 40, [-5, 12, 11, 10, 39], [0, 12, 12, 12, 39]),
+    (2112, 64, 900, [700, 500, 820, 400, 3000], [700, 700, 820, 820, 900]),          # by pairs of CTAs
+    (2112, 64, 900, [250, 900, 100, 2 ** 31 - 1, -2 ** 31], [250, 900, 900, 900, 900])])
+def test_falling_offsets_count_as_the_one_before(N, K, rows, offsets, sound):
+    check_both(*run_both(4, N, K, offsets, rows, np.random.default_rng(17)), sound)
+
+
+def test_more_tiles_than_the_table_holds():
+    """Tiles of many experts past the first 1,024, whose expert is searched for: some experts without rows on both sides, some of one row."""
+    rng = np.random.default_rng(18)
+    E = 512
+    counts = rng.integers(0, 1400, E)
+    counts[rng.random(E) < 0.3] = 0
+    counts[rng.random(E) < 0.1] = 1
+    counts[-1] = 0
+    offsets = np.concatenate([[0], np.cumsum(counts)])
+    tiles = np.cumsum(-(-counts // 208))
+    at = int(np.searchsorted(tiles, 1024, side="right"))
+    counts[at + 1:at + 3] = 0                                                         # behind the expert whose tile is number 1,024 too
+    offsets = np.concatenate([[0], np.cumsum(counts)])
+    tiles = np.cumsum(-(-counts // 208))
+    assert tiles[-1] > 1100 and (counts[:at] == 0).sum() > 50 and (counts[at:] == 0).sum() > 20
+    check_both(*run_both(E, 64, 32, offsets, int(offsets[-1]), rng), offsets)
+
+
+def test_many_rows_of_a_files_blocks():
+    import torch
+
+    rng = np.random.default_rng(19)
+    for rows, K in ((70001, 64), (300, 8224)):
+        code, byte = rng.integers(0, 16, (rows, K), dtype=np.uint8), rng.integers(0, 256, (rows, K // 32), dtype=np.uint8)
+        b = code.reshape(rows, -1, 2, 16)
+        bd = dev(np.concatenate([byte[..., None], b[:, :, 0] | b[:, :, 1] << 4], -1))
+        codes, scales = mx_buffers(rows, K)
+        ops.mx4_from_blocks_device(bd.data_ptr(), rows, K, codes.data_ptr(), scales.data_ptr())
+        torch.cuda.synchronize()
+        want = R.pack(code, byte)
+        assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
+
+
 def test_a_give_up_is_told_to_everyone():
     """A product that gave up is told to every thread for every stream that it asks about, once each, whoever asks first; the count is raised by hand,
     since no sound product gives up."""

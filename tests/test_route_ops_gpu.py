@@ -302,3 +302,10 @@ def test_softmax_weights_over_the_whole_row():
     # and the product once each. The exponentials' errors are in the sum and in the weight alike, so that they count once at most.
     assert np.allclose(w, (p / p.sum(1, keepdims=True))[:, :2], rtol=8 * 2.0 ** -24, atol=0)
     assert np.array_equal(ids[:, 0], l.argmax(1))
+
+
+@pytest.mark.parametrize("E, G, used, k", [(256, 8, 4, 8), (64, 32, 3, 6), (500, 20, 7, 10)])
+def test_groups_in_long_steps(E, G, used, k):
+    rng = np.random.default_rng(E)
+    for T, score, with_bias in ((1500, "sigmoid", True), (901, "softmax", False)):
+        check(rng.standard_normal((T, E)), k, score=score, bias=(0.1 * rng.standard_normal(E)).astype(np.float32) if with_bias else None, n_groups=G, n_groups_used=used)
