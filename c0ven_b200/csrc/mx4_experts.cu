@@ -7,14 +7,14 @@
 // tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
 //
 // What bounds it: few rows an expert (1,000 over 512 experts of 2,048 x 512) HBM, 75 us of gate_up at 6.5 TB/s and 43 of the product at 5.8; many
-// (65,536 over 128 of 2,560 x 768) no one unit, 148 and 107 us at 3.5 and 2.4 PFLOP/s (5.4 on a dense 8,192 x 8,192 x 8,192): without its epilogue an
-// earlier gate_up took 123 of the 148 us it took where that was measured, without scales too 104, and the product 66 of 104 and 57; one row, 7 and 5 us,
+// (65,536 over 128 of 2,560 x 768) no one unit, 150 and 106 us at 3.4 and 2.4 PFLOP/s (5.3 on a dense 8,192 x 8,192 x 8,192). Taken apart in an earlier
+// build on another GPU, where the whole took 148 and 104: 123 and 66 without the epilogues, 104 and 57 without scales too. One row, 7.4 and 5 us, is
 // latency: 1,300 cycles until the experts' first rows are here, 700 for the tables, 2,600 until the first scales are in tensor memory, 490 a stage of
 // MMAs, 1,500 from the last to the end.
 //
 // Roles of a CTA's warps: one thread brings codes by bulk-tensor copies, 256 values of the contraction a stage; three warps bring the scales,
 // four stages (1,024 values: a sector of a row's scales) at a time in turn, word by word into the layout that the tensor core's copy reads
-// (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance); one lane (of a pair's first CTA) issues the copies of
+// (an expert's first row lies anywhere, so rows' scales cannot be laid out in advance; the matrices', which could, have the same form); one lane (of a pair's first CTA) issues the copies of
 // scales to tensor memory, and one the MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
 //
 // Every wait on an mbarrier is bounded: one that runs out raises the CTA's abort flag, the other waits return at once, and the CTA frees its tensor
@@ -618,10 +618,11 @@ void launch_product(const Mx4Args &args, const void *wc, const void *xc, cudaStr
 }
 
 // Tiles of 208 rows by pairs of CTAs where experts have more than 26 rows on average (many then have more than 32, two tiles of a single CTA) and there
-// are 32 items for pairs at least; else of 32 by single CTAs. gate_up and down by pairs and by single CTAs, us: 512 experts of 2,048 x 512, 10 rows
-// 7.7 + 5.6 and 6.7 + 5.1, 1,000 rows 78 + 43 and 75 + 43, 12,000 rows 95 + 53 and 93 + 53, 14,000 rows 96 + 55 and 94 + 58, 16,000 rows 96 + 56 and
-// 104 + 69, 32,000 rows 100 + 65 and 175 + 126; 128 of 2,560 x 768, 2,800 rows 48 + 27 and 47 + 26, skewed 48 + 27 and 49 + 28; one of 2,080 x 1,440, 200
-// rows (12 items for pairs) 10 + 8 and 10 + 6, 777 rows (48) 11 + 8 and 16 + 10; one of 8,192 x 4,096, 128 rows (32) 15 + 10 and 23 + 13.
+// are 32 items for pairs at least; else of 32 by single CTAs. The average is over all experts, as the host does not know which have rows. gate_up and
+// down by pairs and by single CTAs, us: 512 experts of 2,048 x 512, 10 rows 8.4 + 5.6 and 7.4 + 5.0, 1,000 rows 78 + 43 and 75 + 43, 12,000 rows 94 + 54
+// and 92 + 53, 14,000 rows 95 + 55 and 94 + 57, 16,000 rows 95 + 56 and 104 + 68, 32,000 rows 99 + 65 and 177 + 125; 128 of 2,560 x 768, 2,800 rows 48 + 27
+// and 46 + 26, skewed by a Zipf law of 1.1 47 + 28 and 52 + 30; one of 2,080 x 1,440, 200 rows (12 items for pairs) 11 + 8 and 10 + 6, 777 rows (48) 12 + 8
+// and 16 + 10; one of 8,192 x 4,096, 128 rows (32) 15 + 10 and 23 + 13.
 template <class Out>
 void launch(const Mx4Args &a, const void *wc, const void *xc, cudaStream_t st) {
   const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 208 + 1;

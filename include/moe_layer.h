@@ -318,7 +318,7 @@ MOE_API const char *moe_route_rows_static_error(void);
  *   moe_route_logits_device (ids, w, offsets, inv) -> moe_mx4_quantize_rows_device (rows into expert order by inv) ->
  *   moe_mx4_gate_up_device -> moe_mx4_product_device -> moe_combine_rows_device.
  *
- * They keep nothing between calls and allocate nothing: every buffer is the caller's, a DEVICE pointer of the current
+ * They keep nothing between calls (but for what moe_ops_status tells) and allocate nothing: every buffer is the caller's, a DEVICE pointer of the current
  * device (a host pointer or another device's is refused), and every call queues on stream (a cudaStream_t; null: the
  * default stream) without waiting, so a call can be captured into a graph. The first call of each on a device sets
  * kernel attributes; that may happen during a capture too. Calls with different buffers may overlap. T or R of 0 is a
@@ -347,8 +347,8 @@ typedef struct {
 /* A step's routing from its logits, [T] rows of n_experts values, stride values apart (0: n_experts). A row's scores s are
  * the softmax of its logits or their sigmoids; an expert's key is s + bias_dev[expert] (null: the score). With groups, the
  * n_groups_used groups whose two best keys have the largest sums stay (of one expert: its key). ids_dev [T][n_used] are the
- * largest keys' experts, best first; w_dev [T][n_used] their scores (without the bias), renormalised, times scale. Ties go to
- * the lower expert, or group. Which experts are chosen is decided as in 64-bit arithmetic on the given logits and bias; without a
+ * largest keys' experts, best first; w_dev [T][n_used] their scores (without the bias), renormalised, times scale, in f32 and
+ * within 2^-18 of themselves. Ties go to the lower expert, or group. Which experts are chosen is decided as in 64-bit arithmetic on the given logits and bias; without a
  * bias the logits' own order stands for the scores'.
  * An expert whose logit or bias is -infinity or NaN is out: it takes no part in softmax and is never chosen; a row with too few
  * others has id -1 and weight 0 in its last places.
@@ -392,7 +392,8 @@ typedef struct {
  * R counts as R, one below 0 or one before it as that; null: one expert has all R). Rows of no expert are left as they were. Sums are f32.
  *   product: y_dev [R][n_out], f16 or bf16 (MOE_TYPE_F16, MOE_TYPE_BF16), 16-byte aligned: the products, rounded once.
  *   gate_up: w's rows are n_out / 2 gate rows and then as many up rows, n_out a multiple of 64; h = g / (1 + exp(-g)) * u,
- *            with limit > 0 of min(g, limit) and of u held to [-limit, limit], to MX rows of n_out / 2 values.
+ *            with limit > 0 of min(g, limit) and of u held to [-limit, limit], to MX rows of n_out / 2 values. The sums apart, h is within
+ *            2^-17 of itself before its code is chosen: one that near a border between two codes may get either.
  * R at most 2^24. */
 MOE_API moe_status moe_mx4_product_device(const moe_mx4_weights *w, const void *codes_dev, const void *scales_dev, uint32_t R,
                                           const int32_t *offsets_dev, void *y_dev, uint32_t y_type, void *stream);
