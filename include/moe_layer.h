@@ -348,8 +348,8 @@ typedef struct {
  * the softmax of its logits or their sigmoids; an expert's key is s + bias_dev[expert] (null: the score). With groups, the
  * n_groups_used groups whose two best keys have the largest sums stay (of one expert: its key). ids_dev [T][n_used] are the
  * largest keys' experts, best first; w_dev [T][n_used] their scores (without the bias), renormalised, times scale, in f32 and
- * within 2^-18 of themselves. Ties go to the lower expert, or group. Which experts are chosen is decided as in 64-bit arithmetic on the given logits and bias; without a
- * bias the logits' own order stands for the scores'.
+ * within 2^-18 of themselves (one below 10^-37 may be 0). Ties go to the lower expert, or group. Which experts are chosen is
+ * decided as in 64-bit arithmetic on the given logits and bias; without a bias the logits' own order stands for the scores'.
  * An expert whose logit or bias is -infinity or NaN is out: it takes no part in softmax and is never chosen; a row with too few
  * others has id -1 and weight 0 in its last places.
  * offsets_dev (null: no lists; then inv_dev is null too): [n_experts + 1], expert e's rows in expert order are offsets[e] ..
