@@ -21,7 +21,9 @@ SYMBOLS = ("moe_layer_create", "moe_layer_destroy", "moe_layer_forward", "moe_la
            "moe_layer_read_config", "moe_layer_forward_residual_device", "moe_rmsnorm_rows_device", "moe_layer_dispatch_row_bytes", "moe_layer_dispatch_plan_device", "moe_layer_dispatch_rows_device",
            "moe_layer_experts_partial_device", "moe_layer_combine_partials_device", "moe_gguf_open", "moe_gguf_close", "moe_gguf_layers", "moe_gguf_tensors", "moe_layer_create_from_gguf",
            "moe_route_work_bytes", "moe_route_logits_device", "moe_mx4_scale_row_bytes", "moe_mx4_quantize_rows_device", "moe_mx4_dequantize_rows_device",
-           "moe_mx4_from_blocks_device", "moe_mx4_product_device", "moe_mx4_gate_up_device", "moe_combine_rows_device", "moe_ops_status", "moe_ops_note_give_up", "moe_ops_error")
+           "moe_mx4_from_blocks_device", "moe_mx4_product_device", "moe_mx4_gate_up_device", "moe_combine_rows_device", "moe_ops_status", "moe_ops_note_give_up", "moe_ops_error",
+           "moe_sort_rows_device", "moe_sort_rows_grad_device", "moe_combine_rows_grad_device", "moe_route_logits_grad_device", "moe_i8_quantize_rows_device",
+           "moe_i8_dequantize_rows_device", "moe_i8_product_device", "moe_i8_gate_up_device")
 
 
 class Config(C.Structure):
@@ -66,12 +68,17 @@ class Mx4Weights(C.Structure):
                 ("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p)]
 
 
+class I8Weights(C.Structure):
+    _fields_ = [("n_experts", C.c_uint32), ("n_out", C.c_uint32), ("n_in", C.c_uint32), ("reserved", C.c_uint32),
+                ("codes_dev", C.c_void_p), ("scales_dev", C.c_void_p)]
+
+
 class AbiRow(C.Structure):
     _fields_ = [("name", C.c_char_p), ("offset", C.c_uint32), ("size", C.c_uint32)]
 
 
 STRUCTS = {"moe_gguf_tensor": GgufTensor, "moe_layer_config": Config, "moe_layer_weights": Weights, "moe_tile": Tile, "moe_group": Group, "moe_layer_stats": Stats,
-           "moe_route_config": RouteConfig, "moe_mx4_weights": Mx4Weights, "moe_abi_row": AbiRow}
+           "moe_route_config": RouteConfig, "moe_mx4_weights": Mx4Weights, "moe_i8_weights": I8Weights, "moe_abi_row": AbiRow}
 
 _lib = None
 
@@ -148,6 +155,14 @@ def lib():
         L.moe_mx4_product_device.argtypes = [C.POINTER(Mx4Weights), vp, vp, u32, vp, vp, u32, vp]
         L.moe_mx4_gate_up_device.argtypes = [C.POINTER(Mx4Weights), vp, vp, u32, vp, C.c_float, vp, vp, vp]
         L.moe_combine_rows_device.argtypes = [vp, u32, u32, vp, vp, u32, u32, u32, vp, vp, vp]
+        L.moe_sort_rows_device.argtypes = [vp, u32, u64, u32, u32, u32, vp, vp, u32, vp, vp]
+        L.moe_sort_rows_grad_device.argtypes = [vp, u32, u32, vp, vp, vp, u64, u32, u32, u32, vp, vp, vp, vp]
+        L.moe_combine_rows_grad_device.argtypes = [vp, u32, vp, u32, u32, vp, vp, u32, u32, u32, vp, vp, vp]
+        L.moe_route_logits_grad_device.argtypes = [C.POINTER(RouteConfig), vp, u64, vp, u32, vp, vp, vp, u64, vp]
+        L.moe_i8_quantize_rows_device.argtypes = [vp, u32, u64, u32, u32, vp, u32, u32, vp, vp, vp]
+        L.moe_i8_dequantize_rows_device.argtypes = [vp, vp, u32, u32, vp, u32, vp]
+        L.moe_i8_product_device.argtypes = [C.POINTER(I8Weights), vp, vp, u32, vp, vp, u32, vp]
+        L.moe_i8_gate_up_device.argtypes = [C.POINTER(I8Weights), vp, vp, u32, vp, C.c_float, vp, u32, vp]
         L.moe_ops_status.argtypes = [u32, vp]
         L.moe_ops_note_give_up.argtypes = [vp]
         L.moe_ops_error.restype = C.c_char_p

@@ -1,0 +1,482 @@
+// Products of 8-bit rows in expert order with their experts' 8-bit matrices (include/moe_layer.h: moe_i8_product_device, moe_i8_gate_up_device) on the
+// tensor core's integer product: the sums are exact, the scales of the row and of the matrix's row come last.
+//
+// A work item is 128 rows of one expert's matrix for each CTA that works on it (for gate_up 64 features, the gate row and the up row of each next to
+// one another) times up to NT of the expert's rows. The matrix is the instruction's M side and the rows its N side, so a few rows cost a
+// short instruction and what an item costs is bringing the matrix. Persistent units (a CTA, or a pair of CTAs on two SMs that share the rows:
+// tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
+//
+// Roles of a CTA's warps: one thread brings the bytes by bulk-tensor copies, 128 values of the contraction a stage; one lane (of a pair's first CTA)
+// issues the MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
+//
+// Every wait on an mbarrier is bounded: one that runs out raises the CTA's abort flag, the other waits return at once, and the CTA frees its tensor
+// memory and counts itself among the device's CTAs that gave up (moe_ops_status) before it exits.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "i8_mma.cuh"
+#include "mx4.cuh"
+#include "ops_common.h"
+#include "tensor_map.h"
+
+namespace moe {
+namespace {
+
+constexpr uint32_t kMaxExperts = 512;
+constexpr uint32_t kRowsM = 128;        // matrix rows a CTA takes
+constexpr uint32_t kStageK = 128;       // values of the contraction a stage holds: 128 bytes of a row
+constexpr uint32_t kTileTable = 1024;   // tiles whose expert is looked up in a table
+constexpr uint32_t kChunk = 16;         // rows an epilogue warp turns at a time
+
+// min(g, limit) and u held to +-limit. NaN passes through.
+__device__ __forceinline__ void hold(float &g, float &u, float limit) {
+  asm("min.NaN.f32 %0, %0, %2;\n\tmin.NaN.f32 %1, %1, %2;\n\tmax.NaN.f32 %1, %1, %3;" : "+f"(g), "+f"(u) : "f"(limit), "f"(-limit));
+}
+// silu(g) * u in the approximate forms, for g from kFarGate on: the exponential's argument, 116 there, rounds by 2^-18. Below, where 1 / (1 + e^-g) is e^g
+// to f32 and may be too small for it, while u makes of it what the result's type holds: e^(g / 4) four times, the large factor first.
+constexpr float kFarGate = -80.0f;
+__device__ __forceinline__ float swiglu_near(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+__device__ __forceinline__ float swiglu_far(float g, float u) {
+  const float p = expf(0.25f * g);
+  return u * p * p * g * p * p;
+}
+
+__device__ uint32_t g_gave_up;  // CTAs that gave up a wait, ever
+
+struct I8Args {
+  const float *ws, *xs;  // scales of the matrices' rows and of the rows
+  const int32_t *offsets;
+  uint32_t E, N, K, R;
+  uint32_t items_per_tile;  // items that share a tile of rows
+  float limit;
+  void *y;
+};
+
+// Maps over the bytes of the matrices and, in boxes of 16, 32, 64 and 128 rows, of the rows.
+constexpr uint32_t kBoxes = 4;
+__host__ __device__ constexpr uint32_t box_rows(uint32_t i) { return 16u << i; }
+struct I8Maps {
+  CUtensorMap w, x[kBoxes];
+};
+
+// A form of the kernel: what it makes (GU: h of swiglu(gate, up), else the products), CTAs a unit has, and the most rows of a tile. Its shared memory: stages
+// of bytes; the scales of a tile's rows, an epilogue warp its own; barriers; the experts' first rows and first tiles; the tiles' experts.
+template <bool GU, uint32_t CTAS, uint32_t NT>
+struct I8Form {
+  static constexpr uint32_t kGroups = CTAS == 2 && GU ? 4 : 2;  // of four epilogue warps
+  static constexpr uint32_t kThreads = 32 * (2 + 4 * kGroups);
+  static constexpr uint32_t kStageBytes = (kRowsM + NT / CTAS) * 128;
+  static constexpr uint32_t kStages = CTAS == 2 ? 6 : 10;
+  static constexpr uint32_t kRowScales = kStages * kStageBytes;
+  static constexpr uint32_t kWarpScales = NT / kGroups;  // of a warp
+  static constexpr uint32_t kBarriers = kRowScales + 4 * kGroups * kWarpScales * 4;
+  static constexpr uint32_t kTables = kBarriers + 256;
+  static constexpr uint32_t kTileExperts = kTables + 2 * (kMaxExperts + 1) * 4 + 8;
+  static constexpr uint32_t kBytes = kTileExperts + 2 * kTileTable + 1024;  // and room to align the base to 1024
+  static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
+  static_assert(2 * kThreads > kMaxExperts, "two experts a thread");
+  static constexpr uint32_t kCols = 2 * NT;  // of tensor memory: two accumulators
+  static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0 && kCols >= 32, "tensor memory");
+  static_assert(NT % (kChunk * kGroups) == 0, "a group's chunks");
+};
+
+enum : uint32_t { kCopyWarp = 0, kMmaWarp = 1, kEpilogueWarp = 2 };
+
+template <class Out, bool GU, uint32_t CTAS, uint32_t NT>
+__global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_product(const __grid_constant__ I8Args a, const __grid_constant__ I8Maps maps) {
+  using namespace tc;
+  using SM = I8Form<GU, CTAS, NT>;
+  constexpr uint32_t S = SM::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0, unit = blockIdx.x / CTAS, nunits = gridDim.x / CTAS;
+  uint64_t *bars = (uint64_t *)(smem + SM::kBarriers);
+  // Barriers: stages full, empty; accumulators full, empty. Of a pair the first CTA's "full" of stages and "empty" of accumulators take both CTAs' arrivals.
+  constexpr uint32_t kEmpty = S, kAccFull = 2 * S, kAccEmpty = kAccFull + 2, kBars = kAccEmpty + 2;
+  static_assert(8 * kBars + 8 <= 256, "the barriers' room");
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](uint32_t i) { return bar0 + 8 * i; };
+  uint32_t *tmem_slot = (uint32_t *)(bars + kBars);
+  volatile uint32_t *abort = tmem_slot + 1;
+  uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *first_tile = first_row + kMaxExperts + 1;  // [E + 1] each
+  uint16_t *tile_expert = (uint16_t *)(smem + SM::kTileExperts);
+  uint32_t *warp_part = (uint32_t *)smem;  // before the stages come
+  uint32_t *error = (uint32_t *)abort;     // the waits' error word: the flag itself
+
+  if (tid == 0) {
+    for (uint32_t s = 0; s < S; s++) mbar_init(bar(s), CTAS), mbar_init(bar(kEmpty + s), 1);
+    for (uint32_t b = 0; b < 2; b++) mbar_init(bar(kAccFull + b), 1), mbar_init(bar(kAccEmpty + b), CTAS * 4 * SM::kGroups);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if constexpr (CTAS == 2) pair_arrive();
+  // Tensor memory is taken when the kernels before are done, and the next may come when it is: a kernel that held it while it waits for another on the
+  // same SM, which asks for it later, would wait for ever.
+  wait_for_predecessors();
+  if (warp == kMmaWarp) {
+    if constexpr (CTAS == 2)
+      tmem_alloc_pair(smem_u32(tmem_slot), SM::kCols);
+    else
+      tmem_alloc(smem_u32(tmem_slot), SM::kCols);
+  }
+  // The experts' first rows and first tiles, and the tiles' experts, two experts a thread. Offsets are held to 0 .. R, and to rise: each to the largest
+  // before it, which is looked for where one does not.
+  {
+    const uint32_t e = 2 * tid;
+    auto row_of = [&](uint32_t x) { return a.offsets ? min((uint32_t)max(a.offsets[x], 0), a.R) : x ? a.R : 0u; };
+    uint32_t r0 = e <= a.E ? row_of(e) : 0, r1 = e < a.E ? row_of(e + 1) : r0, r2 = e + 1 < a.E ? row_of(e + 2) : r1;
+    if (__syncthreads_or(r1 < r0 || r2 < r1)) {
+      for (uint32_t x = 0; x < min(e, a.E); x++) r0 = max(r0, row_of(x));
+      r1 = max(r0, r1), r2 = max(r1, r2);
+    }
+    dependents_may_launch();
+    const uint32_t t0 = (r1 - r0 + NT - 1) / NT, t1 = (r2 - r1 + NT - 1) / NT;
+    uint32_t sum = t0 + t1;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= (uint32_t)off) sum += o;
+    }
+    if (lane == 31) warp_part[warp] = sum;
+    __syncthreads();
+    sum += __reduce_add_sync(0xffffffffu, lane < warp ? warp_part[lane] : 0) - t0 - t1;
+    if (e <= a.E) first_row[e] = r0, first_tile[e] = sum;
+    if (e < a.E) first_row[e + 1] = r1, first_tile[e + 1] = sum + t0;
+    for (uint32_t t = sum; t < min(sum + t0 + t1, kTileTable); t++) tile_expert[t] = (uint16_t)(t < sum + t0 ? e : e + 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CTAS == 2) pair_wait();  // the other CTA's barriers exist before anything arrives on them
+  tc_fence_after();
+  const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK, ntiles = first_tile[a.E];
+  auto expert_at = [&](uint32_t t) {  // the last expert whose first tile is at most t
+    uint32_t lo = 0, hi = a.E;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (first_tile[mid] <= t)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  };
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t lead0 = CTAS == 2 ? map_to_cta(bar0, 0) : bar0;  // the first CTA's barriers as this CTA names them
+  auto lead = [&](uint32_t i) { return lead0 + 8 * i; };
+  bool ok = true;
+
+  // Item i is piece m = i % M of the matrix for tile t = i / M of the experts' tiles in order; a unit steps by nunits items.
+  struct Item {
+    uint32_t t, m;
+  };
+  const uint32_t step_t = nunits / M, step_m = nunits - step_t * M;
+  const Item first{unit / M, unit % M};
+  auto step = [&](Item &i) {
+    i.t += step_t, i.m += step_m;
+    if (i.m >= M) i.m -= M, i.t++;
+  };
+  // row0: the first of this CTA's matrix rows, or of its features.
+  struct Tile {
+    uint32_t expert, start, count, row0;
+  };
+  auto tile_at = [&](const Item &i) {
+    const uint32_t e = i.t < kTileTable ? tile_expert[i.t] : expert_at(i.t);
+    const uint32_t start = first_row[e] + (i.t - first_tile[e]) * NT;
+    return Tile{e, start, min(NT, first_row[e + 1] - start), (i.m * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
+  };
+  // The rows an instruction takes of a tile: rounded up to 16 for every CTA.
+  auto rounded = [&](uint32_t count) { return (count + 16 * CTAS - 1) & ~(16 * CTAS - 1); };
+
+  if (warp == kCopyWarp) {
+    if (lane == 0) {
+      uint32_t s = 0, phase = 1;  // of the stage's "empty": the first round finds it so
+      for (Item i = first; i.t < ntiles && ok; step(i)) {
+        const Tile t = tile_at(i);
+        // A CTA of a pair brings its half of the instruction's rows, by one copy or two. A copy may run past the tile's rows; what it brings then goes
+        // into columns nobody reads.
+        const uint32_t half = rounded(t.count) / CTAS, x_row = t.start + rank * half;
+        const uint32_t b0 = 27 - __clz(half), rest = half - box_rows(b0), b1 = rest > 16 ? 28 - __clz(rest - 1) : 0;
+        const uint32_t bytes = (kRowsM + box_rows(b0) + (rest ? box_rows(b1) : 0)) * 128;
+        for (uint32_t it = 0; it < KT && ok; it++) {
+          ok = mbar_wait(bar(kEmpty + s), phase, abort, error);
+          if (!ok) break;
+          const uint32_t at = smem_u32(smem + s * SM::kStageBytes), x0 = it * kStageK;
+          if constexpr (CTAS == 2)
+            mbar_arrive_expect_cluster(lead(s), bytes);
+          else
+            mbar_arrive_expect(lead(s), bytes);
+          tma_load_bytes<CTAS>(at, &maps.w, x0, t.row0, t.expert, lead(s));
+          tma_load_bytes<CTAS>(at + kRowsM * 128, &maps.x[b0], x0, x_row, 0, lead(s));
+          if (rest) tma_load_bytes<CTAS>(at + (kRowsM + box_rows(b0)) * 128, &maps.x[b1], x0, x_row + box_rows(b0), 0, lead(s));
+          if (++s == S) s = 0, phase ^= 1;
+        }
+      }
+      if (!ok) {
+        // Copies already issued may still be on their way: give them time to land before the CTA leaves.
+        const long long t0 = clock64();
+        while (clock64() - t0 < 400000) {
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (rank == 0) {
+      const uint32_t leader = elect_leader();
+      auto commit = [&](uint32_t i) {
+        if constexpr (CTAS == 2)
+          mma_commit_pair(leader, bar(i), 3);
+        else
+          mma_commit(leader, bar(i));
+      };
+      uint32_t s = 0, phase = 0, b = 0, acc_phase = 1;
+      for (Item i = first; i.t < ntiles && ok; step(i)) {
+        const Tile t = tile_at(i);
+        const uint32_t acc = tmem_base + b * NT, idesc = i8_instr_desc(rounded(t.count), CTAS * kRowsM);
+        ok = mbar_wait_warp(bar(kAccEmpty + b), acc_phase, abort, error);
+        for (uint32_t it = 0; it < KT && ok; it++) {
+          ok = mbar_wait_warp(bar(s), phase, abort, error);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t stage = smem_u32(smem + s * SM::kStageBytes), rows = stage + kRowsM * 128;
+          const uint32_t steps = min(4u, (K - it * kStageK + 31) / 32);
+#pragma unroll
+          for (uint32_t k = 0; k < 4; k++)
+            if (k < steps) mma_i8<CTAS>(leader, acc, smem_desc_sw128(stage + 32 * k), smem_desc_sw128(rows + 32 * k), idesc, (it | k) != 0);
+          commit(kEmpty + s);
+          if (++s == S) s = 0, phase ^= 1;
+        }
+        if (!ok) break;
+        commit(kAccFull + b);
+        acc_phase ^= b, b ^= 1;
+      }
+    }
+  } else {
+    // Warp w reads tensor memory's lanes 32 (w % 4) ...; the groups take chunks of 16 rows in turn.
+    const uint32_t q = warp % 4, group = (warp - kEpilogueWarp) / 4;
+    constexpr uint32_t dc = SM::kGroups * kChunk;
+    const uint32_t c0 = group * kChunk;
+    float *row_scales = (float *)(smem + SM::kRowScales) + (4 * group + q) * SM::kWarpScales;
+    uint32_t b = 0, phase = 0;
+    for (Item i = first; i.t < ntiles && ok; step(i)) {
+      const Tile t = tile_at(i);
+      const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT;
+      // The scales of the warp's rows, chunk after chunk, and of the lane's matrix rows, while the products run.
+      __syncwarp();  // those of the tile before are read
+#pragma unroll
+      for (uint32_t k = lane; k < SM::kWarpScales; k += 32) {
+        const uint32_t r = c0 + k / kChunk * dc + k % kChunk;
+        row_scales[k] = r < t.count ? a.xs[t.start + r] : 0.0f;
+      }
+      const uint32_t f = GU ? t.row0 + 16 * q + lane / 2 : t.row0 + 32 * q + lane;
+      const bool in = f < (GU ? F : a.N);  // features come 32 together
+      const float *ws = a.ws + (uint64_t)t.expert * a.N + f;
+      const float s0 = in ? ws[0] : 0.0f, s1 = GU && in ? ws[F] : 0.0f;
+      __syncwarp();
+      ok = mbar_wait_warp(bar(kAccFull + b), phase, abort, error);
+      if (!ok) break;
+      tc_fence_after();
+      const float *sx = row_scales;
+      // A chunk's sums are on their way from tensor memory while the one before is turned.
+      auto turn = [&](uint32_t c, const uint32_t *v) {
+        const uint32_t left = t.count - c;
+        if constexpr (!GU) {
+          // A lane holds one feature of 16 rows. Two lanes with neighbouring features share out two rows: the even one stores both features of the
+          // first, the odd one of the second.
+          const uint32_t odd = lane & 1, sel = odd ? 0x3276u : 0x5410u;
+          Out *p = (Out *)a.y + (uint64_t)(t.start + c + odd) * a.N + (f - odd);
+#pragma unroll
+          for (uint32_t j = 0; j < 16; j += 2, p += 2 * (uint64_t)a.N) {
+            const float2 s = *(const float2 *)(sx + j);
+            const uint32_t mine = pack2((float)(int32_t)v[j] * s.x * s0, (float)(int32_t)v[j + 1] * s.y * s0, (const Out *)nullptr);
+            const uint32_t theirs = __shfl_xor_sync(0xffffffffu, mine, 1);
+            if (in && j + odd < left) *(uint32_t *)p = __byte_perm(mine, theirs, sel);
+          }
+        } else {
+          // Even lanes hold gate sums of 16 rows, odd ones the same feature's up sums. They exchange: the even one takes both of the first eight rows, the
+          // odd one of the last eight; then lanes of neighbouring features share out two rows, as above.
+          const uint32_t up = lane & 1, odd = lane / 2 & 1, sel = odd ? 0x3276u : 0x5410u;
+          float h[8];
+          float g[8], u[8];
+#pragma unroll
+          for (uint32_t j = 0; j < 8; j++) {
+            const uint32_t keep = up ? v[8 + j] : v[j], got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[8 + j], 1);
+            const float s = sx[8 * up + j];
+            g[j] = (float)(int32_t)(up ? got : keep) * s * s0, u[j] = (float)(int32_t)(up ? keep : got) * s * s1;
+          }
+          if (a.limit > 0.0f)
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) hold(g[j], u[j], a.limit);
+          float low = 0.0f;
+#pragma unroll
+          for (uint32_t j = 0; j < 8; j++) low = fminf(low, g[j]);
+          if (low < kFarGate) {  // a NaN gate does not count here, and stays one
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) h[j] = g[j] < kFarGate ? swiglu_far(g[j], u[j]) : swiglu_near(g[j], u[j]);
+          } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) h[j] = swiglu_near(g[j], u[j]);
+          }
+          Out *p = (Out *)a.y + (uint64_t)(t.start + c + 8 * up + odd) * F + (f - odd);
+#pragma unroll
+          for (uint32_t j = 0; j < 8; j += 2, p += 2 * (uint64_t)F) {
+            const uint32_t mine = pack2(h[j], h[j + 1], (const Out *)nullptr), theirs = __shfl_xor_sync(0xffffffffu, mine, 2);
+            if (in && 8 * up + j + odd < left) *(uint32_t *)p = __byte_perm(mine, theirs, sel);
+          }
+        }
+      };
+      uint32_t v[16], u[16];
+      if (c0 < t.count) tmem_ld16(from + c0, v);
+      for (uint32_t c = c0; c < t.count; c += 2 * dc, sx += 2 * kChunk) {
+        tmem_ld_wait16(v);
+        if (c + dc < t.count) tmem_ld16(from + c + dc, u);
+        turn(c, v);
+        if (c + dc >= t.count) break;
+        tmem_ld_wait16(u);
+        if (c + 2 * dc < t.count) tmem_ld16(from + c + 2 * dc, v);
+        sx += kChunk;
+        turn(c + dc, u);
+        sx -= kChunk;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CTAS == 2)
+          mbar_arrive_cluster(lead(kAccEmpty + b));
+        else
+          mbar_arrive(lead(kAccEmpty + b));
+      }
+      phase ^= b, b ^= 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort) atomicAdd(&g_gave_up, 1u);
+  if constexpr (CTAS == 2) cluster_sync();  // neither CTA leaves while the other may still read its shared memory or write its tensor memory
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    if constexpr (CTAS == 2)
+      tmem_free_pair(tmem_base, SM::kCols);
+    else
+      tmem_free(tmem_base, SM::kCols);
+  }
+}
+
+template <class Out, bool GU, uint32_t CTAS, uint32_t NT>
+void launch_product(const I8Args &args, const void *wc, const void *xc, cudaStream_t st) {
+  using Form = I8Form<GU, CTAS, NT>;
+  constexpr auto kernel = k_i8_product<Out, GU, CTAS, NT>;
+  I8Args a = args;
+  int device = 0;
+  CUDA_OK(cudaGetDevice(&device));
+  constexpr size_t smem = Form::kBytes;
+  static std::atomic<uint32_t> done{0};
+  CUDA_OK(ensure_dynamic_smem(kernel, smem, done, device));
+  uint32_t units = 0;
+  if constexpr (CTAS == 2) {
+    CUDA_OK(max_pairs<kernel>(Form::kThreads, smem, device, units));
+  } else {
+    int sms = 0;
+    CUDA_OK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    units = (uint32_t)sms;
+  }
+  const uint32_t rows = CTAS * (GU ? kRowsM / 2 : kRowsM), all = GU ? a.N / 2 : a.N;
+  a.items_per_tile = (all + rows - 1) / rows;
+  const uint64_t most = ((uint64_t)a.R / NT + std::min(a.E, a.R)) * a.items_per_tile;  // items there can be
+  I8Maps maps;
+  maps.w = make_bytes_map(wc, a.K, all, GU ? 2 : 1, a.E, GU ? kRowsM / 2 : kRowsM);
+  for (uint32_t i = 0; i < kBoxes; i++)
+    if (box_rows(i) <= NT / CTAS) maps.x[i] = make_bytes_map(xc, a.K, a.R, 1, 1, box_rows(i));
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension, at[1].val.clusterDim = {CTAS, 1, 1};
+  cfg.gridDim = dim3(CTAS * (unsigned)std::min<uint64_t>(most, units)), cfg.blockDim = dim3(Form::kThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+  cfg.attrs = at, cfg.numAttrs = CTAS;  // a single CTA is no cluster
+  CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, maps));
+}
+
+// Tiles of 256 rows by pairs of CTAs where experts have more than 26 rows on average and there are 32 items for pairs at least; else of 32 by single
+// CTAs. The average is over all experts, as the host does not know which have rows.
+template <class Out, bool GU>
+void launch(const I8Args &a, const void *wc, const void *xc, cudaStream_t st) {
+  const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 256 + 1;
+  if (a.R > 26ull * a.E && pieces * tiles >= 32)
+    launch_product<Out, GU, 2, 256>(a, wc, xc, st);
+  else
+    launch_product<Out, GU, 1, 32>(a, wc, xc, st);
+}
+
+I8Args arguments(const moe_i8_weights *w, const float *scales, uint32_t R, const int32_t *offsets) {
+  need(w != nullptr, "weights are required");
+  need(w->n_experts >= 1 && w->n_experts <= kMaxExperts, "n_experts must be 1 .. 512");
+  need(w->n_out >= 32 && w->n_out % 32 == 0 && w->n_out <= kMxMaxValues, "n_out must be a multiple of 32, 32 .. 65536");
+  need(w->n_in >= 32 && w->n_in % 32 == 0 && w->n_in <= kMxMaxValues, "n_in must be a multiple of 32, 32 .. 65536");
+  need(w->reserved == 0, "reserved must be 0");
+  need(offsets || w->n_experts == 1, "offsets are required for more than one expert");
+  need(R <= 1u << 24, "R must be at most 2^24");
+  I8Args a{};
+  a.ws = w->scales_dev, a.xs = scales;
+  a.offsets = offsets, a.E = w->n_experts, a.N = w->n_out, a.K = w->n_in, a.R = R;
+  return a;
+}
+
+template <bool GU>
+void call(const I8Args &a, const moe_i8_weights *w, const void *codes, uint32_t type, cudaStream_t st) {
+  need_device({{w->codes_dev, "weight codes", 16}, {a.ws, "weight scales", 4}, {codes, "codes", 16}, {a.xs, "scales", 4}, {a.offsets, "offsets", 4, true},
+               {a.y, GU ? "h" : "y", 16}});
+  if (type == MOE_TYPE_BF16)
+    launch<__nv_bfloat16, GU>(a, w->codes_dev, codes, st);
+  else
+    launch<__half, GU>(a, w->codes_dev, codes, st);
+}
+
+}  // namespace
+
+uint32_t i8_gave_up(cudaStream_t st, uint32_t timeout_ms) {
+  uint32_t n = 0;
+  CUDA_OK(cudaMemcpyFromSymbolAsync(&n, g_gave_up, sizeof n, 0, cudaMemcpyDeviceToHost, st));
+  Stream::wait_on(st, timeout_ms);
+  return n;
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+MOE_API moe_status moe_i8_product_device(const moe_i8_weights *w, const void *codes_dev, const float *scales_dev, uint32_t R, const int32_t *offsets_dev, void *y_dev,
+                                         uint32_t y_type, void *stream) {
+  return ops_call([&] {
+    need(y_type == MOE_TYPE_F16 || y_type == MOE_TYPE_BF16, "y_type must be MOE_TYPE_F16 or MOE_TYPE_BF16");
+    I8Args a = arguments(w, scales_dev, R, offsets_dev);
+    if (R == 0) return;
+    a.y = y_dev;
+    call<false>(a, w, codes_dev, y_type, (cudaStream_t)stream);
+  });
+}
+
+MOE_API moe_status moe_i8_gate_up_device(const moe_i8_weights *w, const void *codes_dev, const float *scales_dev, uint32_t R, const int32_t *offsets_dev,
+                                         float swiglu_limit, void *h_dev, uint32_t h_type, void *stream) {
+  return ops_call([&] {
+    need(h_type == MOE_TYPE_F16 || h_type == MOE_TYPE_BF16, "h_type must be MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need(!(swiglu_limit < 0.0f) && swiglu_limit - swiglu_limit == 0.0f, "swiglu_limit must be 0 or a positive number");
+    I8Args a = arguments(w, scales_dev, R, offsets_dev);
+    need(a.N % 64 == 0, "gate and up rows together must be a multiple of 64");
+    if (R == 0) return;
+    a.y = h_dev, a.limit = swiglu_limit;
+    call<true>(a, w, codes_dev, h_type, (cudaStream_t)stream);
+  });
+}
+
+}  // extern "C"

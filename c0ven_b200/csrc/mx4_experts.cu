@@ -691,6 +691,7 @@ MOE_API moe_status moe_ops_status(uint32_t timeout_ms, void *stream) {
     uint32_t gave_up = 0;
     CUDA_OK(cudaMemcpyFromSymbolAsync(&gave_up, g_gave_up, sizeof gave_up, 0, cudaMemcpyDeviceToHost, st));
     Stream::wait_on(st, timeout_ms);
+    gave_up += i8_gave_up(st, timeout_ms);
     if (!gave_up) return;
     // What this thread was told about the stream last. Nothing is cleared: others hear of the same products.
     thread_local std::map<std::pair<int, cudaStream_t>, uint32_t> told;

@@ -1,0 +1,292 @@
+// Rows to expert order in their own type, and the gradients of that and of the combine (include/moe_layer.h). Single passes over their data.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "mx4.cuh"
+#include "ops_common.h"
+
+namespace moe {
+namespace {
+
+constexpr uint32_t kRowsMaxUsed = 16;
+constexpr uint32_t kThreads = 256;
+
+// How a step's rows are dealt to a CTA of 256 threads: 2^log2 neighbouring threads a row; of its octets, groups of eight values, thread i takes i,
+// i + 2^log2 and so on.
+struct StepRows {
+  uint32_t T, log2, octets;
+  __device__ uint64_t row() const { return (uint64_t)blockIdx.x * (kThreads >> log2) + (threadIdx.x >> log2); }
+  __device__ uint32_t first() const { return threadIdx.x & ((1u << log2) - 1); }
+  __device__ uint32_t step() const { return 1u << log2; }
+};
+
+template <class X>
+__global__ void __launch_bounds__(kThreads) k_sort_rows(const X *x, uint64_t stride, const StepRows map, const int32_t *inv, const float *w, uint32_t n_used, uint32_t R,
+                                                        X *xs) {
+  dependents_may_launch(), wait_for_predecessors();
+  const uint64_t t = map.row(), D = 8ull * map.octets;
+  if (t >= map.T) return;
+  for (uint32_t o = map.first(); o < map.octets; o += map.step()) {
+    uint4 raw[sizeof(X) / 2];
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(X) / 2; i++) raw[i] = ((const uint4 *)(x + t * stride + 8 * o))[i];
+    float v[8];
+    if (w) load8((const X *)raw, v);
+#pragma unroll 4
+    for (uint32_t j = 0; j < n_used; j++) {
+      const uint32_t r = (uint32_t)inv[t * n_used + j];
+      if (r >= R) continue;
+      X *to = xs + r * D + 8 * o;
+      if (w) {
+        const float f = w[t * n_used + j];
+        float u[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = v[i] * f;
+        store8(to, u);
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(X) / 2; i++) ((uint4 *)to)[i] = raw[i];
+      }
+    }
+  }
+}
+
+// The sums of 16 numbers a thread over a row's 2^log2 threads, written by the row's first ones: n of them to out. The CTA's threads come here
+// together. (Numbers, not lanes, are halved by the first four exchanges, each lane keeping those whose index has its bits: 16 exchanges a warp instead of 80.)
+__device__ __forceinline__ void row_sums(float (&d)[kRowsMaxUsed], uint32_t log2, float (*part)[kRowsMaxUsed], bool in, uint32_t n, float *out) {
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  if (log2 >= 5) {
+#pragma unroll
+    for (uint32_t h = 8, bit = 16; h; h /= 2, bit /= 2) {
+#pragma unroll
+      for (uint32_t i = 0; i < h; i++) {
+        const float keep = lane & bit ? d[i + h] : d[i], give = lane & bit ? d[i] : d[i + h];
+        d[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+      }
+    }
+    d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+    // Lane l has the sum of number l / 2.
+    if (log2 == 5) {
+      if (in && lane % 2 == 0 && lane / 2 < n) out[lane / 2] = d[0];
+      return;
+    }
+    if (lane % 2 == 0) part[warp][lane / 2] = d[0];
+    __syncthreads();
+    const uint32_t i = threadIdx.x & ((1u << log2) - 1), each = 1u << (log2 - 5);
+    if (in && i < n) {
+      float s = 0.0f;
+      for (uint32_t k = 0; k < each; k++) s += part[(warp & ~(each - 1)) + k][i];
+      out[i] = s;
+    }
+    return;
+  }
+  const uint32_t i = lane & ((1u << log2) - 1);
+#pragma unroll
+  for (uint32_t j = 0; j < kRowsMaxUsed; j++) {
+    if (j >= n) break;
+    for (uint32_t off = (1u << log2) / 2; off; off /= 2) d[j] += __shfl_xor_sync(0xffffffffu, d[j], off);
+    if (in && i == 0) out[j] = d[j];
+  }
+}
+
+// dx[t] = (add[t] +) sum_j (w[t][j]) dxs[inv[t][j]], and where dw is wanted dw[t][j] = <x[t], dxs[inv[t][j]]>.
+template <class X, bool DW>
+__global__ void __launch_bounds__(kThreads) k_sort_rows_grad(const X *dxs, const StepRows map, uint32_t R, const int32_t *inv, const float *w, const X *x, uint64_t stride,
+                                                             uint32_t n_used, const X *add, X *dx, float *dw) {
+  __shared__ float part[DW ? kThreads / 32 : 1][kRowsMaxUsed];
+  dependents_may_launch(), wait_for_predecessors();
+  const uint64_t t = map.row(), D = 8ull * map.octets;
+  const bool in = t < map.T;
+  float dot[kRowsMaxUsed];
+#pragma unroll
+  for (uint32_t j = 0; j < kRowsMaxUsed; j++) dot[j] = 0.0f;
+  if (in) {
+    for (uint32_t o = map.first(); o < map.octets; o += map.step()) {
+      float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, xv[8];
+      if constexpr (DW) load8(x + t * stride + 8 * o, xv);
+#pragma unroll
+      for (uint32_t j0 = 0; j0 < kRowsMaxUsed; j0 += 4) {
+        if (j0 >= n_used) break;
+        uint32_t r[4];
+        float v[4][8];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+          r[j] = j0 + j < n_used ? (uint32_t)inv[t * n_used + j0 + j] : 0xFFFFFFFFu;
+          if (r[j] < R) load8(dxs + r[j] * D + 8 * o, v[j]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+          if (r[j] >= R) continue;
+          const float f = w ? w[t * n_used + j0 + j] : 1.0f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) acc[i] = fmaf(f, v[j][i], acc[i]);
+          if constexpr (DW)
+#pragma unroll
+            for (int i = 0; i < 8; i++) dot[j0 + j] = fmaf(xv[i], v[j][i], dot[j0 + j]);
+        }
+      }
+      if (dx) {
+        if (add) {
+          float v[8];
+          load8(add + t * D + 8 * o, v);
+#pragma unroll
+          for (int i = 0; i < 8; i++) acc[i] += v[i];
+        }
+        store8(dx + t * D + 8 * o, acc);
+      }
+    }
+  }
+  if constexpr (DW) row_sums(dot, map.log2, part, in, n_used, dw + t * n_used);
+}
+
+// dy[inv[t][j]] = w[t][j] dout[t], dw[t][j] = <dout[t], y[inv[t][j]]>. dy may be y: a thread has read what it writes over.
+template <class G, class Y>
+__global__ void __launch_bounds__(kThreads) k_combine_rows_grad(const G *dout, const Y *y, const StepRows map, uint32_t R, const int32_t *inv, const float *w,
+                                                                uint32_t n_used, Y *dy, float *dw) {
+  __shared__ float part[kThreads / 32][kRowsMaxUsed];
+  dependents_may_launch(), wait_for_predecessors();
+  const uint64_t t = map.row(), D = 8ull * map.octets;
+  const bool in = t < map.T;
+  float dot[kRowsMaxUsed];
+#pragma unroll
+  for (uint32_t j = 0; j < kRowsMaxUsed; j++) dot[j] = 0.0f;
+  if (in) {
+    for (uint32_t o = map.first(); o < map.octets; o += map.step()) {
+      float g[8];
+      load8(dout + t * D + 8 * o, g);
+#pragma unroll
+      for (uint32_t j0 = 0; j0 < kRowsMaxUsed; j0 += 4) {
+        if (j0 >= n_used) break;
+        uint32_t r[4];
+        float v[4][8];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+          r[j] = j0 + j < n_used ? (uint32_t)inv[t * n_used + j0 + j] : 0xFFFFFFFFu;
+          if (dw && r[j] < R) load8(y + r[j] * D + 8 * o, v[j]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+          if (r[j] >= R) continue;
+          if (dw)
+#pragma unroll
+            for (int i = 0; i < 8; i++) dot[j0 + j] = fmaf(g[i], v[j][i], dot[j0 + j]);
+          if (dy) {
+            const float f = w[t * n_used + j0 + j];
+            float u[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) u[i] = f * g[i];
+            store8(dy + r[j] * D + 8 * o, u);
+          }
+        }
+      }
+    }
+  }
+  if (dw) row_sums(dot, map.log2, part, in, n_used, dw + t * n_used);
+}
+
+template <class F>
+void with_step_rows(uint32_t T, uint32_t n_embd, F &&f) {
+  StepRows map{T, 0, n_embd / 8};
+  while (map.log2 < 8 && (1u << map.log2) < map.octets) map.log2++;
+  const uint32_t rows = kThreads >> map.log2;
+  f(map, dim3((T + rows - 1) / rows));
+}
+
+void need_step(uint32_t T, uint32_t R, uint32_t n_used, uint32_t n_embd) {
+  need(n_used >= 1 && n_used <= kRowsMaxUsed, "n_used must be 1 .. 16");
+  need(n_embd >= 8 && n_embd % 8 == 0 && n_embd <= 1u << 24, "n_embd must be a multiple of 8, at most 2^24");
+  need(T < 1u << 31 && R < 1u << 31, "T and R must be below 2^31");
+}
+
+void need_stride(uint64_t stride, uint32_t n_embd, uint32_t size) {
+  need(stride == 0 || (stride >= n_embd && stride < 1ull << 32 && stride * size % 16 == 0), "stride must be 0, or n_embd at least with rows 16-byte aligned");
+}
+
+// Calls f with a null pointer of the type's element.
+template <class F>
+void with_type(uint32_t type, F &&f) {
+  if (type == MOE_TYPE_F32)
+    f((float *)nullptr);
+  else if (type == MOE_TYPE_F16)
+    f((__half *)nullptr);
+  else
+    f((__nv_bfloat16 *)nullptr);
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+MOE_API moe_status moe_sort_rows_device(const void *x_dev, uint32_t type, uint64_t stride, uint32_t T, uint32_t n_used, uint32_t n_embd, const int32_t *inv_dev,
+                                        const float *w_dev, uint32_t R, void *xs_dev, void *stream) {
+  return ops_call([&] {
+    const uint32_t size = row_type_bytes(type);
+    need(size != 0, "type must be MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need_step(T, R, n_used, n_embd);
+    need_stride(stride, n_embd, size);
+    if (T == 0 || R == 0) return;
+    need_device({{x_dev, "x", 16}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {xs_dev, "xs", 16}});
+    with_step_rows(T, n_embd, [&](StepRows map, dim3 grid) {
+      with_type(type, [&](auto *of) {
+        using X = std::remove_pointer_t<decltype(of)>;
+        CUDA_OK(launch_kernel(true, k_sort_rows<X>, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)x_dev, stride ? stride : n_embd, map, inv_dev, w_dev,
+                              n_used, R, (X *)xs_dev));
+      });
+    });
+  });
+}
+
+MOE_API moe_status moe_sort_rows_grad_device(const void *dxs_dev, uint32_t type, uint32_t R, const int32_t *inv_dev, const float *w_dev, const void *x_dev, uint64_t stride,
+                                             uint32_t T, uint32_t n_used, uint32_t n_embd, const void *add_dev, void *dx_dev, float *dw_dev, void *stream) {
+  return ops_call([&] {
+    const uint32_t size = row_type_bytes(type);
+    need(size != 0, "type must be MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need_step(T, R, n_used, n_embd);
+    need_stride(stride, n_embd, size);
+    need(dx_dev || dw_dev, "dx or dw is required");
+    need(!dw_dev || x_dev, "x is required for dw");
+    need(!add_dev || dx_dev, "dx is required with add");
+    if (T == 0) return;
+    // With R 0 no row of dxs is read: it may be null then.
+    need_device({{dxs_dev, "dxs", 16, R == 0}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {x_dev, "x", 16, true}, {add_dev, "add", 16, true}, {dx_dev, "dx", 16, true},
+                 {dw_dev, "dw", 4, true}});
+    with_step_rows(T, n_embd, [&](StepRows map, dim3 grid) {
+      with_type(type, [&](auto *of) {
+        using X = std::remove_pointer_t<decltype(of)>;
+        const auto kernel = dw_dev ? k_sort_rows_grad<X, true> : k_sort_rows_grad<X, false>;
+        CUDA_OK(launch_kernel(true, kernel, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)dxs_dev, map, R, inv_dev, w_dev, (const X *)x_dev,
+                              stride ? stride : n_embd, n_used, (const X *)add_dev, (X *)dx_dev, dw_dev));
+      });
+    });
+  });
+}
+
+MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t dout_type, const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev,
+                                                const float *w_dev, uint32_t T, uint32_t n_used, uint32_t n_embd, void *dy_dev, float *dw_dev, void *stream) {
+  return ops_call([&] {
+    need(row_type_bytes(dout_type) != 0, "dout_type must be MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need(row_type_bytes(y_type) != 0, "y_type must be MOE_TYPE_F32, MOE_TYPE_F16 or MOE_TYPE_BF16");
+    need_step(T, R, n_used, n_embd);
+    need(dy_dev || dw_dev, "dy or dw is required");
+    need(!dw_dev || y_dev || R == 0, "y is required for dw");
+    need(!dy_dev || w_dev, "w is required for dy");
+    if (T == 0) return;
+    need_device({{dout_dev, "dout", 16}, {y_dev, "y", 16, true}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {dy_dev, "dy", 16, true}, {dw_dev, "dw", 4, true}});
+    with_step_rows(T, n_embd, [&](StepRows map, dim3 grid) {
+      with_type(dout_type, [&](auto *g) {
+        using G = std::remove_pointer_t<decltype(g)>;
+        with_type(y_type, [&](auto *of) {
+          using Y = std::remove_pointer_t<decltype(of)>;
+          CUDA_OK(launch_kernel(true, k_combine_rows_grad<G, Y>, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const G *)dout_dev, (const Y *)y_dev, map, R, inv_dev,
+                                w_dev, n_used, (Y *)dy_dev, dw_dev));
+        });
+      });
+    });
+  });
+}
+
+}  // extern "C"

@@ -63,4 +63,19 @@ CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, 
   return m;
 }
 
+CUtensorMap make_bytes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows) {
+  CUtensorMap m{};
+  const cuuint64_t part = (cuuint64_t)row_bytes * rows;
+  const cuuint64_t dims[4] = {row_bytes, parts, rows, matrices};
+  // A stride that nothing steps by is a row's: the true one may pass what a map holds.
+  const cuuint64_t strides[3] = {parts > 1 ? part : row_bytes, row_bytes, matrices > 1 ? part * parts : row_bytes};
+  const cuuint32_t box[4] = {128, parts, box_rows, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  const CUresult r = tensor_map_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, box, elem,
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw CudaFailure(cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed with driver error " + std::to_string((int)r));
+  return m;
+}
+
 }  // namespace moe

@@ -26,4 +26,9 @@ CUtensorMap make_quants_map(const void *base, uint32_t row_bytes, uint32_t rows,
 // swizzle. What lies past a row's end or past a part's rows reads as zero.
 CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows);
 
+// A map over matrices of bytes, [matrices][parts][rows][row_bytes] one after another (base 16-byte aligned, row_bytes a multiple of 16), whose
+// copies bring 128 bytes of box_rows rows of one matrix, of every part's row r before row r + 1's, with the 128-byte swizzle. What lies past a row's
+// end or past a part's rows reads as zero.
+CUtensorMap make_bytes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows);
+
 }  // namespace moe

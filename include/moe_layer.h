@@ -318,6 +318,11 @@ MOE_API const char *moe_route_rows_static_error(void);
  *   moe_route_logits_device (ids, w, offsets, inv) -> moe_mx4_quantize_rows_device (rows into expert order by inv) ->
  *   moe_mx4_gate_up_device -> moe_mx4_product_device -> moe_combine_rows_device.
  *
+ * or, with experts in 8-bit integers, moe_i8_quantize_rows_device -> moe_i8_gate_up_device -> moe_i8_quantize_rows_device (its h) ->
+ * moe_i8_product_device, or, with experts of the caller's own, moe_sort_rows_device -> the caller's products. A block that trains goes back by
+ * moe_combine_rows_grad_device (results, weights) -> the caller's products' gradients -> moe_sort_rows_grad_device (rows) and
+ * moe_route_logits_grad_device (logits). The products over MX and 8-bit rows have no gradient.
+ *
  * They keep nothing between calls (but for what moe_ops_status tells) and allocate nothing: every buffer is the caller's, a DEVICE pointer of the current
  * device (a host pointer or another device's is refused), and every call queues on stream (a cudaStream_t; null: the
  * default stream) without waiting, so a call can be captured into a graph. The first call of each on a device sets
@@ -405,6 +410,69 @@ MOE_API moe_status moe_mx4_gate_up_device(const moe_mx4_weights *w, const void *
  * n_used 1 .. 16. out_dev may be residual_dev. */
 MOE_API moe_status moe_combine_rows_device(const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev, const float *w_dev, uint32_t T,
                                            uint32_t n_used, uint32_t n_embd, const float *residual_dev, float *out_dev, void *stream);
+
+/* Rows to expert order as they are: xs[inv[t][k]] = x[t], or with w_dev w[t][k] * x[t], worked out in f32. x_dev T rows of n_embd values (type MOE_TYPE_F32, F16 or
+ * BF16), stride values apart (0: n_embd); xs_dev [R][n_embd] of the same type; inv_dev [T][n_used], w_dev [T][n_used] f32 or null. An inv outside 0 .. R - 1
+ * is skipped; a row no entry names is left as it was, a row that two name gets either's, or a mixture. n_used 1 .. 16, n_embd a multiple of 8; rows 16-byte
+ * aligned.
+ * grad: dx[t] = (add[t] +) sum over k, in rank order, of (w[t][k] *) dxs[inv[t][k]], summed in f32 and rounded once, and dw[t][k] = the sum over columns of
+ * x[t] * dxs[inv[t][k]] in f32, 0 for an inv outside 0 .. R - 1. dxs_dev [R][n_embd], x_dev (stride values apart; read for dw alone), add_dev (or null) and dx_dev
+ * [T][n_embd] of type; dx_dev or dw_dev may be null: not wanted. dx_dev may be add_dev. A row of dxs that no entry names is not read. The same call gives the
+ * same bits every time. */
+MOE_API moe_status moe_sort_rows_device(const void *x_dev, uint32_t type, uint64_t stride, uint32_t T, uint32_t n_used, uint32_t n_embd, const int32_t *inv_dev,
+                                        const float *w_dev, uint32_t R, void *xs_dev, void *stream);
+MOE_API moe_status moe_sort_rows_grad_device(const void *dxs_dev, uint32_t type, uint32_t R, const int32_t *inv_dev, const float *w_dev, const void *x_dev, uint64_t stride,
+                                             uint32_t T, uint32_t n_used, uint32_t n_embd, const void *add_dev, void *dx_dev, float *dw_dev, void *stream);
+
+/* The gradient of moe_combine_rows_device: dy[inv[t][k]] = w[t][k] * dout[t], worked out in f32, and dw[t][k] = the sum over columns of dout[t] * y[inv[t][k]] in f32,
+ * 0 for an inv outside 0 .. R - 1; its residual's gradient is dout itself. dout_dev [T][n_embd] of dout_type; y_dev (read for dw alone) and dy_dev [R][n_embd] of
+ * y_type; dy_dev or dw_dev may be null: not wanted. dy_dev may be y_dev, where no two entries name a row. Rows no entry names are left as they were (the lists
+ * of moe_route_logits_device name all rows before offsets[n_experts]). The same call gives the same bits every time. */
+MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t dout_type, const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev,
+                                                const float *w_dev, uint32_t T, uint32_t n_used, uint32_t n_embd, void *dy_dev, float *dw_dev, void *stream);
+
+/* The gradient of moe_route_logits_device's weights with respect to its logits, the chosen experts held fixed (a bias and groups choose but do not
+ * weigh, and have no gradient): dlogits[t][e] = the sum over k of dw[t][k] * the derivative of w[t][k] by logits[t][e]. config, logits_dev, stride, bias_dev and
+ * T are that call's, ids_dev [T][n_used] what it gave (a row's ids differ; one outside 0 .. n_experts - 1 counts for nothing, whatever its dw); groups do not
+ * matter. dlogits_dev T rows of n_experts values of logits_type, dlogits_stride values apart (0: n_experts), every one written: 0 for experts that are out and, but
+ * for a softmax without renormalisation, for those not chosen. Worked out in f32 and rounded once. */
+MOE_API moe_status moe_route_logits_grad_device(const moe_route_config *config, const void *logits_dev, uint64_t stride, const float *bias_dev, uint32_t T,
+                                                const int32_t *ids_dev, const float *dw_dev, void *dlogits_dev, uint64_t dlogits_stride, void *stream);
+
+/* 8-bit rows: K signed codes a row, codes [rows][K], and one f32 scale, scales [rows]; value k is codes[k] * scale. K is a multiple of 32, at most 65,536; codes
+ * pointers are 16-byte aligned.
+ * quantize: rows of K values (type MOE_TYPE_F32, F16 or BF16; stride values apart, 0: K; rows 16-byte aligned). A row's scale is its largest magnitude / 127,
+ * rounded to f32, its codes are 127 x / the largest magnitude to the nearest whole number, ties to even, of exact numbers: -127 .. 127. A row of zeros gets scale 0, a
+ * row with an infinity or NaN scale NaN, both codes 0. inv_dev null: row t to row t of R = T rows. Else [T][n_used], and row t goes to each row inv_dev[t][k] of the R
+ * (one outside 0 .. R - 1 is skipped); a row no entry names is left as it was, a row that two name may get a mixture of them. The experts' matrices are made the
+ * same way, a scale a row of the matrix.
+ * dequantize: code times scale, in f32, rounded to type; [R][K], 16-byte aligned. */
+MOE_API moe_status moe_i8_quantize_rows_device(const void *x_dev, uint32_t type, uint64_t stride, uint32_t T, uint32_t K, const int32_t *inv_dev, uint32_t n_used,
+                                               uint32_t R, void *codes_dev, float *scales_dev, void *stream);
+MOE_API moe_status moe_i8_dequantize_rows_device(const void *codes_dev, const float *scales_dev, uint32_t R, uint32_t K, void *out_dev, uint32_t type, void *stream);
+
+/* Matrices in 8-bit rows, on the device: n_experts (1 .. 512) of n_out rows of n_in values, one after another. n_out and n_in are multiples of 32, at
+ * most 65,536. */
+typedef struct {
+  uint32_t n_experts;
+  uint32_t n_out;
+  uint32_t n_in;
+  uint32_t reserved;       /* 0 */
+  const void *codes_dev;   /* [n_experts][n_out][n_in], -128 .. 127 */
+  const float *scales_dev; /* [n_experts][n_out] */
+} moe_i8_weights;
+
+/* Products of R 8-bit rows in expert order with their experts' matrices, as moe_mx4_product_device and moe_mx4_gate_up_device: the same offsets_dev, the same rows
+ * left as they were. The sums of codes' products are exact; a sum, rounded to f32, times the row's scale, times the matrix's row's, each rounded, is the result.
+ *   product: y_dev [R][n_out], f16 or bf16 (MOE_TYPE_F16, MOE_TYPE_BF16), 16-byte aligned.
+ *   gate_up: w's rows are n_out / 2 gate rows and then as many up rows, n_out a multiple of 64; h = g / (1 + exp(-g)) * u, with limit > 0 of min(g, limit) and of
+ *            u held to [-limit, limit], h_dev [R][n_out / 2], f16 or bf16, 16-byte aligned; within 2^-17 of itself before it is rounded.
+ * R at most 2^24. */
+MOE_API moe_status moe_i8_product_device(const moe_i8_weights *w, const void *codes_dev, const float *scales_dev, uint32_t R, const int32_t *offsets_dev, void *y_dev,
+                                         uint32_t y_type, void *stream);
+MOE_API moe_status moe_i8_gate_up_device(const moe_i8_weights *w, const void *codes_dev, const float *scales_dev, uint32_t R, const int32_t *offsets_dev,
+                                         float swiglu_limit, void *h_dev, uint32_t h_type, void *stream);
+
 /* Waits for stream, timeout_ms at most (0: 60 s). MOE_TIMEOUT when that ran out, or when a product on the current device, on any stream, has given up one
  * of its own waits (each bounded, about a second) since the calling thread last asked about this stream: products' results since then are not to be used.
  * Every thread is told for every stream that it asks about, each once; a thread that has not asked about a stream before is told of all there
