@@ -21,32 +21,45 @@
 #include "mx4.cuh"
 #include "ops_common.h"
 #include "tensor_map.h"
+#include "two.cuh"
 
 namespace moe {
 namespace {
 
 constexpr uint32_t kMaxExperts = 512;
 constexpr uint32_t kRowsM = 128;        // matrix rows a CTA takes
-constexpr uint32_t kStageK = 128;       // values of the contraction a stage holds: 128 bytes of a row
 constexpr uint32_t kTileTable = 1024;   // tiles whose expert is looked up in a table
 constexpr uint32_t kChunk = 16;         // rows an epilogue warp turns at a time
+constexpr uint32_t kItemRing = 16;
 
 // min(g, limit) and u held to +-limit. NaN passes through.
-__device__ __forceinline__ void hold(float &g, float &u, float limit) {
-  asm("min.NaN.f32 %0, %0, %2;\n\tmin.NaN.f32 %1, %1, %2;\n\tmax.NaN.f32 %1, %1, %3;" : "+f"(g), "+f"(u) : "f"(limit), "f"(-limit));
+__device__ __forceinline__ void hold(Two &g, Two &u, float limit) {
+  float a = g.lo(), b = g.hi(), c = u.lo(), d = u.hi();
+  asm("min.NaN.f32 %0, %0, %4;\n\tmin.NaN.f32 %1, %1, %4;\n\tmin.NaN.f32 %2, %2, %4;\n\tmax.NaN.f32 %2, %2, %5;\n\tmin.NaN.f32 %3, %3, %4;\n\tmax.NaN.f32 %3, %3, %5;"
+      : "+f"(a), "+f"(b), "+f"(c), "+f"(d)
+      : "f"(limit), "f"(-limit));
+  g = Two(a, b), u = Two(c, d);
 }
 // silu(g) * u in the approximate forms, for g from kFarGate on: the exponential's argument, 116 there, rounds by 2^-18. Below, where 1 / (1 + e^-g) is e^g
 // to f32 and may be too small for it, while u makes of it what the result's type holds: e^(g / 4) four times, the large factor first.
 constexpr float kFarGate = -80.0f;
-__device__ __forceinline__ float swiglu_near(float g, float u) {
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
+__device__ __forceinline__ Two swiglu_near(const Two &g, const Two &u) {
+  const Two p = g * Two(-1.4426950408889634f);
+  float e0, e1, r0, r1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(p.lo()));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(p.hi()));
+  const Two d = Two(e0, e1) + Two(1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(d.lo()));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(d.hi()));
+  return g * Two(r0, r1) * u;
 }
 __device__ __forceinline__ float swiglu_far(float g, float u) {
   const float p = expf(0.25f * g);
   return u * p * p * g * p * p;
+}
+__device__ __forceinline__ Two swiglu_any(const Two &g, const Two &u) {
+  const Two h = swiglu_near(g, u);
+  return Two(g.lo() < kFarGate ? swiglu_far(g.lo(), u.lo()) : h.lo(), g.hi() < kFarGate ? swiglu_far(g.hi(), u.hi()) : h.hi());
 }
 
 __device__ uint32_t g_gave_up;  // CTAs that gave up a wait, ever
@@ -71,16 +84,21 @@ struct I8Maps {
 // of bytes; the scales of a tile's rows, an epilogue warp its own; barriers; the experts' first rows and first tiles; the tiles' experts.
 template <bool GU, uint32_t CTAS, uint32_t NT>
 struct I8Form {
-  static constexpr uint32_t kGroups = CTAS == 2 && GU ? 4 : 2;  // of four epilogue warps
+  static constexpr uint32_t kGroups = CTAS == 2 ? 4 : 2;  // of four epilogue warps
   static constexpr uint32_t kThreads = 32 * (2 + 4 * kGroups);
-  static constexpr uint32_t kStageBytes = (kRowsM + NT / CTAS) * 128;
-  static constexpr uint32_t kStages = CTAS == 2 ? 6 : 10;
+  // A stage holds 128 values of the contraction, 128 bytes of a row, of single CTAs twice as many: half the hand-overs where a stage's MMAs are short (100 rows
+  // over 512 experts 151 us of gate_up with 128, 145 with 256; pairs 165 with 128, 171 with 256 and half the stages).
+  static constexpr uint32_t kParts = CTAS == 2 ? 1 : 2, kStageK = 128 * kParts;
+  static constexpr uint32_t kPartBytes = (kRowsM + NT / CTAS) * 128;
+  static constexpr uint32_t kStageBytes = kParts * kPartBytes;
+  static constexpr uint32_t kStages = CTAS == 2 ? 6 : 5;
   static constexpr uint32_t kRowScales = kStages * kStageBytes;
   static constexpr uint32_t kWarpScales = NT / kGroups;  // of a warp
   static constexpr uint32_t kBarriers = kRowScales + 4 * kGroups * kWarpScales * 4;
-  static constexpr uint32_t kTables = kBarriers + 256;
+  static constexpr uint32_t kTables = kBarriers + 320;
   static constexpr uint32_t kTileExperts = kTables + 2 * (kMaxExperts + 1) * 4 + 8;
-  static constexpr uint32_t kBytes = kTileExperts + 2 * kTileTable + 1024;  // and room to align the base to 1024
+  static constexpr uint32_t kTileRows = kTileExperts + 2 * kTileTable;
+  static constexpr uint32_t kBytes = kTileRows + 2 * kMaxExperts + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
   static_assert(2 * kThreads > kMaxExperts, "two experts a thread");
   static constexpr uint32_t kCols = 2 * NT;  // of tensor memory: two accumulators
@@ -97,18 +115,20 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_produc
   constexpr uint32_t S = SM::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;  // the same in every lane, and known to be
   const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0, unit = blockIdx.x / CTAS, nunits = gridDim.x / CTAS;
   uint64_t *bars = (uint64_t *)(smem + SM::kBarriers);
   // Barriers: stages full, empty; accumulators full, empty. Of a pair the first CTA's "full" of stages and "empty" of accumulators take both CTAs' arrivals.
   constexpr uint32_t kEmpty = S, kAccFull = 2 * S, kAccEmpty = kAccFull + 2, kBars = kAccEmpty + 2;
-  static_assert(8 * kBars + 8 <= 256, "the barriers' room");
+  static_assert(8 * kBars + 8 + 4 * kItemRing <= 320 && kItemRing > S, "the barriers' room; no more items are under way than stages");
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](uint32_t i) { return bar0 + 8 * i; };
   uint32_t *tmem_slot = (uint32_t *)(bars + kBars);
   volatile uint32_t *abort = tmem_slot + 1;
+  volatile uint32_t *item_rows = abort + 1;  // rows of an instruction of the items under way, from the copies' thread to the MMAs' warp
   uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *first_tile = first_row + kMaxExperts + 1;  // [E + 1] each
   uint16_t *tile_expert = (uint16_t *)(smem + SM::kTileExperts);
+  uint16_t *tile_rows = (uint16_t *)(smem + SM::kTileRows);  // an expert's tiles' rows, but for its last
   uint32_t *warp_part = (uint32_t *)smem;  // before the stages come
   uint32_t *error = (uint32_t *)abort;     // the waits' error word: the flag itself
 
@@ -152,13 +172,18 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_produc
     sum += __reduce_add_sync(0xffffffffu, lane < warp ? warp_part[lane] : 0) - t0 - t1;
     if (e <= a.E) first_row[e] = r0, first_tile[e] = sum;
     if (e < a.E) first_row[e + 1] = r1, first_tile[e + 1] = sum + t0;
+    // An expert's rows are shared out evenly among as few tiles as hold them: a short last tile would cost its matrix's bringing all the same. In steps of 32, its
+    // last tile the rest: of up to 8 tiles, whose rows are 32 (tiles - 1) more than 256 (tiles - 1) at most short of full, none is empty, and of more all are full.
+    auto even = [&](uint32_t rows, uint32_t tiles) { return CTAS == 2 && tiles ? ((rows + tiles - 1) / tiles + 31) & ~31u : NT; };
+    if (e < a.E) tile_rows[e] = (uint16_t)even(r1 - r0, t0);
+    if (e + 1 < a.E) tile_rows[e + 1] = (uint16_t)even(r2 - r1, t1);
     for (uint32_t t = sum; t < min(sum + t0 + t1, kTileTable); t++) tile_expert[t] = (uint16_t)(t < sum + t0 ? e : e + 1);
   }
   tc_fence_before();
   __syncthreads();
   if constexpr (CTAS == 2) pair_wait();  // the other CTA's barriers exist before anything arrives on them
   tc_fence_after();
-  const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + kStageK - 1) / kStageK, ntiles = first_tile[a.E];
+  const uint32_t M = a.items_per_tile, K = a.K, F = a.N / 2, KT = (K + SM::kStageK - 1) / SM::kStageK, ntiles = first_tile[a.E];
   auto expert_at = [&](uint32_t t) {  // the last expert whose first tile is at most t
     uint32_t lo = 0, hi = a.E;
     while (hi - lo > 1) {
@@ -191,16 +216,16 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_produc
   };
   auto tile_at = [&](const Item &i) {
     const uint32_t e = i.t < kTileTable ? tile_expert[i.t] : expert_at(i.t);
-    const uint32_t start = first_row[e] + (i.t - first_tile[e]) * NT;
-    return Tile{e, start, min(NT, first_row[e + 1] - start), (i.m * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
+    const uint32_t rows = tile_rows[e], start = first_row[e] + (i.t - first_tile[e]) * rows;
+    return Tile{e, start, min(rows, first_row[e + 1] - start), (i.m * CTAS + rank) * (GU ? kRowsM / 2 : kRowsM)};
   };
   // The rows an instruction takes of a tile: rounded up to 16 for every CTA.
   auto rounded = [&](uint32_t count) { return (count + 16 * CTAS - 1) & ~(16 * CTAS - 1); };
 
   if (warp == kCopyWarp) {
     if (lane == 0) {
-      uint32_t s = 0, phase = 1;  // of the stage's "empty": the first round finds it so
-      for (Item i = first; i.t < ntiles && ok; step(i)) {
+      uint32_t s = 0, phase = 1, item = 0;  // of the stage's "empty": the first round finds it so
+      for (Item i = first; i.t < ntiles && ok; step(i), item++) {
         const Tile t = tile_at(i);
         // A CTA of a pair brings its half of the instruction's rows, by one copy or two. A copy may run past the tile's rows; what it brings then goes
         // into columns nobody reads.
@@ -210,14 +235,18 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_produc
         for (uint32_t it = 0; it < KT && ok; it++) {
           ok = mbar_wait(bar(kEmpty + s), phase, abort, error);
           if (!ok) break;
-          const uint32_t at = smem_u32(smem + s * SM::kStageBytes), x0 = it * kStageK;
+          uint32_t at = smem_u32(smem + s * SM::kStageBytes), x0 = it * SM::kStageK;
+          const uint32_t parts = SM::kParts == 1 ? 1 : min(SM::kParts, (K - x0 + 127) / 128);
+          if (it == 0 && rank == 0) item_rows[item % kItemRing] = rounded(t.count);
           if constexpr (CTAS == 2)
-            mbar_arrive_expect_cluster(lead(s), bytes);
+            mbar_arrive_expect_cluster(lead(s), parts * bytes);
           else
-            mbar_arrive_expect(lead(s), bytes);
-          tma_load_bytes<CTAS>(at, &maps.w, x0, t.row0, t.expert, lead(s));
-          tma_load_bytes<CTAS>(at + kRowsM * 128, &maps.x[b0], x0, x_row, 0, lead(s));
-          if (rest) tma_load_bytes<CTAS>(at + (kRowsM + box_rows(b0)) * 128, &maps.x[b1], x0, x_row + box_rows(b0), 0, lead(s));
+            mbar_arrive_expect(lead(s), parts * bytes);
+          for (uint32_t part = 0; part < parts; part++, at += SM::kPartBytes, x0 += 128) {
+            tma_load_matrix<CTAS>(at, &maps.w, x0, GU ? 2 * t.expert : t.row0 / 32, GU ? t.row0 / 16 : t.expert, lead(s));
+            tma_load_byte_rows<CTAS>(at + kRowsM * 128, &maps.x[b0], x0, x_row, lead(s));
+            if (rest) tma_load_byte_rows<CTAS>(at + (kRowsM + box_rows(b0)) * 128, &maps.x[b1], x0, x_row + box_rows(b0), lead(s));
+          }
           if (++s == S) s = 0, phase ^= 1;
         }
       }
@@ -237,20 +266,22 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_produc
         else
           mma_commit(leader, bar(i));
       };
-      uint32_t s = 0, phase = 0, b = 0, acc_phase = 1;
-      for (Item i = first; i.t < ntiles && ok; step(i)) {
-        const Tile t = tile_at(i);
-        const uint32_t acc = tmem_base + b * NT, idesc = i8_instr_desc(rounded(t.count), CTAS * kRowsM);
+      const uint32_t stage0 = smem_u32(smem) >> 4, last = (K - 1) % SM::kStageK / 32 + 1;  // steps of the last stage
+      uint32_t s = 0, phase = 0, b = 0, acc_phase = 1, item = 0, idesc = 0;
+      for (Item i = first; i.t < ntiles && ok; step(i), item++) {
+        const uint32_t acc = tmem_base + b * NT;
         ok = mbar_wait_warp(bar(kAccEmpty + b), acc_phase, abort, error);
         for (uint32_t it = 0; it < KT && ok; it++) {
           ok = mbar_wait_warp(bar(s), phase, abort, error);
           if (!ok) break;
+          if (it == 0) idesc = i8_instr_desc(item_rows[item % kItemRing], CTAS * kRowsM);
           tc_fence_after();
-          const uint32_t stage = smem_u32(smem + s * SM::kStageBytes), rows = stage + kRowsM * 128;
-          const uint32_t steps = min(4u, (K - it * kStageK + 31) / 32);
+          const uint32_t stage = stage0 + s * (SM::kStageBytes >> 4), rows = stage + (kRowsM * 128 >> 4), steps = it == KT - 1 ? last : 4 * SM::kParts;
 #pragma unroll
-          for (uint32_t k = 0; k < 4; k++)
-            if (k < steps) mma_i8<CTAS>(leader, acc, smem_desc_sw128(stage + 32 * k), smem_desc_sw128(rows + 32 * k), idesc, (it | k) != 0);
+          for (uint32_t k = 0; k < 4 * SM::kParts; k++) {
+            const uint32_t at = k / 4 * (SM::kPartBytes >> 4) + 2 * (k % 4);
+            if (k < steps) mma_i8<CTAS>(leader, acc, stage + at, rows + at, idesc, (it | k) != 0);
+          }
           commit(kEmpty + s);
           if (++s == S) s = 0, phase ^= 1;
         }
@@ -260,99 +291,115 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_produc
       }
     }
   } else {
-    // Warp w reads tensor memory's lanes 32 (w % 4) ...; the groups take chunks of 16 rows in turn.
-    const uint32_t q = warp % 4, group = (warp - kEpilogueWarp) / 4;
-    constexpr uint32_t dc = SM::kGroups * kChunk;
-    const uint32_t c0 = group * kChunk;
+    // Warp w reads tensor memory's lanes 32 (w % 4) ...; the groups take chunks of 16 rows in turn. Of a chunk a thread has, of four lanes eight apart, the sums of
+    // four rows, two neighbours and two eight on. The four lanes are four neighbouring rows of the matrix, or gate and up of two neighbouring features, as the map
+    // laid them: a thread's results of a row lie side by side, and eight threads' too.
+    const uint32_t q = warp % 4, group = (warp - kEpilogueWarp) / 4, of_eight = lane / 4, pair = 2 * (lane % 4);
+    constexpr uint32_t dc = SM::kGroups * kChunk, kMine = GU ? 2 : 4;  // features of a thread
+    const uint32_t c0 = group * kChunk, width = GU ? F : a.N;
     float *row_scales = (float *)(smem + SM::kRowScales) + (4 * group + q) * SM::kWarpScales;
-    uint32_t b = 0, phase = 0;
-    for (Item i = first; i.t < ntiles && ok; step(i)) {
-      const Tile t = tile_at(i);
-      const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT;
-      // The scales of the warp's rows, chunk after chunk, and of the lane's matrix rows, while the products run.
-      __syncwarp();  // those of the tile before are read
+    // The scales of a tile's rows that the warp turns, chunk after chunk, and of the thread's four matrix rows: loaded while the tile before is turned.
+    constexpr uint32_t kHeld = (SM::kWarpScales + 31) / 32;
+    float held[kHeld], s[4];
+    auto bring = [&](const Tile &t) {
 #pragma unroll
-      for (uint32_t k = lane; k < SM::kWarpScales; k += 32) {
-        const uint32_t r = c0 + k / kChunk * dc + k % kChunk;
-        row_scales[k] = r < t.count ? a.xs[t.start + r] : 0.0f;
+      for (uint32_t k = 0; k < kHeld; k++) {
+        const uint32_t j = 32 * k + lane, r = c0 + j / kChunk * dc + j % kChunk;
+        held[k] = r < t.count ? a.xs[t.start + r] : 0.0f;
       }
-      const uint32_t f = GU ? t.row0 + 16 * q + lane / 2 : t.row0 + 32 * q + lane;
-      const bool in = f < (GU ? F : a.N);  // features come 32 together
-      const float *ws = a.ws + (uint64_t)t.expert * a.N + f;
-      const float s0 = in ? ws[0] : 0.0f, s1 = GU && in ? ws[F] : 0.0f;
+      const uint32_t f = t.row0 + (GU ? 16 : 32) * q;  // features come 32 together
+      const float *ws = a.ws + (uint64_t)t.expert * a.N + f + kMine * of_eight;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; i++) s[i] = f < width ? ws[GU ? i % 2 + i / 2 * F : i] : 0.0f;
+    };
+    uint32_t b = 0, phase = 0;
+    Tile t{};
+    if (first.t < ntiles) bring(t = tile_at(first));
+    for (Item i = first; i.t < ntiles && ok;) {
+      const Tile now = t;
+      const uint32_t from = tmem_base + ((32 * q) << 16) + b * NT, f = now.row0 + (GU ? 16 : 32) * q;
+      const Two w[4] = {Two(s[0]), Two(s[1]), Two(s[2]), Two(s[3])};
+      __syncwarp();  // the scales of the tile before are read
+#pragma unroll
+      for (uint32_t k = 0; k < kHeld; k++)
+        if (32 * k + lane < SM::kWarpScales) row_scales[32 * k + lane] = held[k];
       __syncwarp();
+      step(i);
+      if (i.t < ntiles) bring(t = tile_at(i));
       ok = mbar_wait_warp(bar(kAccFull + b), phase, abort, error);
       if (!ok) break;
       tc_fence_after();
       const float *sx = row_scales;
+      auto load = [&](uint32_t c, uint32_t *v) { tmem_ld_16x16(from + c, v), tmem_ld_16x16(from + (16 << 16) + c, v + 8); };
       // A chunk's sums are on their way from tensor memory while the one before is turned.
-      auto turn = [&](uint32_t c, const uint32_t *v) {
-        const uint32_t left = t.count - c;
-        if constexpr (!GU) {
-          // A lane holds one feature of 16 rows. Two lanes with neighbouring features share out two rows: the even one stores both features of the
-          // first, the odd one of the second.
-          const uint32_t odd = lane & 1, sel = odd ? 0x3276u : 0x5410u;
-          Out *p = (Out *)a.y + (uint64_t)(t.start + c + odd) * a.N + (f - odd);
+      auto turn = [&](uint32_t c, const uint32_t *v, const float *sx) {
+        const float2 a0 = *(const float2 *)(sx + pair), a1 = *(const float2 *)(sx + 8 + pair);
+        const Two x[2] = {Two(a0.x, a0.y), Two(a1.x, a1.y)};
+        // Lane j's two rows, neighbours or (half 1) those eight on: the sums, the rows' scales, the matrix's row's.
+        auto scaled = [&](uint32_t j, uint32_t half) {
+          const uint32_t at = 8 * (j / 2) + 4 * half + 2 * (j % 2);
+          return Two((float)(int32_t)v[at], (float)(int32_t)v[at + 1]) * x[half] * w[j];
+        };
+        auto both = [](float a, float b) { return pack2(a, b, (const Out *)nullptr); };
+        Two r[2][kMine];
 #pragma unroll
-          for (uint32_t j = 0; j < 16; j += 2, p += 2 * (uint64_t)a.N) {
-            const float2 s = *(const float2 *)(sx + j);
-            const uint32_t mine = pack2((float)(int32_t)v[j] * s.x * s0, (float)(int32_t)v[j + 1] * s.y * s0, (const Out *)nullptr);
-            const uint32_t theirs = __shfl_xor_sync(0xffffffffu, mine, 1);
-            if (in && j + odd < left) *(uint32_t *)p = __byte_perm(mine, theirs, sel);
-          }
-        } else {
-          // Even lanes hold gate sums of 16 rows, odd ones the same feature's up sums. They exchange: the even one takes both of the first eight rows, the
-          // odd one of the last eight; then lanes of neighbouring features share out two rows, as above.
-          const uint32_t up = lane & 1, odd = lane / 2 & 1, sel = odd ? 0x3276u : 0x5410u;
-          float h[8];
-          float g[8], u[8];
-#pragma unroll
-          for (uint32_t j = 0; j < 8; j++) {
-            const uint32_t keep = up ? v[8 + j] : v[j], got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[8 + j], 1);
-            const float s = sx[8 * up + j];
-            g[j] = (float)(int32_t)(up ? got : keep) * s * s0, u[j] = (float)(int32_t)(up ? keep : got) * s * s1;
-          }
-          if (a.limit > 0.0f)
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) hold(g[j], u[j], a.limit);
-          float low = 0.0f;
-#pragma unroll
-          for (uint32_t j = 0; j < 8; j++) low = fminf(low, g[j]);
-          if (low < kFarGate) {  // a NaN gate does not count here, and stays one
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) h[j] = g[j] < kFarGate ? swiglu_far(g[j], u[j]) : swiglu_near(g[j], u[j]);
+        for (uint32_t half = 0; half < 2; half++) {
+          if constexpr (GU) {
+            r[half][0] = scaled(0, half), r[half][1] = scaled(1, half);
+            Two u[2] = {scaled(2, half), scaled(3, half)};
+            if (a.limit > 0.0f) hold(r[half][0], u[0], a.limit), hold(r[half][1], u[1], a.limit);
+            const float low = fminf(fminf(r[half][0].lo(), r[half][0].hi()), fminf(r[half][1].lo(), r[half][1].hi()));
+            if (low < kFarGate)  // a NaN gate does not count here, and stays one
+              r[half][0] = swiglu_any(r[half][0], u[0]), r[half][1] = swiglu_any(r[half][1], u[1]);
+            else
+              r[half][0] = swiglu_near(r[half][0], u[0]), r[half][1] = swiglu_near(r[half][1], u[1]);
           } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++) h[j] = swiglu_near(g[j], u[j]);
+            for (uint32_t j = 0; j < 4; j++) r[half][j] = scaled(j, half);
           }
-          Out *p = (Out *)a.y + (uint64_t)(t.start + c + 8 * up + odd) * F + (f - odd);
-#pragma unroll
-          for (uint32_t j = 0; j < 8; j += 2, p += 2 * (uint64_t)F) {
-            const uint32_t mine = pack2(h[j], h[j + 1], (const Out *)nullptr), theirs = __shfl_xor_sync(0xffffffffu, mine, 2);
-            if (in && 8 * up + j + odd < left) *(uint32_t *)p = __byte_perm(mine, theirs, sel);
-          }
+        }
+        Out *p = (Out *)a.y + (uint64_t)(now.start + c + pair) * width + f + kMine * of_eight;
+        const uint32_t left = f < width && now.count > c + pair ? now.count - c - pair : 0;  // rows from the thread's first on
+        auto store = [&](uint32_t row, uint32_t half, bool second) {
+          if (row >= left) return;
+          auto of = [&](uint32_t j) { return second ? r[half][j].hi() : r[half][j].lo(); };
+          if constexpr (GU)
+            *(uint32_t *)(p + (uint64_t)row * width) = both(of(0), of(1));
+          else
+            *(uint2 *)(p + (uint64_t)row * width) = make_uint2(both(of(0), of(1)), both(of(2), of(3)));
+        };
+        store(0, 0, false), store(1, 0, true), store(8, 1, false), store(9, 1, true);
+      };
+      // The accumulator is given back once the warp's last sums are here.
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CTAS == 2)
+            mbar_arrive_cluster(lead(kAccEmpty + b));
+          else
+            mbar_arrive(lead(kAccEmpty + b));
         }
       };
       uint32_t v[16], u[16];
-      if (c0 < t.count) tmem_ld16(from + c0, v);
-      for (uint32_t c = c0; c < t.count; c += 2 * dc, sx += 2 * kChunk) {
+      if (c0 < now.count)
+        load(c0, v);
+      else
+        release();
+      for (uint32_t c = c0; c < now.count; c += 2 * dc, sx += 2 * kChunk) {
         tmem_ld_wait16(v);
-        if (c + dc < t.count) tmem_ld16(from + c + dc, u);
-        turn(c, v);
-        if (c + dc >= t.count) break;
-        tmem_ld_wait16(u);
-        if (c + 2 * dc < t.count) tmem_ld16(from + c + 2 * dc, v);
-        sx += kChunk;
-        turn(c + dc, u);
-        sx -= kChunk;
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CTAS == 2)
-          mbar_arrive_cluster(lead(kAccEmpty + b));
+        if (c + dc < now.count)
+          load(c + dc, u);
         else
-          mbar_arrive(lead(kAccEmpty + b));
+          release();
+        turn(c, v, sx);
+        if (c + dc >= now.count) break;
+        tmem_ld_wait16(u);
+        if (c + 2 * dc < now.count)
+          load(c + 2 * dc, v);
+        else
+          release();
+        turn(c + dc, u, sx + kChunk);
       }
       phase ^= b, b ^= 1;
     }
@@ -393,9 +440,9 @@ void launch_product(const I8Args &args, const void *wc, const void *xc, cudaStre
   a.items_per_tile = (all + rows - 1) / rows;
   const uint64_t most = ((uint64_t)a.R / NT + std::min(a.E, a.R)) * a.items_per_tile;  // items there can be
   I8Maps maps;
-  maps.w = make_bytes_map(wc, a.K, all, GU ? 2 : 1, a.E, GU ? kRowsM / 2 : kRowsM);
+  maps.w = GU ? make_gate_up_map(wc, a.K, all, a.E, kRowsM) : make_matrix_map(wc, a.K, all, a.E, kRowsM);
   for (uint32_t i = 0; i < kBoxes; i++)
-    if (box_rows(i) <= NT / CTAS) maps.x[i] = make_bytes_map(xc, a.K, a.R, 1, 1, box_rows(i));
+    if (box_rows(i) <= NT / CTAS) maps.x[i] = make_byte_rows_map(xc, a.K, a.R, box_rows(i));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute at[2]{};
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, at[0].val.programmaticStreamSerializationAllowed = 1;

@@ -5,21 +5,44 @@
 
 #include "mx4.cuh"
 #include "ops_common.h"
+#include "two.cuh"
 
 namespace moe {
 namespace {
 
 constexpr uint32_t kRowsMaxUsed = 16;
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kHeldOctets = 8;  // groups of eight values a thread holds
+constexpr uint32_t kHeldOctets = 8;             // groups of eight values a thread holds
+constexpr uint32_t kManyOctets = 4 * 148 * 4 * 256;  // a call of so many: eight a thread leave every SM some four CTAs twice over
 
 // How rows are dealt to a CTA of 256 threads: 2^log2 neighbouring threads a row; of its octets, groups of eight values, thread i takes i,
-// i + 2^log2 and so on, V at most.
+// i + 2^log2 and so on.
 struct RowsOfThreads {
   uint32_t T, log2, octets;
   __device__ uint32_t first() const { return threadIdx.x & ((1u << log2) - 1); }
   __device__ uint32_t octet(uint32_t v) const { return first() + (v << log2); }
 };
+
+// The largest magnitude's bits among eight values as f32's, an infinity's or NaN's if there is one: magnitudes order as their bits do, and 16-bit
+// types' are compared two at a time.
+__device__ __forceinline__ uint32_t largest_bits(const uint4 (&raw)[2], const float *) {
+  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) m = max(m, w[i] & 0x7FFFFFFFu);
+  return m;
+}
+__device__ __forceinline__ uint32_t largest_bits(const uint4 (&raw)[1], const __nv_bfloat16 *) {
+  constexpr uint32_t kBits = 0x7FFF7FFFu;
+  const uint32_t m = __vmaxu2(__vmaxu2(raw[0].x & kBits, raw[0].y & kBits), __vmaxu2(raw[0].z & kBits, raw[0].w & kBits));
+  return max(m & 0x7FFF0000u, m << 16);
+}
+__device__ __forceinline__ uint32_t largest_bits(const uint4 (&raw)[1], const __half *) {
+  constexpr uint32_t kBits = 0x7FFF7FFFu;
+  const uint32_t m = __vmaxu2(__vmaxu2(raw[0].x & kBits, raw[0].y & kBits), __vmaxu2(raw[0].z & kBits, raw[0].w & kBits));
+  const float2 f = __half22float2(*(const __half2 *)&m);
+  return max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu);
+}
 
 template <class X>
 struct Octet {
@@ -33,60 +56,77 @@ struct Octet {
     for (uint32_t i = 0; i < sizeof(X) / 2; i++) raw[i] = make_uint4(0, 0, 0, 0);
   }
   __device__ void values(float *v) const { load8((const X *)raw, v); }
-  // The largest magnitude's bits as f32's: magnitudes order as their bits do, an infinity's or NaN's above all numbers'.
-  __device__ uint32_t largest() const {
-    float v[8];
-    values(v);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    return m;
-  }
+  __device__ uint32_t largest() const { return largest_bits(raw, (const X *)nullptr); }
 };
 
-// A row's scale and what its values are multiplied by. bad: it holds an infinity or NaN.
+// A row's scale and what its values are multiplied by: 127 / top is inverse + rest to twice f32's digits. bad: it holds an infinity or NaN. lift: a power of two that
+// takes the row away from the ends of f32's range, where 127 / top, products with 127 or what their roundings leave over would pass it; top, inverse and
+// rest are the lifted row's.
 struct RowScale {
-  float top, scale, inverse;
-  bool bad, small;
+  float top, scale, inverse, rest, lift;
+  bool bad;
   __device__ explicit RowScale(uint32_t bits) {
     bad = bits >= 0x7F800000u;
     top = __uint_as_float(bits);
     scale = bad ? __uint_as_float(0x7FFFFFFFu) : __fdiv_rn(top, 127.0f);
-    small = top < 1e-35f;  // 127 / top would pass f32's range, or x times it be less exact than codes take
+    lift = top < 1e-30f ? 0x1p64f : top > 1e30f ? 0x1p-64f : 1.0f;
+    top *= lift;
     inverse = bad || top == 0.0f ? 0.0f : __fdiv_rn(127.0f, top);
+    rest = fmaf(-inverse, top, 127.0f) * (inverse * (1.0f / 127.0f));
   }
 };
 
-// Eight codes: rint(127 x / top) of exact numbers. x * inverse is within 127 * 2^-23 < 2^-16 of 127 x / top; where it lies nearer than 2^-15 to a border between
-// two codes the quotient is taken in 64 bits. There 127 x is exact, and the quotient's rounding makes no border of what is none: a quotient of numbers of 31 and
-// 24 bits that is not n + 1/2 is 2^-33 of itself away from it at least.
-__device__ __forceinline__ uint2 codes8(const float (&x)[8], const RowScale &s) {
+// Eight codes: rint(127 x / top) of exact numbers, ties to even.
+//
+// Values of 16-bit types: the quotient is worked out to f32's nearest number y. A border between two codes, n + 1/2, is such a number; with x and top whole numbers
+// below 2^11 times powers of two, a quotient in [2^e, 2^(e + 1)) that is not a border lies 2^(e - 20) from one at least, and y 2^(e - 23) from the quotient at most:
+// y is a border where the quotient is, and on its side of it where it is not. (In rows whose largest has few bits one value in some 400 lies on a border.)
+//
+// f32 values: x * inverse, rounded once, is within 127 * 2^-23 < 2^-16 of 127 x / top. Where one lies nearer than 2^-15 to a border the sign of 127 x - border * top
+// decides, from the two products and what their roundings left over: the products are near one another, so their difference is exact, and what was left
+// over has ten bits at most. What a row lifted down loses of its smallest values is far below half a code.
+template <class X>
+__device__ __forceinline__ uint2 codes8(float (&x)[8], const RowScale &s) {
   if (s.bad) return make_uint2(0, 0);
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: sums with it are whole numbers, in the low bits
-  float q[8], far = 0.0f;
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: sums with it are whole numbers, ties to even, in the low bits
+  if (s.lift != 1.0f)
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float y = x[i] * s.inverse;
-    q[i] = y + kMagic;
-    far = fmaxf(far, fabsf(y - (q[i] - kMagic)));
-  }
-  if ((s.small && s.top != 0.0f) || far > 0.5f - 0x1p-15f) {
-#pragma unroll 1
-    for (int i = 0; i < 8; i++) {
-      // Held in registers: no index that the compiler does not know.
-      float v = x[0];
+    for (int i = 0; i < 8; i++) x[i] *= s.lift;
+  const Two inverse(s.inverse), magic(kMagic);
+  Two q[4];
+  if constexpr (sizeof(X) == 2) {
+    const Two rest(s.rest);
 #pragma unroll
-      for (int j = 1; j < 8; j++) v = i == j ? x[j] : v;
-      const float c = (float)rint(127.0 * (double)v / (double)s.top) + kMagic;
+    for (int i = 0; i < 4; i++) {
+      const Two v(x[2 * i], x[2 * i + 1]);
+      q[i] = fma(v, inverse, v * rest) + magic;
+    }
+  } else {
+    const Two minus(-1.0f);
+    float most = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; j++) q[j] = i == j ? c : q[j];
+    for (int i = 0; i < 4; i++) {
+      const Two v(x[2 * i], x[2 * i + 1]);
+      q[i] = fma(v, inverse, magic);
+      const Two off = fma(v, inverse, fma(q[i], minus, magic));
+      most = fmaxf(most, fmaxf(fabsf(off.lo()), fabsf(off.hi())));
+    }
+    if (most > 0.5f - 0x1p-15f) {
+      const Two n(127.0f), top(s.top);
+      auto half = [](float v) { return copysignf(0.5f, v); };
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const Two v(x[2 * i], x[2 * i + 1]), code = q[i] + Two(-kMagic), off = fma(v, inverse, code * minus);
+        const Two border = code + Two(half(off.lo()), half(off.hi())), a = n * v, b = (border * top) * minus;
+        const Two over = (a + b) + fma(fma(border, top, b), minus, fma(n, v, a * minus));
+        q[i] = (border + Two(over.lo() == 0.0f ? 0.0f : half(over.lo()), over.hi() == 0.0f ? 0.0f : half(over.hi()))) + magic;
+      }
     }
   }
-  uint32_t b[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) b[i] = __float_as_uint(q[i]);
-  auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410); };
-  return make_uint2(four(b[0], b[1], b[2], b[3]), four(b[4], b[5], b[6], b[7]));
+  auto four = [](const Two &a, const Two &b) {
+    return __byte_perm(__byte_perm(__float_as_uint(a.lo()), __float_as_uint(a.hi()), 0x0040), __byte_perm(__float_as_uint(b.lo()), __float_as_uint(b.hi()), 0x0040), 0x5410);
+  };
+  return make_uint2(four(q[0], q[1]), four(q[2], q[3]));
 }
 
 // The largest of a row's 2^log2 threads' values. The CTA's threads come here together.
@@ -103,7 +143,7 @@ __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t log2, uint32_t 
 
 // V octets a thread of each of U rows, whose loads are on their way together.
 template <class X, uint32_t V, uint32_t U>
-__global__ void __launch_bounds__(kThreads) k_i8_quantize(const X *x, uint64_t stride, const RowsOfThreads map, uint32_t K, const int32_t *inv, uint32_t n_used, uint32_t R,
+__global__ void __launch_bounds__(kThreads, sizeof(X) == 2 ? 4 : 2) k_i8_quantize(const X *x, uint64_t stride, const RowsOfThreads map, uint32_t K, const int32_t *inv, uint32_t n_used, uint32_t R,
                                                           uint8_t *codes, float *scales) {
   __shared__ uint32_t part[U][kThreads / 32];
   dependents_may_launch(), wait_for_predecessors();
@@ -133,20 +173,26 @@ __global__ void __launch_bounds__(kThreads) k_i8_quantize(const X *x, uint64_t s
     const uint64_t t = t0 + u * rows;
     if (t >= map.T) break;
     const RowScale s(top[u]);
-    uint2 c[V];
+    const int32_t *to = inv + t * n_used;
 #pragma unroll
     for (uint32_t v = 0; v < V; v++) {
+      const uint32_t k = 8 * map.octet(v);
       float f[8];
       o[u][v].values(f);
-      c[v] = codes8(f, s);
+      const uint2 c = codes8<X>(f, s);
+      if (k >= K) break;
+      if (!inv)
+        *(uint2 *)(codes + t * K + k) = c;
+      else
+        for (uint32_t j = 0; j < n_used; j++)
+          if ((uint32_t)to[j] < R) *(uint2 *)(codes + (uint64_t)(uint32_t)to[j] * K + k) = c;
     }
-    for (uint32_t j = 0; j < (inv ? n_used : 1); j++) {
-      const uint64_t r = inv ? (uint64_t)(uint32_t)inv[t * n_used + j] : t;
-      if (r >= R) continue;
-#pragma unroll
-      for (uint32_t v = 0; v < V; v++)
-        if (map.octet(v) < map.octets) *(uint2 *)(codes + r * K + 8 * map.octet(v)) = c[v];
-      if (map.first() == 0) scales[r] = s.scale;
+    if (map.first() == 0) {
+      if (!inv)
+        scales[t] = s.scale;
+      else
+        for (uint32_t j = 0; j < n_used; j++)
+          if ((uint32_t)to[j] < R) scales[(uint32_t)to[j]] = s.scale;
     }
   }
 }
@@ -178,7 +224,7 @@ __global__ void __launch_bounds__(kThreads) k_i8_quantize_long(const X *x, uint6
     o.load(row + k);
     float f[8];
     o.values(f);
-    const uint2 c = codes8(f, s);
+    const uint2 c = codes8<X>(f, s);
     for (uint32_t j = 0; j < (inv ? n_used : 1); j++) {
       const uint64_t r = inv ? (uint64_t)(uint32_t)inv[t * n_used + j] : t;
       if (r < R) *(uint2 *)(codes + r * K + k) = c;
@@ -190,18 +236,28 @@ __global__ void __launch_bounds__(kThreads) k_i8_quantize_long(const X *x, uint6
   }
 }
 
-template <class Y>
+// U rows' octets a thread, whose loads are on their way together.
+template <class Y, uint32_t U>
 __global__ void __launch_bounds__(kThreads) k_i8_dequantize(const uint8_t *codes, const float *scales, const RowsOfThreads map, uint32_t K, Y *out) {
   dependents_may_launch(), wait_for_predecessors();
-  const uint64_t r = (uint64_t)blockIdx.x * (kThreads >> map.log2) + (threadIdx.x >> map.log2);
-  if (r >= map.T) return;
-  const float s = scales[r];
-  for (uint32_t o = map.first(); o < map.octets; o += 1u << map.log2) {
-    const uint2 c = *(const uint2 *)(codes + r * K + 8 * o);
+  const uint32_t rows = kThreads >> map.log2, k = 8 * ((blockIdx.y << map.log2) + map.first());
+  const uint64_t r0 = (uint64_t)blockIdx.x * U * rows + (threadIdx.x >> map.log2);
+  if (k >= K) return;
+  uint2 c[U];
+  float s[U];
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) {
+    const uint64_t r = r0 + u * rows;
+    if (r < map.T) c[u] = *(const uint2 *)(codes + r * K + k), s[u] = scales[r];
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < U; u++) {
+    const uint64_t r = r0 + u * rows;
+    if (r >= map.T) break;
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (float)(int8_t)((i < 4 ? c.x : c.y) >> (8 * (i % 4))) * s;
-    store8(out + r * K + 8 * o, v);
+    for (int i = 0; i < 8; i++) v[i] = (float)(int8_t)((i < 4 ? c[u].x : c[u].y) >> (8 * (i % 4))) * s[u];
+    store8(out + r * K + k, v);
   }
 }
 
@@ -225,22 +281,41 @@ void quantize(const void *x, uint64_t stride, uint32_t T, uint32_t K, const int3
                           n_used, R, (uint8_t *)codes, (float *)scales));
   };
   using std::integral_constant;
-  const uint32_t log2 = std::min(8u, ceil_log2(octets)), held = (octets + (1u << log2) - 1) >> log2;
+  // Long calls: up to eight octets a thread, of one row or more, by threads of one warp where a row has 2,048 values at most. Else an octet a thread where a CTA
+  // has the threads.
+  const bool many = (uint64_t)T * octets >= kManyOctets;
+  const uint32_t log2 = many ? std::max(2u, ceil_log2((octets + kHeldOctets - 1) / kHeldOctets)) : std::min(8u, ceil_log2(octets));
+  const uint32_t held = (octets + (1u << log2) - 1) >> log2;
+  auto with = [&](auto v) {
+    constexpr uint32_t V = decltype(v)::value;
+    if (many)
+      go(v, integral_constant<uint32_t, kHeldOctets / V>{}, log2);
+    else
+      go(v, integral_constant<uint32_t, 1>{}, log2);
+  };
   if (held <= 1)
-    go(integral_constant<uint32_t, 1>{}, integral_constant<uint32_t, 1>{}, log2);
+    with(integral_constant<uint32_t, 1>{});
   else if (held <= 2)
-    go(integral_constant<uint32_t, 2>{}, integral_constant<uint32_t, 1>{}, log2);
+    with(integral_constant<uint32_t, 2>{});
   else if (held <= 4)
-    go(integral_constant<uint32_t, 4>{}, integral_constant<uint32_t, 1>{}, log2);
+    with(integral_constant<uint32_t, 4>{});
   else
-    go(integral_constant<uint32_t, 8>{}, integral_constant<uint32_t, 1>{}, log2);
+    with(integral_constant<uint32_t, 8>{});
 }
 
 template <class Y>
 void dequantize(const void *codes, const void *scales, uint32_t R, uint32_t K, void *out, cudaStream_t st) {
-  const uint32_t octets = K / 8, log2 = std::min(8u, ceil_log2(octets)), rows = kThreads >> log2;
-  CUDA_OK(launch_kernel(true, k_i8_dequantize<Y>, dim3((R + rows - 1) / rows), dim3(kThreads), 0, st, (const uint8_t *)codes, (const float *)scales,
-                        RowsOfThreads{R, log2, octets}, K, (Y *)out));
+  const uint32_t octets = K / 8, log2 = std::min(8u, ceil_log2(octets)), pieces = (octets + (1u << log2) - 1) >> log2;
+  auto go = [&](auto u) {
+    constexpr uint32_t U = decltype(u)::value;
+    const uint32_t rows = U * (kThreads >> log2);
+    CUDA_OK(launch_kernel(true, k_i8_dequantize<Y, U>, dim3((R + rows - 1) / rows, pieces), dim3(kThreads), 0, st, (const uint8_t *)codes, (const float *)scales,
+                          RowsOfThreads{R, log2, octets}, K, (Y *)out));
+  };
+  if ((uint64_t)R * octets >= kManyOctets)
+    go(std::integral_constant<uint32_t, 4>{});
+  else
+    go(std::integral_constant<uint32_t, 1>{});
 }
 
 void need_i8_row(uint32_t K) { need(K >= 32 && K % 32 == 0 && K <= kMxMaxValues, "a row's values must be a multiple of 32, 32 .. 65536"); }

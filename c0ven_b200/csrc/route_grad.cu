@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "ops_common.h"
@@ -52,77 +53,144 @@ __device__ __forceinline__ float warp_max(float v) {
 // e^(l - top), the largest's own 1 even where it is infinite; 0 for an expert that is out.
 __device__ __forceinline__ float part_of(float l, float top) { return l == -INFINITY ? 0.0f : l == top ? 1.0f : expf(l - top); }
 
-// V: columns a lane has at most.
-template <class L, int V>
+// Four neighbouring values of a row as f32, and back. The address is aligned to them.
+__device__ __forceinline__ void load4(const float *p, float *v) { *(float4 *)v = *(const float4 *)p; }
+__device__ __forceinline__ void load4(const __half *p, float *v) {
+  const uint2 u = *(const uint2 *)p;
+  *(float2 *)v = __half22float2(*(const __half2 *)&u.x), *(float2 *)(v + 2) = __half22float2(*(const __half2 *)&u.y);
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16 *p, float *v) {
+  const uint2 u = *(const uint2 *)p;
+  v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xFFFF0000u), v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xFFFF0000u);
+}
+__device__ __forceinline__ void store4(float *p, const float *v) { *(float4 *)p = *(const float4 *)v; }
+__device__ __forceinline__ void store4(__half *p, const float *v) {
+  const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+  *(uint2 *)p = make_uint2(*(const uint32_t *)&a, *(const uint32_t *)&b);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *v) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *(uint2 *)p = make_uint2(*(const uint32_t *)&a, *(const uint32_t *)&b);
+}
+
+// V: columns a lane has at most. W: neighbouring ones it has together, four where the rows' addresses allow, else one. DENSE: softmax weights as they are.
+template <class L, int V, int W, bool DENSE>
 __global__ void __launch_bounds__(32 * kWarps) k_route_grad(const RouteGradArgs a) {
-  __shared__ float rows[kWarps][32 * V];
+  __shared__ __align__(16) float rows[kWarps][32 * V];
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint64_t t = (uint64_t)blockIdx.x * kWarps + warp;
-  if (t >= a.T) return;
   float *row = rows[warp];
+  auto column = [&](int v) { return v / W * 32 * W + lane * W + v % W; };
+#pragma unroll
+  for (int v = 0; v < V; v++) row[column(v)] = 0.0f;
+  // An assignment a lane, and for softmax weights as they are the row's logits: of the warp's next row while this one is worked on.
   uint32_t id = 0xFFFFFFFFu;
-  float d = 0.0f, l = -INFINITY;
-  if (lane < a.k) {
-    id = (uint32_t)a.ids[t * a.k + lane];
-    if (id < a.E) d = a.dw[t * a.k + lane], l = logit_of<L>(a, t, id);
-    if (l == -INFINITY) d = 0.0f;
-  }
-  const bool dense = !a.sigmoid && !a.renorm;
-  float z[V];
-  if (dense) {
+  float d = 0.0f, l = -INFINITY, z[DENSE ? V : 1];
+  auto bring = [&](uint64_t t) {
+    id = 0xFFFFFFFFu, d = 0.0f, l = -INFINITY;
+    if (lane < a.k) {
+      id = (uint32_t)a.ids[t * a.k + lane];
+      if (id < a.E) d = a.dw[t * a.k + lane];
+      if (!DENSE && id < a.E) l = logit_of<L>(a, t, id);
+    }
+    if constexpr (DENSE) {
+      const L *p = (const L *)a.logits + t * a.stride;
 #pragma unroll
-    for (int v = 0; v < V; v++) z[v] = lane + 32 * v < a.E ? logit_of<L>(a, t, lane + 32 * v) : -INFINITY;
-  }
+      for (int v = 0; v < V; v += W) {
+        if constexpr (W == 4) {
+          if (column(v) < a.E)
+            load4(p + column(v), z + v);
+          else
+            z[v] = z[v + 1] = z[v + 2] = z[v + 3] = -INFINITY;
+        } else {
+          z[v] = column(v) < a.E ? (float)p[column(v)] : -INFINITY;
+        }
+      }
+    }
+  };
+  const uint64_t step = (uint64_t)gridDim.x * kWarps;
+  uint64_t t = (uint64_t)blockIdx.x * kWarps + warp;
+  if (t < a.T) bring(t);
+  for (; t < a.T; t += step) {
+    const uint32_t e = id;
+    float y[V], g = d;
+    if constexpr (DENSE) {
+      float top = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < V; v++) row[lane + 32 * v] = 0.0f;
-  __syncwarp();
-  if (dense) {
-    float top = z[0];
+      for (int v = 0; v < V; v++) {
+        y[v] = z[v] > -INFINITY && (!a.bias || (column(v) < a.E && a.bias[column(v)] > -INFINITY)) ? z[v] : -INFINITY;
+        top = fmaxf(top, y[v]);
+      }
+      if (e < a.E) row[e] = g;
+      if (t + step < a.T) bring(t + step);
+      top = warp_max(top);
+      float total = 0.0f;
 #pragma unroll
-    for (int v = 1; v < V; v++) top = fmaxf(top, z[v]);
-    top = warp_max(top);
-    float total = 0.0f;
+      for (int v = 0; v < V; v++) y[v] = part_of(y[v], top), total += y[v];
+      total = warp_sum(total);
+      __syncwarp();
+      float mean = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; v++) z[v] = part_of(z[v], top), total += z[v];
-    total = warp_sum(total);
-    const float mean = total > 0.0f ? warp_sum(part_of(l, top) * d) / total : 0.0f, f = total > 0.0f ? a.scale / total : 0.0f;
-    if (id < a.E) row[id] = d;
-    __syncwarp();
+      for (int v = 0; v < V; v++) {
+        mean += y[v] > 0.0f ? y[v] * row[column(v)] : 0.0f;
+      }
+      mean = warp_sum(mean);
+      const float f = total > 0.0f ? a.scale / total : 0.0f;
+      mean = total > 0.0f ? mean / total : 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; v++) z[v] = f * z[v] * (row[lane + 32 * v] - mean);
-  } else {
-    const float top = warp_max(l);
-    float p = 0.0f, rest = 1.0f;  // rest: 1 - s
-    if (a.sigmoid) {
-      rest = 1.0f / (1.0f + expf(l));
-      // Relative to the largest where all scores are small: from e^-60 on they are e^l to f32.
-      p = l == -INFINITY ? 0.0f : a.renorm && top < -60.0f ? part_of(l, top) : 1.0f / (1.0f + expf(-l));
+      for (int v = 0; v < V; v++) y[v] = y[v] > 0.0f ? f * y[v] * (row[column(v)] - mean) : 0.0f;
     } else {
-      p = part_of(l, top);
+      const float lc = l;
+      if (lc == -INFINITY) g = 0.0f;
+      if (t + step < a.T) bring(t + step);
+      const float top = warp_max(lc);
+      float p = 0.0f, rest = 1.0f;  // rest: 1 - s
+      if (a.sigmoid) {
+        rest = 1.0f / (1.0f + expf(lc));
+        // Relative to the largest where all scores are small: from e^-60 on they are e^l to f32.
+        p = lc == -INFINITY ? 0.0f : a.renorm && top < -60.0f ? part_of(lc, top) : 1.0f / (1.0f + expf(-lc));
+      } else {
+        p = part_of(lc, top);
+      }
+      if (a.renorm) {
+        const float total = warp_sum(p);
+        p = total > 0.0f ? p / total : 0.0f;
+        g -= warp_sum(p * g);
+      }
+      if (e < a.E) row[e] = a.scale * p * rest * g;
+      __syncwarp();
+#pragma unroll
+      for (int v = 0; v < V; v++) y[v] = row[column(v)];
     }
-    if (a.renorm) {
-      const float total = warp_sum(p);
-      p = total > 0.0f ? p / total : 0.0f;
-      const float mean = warp_sum(p * d);
-      if (id < a.E) row[id] = a.scale * p * rest * (d - mean);
-    } else if (id < a.E) {
-      row[id] = a.scale * p * rest * d;
+    L *out = (L *)a.out + t * a.out_stride;
+#pragma unroll
+    for (int v = 0; v < V; v += W) {
+      if constexpr (W == 4) {
+        if (column(v) < a.E) store4(out + column(v), y + v);
+      } else {
+        if (column(v) < a.E) out[column(v)] = (L)y[v];
+      }
     }
     __syncwarp();
-#pragma unroll
-    for (int v = 0; v < V; v++) z[v] = row[lane + 32 * v];
+    if (e < a.E) row[e] = 0.0f;
+    __syncwarp();
   }
-#pragma unroll
-  for (int v = 0; v < V; v++)
-    if (lane + 32 * v < a.E) ((L *)a.out)[t * a.out_stride + lane + 32 * v] = (L)z[v];
+}
+
+template <class L, int W, bool DENSE>
+void launch_grad(const RouteGradArgs &a, cudaStream_t st) {
+  // Rows by warps that stay: as many CTAs as are resident at once for long steps.
+  const dim3 grid(std::min((a.T + kWarps - 1) / kWarps, 148u * 6)), block(32 * kWarps);
+  const auto kernel = a.E <= 128 ? k_route_grad<L, 4, W, DENSE> : a.E <= 256 ? k_route_grad<L, 8, W, DENSE> : k_route_grad<L, 16, W, DENSE>;
+  CUDA_OK(launch_kernel(true, kernel, grid, block, 0, st, a));
 }
 
 template <class L>
 void launch_grad(const RouteGradArgs &a, cudaStream_t st) {
-  const dim3 grid((a.T + kWarps - 1) / kWarps), block(32 * kWarps);
-  const auto kernel = a.E <= 32 ? k_route_grad<L, 1> : a.E <= 64 ? k_route_grad<L, 2> : a.E <= 128 ? k_route_grad<L, 4> : a.E <= 256 ? k_route_grad<L, 8> : k_route_grad<L, 16>;
-  CUDA_OK(launch_kernel(true, kernel, grid, block, 0, st, a));
+  const uint64_t at = (uint64_t)a.logits | (uint64_t)a.out | a.stride * sizeof(L) | a.out_stride * sizeof(L);
+  const bool dense = !a.sigmoid && !a.renorm, four = a.E % 4 == 0 && at % (4 * sizeof(L)) == 0;
+  const auto call = dense ? (four ? launch_grad<L, 4, true> : launch_grad<L, 1, true>) : (four ? launch_grad<L, 4, false> : launch_grad<L, 1, false>);
+  call(a, st);
 }
 
 }  // namespace

@@ -52,26 +52,52 @@ __global__ void __launch_bounds__(kThreads) k_sort_rows(const X *x, uint64_t str
   }
 }
 
-// The sums of 16 numbers a thread over a row's 2^log2 threads, written by the row's first ones: n of them to out. The CTA's threads come here
-// together. (Numbers, not lanes, are halved by the first four exchanges, each lane keeping those whose index has its bits: 16 exchanges a warp instead of 80.)
-__device__ __forceinline__ void row_sums(float (&d)[kRowsMaxUsed], uint32_t log2, float (*part)[kRowsMaxUsed], bool in, uint32_t n, float *out) {
-  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  if (log2 >= 5) {
+// Up to four rows' octets as they were loaded.
+template <class X>
+struct FourRows {
+  uint4 raw[4][sizeof(X) / 2];
+  uint32_t r[4];
+  // Rows inv[j0] .. inv[j0 + 3] of those there are, those of R alone.
+  __device__ void load(const X *rows, uint64_t D, uint32_t c, const int32_t *inv, uint32_t j0, uint32_t n, uint32_t R, bool wanted = true) {
 #pragma unroll
-    for (uint32_t h = 8, bit = 16; h; h /= 2, bit /= 2) {
+    for (uint32_t j = 0; j < 4; j++) r[j] = j0 + j < n ? (uint32_t)inv[j0 + j] : 0xFFFFFFFFu;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+      for (uint32_t i = 0; i < sizeof(X) / 2; i++)
+        if (wanted && r[j] < R) raw[j][i] = ((const uint4 *)(rows + r[j] * D + c))[i];
+  }
+  __device__ void values(uint32_t j, float *v) const { load8((const X *)raw[j], v); }
+};
+
+// The sums of N = 4 Q numbers a thread over a row's 2^log2 threads, n of them to out. The CTA's threads come here together. (Numbers, not lanes, are halved by the
+// first exchanges, each lane keeping those whose index has its bits: 16 exchanges a warp for 16 numbers instead of 80.)
+template <uint32_t Q>
+__device__ __forceinline__ void row_sums(float (&of)[4 * Q], uint32_t log2, float (*part)[kRowsMaxUsed], bool in, uint32_t n, float *out) {
+  constexpr uint32_t N = Q == 1 ? 4 : Q == 2 ? 8 : 16;
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  float d[N];
+#pragma unroll
+  for (uint32_t j = 0; j < N; j++) d[j] = j < 4 * Q ? of[j] : 0.0f;
+  if (log2 >= 5) {
+    uint32_t mine = 0;  // the number whose sum the lane comes to hold
+#pragma unroll
+    for (uint32_t h = N / 2, bit = 16; h; h /= 2, bit /= 2) {
 #pragma unroll
       for (uint32_t i = 0; i < h; i++) {
         const float keep = lane & bit ? d[i + h] : d[i], give = lane & bit ? d[i] : d[i + h];
         d[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
       }
+      mine += lane & bit ? h : 0;
     }
-    d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
-    // Lane l has the sum of number l / 2.
+#pragma unroll
+    for (uint32_t bit = 16 / N; bit; bit /= 2) d[0] += __shfl_xor_sync(0xffffffffu, d[0], bit);
+    const bool first = lane % (32 / N) == 0;
     if (log2 == 5) {
-      if (in && lane % 2 == 0 && lane / 2 < n) out[lane / 2] = d[0];
+      if (in && first && mine < n) out[mine] = d[0];
       return;
     }
-    if (lane % 2 == 0) part[warp][lane / 2] = d[0];
+    if (first) part[warp][mine] = d[0];
     __syncthreads();
     const uint32_t i = threadIdx.x & ((1u << log2) - 1), each = 1u << (log2 - 5);
     if (in && i < n) {
@@ -83,47 +109,46 @@ __device__ __forceinline__ void row_sums(float (&d)[kRowsMaxUsed], uint32_t log2
   }
   const uint32_t i = lane & ((1u << log2) - 1);
 #pragma unroll
-  for (uint32_t j = 0; j < kRowsMaxUsed; j++) {
-    if (j >= n) break;
+  for (uint32_t j = 0; j < 4 * Q; j++) {
     for (uint32_t off = (1u << log2) / 2; off; off /= 2) d[j] += __shfl_xor_sync(0xffffffffu, d[j], off);
-    if (in && i == 0) out[j] = d[j];
+    if (in && i == 0 && j < n) out[j] = d[j];
   }
 }
 
-// dx[t] = (add[t] +) sum_j (w[t][j]) dxs[inv[t][j]], and where dw is wanted dw[t][j] = <x[t], dxs[inv[t][j]]>.
-template <class X, bool DW>
-__global__ void __launch_bounds__(kThreads) k_sort_rows_grad(const X *dxs, const StepRows map, uint32_t R, const int32_t *inv, const float *w, const X *x, uint64_t stride,
-                                                             uint32_t n_used, const X *add, X *dx, float *dw) {
+template <class X>
+constexpr uint32_t grad_ctas() {
+  return sizeof(X) == 4 ? 2 : 4;
+}
+
+// dx[t] = (add[t] +) sum_j (w[t][j]) dxs[inv[t][j]], and where dw is wanted dw[t][j] = <x[t], dxs[inv[t][j]]>. Q: fours of results a row has.
+template <class X, bool DW, uint32_t Q>
+__global__ void __launch_bounds__(kThreads, grad_ctas<X>()) k_sort_rows_grad(const X *dxs, const StepRows map, uint32_t R, const int32_t *inv, const float *w, const X *x,
+                                                                             uint64_t stride, uint32_t n_used, const X *add, X *dx, float *dw) {
   __shared__ float part[DW ? kThreads / 32 : 1][kRowsMaxUsed];
   dependents_may_launch(), wait_for_predecessors();
   const uint64_t t = map.row(), D = 8ull * map.octets;
   const bool in = t < map.T;
-  float dot[kRowsMaxUsed];
-#pragma unroll
-  for (uint32_t j = 0; j < kRowsMaxUsed; j++) dot[j] = 0.0f;
+  float dot[DW ? 4 * Q : 1] = {};
   if (in) {
+    inv += t * n_used, w += w ? t * n_used : 0;
     for (uint32_t o = map.first(); o < map.octets; o += map.step()) {
       float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, xv[8];
       if constexpr (DW) load8(x + t * stride + 8 * o, xv);
 #pragma unroll
-      for (uint32_t j0 = 0; j0 < kRowsMaxUsed; j0 += 4) {
-        if (j0 >= n_used) break;
-        uint32_t r[4];
-        float v[4][8];
+      for (uint32_t j0 = 0; j0 < 4 * Q; j0 += 4) {
+        FourRows<X> rows;
+        rows.load(dxs, D, 8 * o, inv, j0, n_used, R);
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-          r[j] = j0 + j < n_used ? (uint32_t)inv[t * n_used + j0 + j] : 0xFFFFFFFFu;
-          if (r[j] < R) load8(dxs + r[j] * D + 8 * o, v[j]);
-        }
+          if (rows.r[j] >= R) continue;
+          const float f = w ? w[j0 + j] : 1.0f;
+          float v[8];
+          rows.values(j, v);
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-          if (r[j] >= R) continue;
-          const float f = w ? w[t * n_used + j0 + j] : 1.0f;
-#pragma unroll
-          for (int i = 0; i < 8; i++) acc[i] = fmaf(f, v[j][i], acc[i]);
+          for (int i = 0; i < 8; i++) acc[i] = fmaf(f, v[i], acc[i]);
           if constexpr (DW)
 #pragma unroll
-            for (int i = 0; i < 8; i++) dot[j0 + j] = fmaf(xv[i], v[j][i], dot[j0 + j]);
+            for (int i = 0; i < 8; i++) dot[j0 + j] = fmaf(xv[i], v[i], dot[j0 + j]);
         }
       }
       if (dx) {
@@ -137,52 +162,62 @@ __global__ void __launch_bounds__(kThreads) k_sort_rows_grad(const X *dxs, const
       }
     }
   }
-  if constexpr (DW) row_sums(dot, map.log2, part, in, n_used, dw + t * n_used);
+  if constexpr (DW) row_sums<Q>(dot, map.log2, part, in, n_used, dw + t * n_used);
 }
 
 // dy[inv[t][j]] = w[t][j] dout[t], dw[t][j] = <dout[t], y[inv[t][j]]>. dy may be y: a thread has read what it writes over.
-template <class G, class Y>
-__global__ void __launch_bounds__(kThreads) k_combine_rows_grad(const G *dout, const Y *y, const StepRows map, uint32_t R, const int32_t *inv, const float *w,
-                                                                uint32_t n_used, Y *dy, float *dw) {
+template <class G, class Y, uint32_t Q>
+__global__ void __launch_bounds__(kThreads, grad_ctas<Y>()) k_combine_rows_grad(const G *dout, const Y *y, const StepRows map, uint32_t R, const int32_t *inv, const float *w,
+                                                                                uint32_t n_used, Y *dy, float *dw) {
   __shared__ float part[kThreads / 32][kRowsMaxUsed];
   dependents_may_launch(), wait_for_predecessors();
   const uint64_t t = map.row(), D = 8ull * map.octets;
   const bool in = t < map.T;
-  float dot[kRowsMaxUsed];
-#pragma unroll
-  for (uint32_t j = 0; j < kRowsMaxUsed; j++) dot[j] = 0.0f;
+  float dot[4 * Q] = {};
   if (in) {
+    inv += t * n_used, w += w ? t * n_used : 0;
     for (uint32_t o = map.first(); o < map.octets; o += map.step()) {
       float g[8];
       load8(dout + t * D + 8 * o, g);
 #pragma unroll
-      for (uint32_t j0 = 0; j0 < kRowsMaxUsed; j0 += 4) {
-        if (j0 >= n_used) break;
-        uint32_t r[4];
-        float v[4][8];
+      for (uint32_t j0 = 0; j0 < 4 * Q; j0 += 4) {
+        FourRows<Y> rows;
+        rows.load(y, D, 8 * o, inv, j0, n_used, R, dw);
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
-          r[j] = j0 + j < n_used ? (uint32_t)inv[t * n_used + j0 + j] : 0xFFFFFFFFu;
-          if (dw && r[j] < R) load8(y + r[j] * D + 8 * o, v[j]);
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-          if (r[j] >= R) continue;
-          if (dw)
-#pragma unroll
-            for (int i = 0; i < 8; i++) dot[j0 + j] = fmaf(g[i], v[j][i], dot[j0 + j]);
+          if (rows.r[j] >= R) continue;
           if (dy) {
-            const float f = w[t * n_used + j0 + j];
+            const float f = w[j0 + j];
             float u[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) u[i] = f * g[i];
-            store8(dy + r[j] * D + 8 * o, u);
+            store8(dy + rows.r[j] * D + 8 * o, u);
+          }
+          if (dw) {
+            float v[8];
+            rows.values(j, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) dot[j0 + j] = fmaf(g[i], v[i], dot[j0 + j]);
           }
         }
       }
     }
   }
-  if (dw) row_sums(dot, map.log2, part, in, n_used, dw + t * n_used);
+  if (dw) row_sums<Q>(dot, map.log2, part, in, n_used, dw + t * n_used);
+}
+
+// Calls f with the fours of results a row has, as a type.
+template <class F>
+void with_fours(uint32_t n_used, F &&f) {
+  using std::integral_constant;
+  if (n_used <= 4)
+    f(integral_constant<uint32_t, 1>{});
+  else if (n_used <= 8)
+    f(integral_constant<uint32_t, 2>{});
+  else if (n_used <= 12)
+    f(integral_constant<uint32_t, 3>{});
+  else
+    f(integral_constant<uint32_t, 4>{});
 }
 
 template <class F>
@@ -257,9 +292,12 @@ MOE_API moe_status moe_sort_rows_grad_device(const void *dxs_dev, uint32_t type,
     with_step_rows(T, n_embd, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
-        const auto kernel = dw_dev ? k_sort_rows_grad<X, true> : k_sort_rows_grad<X, false>;
-        CUDA_OK(launch_kernel(true, kernel, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)dxs_dev, map, R, inv_dev, w_dev, (const X *)x_dev,
-                              stride ? stride : n_embd, n_used, (const X *)add_dev, (X *)dx_dev, dw_dev));
+        with_fours(n_used, [&](auto q) {
+          constexpr uint32_t Q = decltype(q)::value;
+          const auto kernel = dw_dev ? k_sort_rows_grad<X, true, Q> : k_sort_rows_grad<X, false, Q>;
+          CUDA_OK(launch_kernel(true, kernel, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)dxs_dev, map, R, inv_dev, w_dev, (const X *)x_dev,
+                                stride ? stride : n_embd, n_used, (const X *)add_dev, (X *)dx_dev, dw_dev));
+        });
       });
     });
   });
@@ -281,8 +319,10 @@ MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t d
         using G = std::remove_pointer_t<decltype(g)>;
         with_type(y_type, [&](auto *of) {
           using Y = std::remove_pointer_t<decltype(of)>;
-          CUDA_OK(launch_kernel(true, k_combine_rows_grad<G, Y>, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const G *)dout_dev, (const Y *)y_dev, map, R, inv_dev,
-                                w_dev, n_used, (Y *)dy_dev, dw_dev));
+          with_fours(n_used, [&](auto q) {
+            CUDA_OK(launch_kernel(true, k_combine_rows_grad<G, Y, decltype(q)::value>, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const G *)dout_dev,
+                                  (const Y *)y_dev, map, R, inv_dev, w_dev, n_used, (Y *)dy_dev, dw_dev));
+          });
         });
       });
     });

@@ -63,19 +63,31 @@ CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, 
   return m;
 }
 
-CUtensorMap make_bytes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows) {
+static CUtensorMap bytes_map(const void *base, uint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
   CUtensorMap m{};
-  const cuuint64_t part = (cuuint64_t)row_bytes * rows;
-  const cuuint64_t dims[4] = {row_bytes, parts, rows, matrices};
-  // A stride that nothing steps by is a row's: the true one may pass what a map holds.
-  const cuuint64_t strides[3] = {parts > 1 ? part : row_bytes, row_bytes, matrices > 1 ? part * parts : row_bytes};
-  const cuuint32_t box[4] = {128, parts, box_rows, 1};
-  const cuuint32_t elem[4] = {1, 1, 1, 1};
-  const CUresult r = tensor_map_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, box, elem,
-                                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  const CUresult r = tensor_map_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw CudaFailure(cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed with driver error " + std::to_string((int)r));
   return m;
+}
+
+CUtensorMap make_matrix_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t matrices, uint32_t box_rows) {
+  const cuuint64_t row = row_bytes, dims[5] = {row, 8, 4, rows / 32, matrices}, strides[4] = {4 * row, row, 32 * row, rows * row};
+  const cuuint32_t box[5] = {128, 8, 4, box_rows / 32, 1};
+  return bytes_map(base, 5, dims, strides, box);
+}
+
+CUtensorMap make_gate_up_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t matrices, uint32_t box_rows) {
+  const cuuint64_t row = row_bytes, dims[5] = {row, 8, 2, 2ull * matrices, rows / 16}, strides[4] = {2 * row, row, rows * row, 16 * row};
+  const cuuint32_t box[5] = {128, 8, 2, 2, box_rows / 32};
+  return bytes_map(base, 5, dims, strides, box);
+}
+
+CUtensorMap make_byte_rows_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t box_rows) {
+  const cuuint64_t dims[2] = {row_bytes, rows}, strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {128, box_rows};
+  return bytes_map(base, 2, dims, strides, box);
 }
 
 }  // namespace moe

@@ -26,9 +26,16 @@ CUtensorMap make_quants_map(const void *base, uint32_t row_bytes, uint32_t rows,
 // swizzle. What lies past a row's end or past a part's rows reads as zero.
 CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows);
 
-// A map over matrices of bytes, [matrices][parts][rows][row_bytes] one after another (base 16-byte aligned, row_bytes a multiple of 16), whose
-// copies bring 128 bytes of box_rows rows of one matrix, of every part's row r before row r + 1's, with the 128-byte swizzle. What lies past a row's
-// end or past a part's rows reads as zero.
-CUtensorMap make_bytes_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t parts, uint32_t matrices, uint32_t box_rows);
+// Maps over matrices of bytes, [matrices][rows][row_bytes] one after another (base 16-byte aligned, row_bytes a multiple of 16, rows of 32), whose copies bring 128
+// bytes of box_rows rows (a multiple of 32) of one matrix with the 128-byte swizzle. Every 32 of them come in the order 0, 4, ... 28, 1, 5, ... 29, 2, ... 30, 3, ... 31: a
+// thread that has four lanes eight apart of a product has four neighbouring rows of the matrix. Places: of 32 rows, of matrices.
+CUtensorMap make_matrix_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t matrices, uint32_t box_rows);
+// The same of matrices of rows gate and then rows up rows, whose copies bring box_rows / 2 of each: 0, 2, ... 14, 1, 3, ... 15 of 16 gate rows, then the same of 16 up
+// rows, and so on. Places: of gate and of up matrices (matrix m's gate is 2 m), of 16 rows.
+CUtensorMap make_gate_up_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t matrices, uint32_t box_rows);
+
+// A map over rows of bytes [rows][row_bytes] (base 16-byte aligned, row_bytes a multiple of 16), whose copies bring 128 bytes of box_rows rows with the 128-byte
+// swizzle; zeros past the end.
+CUtensorMap make_byte_rows_map(const void *base, uint32_t row_bytes, uint32_t rows, uint32_t box_rows);
 
 }  // namespace moe
