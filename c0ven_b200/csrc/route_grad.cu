@@ -15,6 +15,7 @@
 #include <cstdint>
 
 #include "ops_common.h"
+#include "two.cuh"
 
 namespace moe {
 namespace {
@@ -52,6 +53,11 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 // e^(l - top), the largest's own 1 even where it is infinite; 0 for an expert that is out.
 __device__ __forceinline__ float part_of(float l, float top) { return l == -INFINITY ? 0.0f : l == top ? 1.0f : expf(l - top); }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 // Four neighbouring values of a row as f32, and back. The address is aligned to them.
 __device__ __forceinline__ void load4(const float *p, float *v) { *(float4 *)v = *(const float4 *)p; }
@@ -115,30 +121,55 @@ __global__ void __launch_bounds__(32 * kWarps) k_route_grad(const RouteGradArgs 
     const uint32_t e = id;
     float y[V], g = d;
     if constexpr (DENSE) {
+      // An expert that is out, NaN among them, counts as -infinity. The exponentials are approximate, off by 2^-22 and by what the argument's two roundings
+      // make of it, a part in 2^23 of l - top: as much as rounding l - top alone does to an accurate one.
       float top = -INFINITY;
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        y[v] = z[v] > -INFINITY && (!a.bias || (column(v) < a.E && a.bias[column(v)] > -INFINITY)) ? z[v] : -INFINITY;
+        y[v] = fmaxf(z[v], -INFINITY);
+        if (a.bias && column(v) < a.E && !(a.bias[column(v)] > -INFINITY)) y[v] = -INFINITY;
         top = fmaxf(top, y[v]);
       }
       if (e < a.E) row[e] = g;
+      const bool odd = __any_sync(0xffffffffu, !(fabsf(g) < INFINITY));
       if (t + step < a.T) bring(t + step);
       top = warp_max(top);
-      float total = 0.0f;
+      if (top == INFINITY) {  // those alone share the row
 #pragma unroll
-      for (int v = 0; v < V; v++) y[v] = part_of(y[v], top), total += y[v];
-      total = warp_sum(total);
-      __syncwarp();
-      float mean = 0.0f;
-#pragma unroll
-      for (int v = 0; v < V; v++) {
-        mean += y[v] > 0.0f ? y[v] * row[column(v)] : 0.0f;
+        for (int v = 0; v < V; v++) y[v] = y[v] == INFINITY ? 0.0f : -INFINITY;
       }
-      mean = warp_sum(mean);
-      const float f = total > 0.0f ? a.scale / total : 0.0f;
-      mean = total > 0.0f ? mean / total : 0.0f;
+      const Two less(fabsf(top) < INFINITY ? -top : 0.0f), log2e(1.4426950408889634f);
+      Two total(0.0f);
 #pragma unroll
-      for (int v = 0; v < V; v++) y[v] = y[v] > 0.0f ? f * y[v] * (row[column(v)] - mean) : 0.0f;
+      for (int v = 0; v < V; v += 2) {
+        const Two p = (Two(y[v], y[v + 1]) + less) * log2e;
+        y[v] = exp2_approx(p.lo()), y[v + 1] = exp2_approx(p.hi());
+        total = total + Two(y[v], y[v + 1]);
+      }
+      const float sum = warp_sum(total.lo() + total.hi());
+      __syncwarp();
+      Two part(0.0f);
+      float c[V];
+#pragma unroll
+      for (int v = 0; v < V; v++) c[v] = row[column(v)];
+      if (odd) {  // a weight's gradient that is no number reaches those its expert's share does
+        float m = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; v++) m += y[v] > 0.0f ? y[v] * c[v] : 0.0f;
+        const float mean = sum > 0.0f ? warp_sum(m) / sum : 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; v++) y[v] = y[v] > 0.0f ? a.scale / sum * y[v] * (c[v] - mean) : 0.0f;
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) part = fma(Two(y[v], y[v + 1]), Two(c[v], c[v + 1]), part);
+        const float f = sum > 0.0f ? a.scale / sum : 0.0f, mean = sum > 0.0f ? warp_sum(part.lo() + part.hi()) / sum : 0.0f;
+        const Two factor(f), minus(-mean);
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+          const Two r = (Two(c[v], c[v + 1]) + minus) * (Two(y[v], y[v + 1]) * factor);
+          y[v] = r.lo(), y[v + 1] = r.hi();
+        }
+      }
     } else {
       const float lc = l;
       if (lc == -INFINITY) g = 0.0f;

@@ -1,7 +1,9 @@
 // Rows to expert order in their own type, and the gradients of that and of the combine (include/moe_layer.h). Single passes over their data.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "mx4.cuh"
 #include "ops_common.h"
@@ -11,6 +13,7 @@ namespace {
 
 constexpr uint32_t kRowsMaxUsed = 16;
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kLongStep = 1024;  // rows
 
 // How a step's rows are dealt to a CTA of 256 threads: 2^log2 neighbouring threads a row; of its octets, groups of eight values, thread i takes i,
 // i + 2^log2 and so on.
@@ -115,9 +118,11 @@ __device__ __forceinline__ void row_sums(float (&of)[4 * Q], uint32_t log2, floa
   }
 }
 
+// CTAs an SM of the gradients' kernels, by the registers that four rows' octets as they were loaded, their sums and the row's own values take: 8,192 rows of 2,048 bf16
+// values, dx and dw, 63 us with four, 71 with three, 75 with five (which spill); 4,096 of 4,096 f32 values 101 with three, 132 with two.
 template <class X>
 constexpr uint32_t grad_ctas() {
-  return sizeof(X) == 4 ? 2 : 4;
+  return sizeof(X) == 4 ? 3 : 4;
 }
 
 // dx[t] = (add[t] +) sum_j (w[t][j]) dxs[inv[t][j]], and where dw is wanted dw[t][j] = <x[t], dxs[inv[t][j]]>. Q: fours of results a row has.
@@ -220,10 +225,20 @@ void with_fours(uint32_t n_used, F &&f) {
     f(integral_constant<uint32_t, 4>{});
 }
 
+// Calls f with the map for a step's rows, and its grid. Rows of more than 32 octets get up to a CTA of threads. most_log2 is for long steps: as many threads a row, that
+// many at most, as leave fewer than an eighth of them idle in a row's last round. What only reads rows does best with a warp a row, which meets at no barrier
+// (8,192 rows of 2,048 bf16 values, eight places each, dx and dw: 57 us, 59 with 64 threads a row, 62 with 256; of 1,536 44, 46 and 56); what writes them, with as
+// many threads as fit (16,384 of 2,048, ten places: 232 us with 256, 244 with 32; 4,096 of 2,880, six places: 58 with 64, 61 with 256, 64 with 32).
 template <class F>
-void with_step_rows(uint32_t T, uint32_t n_embd, F &&f) {
+void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t most_log2, F &&f) {
   StepRows map{T, 0, n_embd / 8};
   while (map.log2 < 8 && (1u << map.log2) < map.octets) map.log2++;
+  if (T >= kLongStep && map.log2 > 5) {
+    auto slots = [&](uint32_t log2) { return (uint64_t)((map.octets + (1u << log2) - 1) >> log2) << log2; };
+    uint32_t log2 = std::min(most_log2, map.log2);
+    while (log2 > 5 && slots(log2) * 8 > map.octets * 9ull) log2--;
+    map.log2 = log2;
+  }
   const uint32_t rows = kThreads >> map.log2;
   f(map, dim3((T + rows - 1) / rows));
 }
@@ -265,7 +280,7 @@ MOE_API moe_status moe_sort_rows_device(const void *x_dev, uint32_t type, uint64
     need_stride(stride, n_embd, size);
     if (T == 0 || R == 0) return;
     need_device({{x_dev, "x", 16}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {xs_dev, "xs", 16}});
-    with_step_rows(T, n_embd, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, 8, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
         CUDA_OK(launch_kernel(true, k_sort_rows<X>, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)x_dev, stride ? stride : n_embd, map, inv_dev, w_dev,
@@ -289,7 +304,7 @@ MOE_API moe_status moe_sort_rows_grad_device(const void *dxs_dev, uint32_t type,
     // With R 0 no row of dxs is read: it may be null then.
     need_device({{dxs_dev, "dxs", 16, R == 0}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {x_dev, "x", 16, true}, {add_dev, "add", 16, true}, {dx_dev, "dx", 16, true},
                  {dw_dev, "dw", 4, true}});
-    with_step_rows(T, n_embd, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, dw_dev ? 5 : 8, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
         with_fours(n_used, [&](auto q) {
@@ -314,7 +329,7 @@ MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t d
     need(!dy_dev || w_dev, "w is required for dy");
     if (T == 0) return;
     need_device({{dout_dev, "dout", 16}, {y_dev, "y", 16, true}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {dy_dev, "dy", 16, true}, {dw_dev, "dw", 4, true}});
-    with_step_rows(T, n_embd, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, 8, [&](StepRows map, dim3 grid) {
       with_type(dout_type, [&](auto *g) {
         using G = std::remove_pointer_t<decltype(g)>;
         with_type(y_type, [&](auto *of) {
