@@ -79,9 +79,17 @@ __device__ __forceinline__ void store4(__nv_bfloat16 *p, const float *v) {
   *(uint2 *)p = make_uint2(*(const uint32_t *)&a, *(const uint32_t *)&b);
 }
 
+// CTAs an SM. Softmax weights as they are: as many as are resident at once, whose warps bring their next row while they work on one, with registers for three (32,768
+// rows of 512 f32 logits: 25 us, 30 without that bound and with six CTAs an SM, 34 with two resident and three launched; the bytes alone 20.5). Else a row
+// is short work (32,768 rows of 512 f32 values 19 us, of 256 bf16 ones 12.6 with 16 an SM, 19 and 12.7 with 8, 19 and 13.4 with 28).
+template <int V, bool DENSE>
+constexpr uint32_t grad_ctas() {
+  return !DENSE ? 16 : V == 16 ? 3 : V == 8 ? 4 : 6;
+}
+
 // V: columns a lane has at most. W: neighbouring ones it has together, four where the rows' addresses allow, else one. DENSE: softmax weights as they are.
 template <class L, int V, int W, bool DENSE>
-__global__ void __launch_bounds__(32 * kWarps) k_route_grad(const RouteGradArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8) k_route_grad(const RouteGradArgs a) {
   __shared__ __align__(16) float rows[kWarps][32 * V];
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -208,12 +216,20 @@ __global__ void __launch_bounds__(32 * kWarps) k_route_grad(const RouteGradArgs 
   }
 }
 
+template <class L, int V, int W, bool DENSE>
+void launch_columns(const RouteGradArgs &a, cudaStream_t st) {
+  const dim3 grid(std::min((a.T + kWarps - 1) / kWarps, 148 * grad_ctas<V, DENSE>())), block(32 * kWarps);
+  CUDA_OK(launch_kernel(true, k_route_grad<L, V, W, DENSE>, grid, block, 0, st, a));
+}
+
 template <class L, int W, bool DENSE>
 void launch_grad(const RouteGradArgs &a, cudaStream_t st) {
-  // Rows by warps that stay: as many CTAs as are resident at once for long steps.
-  const dim3 grid(std::min((a.T + kWarps - 1) / kWarps, 148u * 6)), block(32 * kWarps);
-  const auto kernel = a.E <= 128 ? k_route_grad<L, 4, W, DENSE> : a.E <= 256 ? k_route_grad<L, 8, W, DENSE> : k_route_grad<L, 16, W, DENSE>;
-  CUDA_OK(launch_kernel(true, kernel, grid, block, 0, st, a));
+  if (a.E <= 128)
+    launch_columns<L, 4, W, DENSE>(a, st);
+  else if (a.E <= 256)
+    launch_columns<L, 8, W, DENSE>(a, st);
+  else
+    launch_columns<L, 16, W, DENSE>(a, st);
 }
 
 template <class L>

@@ -16,12 +16,12 @@ constexpr uint32_t kThreads = 256;
 constexpr uint32_t kLongStep = 1024;  // rows
 
 // How a step's rows are dealt to a CTA of 256 threads: 2^log2 neighbouring threads a row; of its octets, groups of eight values, thread i takes i,
-// i + 2^log2 and so on.
+// i + 2^log2 and so on; with several CTAs a row (grid.y) they take turns.
 struct StepRows {
   uint32_t T, log2, octets;
   __device__ uint64_t row() const { return (uint64_t)blockIdx.x * (kThreads >> log2) + (threadIdx.x >> log2); }
-  __device__ uint32_t first() const { return threadIdx.x & ((1u << log2) - 1); }
-  __device__ uint32_t step() const { return 1u << log2; }
+  __device__ uint32_t first() const { return (threadIdx.x & ((1u << log2) - 1)) + (blockIdx.y << log2); }
+  __device__ uint32_t step() const { return gridDim.y << log2; }
 };
 
 template <class X>
@@ -229,8 +229,9 @@ void with_fours(uint32_t n_used, F &&f) {
 // many at most, as leave fewer than an eighth of them idle in a row's last round. What only reads rows does best with a warp a row, which meets at no barrier
 // (8,192 rows of 2,048 bf16 values, eight places each, dx and dw: 57 us, 59 with 64 threads a row, 62 with 256; of 1,536 44, 46 and 56); what writes them, with as
 // many threads as fit (16,384 of 2,048, ten places: 232 us with 256, 244 with 32; 4,096 of 2,880, six places: 58 with 64, 61 with 256, 64 with 32).
+// whole: a row is one CTA's; else a short step's rows are up to 16 CTAs'.
 template <class F>
-void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t most_log2, F &&f) {
+void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t most_log2, bool whole, F &&f) {
   StepRows map{T, 0, n_embd / 8};
   while (map.log2 < 8 && (1u << map.log2) < map.octets) map.log2++;
   if (T >= kLongStep && map.log2 > 5) {
@@ -239,8 +240,8 @@ void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t most_log2, F &&f) {
     while (log2 > 5 && slots(log2) * 8 > map.octets * 9ull) log2--;
     map.log2 = log2;
   }
-  const uint32_t rows = kThreads >> map.log2;
-  f(map, dim3((T + rows - 1) / rows));
+  const uint32_t rows = kThreads >> map.log2, rounds = (map.octets + (1u << map.log2) - 1) >> map.log2;
+  f(map, dim3((T + rows - 1) / rows, whole || T >= kLongStep ? 1 : std::min(rounds, 16u)));
 }
 
 void need_step(uint32_t T, uint32_t R, uint32_t n_used, uint32_t n_embd) {
@@ -280,7 +281,7 @@ MOE_API moe_status moe_sort_rows_device(const void *x_dev, uint32_t type, uint64
     need_stride(stride, n_embd, size);
     if (T == 0 || R == 0) return;
     need_device({{x_dev, "x", 16}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {xs_dev, "xs", 16}});
-    with_step_rows(T, n_embd, 8, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, 8, false, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
         CUDA_OK(launch_kernel(true, k_sort_rows<X>, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)x_dev, stride ? stride : n_embd, map, inv_dev, w_dev,
@@ -304,7 +305,7 @@ MOE_API moe_status moe_sort_rows_grad_device(const void *dxs_dev, uint32_t type,
     // With R 0 no row of dxs is read: it may be null then.
     need_device({{dxs_dev, "dxs", 16, R == 0}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {x_dev, "x", 16, true}, {add_dev, "add", 16, true}, {dx_dev, "dx", 16, true},
                  {dw_dev, "dw", 4, true}});
-    with_step_rows(T, n_embd, dw_dev ? 5 : 8, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, dw_dev ? 5 : 8, dw_dev, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
         with_fours(n_used, [&](auto q) {
@@ -329,7 +330,7 @@ MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t d
     need(!dy_dev || w_dev, "w is required for dy");
     if (T == 0) return;
     need_device({{dout_dev, "dout", 16}, {y_dev, "y", 16, true}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {dy_dev, "dy", 16, true}, {dw_dev, "dw", 4, true}});
-    with_step_rows(T, n_embd, 8, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, 8, dw_dev, [&](StepRows map, dim3 grid) {
       with_type(dout_type, [&](auto *g) {
         using G = std::remove_pointer_t<decltype(g)>;
         with_type(y_type, [&](auto *of) {
