@@ -452,12 +452,16 @@ void launch_product(const I8Args &args, const void *wc, const void *xc, cudaStre
   CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a, maps));
 }
 
-// Tiles of 256 rows by pairs of CTAs where experts have more than 26 rows on average and there are 32 items for pairs at least; else of 32 by single
-// CTAs. The average is over all experts, as the host does not know which have rows.
+// Tiles of 256 rows by pairs of CTAs where experts have more than 28 rows on average (many then have more than 32, two tiles of a single CTA) and there are 32 items
+// for pairs at least and more than a round of them for single CTAs; else of 32 by single CTAs. The average is over all experts, as the host does not know
+// which have rows. gate_up and down by single CTAs and by pairs, us from a graph: 512 experts of 2,048 x 512, 10,000 rows 174 + 90 and 175 + 92, 16,000 173 + 93 and
+// 176 + 97, 24,000 204 + 126 and 179 + 105; 128 of 2,560 x 768, 2,000 rows 80 + 44 and 82 + 46, 3,200 84 + 45 and 83 + 46, skewed by a Zipf law of 1.1 86 + 48 and
+// 83 + 47, 4,800 88 + 51 and 84 + 48. One matrix: 2,080 x 1,440, 200 rows (9 items for pairs) 5.9 and 8.5, 400 (18) 8.7 and 8.7, 777 (36) 11.5 and 9.0; 8,192 x
+// 4,096, 64 rows (32, and 128 for single CTAs) 11.2 and 13.9, 128 rows (32, and 256) 16.9 and 14.6.
 template <class Out, bool GU>
 void launch(const I8Args &a, const void *wc, const void *xc, cudaStream_t st) {
-  const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 256 + 1;
-  if (a.R > 26ull * a.E && pieces * tiles >= 32)
+  const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 256 + 1, single = ((uint64_t)a.R + 31) / 32 * ((a.N + 127) / 128);
+  if (a.R > 28ull * a.E && pieces * tiles >= 32 && single > 148)
     launch_product<Out, GU, 2, 256>(a, wc, xc, st);
   else
     launch_product<Out, GU, 1, 32>(a, wc, xc, st);

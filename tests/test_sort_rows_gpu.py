@@ -36,7 +36,9 @@ def places(rng, T, n, R, dropped=0.1):
     return inv
 
 
-SHAPES = [(1, 1, 8), (1, 16, 2560), (3, 2, 16), (7, 3, 4104), (300, 10, 64), (13, 8, 2560), (33, 5, 24), (21, 4, 264), (2, 6, 2056), (65, 16, 1024), (1001, 7, 520), (5, 2, 65536)]
+SHAPES = [(1, 1, 8), (1, 16, 2560), (3, 2, 16), (7, 3, 4104), (300, 10, 64), (13, 8, 2560), (33, 5, 24), (21, 4, 264), (2, 6, 2056), (65, 16, 1024), (1001, 7, 520), (5, 2, 65536),
+          # Long steps: a warp a row, 64 and 128 threads a row, a CTA; rows that leave the last CTA half empty.
+          (1203, 3, 2560), (1100, 16, 1032), (1024, 5, 2880), (1501, 2, 3088), (1027, 12, 264), (2050, 8, 64)]
 
 
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
@@ -223,8 +225,8 @@ def route_case(rng, T, E, n, type, spread=1.0):
     return l, ids
 
 
-def check_route_grad(got, l, ids, dw, score, renorm, scale, type):
-    want, size = M.route_grad(l, ids, dw.astype(np.float64), score, renorm, scale)
+def check_route_grad(got, l, ids, dw, score, renorm, scale, type, known=None):
+    want, size = known or M.route_grad(l, ids, dw.astype(np.float64), score, renorm, scale)
     # What a share p is off by: its exponential 2 ulp (4 U) and its argument's rounding, U of the largest difference in use, which for a sigmoid is the logit
     # itself; the sum over the row 21 U (16 a lane, 5 exchanges) with the terms' own; the division, and 1 - s likewise. The mean of d: those and 6 U more. Five products.
     finite = l[np.isfinite(l)]
@@ -238,7 +240,9 @@ def check_route_grad(got, l, ids, dw, score, renorm, scale, type):
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [True, False])
-@pytest.mark.parametrize("T, E, n", [(1, 1, 1), (1, 512, 10), (9, 512, 16), (37, 160, 6), (13, 33, 4), (100, 8, 2), (5, 64, 8), (3, 255, 16), (700, 96, 1), (2, 16, 16)])
+@pytest.mark.parametrize("T, E, n", [(1, 1, 1), (1, 512, 10), (9, 512, 16), (37, 160, 6), (13, 33, 4), (100, 8, 2), (5, 64, 8), (3, 255, 16), (700, 96, 1), (2, 16, 16),
+                                     # More rows than warps that stay.
+                                     (4001, 512, 10), (5003, 200, 8), (8005, 64, 4)])
 def test_route_grad(T, E, n, score, renorm, type):
     import torch
 
@@ -253,13 +257,14 @@ def test_route_grad(T, E, n, score, renorm, type):
         out = torch.full((T + 1, E + 3), 7.0, dtype=dtype(type), device="cuda")
         wide = torch.zeros((T, E + 5), dtype=dtype(type), device="cuda")
         wide[:, :E] = l
+        known = M.route_grad(host(l), ids.cpu().numpy(), dw.astype(np.float64), score, renorm, 2.5)
         for src, stride, dst in ((l, 0, 0), (wide, E + 5, E + 3)):
             out[:] = 7.0
             ops.route_logits_grad_device(src.data_ptr(), TYPES[type], T, E, n, ids.data_ptr(), dd.data_ptr(), out.data_ptr(), score=TYPES_OF_SCORE[score], renorm=renorm,
                                          scale=2.5, stride=stride, dlogits_stride=dst)
             flat = out.view(-1)
             got = out[:T, :E] if dst else flat[:T * E].view(T, E)
-            check_route_grad(host(got), host(l), ids.cpu().numpy(), dw, score, renorm, 2.5, type)
+            check_route_grad(host(got), host(l), ids.cpu().numpy(), dw, score, renorm, 2.5, type, known)
             assert (out[T] == 7.0).all() and (not dst or (out[:T, E:] == 7.0).all()) and (dst or (flat[T * E:] == 7.0).all())
 
 
@@ -319,6 +324,33 @@ def test_route_grad_against_differences(score, renorm):
         d = (M.weights_by_logits(hi, i, score, renorm, 2.0) - M.weights_by_logits(lo, i, score, renorm, 2.0)) / (2 * step)
         # The f32 result is within some 60 half steps of terms of 2 at most.
         assert np.allclose((d * dw).sum(1), host(out)[:, e], rtol=0, atol=4 * n * 2 * step ** 2 + 120 * U)
+
+
+@pytest.mark.parametrize("T, n, D", [(3, 4, 40), (50, 7, 264), (1300, 5, 2880)])
+def test_gradients_are_the_linear_calls_transposes(T, n, D):
+    """Sorting and the combine are linear in rows, results and weights: the change that a change of one of them makes, times a gradient, is that change times the
+    gradient's. (Differences of linear calls are the calls of differences.) Sums in 64 bits of f32 results, each within a few half steps of its terms' sizes."""
+    import torch
+
+    rng = np.random.default_rng(T)
+    rows = T * n
+    inv = dev(rng.permutation(rows).reshape(T, n).astype(np.int32))
+    f = lambda *s: dev(rng.standard_normal(s).astype(np.float32))  # noqa: E731
+    x, v, g, w, u, dout = f(T, D), f(T, D), f(rows, D), f(T, n), f(T, n), f(T, D)
+    y, z = f(rows, D), f(rows, D)
+    out = lambda *s: torch.empty(s, device="cuda")  # noqa: E731
+    dx, dw, dy, dw2, xs, xu, cz, cu = out(T, D), out(T, n), out(rows, D), out(T, n), out(rows, D), out(rows, D), out(T, D), out(T, D)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    ops.sort_rows_grad_device(p(g), ops.F32, rows, p(inv), T, n, D, dx_ptr=p(dx), w_ptr=p(w), x_ptr=p(x), dw_ptr=p(dw))
+    ops.sort_rows_device(p(v), ops.F32, T, n, D, p(inv), rows, p(xs), w_ptr=p(w))   # along v, the weights as they are
+    ops.sort_rows_device(p(x), ops.F32, T, n, D, p(inv), rows, p(xu), w_ptr=p(u))   # along u, the rows as they are
+    ops.combine_rows_grad_device(p(dout), ops.F32, p(y), ops.F32, rows, p(inv), p(w), T, n, D, dy_ptr=p(dy), dw_ptr=p(dw2))
+    ops.combine_rows_device(p(z), ops.F32, rows, p(inv), p(w), T, n, D, p(cz))
+    ops.combine_rows_device(p(y), ops.F32, rows, p(inv), p(u), T, n, D, p(cu))
+    for a, b, c, d in ((xs, g, v, dx), (xu, g, u, dw), (cz, dout, z, dy), (cu, dout, u, dw2)):
+        one, two = host(a) * host(b), host(c) * host(d)
+        size = np.abs(host(g)).sum() * 8 if a is xs or a is xu else np.abs(host(dout)).sum() * 8 * n
+        assert abs(one.sum() - two.sum()) <= (chain(D) + n + 4) * U * max(np.abs(one).sum(), np.abs(two).sum(), size)
 
 
 def test_streams_and_captured_graphs():
