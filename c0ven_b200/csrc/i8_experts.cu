@@ -6,13 +6,13 @@
 // short instruction and what an item costs is bringing the matrix. Persistent units (a CTA, or a pair of CTAs on two SMs that share the rows:
 // tcgen05's cta_group::2) take items in turn; items of one expert are neighbours.
 //
-// What bounds it: few rows an expert (1,000 over 512 experts of 2,048 x 512, of which 440 have some) HBM, 143 us of gate_up at 6.5 TB/s and 73 of the product at
+// What bounds it: few rows an expert (1,000 over 512 experts of 2,048 x 512, of which 440 have some) HBM, 139 us of gate_up at 6.7 TB/s and 73 of the product at
 // 6.3; many (65,536 over 128 of 2,560 x 768) what an SM takes in, 52 to 57 bytes a clock: a pair's stage brings each CTA 16 KB of the matrix and 64 bytes a
-// row, which at 256 rows is 64 bytes for every clock of its MMAs, and more at fewer rows. 218 and 147 us (2.4 and 1.8 PTOP/s) at the 1.6 GHz that the tensor
-// load leaves, 270 and 175 under a second of load; with two experts, whose matrices stay in the L2, 165 and 117. Without an epilogue 199 and 101; one large 8,192 x
-// 8,192 x 8,192 370, 335 without (3.3 PTOP/s). Tried, and not faster: results through shared memory, by 16-byte stores or bulk-tensor copies; items of two
-// pieces of the matrix, which bring a quarter less but leave no second accumulator (the large one 339, gate_up 228); stages of 256 values for pairs. One row, 6.9
-// and 4.9 us, is latency.
+// row, which at 256 rows is 64 bytes for every clock of its MMAs, and more at fewer rows. 217 and 134 us (2.4 and 1.9 PTOP/s; HBM alone would take 118 and
+// 97) at the 1.6 GHz that the tensor load leaves, 250 and 155 to 165 under a second of load; with two experts, whose matrices stay in the L2, 164 and 110. Without
+// stores 214 and 112, without an epilogue 203 and 103; one large 8,192 x 8,192 x 8,192 370, 335 without (3.3 PTOP/s). Tried, and not faster: results through shared
+// memory, by 16-byte stores or bulk-tensor copies; items of two pieces of the matrix, which bring a quarter less but leave no second accumulator (the large
+// one 339, gate_up 228); stages of 256 values for pairs; 32 rows from tensor memory at a time. One row, 6.8 and 4.9 us, is latency.
 //
 // Roles of a CTA's warps: one thread brings the bytes by bulk-tensor copies, a stage of the contraction at a time; one lane (of a pair's first CTA)
 // issues the MMAs; groups of four warps turn accumulators, of which there are two sets, into results.
@@ -92,7 +92,9 @@ struct I8Maps {
 // of bytes; the scales of a tile's rows, an epilogue warp its own; barriers; the experts' first rows and first tiles; the tiles' experts.
 template <bool GU, uint32_t CTAS, uint32_t NT>
 struct I8Form {
-  static constexpr uint32_t kGroups = CTAS == 2 ? 4 : 2;  // of four epilogue warps
+  // Groups of four epilogue warps. With four of them for pairs (and as many stores and waits on their way) the product of 65,536 rows over 128 experts took 147 us, 134 with
+  // two, 144 with one; gate_up 220, 217 and 226.
+  static constexpr uint32_t kGroups = 2;
   static constexpr uint32_t kThreads = 32 * (2 + 4 * kGroups);
   // A stage holds 128 values of the contraction, 128 bytes of a row, of single CTAs twice as many: half the hand-overs where a stage's MMAs are short (100 rows
   // over 512 experts 151 us of gate_up with 128, 145 with 256; pairs 165 with 128, 171 with 256 and half the stages).

@@ -63,11 +63,12 @@ CUtensorMap make_codes_map(const void *base, uint32_t row_bytes, uint32_t rows, 
   return m;
 }
 
+// The L2 fetches 256 bytes of a row at once, as the next stage wants the next 128 (100 rows over 512 experts of 2,048 x 512: gate_up 140 us, 144 with 128).
 static CUtensorMap bytes_map(const void *base, uint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
   CUtensorMap m{};
   const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
   const CUresult r = tensor_map_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw CudaFailure(cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed with driver error " + std::to_string((int)r));
   return m;
 }
