@@ -1,10 +1,12 @@
 // Rows to and from 8-bit integers with a scale each (include/moe_layer.h, "8-bit rows"). Single passes over their data: what bounds long calls is HBM. A row's values
-// stay in its threads' registers, as they were loaded, from its largest magnitude to its codes. 32,768 rows of 2,048 bf16 values to 8-bit rows 38.7 us
-// (5.2 TB/s) and back 31.5 (6.4); f32 values 61 (5.5); 65,536 rows of 768 bf16 values 33 (4.5), 300,000 of 64 15; 4,096 of 2,880 to six places each 22. 13 rows of
+// stay in its threads' registers, as they were loaded, from its largest magnitude to its codes. 32,768 rows of 2,048 bf16 values to 8-bit rows 35.5 us
+// (5.7 TB/s) and back 31.5 (6.4); f32 values 58 (5.7); 65,536 rows of 768 bf16 values 30 (5.0), 300,000 of 64 15; 4,096 of 2,880 to six places each 22. 13 rows of
 // 2,560 f32 values to eight places each and back 2.6 + 1.6 us, one round trip after another.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "mx4.cuh"
 #include "ops_common.h"
@@ -68,15 +70,17 @@ struct Octet {
 struct RowScale {
   float top, scale, inverse, rest, lift;
   bool bad;
+  RowScale() = default;
   __device__ explicit RowScale(uint32_t bits) {
     bad = bits >= 0x7F800000u;
     top = __uint_as_float(bits);
     scale = bad ? __uint_as_float(0x7FFFFFFFu) : __fdiv_rn(top, 127.0f);
-    lift = top < 1e-30f ? 0x1p64f : top > 1e30f ? 0x1p-64f : 1.0f;
+    lift = top < 1e-30f && top != 0.0f ? 0x1p64f : top > 1e30f ? 0x1p-64f : 1.0f;
     top *= lift;
     inverse = bad || top == 0.0f ? 0.0f : __fdiv_rn(127.0f, top);
     rest = fmaf(-inverse, top, 127.0f) * (inverse * (1.0f / 127.0f));
   }
+  __device__ bool odd() const { return bad || lift != 1.0f; }
 };
 
 // Eight codes: rint(127 x / top) of exact numbers, ties to even.
@@ -88,11 +92,13 @@ struct RowScale {
 // f32 values: x * inverse, rounded once, is within 127 * 2^-23 < 2^-16 of 127 x / top. Where one lies nearer than 2^-15 to a border the sign of 127 x - border * top
 // decides, from the two products and what their roundings left over: the products are near one another, so their difference is exact, and what was left
 // over has ten bits at most. What a row lifted down loses of its smallest values is far below half a code.
-template <class X>
+//
+// ODD: the row may be bad or lifted. (Looking for that at every eight values took 39 us where 35.5 do.)
+template <class X, bool ODD>
 __device__ __forceinline__ uint2 codes8(float (&x)[8], const RowScale &s) {
-  if (s.bad) return make_uint2(0, 0);
+  if (ODD && s.bad) return make_uint2(0, 0);
   constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: sums with it are whole numbers, ties to even, in the low bits
-  if (s.lift != 1.0f)
+  if (ODD && s.lift != 1.0f)
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] *= s.lift;
   const Two inverse(s.inverse), magic(kMagic);
@@ -144,10 +150,11 @@ __device__ __forceinline__ uint32_t row_max(uint32_t m, uint32_t log2, uint32_t 
   return m;
 }
 
-// V octets a thread of each of U rows, whose loads are on their way together.
+// V octets a thread of each of U rows, whose loads are on their way together. CTAs an SM by the registers: five of 16-bit rows of one row a thread (35.5 us where four take
+// 37.5), four where it has more (15 us of 300,000 rows of 64; five spill and take 17.7), two of f32 rows.
 template <class X, uint32_t V, uint32_t U>
-__global__ void __launch_bounds__(kThreads, sizeof(X) == 2 ? 4 : 2) k_i8_quantize(const X *x, uint64_t stride, const RowsOfThreads map, uint32_t K, const int32_t *inv, uint32_t n_used, uint32_t R,
-                                                          uint8_t *codes, float *scales) {
+__global__ void __launch_bounds__(kThreads, sizeof(X) == 4 ? 2 : U == 1 ? 5 : 4) k_i8_quantize(const X *x, uint64_t stride, const RowsOfThreads map, uint32_t K, const int32_t *inv,
+                                                                                              uint32_t n_used, uint32_t R, uint8_t *codes, float *scales) {
   __shared__ uint32_t part[U][kThreads / 32];
   dependents_may_launch(), wait_for_predecessors();
   const uint32_t rows = kThreads >> map.log2;
@@ -171,33 +178,42 @@ __global__ void __launch_bounds__(kThreads, sizeof(X) == 2 ? 4 : 2) k_i8_quantiz
     for (uint32_t v = 0; v < V; v++) top[u] = max(top[u], o[u][v].largest());
     top[u] = row_max(top[u], map.log2, part[u]);
   }
+  RowScale s[U];
+  bool odd = false;
 #pragma unroll
-  for (uint32_t u = 0; u < U; u++) {
-    const uint64_t t = t0 + u * rows;
-    if (t >= map.T) break;
-    const RowScale s(top[u]);
-    const int32_t *to = inv + t * n_used;
+  for (uint32_t u = 0; u < U; u++) s[u] = RowScale(top[u]), odd |= s[u].odd();
+  auto write = [&](auto is_odd) {
 #pragma unroll
-    for (uint32_t v = 0; v < V; v++) {
-      const uint32_t k = 8 * map.octet(v);
-      float f[8];
-      o[u][v].values(f);
-      const uint2 c = codes8<X>(f, s);
-      if (k >= K) break;
-      if (!inv)
-        *(uint2 *)(codes + t * K + k) = c;
-      else
-        for (uint32_t j = 0; j < n_used; j++)
-          if ((uint32_t)to[j] < R) *(uint2 *)(codes + (uint64_t)(uint32_t)to[j] * K + k) = c;
+    for (uint32_t u = 0; u < U; u++) {
+      const uint64_t t = t0 + u * rows;
+      if (t >= map.T) break;
+      const int32_t *to = inv + t * n_used;
+#pragma unroll
+      for (uint32_t v = 0; v < V; v++) {
+        const uint32_t k = 8 * map.octet(v);
+        float f[8];
+        o[u][v].values(f);
+        const uint2 c = codes8<X, decltype(is_odd)::value>(f, s[u]);
+        if (k >= K) break;
+        if (!inv)
+          *(uint2 *)(codes + t * K + k) = c;
+        else
+          for (uint32_t j = 0; j < n_used; j++)
+            if ((uint32_t)to[j] < R) *(uint2 *)(codes + (uint64_t)(uint32_t)to[j] * K + k) = c;
+      }
+      if (map.first() == 0) {
+        if (!inv)
+          scales[t] = s[u].scale;
+        else
+          for (uint32_t j = 0; j < n_used; j++)
+            if ((uint32_t)to[j] < R) scales[(uint32_t)to[j]] = s[u].scale;
+      }
     }
-    if (map.first() == 0) {
-      if (!inv)
-        scales[t] = s.scale;
-      else
-        for (uint32_t j = 0; j < n_used; j++)
-          if ((uint32_t)to[j] < R) scales[(uint32_t)to[j]] = s.scale;
-    }
-  }
+  };
+  if (__any_sync(0xffffffffu, odd))
+    write(std::true_type{});
+  else
+    write(std::false_type{});
 }
 
 // Rows longer than threads hold, a CTA each: read twice, the second time from the L2.
@@ -227,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) k_i8_quantize_long(const X *x, uint6
     o.load(row + k);
     float f[8];
     o.values(f);
-    const uint2 c = codes8<X>(f, s);
+    const uint2 c = codes8<X, true>(f, s);
     for (uint32_t j = 0; j < (inv ? n_used : 1); j++) {
       const uint64_t r = inv ? (uint64_t)(uint32_t)inv[t * n_used + j] : t;
       if (r < R) *(uint2 *)(codes + r * K + k) = c;
