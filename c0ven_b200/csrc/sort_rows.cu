@@ -18,6 +18,7 @@ namespace {
 constexpr uint32_t kRowsMaxUsed = 16;
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kLongStep = 1024;  // rows
+constexpr uint32_t kFewThreads = 148 * 512;  // a step's, at least
 
 // How a step's rows are dealt to a CTA of 256 threads: 2^log2 neighbouring threads a row; of its octets, groups of eight values, thread i takes i,
 // i + 2^log2 and so on; with several CTAs a row (grid.y) they take turns.
@@ -28,32 +29,39 @@ struct StepRows {
   __device__ uint32_t step() const { return gridDim.y << log2; }
 };
 
-template <class X>
+// U octets of a row at a time, whose loads are on their way together.
+template <class X, uint32_t U>
 __global__ void __launch_bounds__(kThreads) k_sort_rows(const X *x, uint64_t stride, const StepRows map, const int32_t *inv, const float *w, uint32_t n_used, uint32_t R,
                                                         X *xs) {
   dependents_may_launch(), wait_for_predecessors();
   const uint64_t t = map.row(), D = 8ull * map.octets;
   if (t >= map.T) return;
-  for (uint32_t o = map.first(); o < map.octets; o += map.step()) {
-    uint4 raw[sizeof(X) / 2];
+  for (uint32_t o = map.first(); o < map.octets; o += U * map.step()) {
+    uint4 raw[U][sizeof(X) / 2];
 #pragma unroll
-    for (uint32_t i = 0; i < sizeof(X) / 2; i++) raw[i] = ((const uint4 *)(x + t * stride + 8 * o))[i];
-    float v[8];
-    if (w) load8((const X *)raw, v);
+    for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+      for (uint32_t i = 0; i < sizeof(X) / 2; i++)
+        if (o + u * map.step() < map.octets) raw[u][i] = ((const uint4 *)(x + t * stride + 8 * (o + u * map.step())))[i];
 #pragma unroll 4
     for (uint32_t j = 0; j < n_used; j++) {
       const uint32_t r = (uint32_t)inv[t * n_used + j];
       if (r >= R) continue;
-      X *to = xs + r * D + 8 * o;
-      if (w) {
-        const float f = w[t * n_used + j];
-        float u[8];
+      const float f = w ? w[t * n_used + j] : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) u[i] = v[i] * f;
-        store8(to, u);
-      } else {
+      for (uint32_t u = 0; u < U; u++) {
+        if (o + u * map.step() >= map.octets) break;
+        X *to = xs + r * D + 8 * (o + u * map.step());
+        if (w) {
+          float v[8];
+          load8((const X *)raw[u], v);
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(X) / 2; i++) ((uint4 *)to)[i] = raw[i];
+          for (int i = 0; i < 8; i++) v[i] *= f;
+          store8(to, v);
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < sizeof(X) / 2; i++) ((uint4 *)to)[i] = raw[u][i];
+        }
       }
     }
   }
@@ -230,7 +238,8 @@ void with_fours(uint32_t n_used, F &&f) {
 }
 
 // Calls f with the map for a step's rows, and its grid. Rows of more than 32 octets get up to a CTA of threads. most_log2 is for long steps: as many threads a row, that
-// many at most, as leave fewer than an eighth of them idle in a row's last round. What only reads rows does best with a warp a row, which meets at no barrier
+// many at most, as leave fewer than an eighth of them idle in a row's last round, but enough to fill the GPU (1,030 rows of 1,320, twelve places: the combine's gradients
+// 17 us so, 29 with a warp a row). What only reads rows does best with a warp a row, which meets at no barrier
 // (8,192 rows of 2,048 bf16 values, eight places each, dx and dw: 57 us, 59 with 64 threads a row, 62 with 256; of 1,536 44, 46 and 56); what writes them, with as
 // many threads as fit (16,384 of 2,048, ten places: 232 us with 256, 244 with 32; 4,096 of 2,880, six places: 58 with 64, 61 with 256, 64 with 32).
 // whole: a row is one CTA's; else a short step's rows are up to 16 CTAs'.
@@ -242,6 +251,7 @@ void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t most_log2, bool whole,
     auto slots = [&](uint32_t log2) { return (uint64_t)((map.octets + (1u << log2) - 1) >> log2) << log2; };
     uint32_t log2 = std::min(most_log2, map.log2);
     while (log2 > 5 && slots(log2) * 8 > map.octets * 9ull) log2--;
+    while (log2 < map.log2 && (uint64_t)T << log2 < kFewThreads) log2++;
     map.log2 = log2;
   }
   const uint32_t rows = kThreads >> map.log2, rounds = (map.octets + (1u << map.log2) - 1) >> map.log2;
@@ -288,8 +298,12 @@ MOE_API moe_status moe_sort_rows_device(const void *x_dev, uint32_t type, uint64
     with_step_rows(T, n_embd, 8, false, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
-        CUDA_OK(launch_kernel(true, k_sort_rows<X>, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)x_dev, stride ? stride : n_embd, map, inv_dev, w_dev,
-                              n_used, R, (X *)xs_dev));
+        // Octets a thread has of a row: of 16-bit types up to four at a time (13,516 rows of 3,768 weighted bf16 values, three places each, 70 us, one at a time 79; 32,768
+        // of 2,048, one place, 45 and 50), of f32 one (16,384 of 2,048, two places, 66, two at a time 70).
+        const uint32_t mine = (map.octets + (grid.y << map.log2) - 1) / (grid.y << map.log2);
+        const auto kernel = mine == 1 || sizeof(X) == 4 ? k_sort_rows<X, 1> : mine == 2 ? k_sort_rows<X, 2> : k_sort_rows<X, 4>;
+        CUDA_OK(launch_kernel(true, kernel, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)x_dev, stride ? stride : n_embd, map, inv_dev, w_dev, n_used, R,
+                              (X *)xs_dev));
       });
     });
   });
