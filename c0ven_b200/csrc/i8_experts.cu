@@ -88,13 +88,11 @@ struct I8Maps {
   CUtensorMap w, x[kBoxes];
 };
 
-// A form of the kernel: what it makes (GU: h of swiglu(gate, up), else the products), CTAs a unit has, and the most rows of a tile. Its shared memory: stages
+// A form of the kernel: what it makes (GU: h of swiglu(gate, up), else the products), CTAs a unit has, the most rows of a tile, and its groups of four epilogue warps. Its shared memory: stages
 // of bytes; the scales of a tile's rows, an epilogue warp its own; barriers; the experts' first rows and first tiles; the tiles' experts.
-template <bool GU, uint32_t CTAS, uint32_t NT>
+template <bool GU, uint32_t CTAS, uint32_t NT, uint32_t G>
 struct I8Form {
-  // Groups of four epilogue warps. With four of them for pairs (and as many stores and waits on their way) the product of 65,536 rows over 128 experts took 147 us, 134 with
-  // two, 144 with one; gate_up 220, 217 and 226.
-  static constexpr uint32_t kGroups = 2;
+  static constexpr uint32_t kGroups = G;
   static constexpr uint32_t kThreads = 32 * (2 + 4 * kGroups);
   // A stage holds 128 values of the contraction, 128 bytes of a row, of single CTAs twice as many: half the hand-overs where a stage's MMAs are short (100 rows
   // over 512 experts 151 us of gate_up with 128, 145 with 256; pairs 165 with 128, 171 with 256 and half the stages).
@@ -118,10 +116,10 @@ struct I8Form {
 
 enum : uint32_t { kCopyWarp = 0, kMmaWarp = 1, kEpilogueWarp = 2 };
 
-template <class Out, bool GU, uint32_t CTAS, uint32_t NT>
-__global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_product(const __grid_constant__ I8Args a, const __grid_constant__ I8Maps maps) {
+template <class Out, bool GU, uint32_t CTAS, uint32_t NT, uint32_t G>
+__global__ void __launch_bounds__(I8Form<GU, CTAS, NT, G>::kThreads, 1) k_i8_product(const __grid_constant__ I8Args a, const __grid_constant__ I8Maps maps) {
   using namespace tc;
-  using SM = I8Form<GU, CTAS, NT>;
+  using SM = I8Form<GU, CTAS, NT, G>;
   constexpr uint32_t S = SM::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -428,10 +426,10 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT>::kThreads, 1) k_i8_produc
   }
 }
 
-template <class Out, bool GU, uint32_t CTAS, uint32_t NT>
+template <class Out, bool GU, uint32_t CTAS, uint32_t NT, uint32_t G>
 void launch_product(const I8Args &args, const void *wc, const void *xc, cudaStream_t st) {
-  using Form = I8Form<GU, CTAS, NT>;
-  constexpr auto kernel = k_i8_product<Out, GU, CTAS, NT>;
+  using Form = I8Form<GU, CTAS, NT, G>;
+  constexpr auto kernel = k_i8_product<Out, GU, CTAS, NT, G>;
   I8Args a = args;
   int device = 0;
   CUDA_OK(cudaGetDevice(&device));
@@ -468,13 +466,20 @@ void launch_product(const I8Args &args, const void *wc, const void *xc, cudaStre
 // 176 + 97, 24,000 204 + 126 and 179 + 105; 128 of 2,560 x 768, 2,000 rows 80 + 44 and 82 + 46, 3,200 84 + 45 and 83 + 46, skewed by a Zipf law of 1.1 86 + 48 and
 // 83 + 47, 4,800 88 + 51 and 84 + 48. One matrix: 2,080 x 1,440, 200 rows (9 items for pairs) 5.9 and 8.5, 400 (18) 8.7 and 8.7, 777 (36) 11.5 and 9.0; 8,192 x
 // 4,096, 64 rows (32, and 128 for single CTAs) 11.2 and 13.9, 128 rows (32, and 256) 16.9 and 14.6.
+//
+// Two groups of epilogue warps, as more warps' stores and waits stand in the way of the two that bring bytes and issue MMAs (pairs, 65,536 rows over 128 experts of 2,560 x
+// 768: the product 134 us, 147 with four groups, 144 with one); four for gate_up by pairs where the contraction is too short for two to be done beside it
+// (16,384 rows over 32 experts, n_in and features 256 and 128 9.3 us, 11.3 with two; 768 and 384 17.4 and 20.7; 1,280 and 768 33.1 and 34.8; 1,536 and 1,024 46.7 and
+// 47.2; 2,048 and 1,536 85.6 and 85.1, 111 and 102 under load).
 template <class Out, bool GU>
 void launch(const I8Args &a, const void *wc, const void *xc, cudaStream_t st) {
   const uint64_t pieces = (a.N + 255) / 256, tiles = (uint64_t)a.R / 256 + 1, single = ((uint64_t)a.R + 31) / 32 * ((a.N + 127) / 128);
-  if (a.R > 28ull * a.E && pieces * tiles >= 32 && single > 148)
-    launch_product<Out, GU, 2, 256>(a, wc, xc, st);
+  if (a.R <= 28ull * a.E || pieces * tiles < 32 || single <= 148)
+    launch_product<Out, GU, 1, 32, 2>(a, wc, xc, st);
+  else if (GU && a.K <= 1536)
+    launch_product<Out, GU, 2, 256, GU ? 4 : 2>(a, wc, xc, st);
   else
-    launch_product<Out, GU, 1, 32>(a, wc, xc, st);
+    launch_product<Out, GU, 2, 256, 2>(a, wc, xc, st);
 }
 
 I8Args arguments(const moe_i8_weights *w, const float *scales, uint32_t R, const int32_t *offsets) {

@@ -237,20 +237,20 @@ void with_fours(uint32_t n_used, F &&f) {
     f(integral_constant<uint32_t, 4>{});
 }
 
-// Calls f with the map for a step's rows, and its grid. Rows of more than 32 octets get up to a CTA of threads. most_log2 is for long steps: as many threads a row, that
-// many at most, as leave fewer than an eighth of them idle in a row's last round, but enough to fill the GPU (1,030 rows of 1,320, twelve places: the combine's gradients
+// Calls f with the map for a step's rows, and its grid. Rows of more than 32 octets get up to a CTA of threads. least_log2 and most_log2 are for long steps: as many threads a row, within them, as
+// leave fewer than an eighth of them idle in a row's last round, but enough to fill the GPU (1,030 rows of 1,320, twelve places: the combine's gradients
 // 17 us so, 29 with a warp a row). What only reads rows does best with a warp a row, which meets at no barrier
 // (8,192 rows of 2,048 bf16 values, eight places each, dx and dw: 57 us, 59 with 64 threads a row, 62 with 256; of 1,536 44, 46 and 56); what writes them, with as
 // many threads as fit (16,384 of 2,048, ten places: 232 us with 256, 244 with 32; 4,096 of 2,880, six places: 58 with 64, 61 with 256, 64 with 32).
 // whole: a row is one CTA's; else a short step's rows are up to 16 CTAs'.
 template <class F>
-void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t most_log2, bool whole, F &&f) {
+void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t least_log2, uint32_t most_log2, bool whole, F &&f) {
   StepRows map{T, 0, n_embd / 8};
   while (map.log2 < 8 && (1u << map.log2) < map.octets) map.log2++;
   if (T >= kLongStep && map.log2 > 5) {
     auto slots = [&](uint32_t log2) { return (uint64_t)((map.octets + (1u << log2) - 1) >> log2) << log2; };
     uint32_t log2 = std::min(most_log2, map.log2);
-    while (log2 > 5 && slots(log2) * 8 > map.octets * 9ull) log2--;
+    while (log2 > least_log2 && slots(log2) * 8 > map.octets * 9ull) log2--;
     while (log2 < map.log2 && (uint64_t)T << log2 < kFewThreads) log2++;
     map.log2 = log2;
   }
@@ -295,7 +295,7 @@ MOE_API moe_status moe_sort_rows_device(const void *x_dev, uint32_t type, uint64
     need_stride(stride, n_embd, size);
     if (T == 0 || R == 0) return;
     need_device({{x_dev, "x", 16}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {xs_dev, "xs", 16}});
-    with_step_rows(T, n_embd, 8, false, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, type == MOE_TYPE_F32 ? 8 : 5, 8, false, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
         // Octets a thread has of a row: of 16-bit types up to four at a time (13,516 rows of 3,768 weighted bf16 values, three places each, 70 us, one at a time 79; 32,768
@@ -323,7 +323,7 @@ MOE_API moe_status moe_sort_rows_grad_device(const void *dxs_dev, uint32_t type,
     // With R 0 no row of dxs is read: it may be null then.
     need_device({{dxs_dev, "dxs", 16, R == 0}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {x_dev, "x", 16, true}, {add_dev, "add", 16, true}, {dx_dev, "dx", 16, true},
                  {dw_dev, "dw", 4, true}});
-    with_step_rows(T, n_embd, dw_dev ? 5 : 8, dw_dev, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, 5, dw_dev ? 5 : 8, dw_dev, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
         with_fours(n_used, [&](auto q) {
@@ -348,7 +348,7 @@ MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t d
     need(!dy_dev || w_dev, "w is required for dy");
     if (T == 0) return;
     need_device({{dout_dev, "dout", 16}, {y_dev, "y", 16, true}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {dy_dev, "dy", 16, true}, {dw_dev, "dw", 4, true}});
-    with_step_rows(T, n_embd, 8, dw_dev, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd, 5, 8, dw_dev, [&](StepRows map, dim3 grid) {
       with_type(dout_type, [&](auto *g) {
         using G = std::remove_pointer_t<decltype(g)>;
         with_type(y_type, [&](auto *of) {

@@ -426,8 +426,8 @@ MOE_API moe_status moe_sort_rows_grad_device(const void *dxs_dev, uint32_t type,
 
 /* The gradient of moe_combine_rows_device: dy[inv[t][k]] = w[t][k] * dout[t], worked out in f32, and dw[t][k] = the sum over columns of dout[t] * y[inv[t][k]] in f32,
  * 0 for an inv outside 0 .. R - 1; its residual's gradient is dout itself. dout_dev [T][n_embd] of dout_type; y_dev (read for dw alone) and dy_dev [R][n_embd] of
- * y_type; dy_dev or dw_dev may be null: not wanted. dy_dev may be y_dev, where no two entries name a row. Rows no entry names are left as they were (the lists
- * of moe_route_logits_device name all rows before offsets[n_experts]). The same call gives the same bits every time. */
+ * y_type; dy_dev or dw_dev may be null: not wanted. dy_dev may be y_dev, where no two entries name a row. Rows of dy no entry names are left as they were (the
+ * lists of moe_route_logits_device name all rows before offsets[n_experts], each once); one that two name gets either's, or a mixture. The same call gives the same bits every time. */
 MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t dout_type, const void *y_dev, uint32_t y_type, uint32_t R, const int32_t *inv_dev,
                                                 const float *w_dev, uint32_t T, uint32_t n_used, uint32_t n_embd, void *dy_dev, float *dw_dev, void *stream);
 

@@ -224,7 +224,9 @@ def swiglu_near(h, g, u, limit, type):
 @pytest.mark.parametrize("limited", [False, True])
 @pytest.mark.parametrize("E, F, K, counts", [(1, 32, 32, [5]), (1, 64, 96, [1]), (3, 96, 544, [0, 7, 130]), (5, 288, 2880, [16, 15, 0, 33, 1]), (70, 32, 128, [1] * 70),
                                              (1, 544, 160, [1793]), (512, 32, 32, [0, 1] * 256), (1, 32768, 32, [40]), (3, 1056, 1312, [209, 0, 1100]),
-                                             (8, 544, 544, [32, 96, 160, 192, 224, 256, 257, 511]), (2, 4128, 416, [417, 16]), (1, 32, 65536, [2])])
+                                             (8, 544, 544, [32, 96, 160, 192, 224, 256, 257, 511]), (2, 4128, 416, [417, 16]), (1, 32, 65536, [2]),
+                                             # By pairs with a contraction long enough for two groups of epilogue warps.
+                                             (2, 1056, 1696, [600, 217])])
 def test_gate_up(E, F, K, counts, limited, h_type):
     import torch
 
