@@ -2,7 +2,7 @@
 // a row is read once and written to its places, or its places are read four rows at a time and summed. No sum is by atomics, and each has one order.
 // 32,768 rows of 2,048 bf16 values to ten places each 234 us (6.3 TB/s); the combine's gradients of 16,384 such rows 235 (6.3); rows' and weights' gradients of 3,521
 // rows of 2,560 f16 values, eight places each, 31.5 (5.2), of 8,192 of 2,048 bf16 57 (5.9), rows' alone 50 (6.0); of 90,000 rows of 64 29 (3.9). 13 rows of 2,560 f32
-// values to eight places each 2.6 us.
+// values to eight places each 1.8 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -29,20 +29,20 @@ struct StepRows {
   __device__ uint32_t step() const { return gridDim.y << log2; }
 };
 
-// U octets of a row at a time, whose loads are on their way together.
+// Here the map's octets are pieces of 16 bytes, so that neighbouring threads store neighbouring ones (of f32 rows two pieces a thread, every other one at a time, took 74 us
+// of 7,787 rows of 768, eleven places each, where this takes 47). U of them at a time, whose loads are on their way together.
 template <class X, uint32_t U>
 __global__ void __launch_bounds__(kThreads) k_sort_rows(const X *x, uint64_t stride, const StepRows map, const int32_t *inv, const float *w, uint32_t n_used, uint32_t R,
                                                         X *xs) {
   dependents_may_launch(), wait_for_predecessors();
-  const uint64_t t = map.row(), D = 8ull * map.octets;
+  constexpr uint32_t V = 16 / sizeof(X);
+  const uint64_t t = map.row(), D = (uint64_t)V * map.octets;
   if (t >= map.T) return;
   for (uint32_t o = map.first(); o < map.octets; o += U * map.step()) {
-    uint4 raw[U][sizeof(X) / 2];
+    uint4 raw[U];
 #pragma unroll
     for (uint32_t u = 0; u < U; u++)
-#pragma unroll
-      for (uint32_t i = 0; i < sizeof(X) / 2; i++)
-        if (o + u * map.step() < map.octets) raw[u][i] = ((const uint4 *)(x + t * stride + 8 * (o + u * map.step())))[i];
+      if (o + u * map.step() < map.octets) raw[u] = *(const uint4 *)(x + t * stride + V * (o + u * map.step()));
 #pragma unroll 4
     for (uint32_t j = 0; j < n_used; j++) {
       const uint32_t r = (uint32_t)inv[t * n_used + j];
@@ -51,16 +51,18 @@ __global__ void __launch_bounds__(kThreads) k_sort_rows(const X *x, uint64_t str
 #pragma unroll
       for (uint32_t u = 0; u < U; u++) {
         if (o + u * map.step() >= map.octets) break;
-        X *to = xs + r * D + 8 * (o + u * map.step());
-        if (w) {
+        X *to = xs + r * D + V * (o + u * map.step());
+        if (!w) {
+          *(uint4 *)to = raw[u];
+        } else if constexpr (V == 4) {
+          const float4 v = *(const float4 *)&raw[u];
+          *(float4 *)to = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+        } else {
           float v[8];
-          load8((const X *)raw[u], v);
+          load8((const X *)&raw[u], v);
 #pragma unroll
           for (int i = 0; i < 8; i++) v[i] *= f;
           store8(to, v);
-        } else {
-#pragma unroll
-          for (uint32_t i = 0; i < sizeof(X) / 2; i++) ((uint4 *)to)[i] = raw[u][i];
         }
       }
     }
@@ -237,12 +239,12 @@ void with_fours(uint32_t n_used, F &&f) {
     f(integral_constant<uint32_t, 4>{});
 }
 
-// Calls f with the map for a step's rows, and its grid. Rows of more than 32 octets get up to a CTA of threads. least_log2 and most_log2 are for long steps: as many threads a row, within them, as
-// leave fewer than an eighth of them idle in a row's last round, but enough to fill the GPU (1,030 rows of 1,320, twelve places: the combine's gradients
-// 17 us so, 29 with a warp a row). What only reads rows does best with a warp a row, which meets at no barrier
-// (8,192 rows of 2,048 bf16 values, eight places each, dx and dw: 57 us, 59 with 64 threads a row, 62 with 256; of 1,536 44, 46 and 56); what writes them, with as
-// many threads as fit (16,384 of 2,048, ten places: 232 us with 256, 244 with 32; 4,096 of 2,880, six places: 58 with 64, 61 with 256, 64 with 32).
-// whole: a row is one CTA's; else a short step's rows are up to 16 CTAs'.
+// Calls f with the map for a step's rows, and its grid. Rows of more than 32 octets get up to a CTA of threads. least_log2 and most_log2 are for long steps: as many
+// threads a row, within them, as leave fewer than an eighth of them idle in a row's last round, but enough to fill the GPU (1,030 rows of 1,320, twelve places: the
+// combine's gradients 17 us so, 29 with a warp a row). What only reads rows does best with a warp a row, which meets at no barrier (8,192 rows of 2,048 bf16 values, eight
+// places each, dx and dw: 57 us, 59 with 64 threads a row, 62 with 256; of 1,536 44, 46 and 56); the combine's gradients, which write them too, with as many threads as
+// fit (16,384 of 2,048, ten places: 232 us with 256, 244 with 32; 4,096 of 2,880, six places: 58 with 64, 61 with 256, 64 with 32); sorting with 256 whatever is
+// idle (3,163 of 1,776 bf16 values, thirteen places: 28.6 us, 35.6 with 32). whole: a row is one CTA's; else a short step's rows are up to 16 CTAs'.
 template <class F>
 void with_step_rows(uint32_t T, uint32_t n_embd, uint32_t least_log2, uint32_t most_log2, bool whole, F &&f) {
   StepRows map{T, 0, n_embd / 8};
@@ -295,13 +297,13 @@ MOE_API moe_status moe_sort_rows_device(const void *x_dev, uint32_t type, uint64
     need_stride(stride, n_embd, size);
     if (T == 0 || R == 0) return;
     need_device({{x_dev, "x", 16}, {inv_dev, "inv", 4}, {w_dev, "w", 4, true}, {xs_dev, "xs", 16}});
-    with_step_rows(T, n_embd, type == MOE_TYPE_F32 ? 8 : 5, 8, false, [&](StepRows map, dim3 grid) {
+    with_step_rows(T, n_embd / 2 * size, 8, 8, false, [&](StepRows map, dim3 grid) {
       with_type(type, [&](auto *of) {
         using X = std::remove_pointer_t<decltype(of)>;
-        // Octets a thread has of a row: of 16-bit types up to four at a time (13,516 rows of 3,768 weighted bf16 values, three places each, 70 us, one at a time 79; 32,768
-        // of 2,048, one place, 45 and 50), of f32 one (16,384 of 2,048, two places, 66, two at a time 70).
+        // Pieces a thread has of a row, up to four at a time (13,516 rows of 3,768 weighted bf16 values, three places each, 70 us, one at a time 79; 32,768 of 2,048, one
+        // place, 45 and 50).
         const uint32_t mine = (map.octets + (grid.y << map.log2) - 1) / (grid.y << map.log2);
-        const auto kernel = mine == 1 || sizeof(X) == 4 ? k_sort_rows<X, 1> : mine == 2 ? k_sort_rows<X, 2> : k_sort_rows<X, 4>;
+        const auto kernel = mine == 1 ? k_sort_rows<X, 1> : mine == 2 ? k_sort_rows<X, 2> : k_sort_rows<X, 4>;
         CUDA_OK(launch_kernel(true, kernel, grid, dim3(kThreads), 0, (cudaStream_t)stream, (const X *)x_dev, stride ? stride : n_embd, map, inv_dev, w_dev, n_used, R,
                               (X *)xs_dev));
       });
