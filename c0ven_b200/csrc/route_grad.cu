@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8
   auto column = [&](int v) { return v / W * 32 * W + lane * W + v % W; };
 #pragma unroll
   for (int v = 0; v < V; v++) row[column(v)] = 0.0f;
+  __syncwarp();
   // An assignment a lane, and for softmax weights as they are the row's logits: of the warp's next row while this one is worked on.
   uint32_t id = 0xFFFFFFFFu;
   float d = 0.0f, l = -INFINITY, z[DENSE ? V : 1];
