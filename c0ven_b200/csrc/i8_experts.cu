@@ -109,6 +109,7 @@ struct I8Form {
   static constexpr uint32_t kBytes = kTileRows + 2 * kMaxExperts + 1024;  // and room to align the base to 1024
   static_assert(kBytes <= 227 * 1024, "a CTA's shared memory");
   static_assert(2 * kThreads > kMaxExperts, "two experts a thread");
+  static_assert(kThreads / 32 * 4 <= kBarriers - kRowScales, "a word a warp in the scales' room");
   static constexpr uint32_t kCols = 2 * NT;  // of tensor memory: two accumulators
   static_assert(kCols <= 512 && (kCols & (kCols - 1)) == 0 && kCols >= 32, "tensor memory");
   static_assert(NT % (kChunk * kGroups) == 0, "a group's chunks");
@@ -137,7 +138,8 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT, G>::kThreads, 1) k_i8_pro
   uint32_t *first_row = (uint32_t *)(smem + SM::kTables), *first_tile = first_row + kMaxExperts + 1;  // [E + 1] each
   uint16_t *tile_expert = (uint16_t *)(smem + SM::kTileExperts);
   uint16_t *tile_rows = (uint16_t *)(smem + SM::kTileRows);  // an expert's tiles' rows, but for its last
-  uint32_t *warp_part = (uint32_t *)smem;  // before the stages come
+  // The warps' sums of tiles, before the scales come: where no copy writes, as one was seen to overtake ordinary reads that only a barrier stands behind.
+  uint32_t *warp_part = (uint32_t *)(smem + SM::kRowScales);
   uint32_t *error = (uint32_t *)abort;     // the waits' error word: the flag itself
 
   if (tid == 0) {
