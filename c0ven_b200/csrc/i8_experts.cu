@@ -70,8 +70,6 @@ __device__ __forceinline__ Two swiglu_any(const Two &g, const Two &u) {
   return Two(g.lo() < kFarGate ? swiglu_far(g.lo(), u.lo()) : h.lo(), g.hi() < kFarGate ? swiglu_far(g.hi(), u.hi()) : h.hi());
 }
 
-__device__ uint32_t g_gave_up;  // CTAs that gave up a wait, ever
-
 struct I8Args {
   const float *ws, *xs;  // scales of the matrices' rows and of the rows
   const int32_t *offsets;
@@ -79,6 +77,7 @@ struct I8Args {
   uint32_t items_per_tile;  // items that share a tile of rows
   float limit;
   void *y;
+  uint32_t *gave_up;  // the device's count
 };
 
 // Maps over the bytes of the matrices and, in boxes of 16, 32, 64 and 128 rows, of the rows.
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(I8Form<GU, CTAS, NT, G>::kThreads, 1) k_i8_pro
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort) atomicAdd(&g_gave_up, 1u);
+  if (tid == 0 && *abort) atomicAdd(a.gave_up, 1u);
   if constexpr (CTAS == 2) cluster_sync();  // neither CTA leaves while the other may still read its shared memory or write its tensor memory
   if (warp == kMmaWarp) {
     __syncwarp();
@@ -435,6 +434,7 @@ void launch_product(const I8Args &args, const void *wc, const void *xc, cudaStre
   I8Args a = args;
   int device = 0;
   CUDA_OK(cudaGetDevice(&device));
+  a.gave_up = gave_up_count(device);
   constexpr size_t smem = Form::kBytes;
   static std::atomic<uint32_t> done{0};
   CUDA_OK(ensure_dynamic_smem(kernel, smem, done, device));
@@ -509,13 +509,6 @@ void call(const I8Args &a, const moe_i8_weights *w, const void *codes, uint32_t 
 }
 
 }  // namespace
-
-uint32_t i8_gave_up(cudaStream_t st, uint32_t timeout_ms) {
-  uint32_t n = 0;
-  CUDA_OK(cudaMemcpyFromSymbolAsync(&n, g_gave_up, sizeof n, 0, cudaMemcpyDeviceToHost, st));
-  Stream::wait_on(st, timeout_ms);
-  return n;
-}
 
 }  // namespace moe
 

@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <map>
 #include <type_traits>
@@ -646,7 +647,31 @@ Mx4Args arguments(const moe_mx4_weights *w, const void *scales, uint32_t R, cons
   return a;
 }
 
+// A stream of the current device for moe_ops_status alone, made when it first asks: no work of a caller's ever stands before a copy on it.
+cudaStream_t status_stream(int device) {
+  static std::atomic<cudaStream_t> made[64];
+  if (device < 0 || device >= 64) throw CudaFailure(cudaErrorInvalidDevice, "a device past the 64th");
+  cudaStream_t known = made[device].load(std::memory_order_acquire);
+  if (known) return known;
+  cudaStream_t mine = nullptr;
+  CUDA_OK(cudaStreamCreateWithFlags(&mine, cudaStreamNonBlocking));
+  if (made[device].compare_exchange_strong(known, mine)) return mine;
+  cudaStreamDestroy(mine);  // another thread's came first
+  return known;
+}
+
 }  // namespace
+
+uint32_t *gave_up_count(int device) {
+  static std::atomic<uint32_t *> known[64];
+  if (device < 0 || device >= 64) throw CudaFailure(cudaErrorInvalidDevice, "a device past the 64th");
+  uint32_t *at = known[device].load(std::memory_order_acquire);
+  if (at) return at;
+  CUDA_OK(cudaGetSymbolAddress((void **)&at, g_gave_up));
+  known[device].store(at, std::memory_order_release);
+  return at;
+}
+
 }  // namespace moe
 
 using namespace moe;
@@ -688,10 +713,10 @@ MOE_API moe_status moe_ops_status(uint32_t timeout_ms, void *stream) {
     Stream::wait_on(st, timeout_ms);
     int device = 0;
     CUDA_OK(cudaGetDevice(&device));
+    // The one wait is above: this copy, to pageable memory, returns when it is done, and waits for nothing. On st it would wait for what other threads have queued
+    // there by now, and for the default stream's work where the two wait for one another.
     uint32_t gave_up = 0;
-    CUDA_OK(cudaMemcpyFromSymbolAsync(&gave_up, g_gave_up, sizeof gave_up, 0, cudaMemcpyDeviceToHost, st));
-    Stream::wait_on(st, timeout_ms);
-    gave_up += i8_gave_up(st, timeout_ms);
+    CUDA_OK(cudaMemcpyAsync(&gave_up, gave_up_count(device), sizeof gave_up, cudaMemcpyDeviceToHost, status_stream(device)));
     if (!gave_up) return;
     // What this thread was told about the stream last. Nothing is cleared: others hear of the same products.
     thread_local std::map<std::pair<int, cudaStream_t>, uint32_t> told;

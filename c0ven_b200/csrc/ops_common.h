@@ -15,8 +15,8 @@ namespace moe {
 
 std::string &ops_error();  // the calling thread's
 
-// CTAs of products of 8-bit rows that gave up a wait on the current device, ever; waits for st.
-uint32_t i8_gave_up(cudaStream_t st, uint32_t timeout_ms);
+// Where the current device, whose ordinal device is, counts the products' CTAs that gave up a wait, ever: one count for all kinds of products.
+uint32_t *gave_up_count(int device);
 
 inline void need(bool ok, const char *what) {
   if (!ok) throw BadArgument(what);

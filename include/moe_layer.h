@@ -476,7 +476,7 @@ MOE_API moe_status moe_i8_gate_up_device(const moe_i8_weights *w, const void *co
 /* Waits for stream, timeout_ms at most (0: 60 s). MOE_TIMEOUT when that ran out, or when a product on the current device, on any stream, has given up one
  * of its own waits (each bounded, about a second) since the calling thread last asked about this stream: products' results since then are not to be used.
  * Every thread is told for every stream that it asks about, each once; a thread that has not asked about a stream before is told of all there
- * ever were. Not while stream is captured.
+ * ever were. Not while stream is captured. It waits for stream's work alone, and keeps a stream of its own on each device from its first call there on.
  * moe_ops_note_give_up: counts one, queued on stream, as a product that gave up would, for tests of a caller's handling. */
 MOE_API moe_status moe_ops_status(uint32_t timeout_ms, void *stream);
 MOE_API moe_status moe_ops_note_give_up(void *stream);
