@@ -56,6 +56,8 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 // e^(l - top), the largest's own 1 even where it is infinite; 0 for an expert that is out.
 __device__ __forceinline__ float part_of(float l, float top) { return l == -INFINITY ? 0.0f : l == top ? 1.0f : expf(l - top); }
+// f d, 0 for a factor that vanished whatever d is: a weight's gradient that is no number reaches no expert by a share of 0.
+__device__ __forceinline__ float weighed(float f, float d) { return f != 0.0f ? f * d : 0.0f; }
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -164,13 +166,13 @@ __global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8
       float c[V];
 #pragma unroll
       for (int v = 0; v < V; v++) c[v] = row[column(v)];
-      if (odd) {  // a weight's gradient that is no number reaches those its expert's share does
+      if (odd) {  // a weight's gradient that is no number reaches those that its expert's share does
         float m = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; v++) m += y[v] > 0.0f ? y[v] * c[v] : 0.0f;
         const float mean = sum > 0.0f ? warp_sum(m) / sum : 0.0f;
 #pragma unroll
-        for (int v = 0; v < V; v++) y[v] = y[v] > 0.0f ? a.scale / sum * y[v] * (c[v] - mean) : 0.0f;
+        for (int v = 0; v < V; v++) y[v] = y[v] > 0.0f ? weighed(a.scale / sum * y[v], c[v] - mean) : 0.0f;
       } else {
 #pragma unroll
         for (int v = 0; v < V; v += 2) part = fma(Two(y[v], y[v + 1]), Two(c[v], c[v + 1]), part);
@@ -198,9 +200,9 @@ __global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8
       if (a.renorm) {
         const float total = warp_sum(p);
         p = total > 0.0f ? p / total : 0.0f;
-        g -= warp_sum(p * g);
+        g -= warp_sum(weighed(p, g));
       }
-      if (e < a.E) row[e] = a.scale * p * rest * g;
+      if (e < a.E) row[e] = weighed(a.scale * p * rest, g);
       __syncwarp();
 #pragma unroll
       for (int v = 0; v < V; v++) y[v] = row[column(v)];

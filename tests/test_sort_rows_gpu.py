@@ -467,3 +467,47 @@ def test_a_block_that_trains(T, score):
     close(dl.double().T @ x.double(), WR.grad, 2.0 ** -16)
     close(m1.grad, W1.grad, 2.0 ** -16)
     close(m2.grad, W2.grad, 2.0 ** -16)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_odd_weights_gradients_reach_no_vanished_share(score, renorm):
+    """Infinities and NaN in the weights' gradients of experts whose factor is 0 in f32 reach nothing; in the others what the formulas make of them."""
+    import torch
+
+    T, E, n = 6, 40, 3
+    l = np.full((T, E), -300.0, np.float32)
+    ids = np.tile(np.array([3, 17, 8], np.int32), (T, 1))
+    l[:, 3] = [0.5, 0.5, 200, 200, -150, 0.5]    # by sigmoids 200 is 1 - s of 0
+    l[:, 17] = [-200, 0.25, 0, 200, -152, 0.25]  # by softmax 200 apart is a share of 0
+    l[:, 8] = [-200, 0, -200, 200, -400, -200]
+    odd = np.array([[1, np.inf, np.nan], [1, np.inf, 2], [np.nan, 1, -np.inf], [np.inf, 1, 2], [1, 2, np.nan], [-1, 3, np.nan]], np.float32)
+    dl, di, dd, out = dev(l), dev(ids), dev(odd), torch.full((T, E), 7.0, device="cuda")
+    ops.route_logits_grad_device(dl.data_ptr(), ops.F32, T, E, n, di.data_ptr(), dd.data_ptr(), out.data_ptr(), score=TYPES_OF_SCORE[score], renorm=renorm)
+    l64, d64, want = l.astype(np.float64), odd.astype(np.float64), np.zeros((T, E))
+    small = 2.0 ** -150  # half of f32's least number: all factors here are far above it or below
+
+    def share(p):
+        return np.where(p < small, 0.0, p)
+
+    for t in range(T):
+        lc, factor, p = l64[t, ids[t]], np.ones(n), None
+        if score == "softmax":
+            of = lc if renorm else l64[t]
+            p = share(np.exp(of - of.max()) / np.exp(of - of.max()).sum())
+        else:
+            factor = share(np.exp(-np.logaddexp(0, lc)))
+            s = -np.logaddexp(0, -lc)
+            p = share(np.exp(s - s.max()) / np.exp(s - s.max()).sum()) if renorm else share(np.exp(s))
+        dense = score == "softmax" and not renorm
+        d = np.zeros(E) if dense else d64[t]
+        if dense:
+            d[ids[t]] = d64[t]
+        with np.errstate(invalid="ignore"):
+            mean = np.where(p > 0, p * d, 0.0)[p > 0].sum() if score == "softmax" or renorm else 0.0
+            v = np.where(p > 0, p, 0.0) * (factor if not dense else 1.0)
+            v = np.where(v > 0, v * (d - mean), 0.0)
+        want[t, slice(None) if dense else ids[t]] = v
+    got = host(out)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), (got[:, [3, 17, 8]], want[:, [3, 17, 8]])
+    assert np.allclose(got, want, rtol=2.0 ** -18, atol=2.0 ** -20, equal_nan=True)
