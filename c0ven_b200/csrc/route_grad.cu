@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8
         top = fmaxf(top, y[v]);
       }
       if (e < a.E) row[e] = g;
-      const bool odd = __any_sync(0xffffffffu, !(fabsf(g) < INFINITY));
+      const bool odd = __any_sync(0xffffffffu, !(fabsf(g) < 1e30f));
       if (t + step < a.T) bring(t + step);
       top = warp_max(top);
       if (top == INFINITY) {  // those alone share the row
@@ -166,11 +166,11 @@ __global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8
       float c[V];
 #pragma unroll
       for (int v = 0; v < V; v++) c[v] = row[column(v)];
-      if (odd) {  // a weight's gradient that is no number reaches those that its expert's share does
+      if (odd) {  // a weight's gradient that is no number reaches those that its expert's share does; one so large is weighed before it is summed
         float m = 0.0f;
 #pragma unroll
-        for (int v = 0; v < V; v++) m += y[v] > 0.0f ? y[v] * c[v] : 0.0f;
-        const float mean = sum > 0.0f ? warp_sum(m) / sum : 0.0f;
+        for (int v = 0; v < V; v++) m += y[v] > 0.0f ? y[v] / sum * c[v] : 0.0f;
+        const float mean = warp_sum(m);
 #pragma unroll
         for (int v = 0; v < V; v++) y[v] = y[v] > 0.0f ? weighed(a.scale / sum * y[v], c[v] - mean) : 0.0f;
       } else {

@@ -435,8 +435,8 @@ MOE_API moe_status moe_combine_rows_grad_device(const void *dout_dev, uint32_t d
  * weigh, and have no gradient): dlogits[t][e] = the sum over k of dw[t][k] * the derivative of w[t][k] by logits[t][e]. config, logits_dev, stride, bias_dev and
  * T are that call's, ids_dev [T][n_used] what it gave (a row's ids differ; one outside 0 .. n_experts - 1 counts for nothing, whatever its dw); groups do not
  * matter. dlogits_dev T rows of n_experts values of logits_type, dlogits_stride values apart (0: n_experts), every one written: 0 for experts that are out and, but
- * for a softmax without renormalisation, for those not chosen. Worked out in f32 and rounded once. A dw that is infinite or NaN reaches no expert by a factor that is
- * 0 in f32 (a share of scores so far apart, a sigmoid so near 1): such an expert's part of the sums, and its gradient, are 0. */
+ * for a softmax without renormalisation, for those not chosen. Worked out in f32 and rounded once. Whatever dw is, infinite or NaN,
+ * an expert whose share is 0 in f32 (scores so far apart) adds nothing to the sums, and one whose share or 1 - s (a sigmoid so near 1) is 0 has the gradient 0. */
 MOE_API moe_status moe_route_logits_grad_device(const moe_route_config *config, const void *logits_dev, uint64_t stride, const float *bias_dev, uint32_t T,
                                                 const int32_t *ids_dev, const float *dw_dev, void *dlogits_dev, uint64_t dlogits_stride, void *stream);
 

@@ -511,3 +511,16 @@ def test_odd_weights_gradients_reach_no_vanished_share(score, renorm):
     got = host(out)
     assert np.array_equal(np.isnan(got), np.isnan(want)), (got[:, [3, 17, 8]], want[:, [3, 17, 8]])
     assert np.allclose(got, want, rtol=2.0 ** -18, atol=2.0 ** -20, equal_nan=True)
+
+
+def test_weights_gradients_as_large_as_f32_holds():
+    """A softmax as it is: shares times gradients whose sum f32 does not hold before it is divided by the row's sum of exponentials."""
+    import torch
+
+    E = 64
+    l, ids, dw = torch.zeros((2, E), device="cuda"), dev(np.array([[1, 2, 40], [0, 3, 63]], np.int32)), torch.full((2, 3), 3e38, device="cuda")
+    dw[1, 1] = 1e38
+    out = torch.empty((2, E), device="cuda")
+    ops.route_logits_grad_device(l.data_ptr(), ops.F32, 2, E, 3, ids.data_ptr(), dw.data_ptr(), out.data_ptr(), renorm=False)
+    want, _ = M.route_grad(host(l), ids.cpu().numpy(), dw.double().cpu().numpy(), "softmax", False, 1.0)
+    assert np.allclose(host(out), want, rtol=2.0 ** -18, atol=0)
