@@ -56,6 +56,9 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 // e^(l - top), the largest's own 1 even where it is infinite; 0 for an expert that is out.
 __device__ __forceinline__ float part_of(float l, float top) { return l == -INFINITY ? 0.0f : l == top ? 1.0f : expf(l - top); }
+constexpr float kLog2e = 1.4426950408889634f;
+// A row's largest logit from which on its product with log2(e) might be rounded by what 2^ of passes f32: by 1/16 below.
+constexpr float kFarTop = 0x1p20f;
 // f d, 0 for a factor that vanished whatever d is: a weight's gradient that is no number reaches no expert by a share of 0.
 __device__ __forceinline__ float weighed(float f, float d) { return f != 0.0f ? f * d : 0.0f; }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -135,8 +138,9 @@ __global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8
     const uint32_t e = id;
     float y[V], g = d;
     if constexpr (DENSE) {
-      // An expert that is out, NaN among them, counts as -infinity. The exponentials are approximate, off by 2^-22 and by what the argument's two roundings
-      // make of it, a part in 2^23 of l - top: as much as rounding l - top alone does to an accurate one.
+      // An expert that is out, NaN among them, counts as -infinity. The exponentials are 2^(l log2(e) - top log2(e)), approximate, off by 2^-22 and by the argument's one
+      // rounding and its factor's, 1.22 parts in 2^24 of l - top: some more than rounding l - top does to an accurate one. How the second product was rounded is
+      // one factor of the whole row, which its shares do not have.
       float top = -INFINITY;
 #pragma unroll
       for (int v = 0; v < V; v++) {
@@ -148,15 +152,16 @@ __global__ void __launch_bounds__(32 * kWarps, DENSE ? grad_ctas<V, DENSE>() : 8
       const bool odd = __any_sync(0xffffffffu, !(fabsf(g) < 1e30f));
       if (t + step < a.T) bring(t + step);
       top = warp_max(top);
-      if (top == INFINITY) {  // those alone share the row
+      if (!(fabsf(top) < kFarTop)) {
 #pragma unroll
-        for (int v = 0; v < V; v++) y[v] = y[v] == INFINITY ? 0.0f : -INFINITY;
+        for (int v = 0; v < V; v++) y[v] = top == INFINITY ? (y[v] == INFINITY ? 0.0f : -INFINITY) : top == -INFINITY ? y[v] : y[v] - top;  // infinite ones alone share the row
+        top = 0.0f;
       }
-      const Two less(fabsf(top) < INFINITY ? -top : 0.0f), log2e(1.4426950408889634f);
+      const Two log2e(kLog2e), less(-top * kLog2e);
       Two total(0.0f);
 #pragma unroll
       for (int v = 0; v < V; v += 2) {
-        const Two p = (Two(y[v], y[v + 1]) + less) * log2e;
+        const Two p = fma(Two(y[v], y[v + 1]), log2e, less);
         y[v] = exp2_approx(p.lo()), y[v + 1] = exp2_approx(p.hi());
         total = total + Two(y[v], y[v + 1]);
       }

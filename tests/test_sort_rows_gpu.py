@@ -524,3 +524,28 @@ def test_weights_gradients_as_large_as_f32_holds():
     ops.route_logits_grad_device(l.data_ptr(), ops.F32, 2, E, 3, ids.data_ptr(), dw.data_ptr(), out.data_ptr(), renorm=False)
     want, _ = M.route_grad(host(l), ids.cpu().numpy(), dw.double().cpu().numpy(), "softmax", False, 1.0)
     assert np.allclose(host(out), want, rtol=2.0 ** -18, atol=0)
+
+
+@pytest.mark.parametrize("shift", [0.0, 1000.0, -1000.0, 3e6])
+def test_small_shares_by_one_rounding_of_their_exponents(shift):
+    """Softmax weights as they are, f32, a chosen expert so far above the others that the row's sum is its exponential alone, and dw 1: a gradient is the share itself, off by
+    its exponent's one rounding (in units of log 2, so half a step of numbers from 64 on), by log2(e)'s own to f32, 1.34e-8 of it, by two approximate exponentials of 2^-22, a
+    quotient and a product. Of rows whose logits are all beyond 2^20 the difference itself is rounded first: half a step more."""
+    import torch
+
+    rng = np.random.default_rng(21)
+    T, E = 128, 512
+    l = (rng.uniform(-63, -46, (T, E)) + shift).astype(np.float32)
+    top = rng.integers(0, E, T)
+    l[np.arange(T), top] = (rng.uniform(0, 1, T) + shift).astype(np.float32)
+    dl, di, dd, out = dev(l), dev(top.astype(np.int32)[:, None]), torch.ones((T, 1), device="cuda"), torch.empty((T, E), device="cuda")
+    ops.route_logits_grad_device(dl.data_ptr(), ops.F32, T, E, 1, di.data_ptr(), dd.data_ptr(), out.data_ptr(), renorm=False)
+    want, _ = M.route_grad(l.astype(np.float64), top[:, None], np.ones((T, 1)), "softmax", False, 1.0)
+    rest = np.ones((T, E), bool)
+    rest[np.arange(T), top] = False
+    d = (l[np.arange(T), top].astype(np.float64)[:, None] - l)[rest]
+    arg = d * np.log2(np.e)
+    assert arg.min() > 65 and arg.max() < 127  # a step is 2^-17
+    bound = np.log(2) * 2.0 ** -18 + 1.34e-8 * d + 2 * 2.0 ** -22 + 4 * U + (2.0 ** -19 if shift > 2 ** 20 else 0.0)
+    off = np.abs(host(out)[rest] / want[rest] - 1)
+    assert (off <= bound).all(), (off / bound).max()
