@@ -328,7 +328,9 @@ MOE_API const char *moe_route_rows_static_error(void);
  * default stream) without waiting, so a call can be captured into a graph. The first call of each on a device sets
  * kernel attributes; that may happen during a capture too. Calls with different buffers may overlap. T or R of 0 is a
  * call with nothing to do (offsets become 0). A call's outputs share no bytes with its inputs or with one another, but for
- * moe_combine_rows_device's residual. moe_ops_error: the calling thread's last message from any of them.
+ * those that may be one of its inputs as a whole: moe_combine_rows_device's out_dev its residual_dev, moe_sort_rows_grad_device's dx_dev its add_dev,
+ * moe_combine_rows_grad_device's dy_dev its y_dev. Where a call says no less, T and R are below 2^31, strides below 2^32 and n_embd is at most 2^24.
+ * moe_ops_error: the calling thread's last message from any of them.
  *
  * MX rows: values in blocks of 32 along the row, a value an e2m1 code (sign, 0 0.5 1 1.5 2 3 4 6), a block one e8m0 scale
  * byte (2^(byte - 127); 255: the block is NaN). codes [rows][K / 2]: value 2i in the low half of byte i, 2i + 1 in the high

@@ -2,6 +2,7 @@
 import ctypes as C
 import importlib.util
 import os
+import re
 
 import numpy as np
 import pytest
@@ -199,3 +200,19 @@ def test_the_plain_forms_agree_with_the_cases_plain_forms():
     assert np.array_equal(g, M.gathered(rows, inv).astype(np.float32))
     s = cases._scattered(torch.from_numpy(inv), torch.from_numpy(w[..., None] * dout[:, None]), 4).numpy()
     assert np.array_equal(s, M.sort(dout, inv, w, np.zeros((4, 8), np.float32)))
+
+
+def test_the_header_says_what_may_be_in_place_and_how_far_numbers_go():
+    """The operators' general rule on shared bytes names every output that a call's own text lets be an input, and the limits that the calls hold to."""
+    header = open(os.path.join(os.path.dirname(__file__), "..", "include", "moe_layer.h")).read()
+    part = header[header.index("/* Operators without a layer"):]
+    rule, rest = part.split("*/", 1)
+    rule, texts = " ".join(rule.replace("\n *", " ").split()), re.findall(r"/\*(.*?)\*/", rest, re.S)
+    allowed = [pair for t in texts for pair in re.findall(r"(\w+_dev) may be (\w+_dev)", t)]
+    assert len(allowed) == 3
+    for out, of in allowed:
+        assert f"{out} its {of}" in rule, (out, of)
+    for limit, args in (("T and R are below 2^31", dict(T=1 << 31)), ("T and R are below 2^31", dict(R=1 << 31)), ("strides below 2^32", dict(stride=1 << 32)),
+                        ("n_embd is at most 2^24", dict(n_embd=(1 << 24) + 8))):
+        assert limit in rule
+        refused(lambda: ops.sort_rows_device(**(SORT | args)))
