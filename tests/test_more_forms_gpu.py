@@ -34,3 +34,59 @@ def test_route_grad_of_more_rows_than_warps(T, E, n, score, renorm, type):
     ops.route_logits_grad_device(l.data_ptr(), TYPES[type], T, E, n, ids.data_ptr(), dd.data_ptr(), out.data_ptr(), score=S.TYPES_OF_SCORE[score], renorm=renorm, scale=2.5)
     S.check_route_grad(S.host(out[:T]), S.host(l), ids.cpu().numpy(), dw, score, renorm, 2.5, type)
     assert (out[T] == 7.0).all()
+
+
+# --- gradients by 16 and by 32 threads a row ------------------------------------------------------------------------------
+
+
+def additions(D):
+    """Of a sum over D columns one after another, at most: a thread's share, by 32 threads a row at least where there are as many octets, and exchanges after it."""
+    octets = D // 8
+    threads = min(32, 1 << max(0, (octets - 1).bit_length()))
+    return 8 * -(-octets // threads) + 5 + 8
+
+
+def gathered64(rows, inv):
+    """rows[inv] on the device, zeros where an entry names none: [T][n][D]."""
+    import torch
+
+    there = (inv >= 0) & (inv < len(rows))
+    return torch.where(there[..., None], rows.double()[torch.where(there, inv, 0).long()], torch.zeros((), dtype=torch.float64, device="cuda"))
+
+
+# Rows of 17 to 32 octets by 32 threads; so the rows' and weights' gradients of longer rows from 2,368 rows on, and all gradients where no more threads fit
+# (264, 1,032 and 1,320 columns of 2,368 rows and more). Rows of 9 to 16 octets by 16.
+HALF_AND_WHOLE_WARPS = [(2370, 3, 2560), (2370, 8, 2560), (2368, 11, 2560), (2369, 16, 2560), (2400, 2, 264), (2401, 16, 1032), (2500, 7, 1320), (37, 4, 136), (51, 10, 200),
+                        (9, 13, 256), (1501, 6, 256), (50, 1, 72), (33, 16, 128), (5003, 5, 72), (1501, 9, 128)]
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T, n, D", HALF_AND_WHOLE_WARPS)
+def test_gradients_by_half_and_whole_warps(T, n, D, type):
+    import torch
+
+    rng = np.random.default_rng(T + n + D)
+    g = torch.Generator(device="cuda").manual_seed(T + n)
+    rows = max(1, T * n - T * n // 7)
+    randn = lambda s, t=type: torch.randn(s, generator=g, device="cuda").to(S.dtype(t))  # noqa: E731
+    inv = S.dev(S.places(rng, T, n, rows))
+    x, dxs, y, dout, w = randn((T, D)), randn((rows, D)), randn((rows, D)), randn((T, D), "f32"), randn((T, n), "f32")
+    dx, dw = torch.full((T + 1, D), 7.0, dtype=S.dtype(type), device="cuda"), torch.full((T + 1, n), 7.0, device="cuda")
+    ops.sort_rows_grad_device(dxs.data_ptr(), TYPES[type], rows, inv.data_ptr(), T, n, D, dx_ptr=dx.data_ptr(), w_ptr=w.data_ptr(), x_ptr=x.data_ptr(), dw_ptr=dw.data_ptr())
+    v = gathered64(dxs, inv)
+    f = w.double()[..., None]
+    S.near(S.host(dx[:T]), S.host((f * v).sum(1)), S.host((f * v).abs().sum(1)), type, n + 2)
+    terms = x.double()[:, None] * v
+    S.near(S.host(dw[:T]), S.host(terms.sum(2)), S.host(terms.abs().sum(2)), "f32", additions(D))
+    assert (dx[T] == 7.0).all() and (dw[T] == 7.0).all()
+    alone = torch.full((T, D), 7.0, dtype=S.dtype(type), device="cuda")
+    ops.sort_rows_grad_device(dxs.data_ptr(), TYPES[type], rows, inv.data_ptr(), T, n, D, dx_ptr=alone.data_ptr(), w_ptr=w.data_ptr())
+    assert torch.equal(alone, dx[:T])  # a column's sum has one order
+    del v, terms
+    dy, dw = y.clone(), torch.full((T + 1, n), 7.0, device="cuda")
+    ops.combine_rows_grad_device(dout.data_ptr(), ops.F32, dy.data_ptr(), TYPES[type], rows, inv.data_ptr(), w.data_ptr(), T, n, D, dy_ptr=dy.data_ptr(), dw_ptr=dw.data_ptr())
+    terms = dout.double()[:, None] * gathered64(y, inv)
+    S.near(S.host(dw[:T]), S.host(terms.sum(2)), S.host(terms.abs().sum(2)), "f32", additions(D))
+    want, there = y.clone(), (inv >= 0) & (inv < rows)
+    want[inv[there].long()] = (w[..., None] * dout[:, None])[there].to(S.dtype(type))
+    assert torch.equal(dy, want) and (dw[T] == 7.0).all()
