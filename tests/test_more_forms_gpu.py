@@ -90,3 +90,96 @@ def test_gradients_by_half_and_whole_warps(T, n, D, type):
     want, there = y.clone(), (inv >= 0) & (inv < rows)
     want[inv[there].long()] = (w[..., None] * dout[:, None])[there].to(S.dtype(type))
     assert torch.equal(dy, want) and (dw[T] == 7.0).all()
+
+
+# --- 8-bit rows: several rows a thread --------------------------------------------------------------------------------------
+
+
+def quantized64(x):
+    """Codes and scales of rows x on the device, in 64 bits: the quotient's rounding makes no border between two codes of what is none."""
+    import torch
+
+    x = x.double()
+    top = x.abs().amax(1)
+    bad = ~torch.isfinite(top)
+    safe = torch.where(bad | (top == 0), torch.ones_like(top), top)
+    codes = torch.round(127 * torch.where(bad[:, None], torch.zeros_like(x), x) / safe[:, None])
+    scales = torch.where(bad, torch.full_like(top, float("nan")), top).float() / torch.full_like(top, 127, dtype=torch.float32)
+    return codes.to(torch.int8), scales
+
+
+def same(codes, scales, want):
+    import torch
+
+    return torch.equal(codes, want[0]) and torch.equal(scales.view(torch.int32)[~torch.isnan(want[1])], want[1].view(torch.int32)[~torch.isnan(want[1])]) and \
+        torch.equal(torch.isnan(scales), torch.isnan(want[1]))
+
+
+# Calls of 606,208 octets and more whose rows have 4, 8, 12 and 16: four threads a row, eight, four, three and two rows a thread at the same time.
+SHORT_ROWS = [(151_553, 32), (75_787, 64), (50_533, 96), (37_891, 128)]
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T, K", SHORT_ROWS)
+def test_quantize_many_short_rows(T, K, type):
+    """As they lie; rows of ordinary sizes, and among them rows of zeros, of f32's ends, denormals, infinities and NaN, so that a thread's rows differ in kind."""
+    import torch
+
+    rng = np.random.default_rng(K)
+    x = I.rows_of(rng, T, K).astype(np.float32) if type != "f16" else np.clip(I.rows_of(rng, T, K), -6e4, 6e4).astype(np.float32)
+    plain = S.dev(x, type)
+    odd = x.copy()
+    pick = rng.integers(0, 40, T)
+    odd[pick == 1] *= np.float32(2.0 ** -100)
+    odd[pick == 2] *= np.float32(2.0 ** 70)
+    odd[pick == 3] = 0
+    odd[np.flatnonzero(pick == 4), rng.integers(0, K, (pick == 4).sum())] = np.inf
+    odd[np.flatnonzero(pick == 5), rng.integers(0, K, (pick == 5).sum())] = np.nan
+    odd[pick == 6] = np.float32(2.0 ** -149) * rng.integers(-200, 201, ((pick == 6).sum(), K))
+    for t in (plain, S.dev(odd, type)):
+        codes, scales = I.buffers(T + 1, K)
+        ops.i8_quantize_rows_device(t.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), T)
+        assert same(codes[:T], scales[:T], quantized64(t))
+        assert (codes[T] == 0x6E).all() and scales[T] == 7.0
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("T, K", SHORT_ROWS)
+def test_quantize_scatters_many_short_rows(T, K, type):
+    """To two places each, some of none, from rows that lie apart; rows no entry names are left as they were."""
+    import torch
+
+    rng, n = np.random.default_rng(K + 1), 2
+    rows = T * n * 7 // 8
+    full = S.dev(rng.standard_normal((T, K + 8)).astype(np.float32), type)
+    inv = S.dev(S.places(rng, T, n, rows, 0.05))
+    codes, scales = I.buffers(rows + 1, K)
+    ops.i8_quantize_rows_device(full.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), rows, stride=K + 8, inv_ptr=inv.data_ptr(), n_used=n)
+    want, (c, s) = I.buffers(rows + 1, K), quantized64(full[:, :K])
+    for k in range(n):
+        there = (inv[:, k] >= 0) & (inv[:, k] < rows)
+        want[0][inv[there, k].long()], want[1][inv[there, k].long()] = c[there], s[there]
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1])
+
+
+def test_the_device_form_of_the_definition_is_the_hosts():
+    rng = np.random.default_rng(3)
+    x = I.rows_of(rng, 500, 96).astype(np.float32)
+    x[7, 3], x[8, 4] = np.inf, np.nan
+    c, s = quantized64(S.dev(x))
+    want = M.quantize(x)
+    assert np.array_equal(c.cpu().numpy(), want[0]) and np.array_equal(s.cpu().numpy(), want[1], equal_nan=True)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_quantize_every_significand_by_every_other(type):
+    """Rows whose largest has every significand of the type, in [2, 4), and beside it all significands of each of the nine powers of two below."""
+    n = 1 << (7 if type == "bf16" else 10)
+    sig = 1 + np.arange(n) / n
+    x = np.concatenate([np.repeat(2 * sig[:, None], 32, 1)] + [np.tile(sig * 2.0 ** -j, (n, 1)) for j in range(9)], 1).astype(np.float32)
+    t = S.dev(x, type)
+    T, K = x.shape
+    assert K % 32 == 0 and np.array_equal(S.host(t), x)  # nothing was rounded
+    codes, scales = I.buffers(T, K)
+    ops.i8_quantize_rows_device(t.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), T)
+    assert same(codes, scales, quantized64(t))
