@@ -183,3 +183,34 @@ def test_quantize_every_significand_by_every_other(type):
     codes, scales = I.buffers(T, K)
     ops.i8_quantize_rows_device(t.data_ptr(), TYPES[type], T, K, codes.data_ptr(), scales.data_ptr(), T)
     assert same(codes, scales, quantized64(t))
+
+
+# --- products: the same bits again ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("y_type", ["f16", "bf16"])
+@pytest.mark.parametrize("E, T, k, D, F", [(512, 100, 10, 2048, 512), (16, 300, 4, 2560, 768), (1, 1, 1, 288, 64)])
+def test_gate_up_rows_and_product_repeat_themselves(E, T, k, D, F, y_type):
+    """Gate and up, its result in 8-bit rows, the product: twenty times over on buffers that held something else, bit for bit."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(E)
+    rows = T * k
+    w1, w2 = (torch.randint(-40, 41, s, generator=g, device="cuda", dtype=torch.int8) for s in ((E, 2 * F, D), (E, D, F)))
+    s1, s2 = (0.01 + 0.01 * torch.rand(s, generator=g, device="cuda") for s in ((E, 2 * F), (E, D)))
+    c, s = torch.randint(-127, 128, (rows, D), generator=g, device="cuda", dtype=torch.int8), 0.001 * torch.rand(rows, generator=g, device="cuda")
+    offsets = torch.sort(torch.randint(0, rows + 1, (E + 1,), generator=g, device="cuda"))[0].to(torch.int32)
+    offsets[0], offsets[E] = 0, rows
+    a, b = ops.I8Weights(E, 2 * F, D, w1.data_ptr(), s1.data_ptr()), ops.I8Weights(E, D, F, w2.data_ptr(), s2.data_ptr())
+    first = None
+    for i in range(20):
+        h, y = (torch.full(z, float(i), dtype=S.dtype(y_type), device="cuda") for z in ((rows, F), (rows, D)))
+        hc, hs = I.buffers(rows, F)
+        ops.i8_gate_up_device(a, c.data_ptr(), s.data_ptr(), rows, offsets.data_ptr(), h.data_ptr(), TYPES[y_type])
+        ops.i8_quantize_rows_device(h.data_ptr(), TYPES[y_type], rows, F, hc.data_ptr(), hs.data_ptr(), rows)
+        ops.i8_product_device(b, hc.data_ptr(), hs.data_ptr(), rows, offsets.data_ptr(), y.data_ptr(), TYPES[y_type])
+        if first is None:
+            first = h, hc, hs, y
+            assert torch.isfinite(y).all() and (y != 0).any()
+        assert all(torch.equal(p, q) for p, q in zip(first, (h, hc, hs, y)))
+    ops.status()
