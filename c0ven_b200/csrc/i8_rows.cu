@@ -1,8 +1,7 @@
 // Rows to and from 8-bit integers with a scale each (include/moe_layer.h, "8-bit rows"). Single passes over their data: what bounds long calls is HBM. A row's values
 // stay in its threads' registers, as they were loaded, from its largest magnitude to its codes. 32,768 rows of 2,048 bf16 values to 8-bit rows 35.5 us
 // (5.7 TB/s) and back 31.5 (6.4); f32 values 58 (5.7); 65,536 rows of 768 bf16 values 30 (5.0), f32 49 (5.1); 300,000 of 64 bf16 15, f32 24.8; 4,096 of 2,880 bf16 to six
-// places each 22, f32 31.7. 13 rows of 2,560 f32 values
-// to eight places each and back 2.6 + 1.6 us, one round trip after another.
+// places each 22, f32 31.7. 13 rows of 2,560 f32 values to eight places each and back 2.6 + 1.6 us, one round trip after another.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -19,9 +18,10 @@ namespace {
 constexpr uint32_t kRowsMaxUsed = 16;
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kHeldOctets = 8;             // groups of eight values a thread holds
-// Octets of a call from which on a thread has up to eight of one row or more: as many as two CTAs an SM hold so. To 8-bit rows, by an octet a thread and by up to eight: 2,048 bf16 values, 2,048 rows 5.7 and 5.6 us, 2,400 6.1 and 5.3, 4,800 11.0 and 7.2, 9,500 21 and 13.4; f32, 1,024 rows 4.2 and 4.6, 2,400 7.9 and 7.1, 9,500 31
-// and 21.5; 64 bf16 values, 75,800 rows 5.6 and 6.9, 152,000 9.3 and 8.9, 300,000 17.8 and 15.1. Back, by an octet a thread and by four: 2,400 of 2,048 3.4 and 3.8, 3,200
-// 4.2 and 4.1, 9,500 12.6 and 10.7.
+// Octets of a call from which on a thread has up to eight of one row or more: as many as two CTAs an SM hold so. To 8-bit rows, us by an octet a thread and by up
+// to eight: 2,048 bf16 values, 2,048 rows 5.7 and 5.6, 2,400 6.1 and 5.3, 4,800 11.0 and 7.2, 9,500 21 and 13.4; f32, 1,024 rows 4.2 and 4.6, 2,400 7.9 and 7.1, 9,500
+// 31 and 21.5; 64 bf16 values, 75,800 rows 5.6 and 6.9, 152,000 9.3 and 8.9, 300,000 17.8 and 15.1. Back, by an octet a thread and by four: 2,400 rows of 2,048 3.4 and
+// 3.8, 3,200 4.2 and 4.1, 9,500 12.6 and 10.7.
 constexpr uint32_t kManyOctets = 2 * 148 * 256 * kHeldOctets;
 
 // How rows are dealt to a CTA of 256 threads: 2^log2 neighbouring threads a row; of its octets, groups of eight values, thread i takes i,
